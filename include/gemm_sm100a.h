@@ -263,6 +263,137 @@ int gemm_sm100a_umma_peak(int32_t dtype, int32_t cta_group, int32_t num_ctas, in
 int gemm_sm100a_tma_read_probe(const void* buf, int64_t bytes, int32_t box_width, int32_t box_rows,
                                int32_t stages, int32_t ctas_per_sm, unsigned long long* results, void* stream);
 
+/* ------------------------------------------------------------------------
+ * 8-bit integer linear layers: the product of int8 operands with one scale per
+ * token and channel, the quantiser that makes such operands, and dropout.
+ * ------------------------------------------------------------------------ */
+
+/* Element types of the floating tensors these calls read and write. */
+enum {
+  GEMM_TYPE_BF16 = 0,
+  GEMM_TYPE_FP16 = 1,
+  GEMM_TYPE_FP32 = 2
+};
+
+/*
+ * Dropout of element (r, c) of a matrix, from the generator's counter (see
+ * gemm_sm100a_generate): nothing is stored, the mask is a pure function of
+ * (seed, stream_id, index), so the backward pass and every rank of an N-split
+ * regenerate exactly their part of it.
+ *   index = (row0 + r) * row_elems + col0 + c
+ *   h     = mix64(key(seed, stream_id) + (index / 2 + 1) * 0x9E3779B97F4A7C15)
+ *   word  = index odd ? h >> 32 : h & 0xFFFFFFFF
+ *   kept iff word >= rint(p * 2^32); a kept value is multiplied by 1 / (1 - p),
+ *   a dropped one is replaced by 0 whatever it was (NaN and Inf included).
+ * p = 0 disables it (no other field is read), p = 1 drops everything.
+ * row0, col0 >= 0, row_elems >= col0 + columns, all indices below 2^62.
+ */
+typedef struct DropoutArgs {
+  double   p;
+  uint64_t seed, stream_id;
+  const uint64_t* seed_offset; /* optional device word added to seed when the kernel runs, so that
+                                  a captured graph draws a new mask at each replay; 8-byte aligned */
+  int64_t  row0, col0, row_elems;
+} DropoutArgs;
+
+/*
+ *   D = C + dropout( scale_a[i] * scale_b[j] * sum_k A[i][k] B[j][k] + bias[j] )
+ *
+ *   A  m x k int8 (tokens), B  n x k int8 (channels), K contiguous, rows of
+ *   lda / ldb bytes (multiples of 16, bases 16-byte aligned); bytes between k
+ *   and the row stride are not used.  The sum is exact in int32 (k <= 131071),
+ *   everything after it fp32, rounded once to d_type.  The result has the
+ *   same bits for every tile, split and size of the batch.
+ *   scale_a (m) and scale_b (n) fp32; NULL means 1.
+ *   D  m x n row-major (N contiguous), leading dimension ldd >= n elements,
+ *   any alignment of its own type; C (optional) like D with ldc, may be D.
+ *   bias (optional): n elements of bias_type.
+ * m or n of 0: nothing is launched.  D must not overlap A, B, scales or bias.
+ */
+typedef struct Int8GemmArgs {
+  uint32_t struct_size;    /* sizeof(Int8GemmArgs) */
+  int32_t  d_type;         /* GEMM_TYPE_*: D and C */
+  int64_t  m, n, k;
+  const void* a;  int64_t lda;
+  const void* b;  int64_t ldb;
+  void*       d;  int64_t ldd;
+  const void* c;  int64_t ldc;
+  const float* scale_a;
+  const float* scale_b;
+  const void* bias;
+  int32_t  bias_type;      /* GEMM_TYPE_* */
+  int32_t  tile_n;         /* tokens per tile; 0 = chosen from the sizes */
+  int32_t  cta_group;      /* 1 or 2 (CTA pair); 0 = chosen */
+  int32_t  split_k;        /* CTAs that share one tile's K; 0 = chosen */
+  DropoutArgs drop;
+  int32_t* status;         /* optional device int32, as in GemmArgs */
+  uint32_t timeout_ms;     /* device wait budget; 0 = 4000 ms */
+  uint32_t flags;          /* 0 or GEMM_FLAG_INJECT_STALL */
+} Int8GemmArgs;
+
+/* Validate and resolve without launching (GemmInfo.tile_m is the channels of a
+ * tile, tile_n its tokens). */
+int gemm_sm100a_int8_query(const Int8GemmArgs* args, GemmInfo* info);
+
+/* Enqueue one product; asynchronous, allocates nothing, capturable. */
+int gemm_sm100a_int8_launch(const Int8GemmArgs* args, void* stream);
+
+/*
+ * Quantise the rows of X (m x k of x_type, row stride ldx elements) and multiply:
+ * gemm_sm100a_quantize_int8 followed by gemm_sm100a_int8_launch, bit for bit, in one
+ * or two launches.  args->a and args->scale_a are workspace of the caller
+ * (m * lda bytes and m floats; their content afterwards is unspecified).
+ */
+int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream);
+
+/*
+ * Symmetric int8 quantisation with one scale per row:
+ *   amax_i = max(max_j |x_ij|, 127 * 2^-126),  scale_i = amax_i / 127,
+ *   q_ij   = 127 * x_ij / amax_i rounded to the nearest integer, ties to even
+ * (decided exactly, not from a rounded quotient).  A row with a NaN or an
+ * infinity gets that as its scale and zeros as q, which makes NaN of what is
+ * computed from it and touches no other row.
+ * With transpose: one scale per COLUMN, q stored cols x rows (ldq >= rows), and
+ * optionally the sum of each column (fp32) in col_sums.
+ * With drop.p > 0, x is first masked; the factor 1 / (1 - p) enters scale and
+ * col_sums (indices count elements of X as stored, transposed or not).
+ * ldq is a multiple of 16 bytes, q 16-byte aligned; bytes of q beyond the last
+ * element of a row are left as they were.  rows or cols of 0: with transpose
+ * and rows = 0 the scales are 2^-126 and the sums 0, else nothing is written.
+ */
+typedef struct Int8QuantArgs {
+  uint32_t struct_size;    /* sizeof(Int8QuantArgs) */
+  int32_t  x_type;         /* GEMM_TYPE_* */
+  int64_t  rows, cols;
+  const void* x;  int64_t ldx;
+  void*    q;     int64_t ldq;
+  float*   scale;
+  float*   col_sums;       /* transpose only; NULL = not wanted */
+  int32_t  transpose;
+  int32_t  reserved;       /* 0 */
+  DropoutArgs drop;
+} Int8QuantArgs;
+
+int gemm_sm100a_quantize_int8(const Int8QuantArgs* args, void* stream);
+
+/*
+ * Y = residual + dropout(X), rows x cols row-major with their own row strides
+ * (elements), all of one type, any alignment of that type; computed in fp32 and
+ * rounded once.  Its gradient is the same call on dY without the residual.
+ * Y may be X or residual (same stride).
+ */
+typedef struct DropoutOpArgs {
+  uint32_t struct_size;    /* sizeof(DropoutOpArgs) */
+  int32_t  type;           /* GEMM_TYPE_* */
+  int64_t  rows, cols;
+  const void* x;         int64_t ldx;
+  const void* residual;  int64_t ldr;   /* NULL = none */
+  void*    y;            int64_t ldy;
+  DropoutArgs drop;
+} DropoutOpArgs;
+
+int gemm_sm100a_dropout(const DropoutOpArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,3 +35,25 @@ struct StreamDeviceGuard {
     if (prev >= 0 && prev != dev) cudaSetDevice(prev);
   }
 };
+
+// The same for a call that names no owner of its stream: the device is that of
+// `ptr`, a buffer the call writes.  It is right on every stream (the legacy
+// default stream belongs to whichever device is current), does not touch a
+// capturing stream, and turns a pointer to host memory into an error.
+struct PointerDeviceGuard {
+  int prev = -1;
+  int dev = 0;
+  bool ok = false;
+  explicit PointerDeviceGuard(const void* ptr) {
+    if (cudaGetDevice(&prev) != cudaSuccess) { prev = -1; cudaGetLastError(); }
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, ptr) != cudaSuccess) { cudaGetLastError(); return; }
+    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) return;
+    dev = at.device;
+    if (dev != prev && cudaSetDevice(dev) != cudaSuccess) { cudaGetLastError(); return; }
+    ok = true;
+  }
+  ~PointerDeviceGuard() {
+    if (prev >= 0 && prev != dev) cudaSetDevice(prev);
+  }
+};

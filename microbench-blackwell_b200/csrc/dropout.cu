@@ -1,0 +1,98 @@
+// dropout.cu -- Y = residual + dropout(X) with a mask that is never stored: it
+// is drawn again from the counter of each element (counter_rng.cuh) wherever it
+// is needed.  Bound by the bytes of X, residual and Y.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+
+#include "device_guard.cuh"
+#include "gemm_sm100a.h"
+#include "int8_common.cuh"
+
+using namespace int8op;
+
+namespace {
+
+struct DropoutParams {
+  const void* x; int64_t ldx;
+  const void* res; int64_t ldr;
+  void* y; int64_t ldy;
+  int64_t rows, cols;
+  Drop drop;
+  int32_t wide;
+};
+
+// One 16-byte vector per thread and row; blockDim.x threads cover a segment of
+// the row, blockDim.y rows.
+template <typename T, bool RES>
+__global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
+  constexpr int V = Vec<T>::N;
+  const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
+  if (c >= p.cols) return;
+  const int n = (int)min((int64_t)V, p.cols - c);
+  const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
+  const float grow = p.drop.on ? p.drop.grow : 1.f;
+  for (int64_t r = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r < p.rows; r += (int64_t)gridDim.y * blockDim.y) {
+    const Vec<T> v = load_vec<T>(static_cast<const T*>(p.x) + r * p.ldx + c, n, p.wide);
+    Vec<T> b = {};
+    if constexpr (RES) b = load_vec<T>(static_cast<const T*>(p.res) + r * p.ldr + c, n, p.wide);
+    const uint32_t keep = p.drop.on ? drop_mask<V>(key, p.drop.threshold, drop_index(p.drop, r, c)) : 0xFFFFFFFFu;
+    Vec<T> o;
+    o.w[0] = o.w[1] = o.w[2] = o.w[3] = 0u;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float f = keep >> j & 1u ? v.get(j) * grow : 0.f;
+      if constexpr (RES) f += b.get(j);
+      o.set(j, f);
+    }
+    store_vec<T>(static_cast<T*>(p.y) + r * p.ldy + c, o, n, p.wide);
+  }
+}
+
+template <typename T>
+cudaError_t launch(const DropoutParams& p, cudaStream_t st) {
+  const int64_t nvec = (p.cols + Vec<T>::N - 1) / Vec<T>::N;
+  int tx = 32;
+  while (tx < 256 && tx < nvec) tx *= 2;
+  const int ty = 256 / tx;
+  const int64_t gx = (nvec + tx - 1) / tx;
+  int64_t gy = (p.rows + ty - 1) / ty;
+  if (gy > 65535) gy = 65535;
+  const dim3 grid((unsigned)gx, (unsigned)gy), block((unsigned)tx, (unsigned)ty);
+  if (p.res) dropout_kernel<T, true><<<grid, block, 0, st>>>(p);
+  else dropout_kernel<T, false><<<grid, block, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+extern "C" int gemm_sm100a_dropout(const DropoutOpArgs* a, void* stream) {
+  if (!a || a->struct_size != sizeof(DropoutOpArgs)) return GEMM_ERR_BAD_ARGS;
+  if (!type_ok(a->type) || a->rows < 0 || a->cols < 0 || a->cols > INT32_MAX / 2 || a->rows > INT32_MAX / 2)
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  DropoutParams p;
+  memset(&p, 0, sizeof(p));
+  const char* why = "";
+  const int rc = drop_resolve(a->drop, a->rows, a->cols, p.drop, &why);
+  if (rc != GEMM_OK) return rc;
+  if (a->rows == 0 || a->cols == 0) return GEMM_OK;
+  if (!a->x || !a->y) return GEMM_ERR_BAD_ARGS;
+  const int e = type_bytes(a->type);
+  if (a->ldx < a->cols || a->ldy < a->cols || (a->residual && a->ldr < a->cols)) return GEMM_ERR_CANNOT_IMPLEMENT;
+  if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->y) | reinterpret_cast<uintptr_t>(a->residual)) % e)
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  p.x = a->x; p.ldx = a->ldx; p.res = a->residual; p.ldr = a->ldr; p.y = a->y; p.ldy = a->ldy;
+  p.rows = a->rows; p.cols = a->cols;
+  p.wide = rows_16b(a->x, a->ldx, e) && rows_16b(a->y, a->ldy, e) && (!a->residual || rows_16b(a->residual, a->ldr, e));
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  PointerDeviceGuard guard(a->y);
+  if (!guard.ok) return GEMM_ERR_LAUNCH;
+  const cudaError_t err = a->type == GEMM_TYPE_BF16 ? launch<__nv_bfloat16>(p, st)
+                        : a->type == GEMM_TYPE_FP16 ? launch<__half>(p, st) : launch<float>(p, st);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    return GEMM_ERR_LAUNCH;
+  }
+  return GEMM_OK;
+}

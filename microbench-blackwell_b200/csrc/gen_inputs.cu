@@ -15,23 +15,13 @@
 #include <cstdint>
 
 #include "gemm_sm100a.h"
+#include "counter_rng.cuh"
 #include "device_guard.cuh"
 
 namespace {
 
-__device__ __forceinline__ uint64_t mix64(uint64_t z) {
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ULL;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBULL;
-  return z ^ (z >> 31);
-}
-constexpr uint64_t kGolden = 0x9E3779B97F4A7C15ULL;
-
-__host__ __device__ inline uint64_t mix64_hd(uint64_t z) {
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ULL;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBULL;
-  return z ^ (z >> 31);
-}
-inline uint64_t stream_key(uint64_t seed, uint64_t stream) { return mix64_hd(seed + mix64_hd(stream + kGolden)); }
+using counter_rng::draw;
+using counter_rng::stream_key;
 
 __device__ __forceinline__ float uniform_from_bits(uint64_t r) {
   return __fsub_rn(__fmul_rn((float)(int32_t)(r >> 40), 1.0f / 8388608.0f), 1.0f);
@@ -151,7 +141,7 @@ __global__ void generate_kernel(void* out, int out_dtype, int dist, float scale,
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / cols, c = i - r * cols;
     const uint64_t idx = (uint64_t)((row0 + r) * cols + c);
-    const uint64_t bits = mix64(key + (idx + 1) * kGolden);
+    const uint64_t bits = draw(key, idx);
     float v = dist ? normal_from_bits(bits) : uniform_from_bits(bits);
     v = __fmul_rn(v, scale);
     if (out_dtype == GEMM_DTYPE_BF16)
@@ -174,7 +164,7 @@ __global__ void generate_nvfp4_kernel(uint8_t* packed, uint8_t* scales, float sc
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const uint64_t idx = (uint64_t)((row0 + r) * cols + cb * 16 + j);
-      v[j] = __fmul_rn(normal_from_bits(mix64(key + (idx + 1) * kGolden)), scale);
+      v[j] = __fmul_rn(normal_from_bits(draw(key, idx)), scale);
       amax = fmaxf(amax, fabsf(v[j]));
     }
     const uint8_t sq = ue4m3_round_up(__fdiv_rn(amax, 6.0f));

@@ -1,0 +1,245 @@
+// int8_common.cuh -- what the 8-bit integer operators share: element types,
+// the dropout mask, exact int8 rounding and host-side argument checks.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "counter_rng.cuh"
+#include "gemm_sm100a.h"
+
+namespace int8op {
+
+__host__ __device__ constexpr int type_bytes(int t) { return t == GEMM_TYPE_FP32 ? 4 : 2; }
+__host__ __device__ constexpr bool type_ok(int t) { return t >= GEMM_TYPE_BF16 && t <= GEMM_TYPE_FP32; }
+
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+
+// Element i of a vector of run-time type t.
+__device__ __forceinline__ float load_as_f32(const void* p, int t, int64_t i) {
+  if (t == GEMM_TYPE_FP32) return static_cast<const float*>(p)[i];
+  if (t == GEMM_TYPE_BF16) return to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
+  return to_f32(static_cast<const __half*>(p)[i]);
+}
+
+// 16 bytes of T as registers; element access is compile-time indexed.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / (int)sizeof(T);
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint16_t h = (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu);
+      T v;
+      __builtin_memcpy(&v, &h, 2);
+      return to_f32(v);
+    }
+  }
+  __device__ __forceinline__ void set(int i, float f) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(f);
+    } else {
+      const T v = from_f32<T>(f);
+      uint16_t h;
+      __builtin_memcpy(&h, &v, 2);
+      w[i / 2] = i & 1 ? (w[i / 2] & 0xFFFFu) | ((uint32_t)h << 16) : (w[i / 2] & 0xFFFF0000u) | h;
+    }
+  }
+  __device__ __forceinline__ void zero(int i) {
+    if constexpr (sizeof(T) == 4) w[i] = 0u;
+    else w[i / 2] &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+  }
+};
+
+// Elements [0, n) of p (n <= Vec<T>::N; the rest reads as 0).  `wide`: p is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p, int n, bool wide) {
+  Vec<T> v;
+  if (n >= Vec<T>::N && wide) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
+  } else {
+    v.w[0] = v.w[1] = v.w[2] = v.w[3] = 0u;
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i)
+      if (i < n) {
+        if constexpr (sizeof(T) == 4) {
+          v.w[i] = __float_as_uint(reinterpret_cast<const float*>(p)[i]);
+        } else {
+          const uint32_t h = reinterpret_cast<const uint16_t*>(p)[i];
+          v.w[i / 2] |= i & 1 ? h << 16 : h;
+        }
+      }
+  }
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T>& v, int n, bool wide) {
+  if (n >= Vec<T>::N && wide) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i)
+      if (i < n) {
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[i] = v.w[i];
+        else reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(i & 1 ? v.w[i / 2] >> 16 : v.w[i / 2] & 0xFFFFu);
+      }
+  }
+}
+
+// ------------------------------------------------------------------ dropout
+// Kernel-side form of DropoutArgs.
+struct Drop {
+  uint64_t seed_mix;            // seed + mix64(stream_id + golden)
+  const uint64_t* seed_offset;
+  uint64_t threshold;           // rint(p * 2^32): a word below it is dropped
+  float grow;                   // 1 / (1 - p), 0 for p = 1
+  int32_t on;
+  int64_t row0, col0, row_elems;
+};
+
+__device__ __forceinline__ uint64_t drop_key(const Drop& d) {
+  return counter_rng::mix64(d.seed_mix + (d.seed_offset ? *d.seed_offset : 0ull));
+}
+__device__ __forceinline__ int64_t drop_index(const Drop& d, int64_t r, int64_t c) {
+  return (d.row0 + r) * d.row_elems + d.col0 + c;
+}
+__device__ __forceinline__ bool drop_keeps(uint64_t key, uint64_t threshold, int64_t index) {
+  const uint64_t h = counter_rng::draw(key, (uint64_t)index >> 1);
+  return (index & 1 ? h >> 32 : h & 0xFFFFFFFFull) >= threshold;
+}
+// Bit e of the result: element `index` + e is kept, e < N (N even).  One draw
+// serves the two elements of an aligned pair.
+template <int N>
+__device__ __forceinline__ uint32_t drop_mask(uint64_t key, uint64_t threshold, int64_t index) {
+  const uint64_t first = (uint64_t)index >> 1;
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < N / 2; ++j) {
+    const uint64_t h = counter_rng::draw(key, first + j);
+    m |= ((h & 0xFFFFFFFFull) >= threshold ? 1u : 0u) << (2 * j);
+    m |= ((h >> 32) >= threshold ? 1u : 0u) << (2 * j + 1);
+  }
+  if (index & 1) {
+    const uint64_t h = counter_rng::draw(key, first + N / 2);
+    m = (m >> 1) | (((h & 0xFFFFFFFFull) >= threshold ? 1u : 0u) << (N - 1));
+  }
+  return m;
+}
+
+// ------------------------------------------------------------------ int8 rounding
+// q = 127 * x / amax to the nearest integer, ties to even, decided exactly.
+// Everything is scaled by a power of two g so that neither the products nor
+// the reciprocal leave the normal range.
+constexpr float kAmaxMin = 127.0f * 1.17549435e-38f;   // 127 * 2^-126
+
+struct RowScale {
+  float c;      // 127 * g, 0 for a row with NaN or Inf
+  float a;      // amax * g
+  float ra;     // 1 / a
+  float scale;  // amax / 127
+};
+
+// `bits`: the largest |x| of the row as fp32 bits (integer maximum, so NaN > Inf > finite).
+__device__ __forceinline__ RowScale row_scale(uint32_t bits) {
+  RowScale s;
+  if (bits >= 0x7F800000u) {
+    s.c = 0.f; s.a = 1.f; s.ra = 1.f; s.scale = __uint_as_float(bits);
+    return s;
+  }
+  const float amax = fmaxf(__uint_as_float(bits), kAmaxMin);
+  const float g = amax < 0x1p-60f ? 0x1p64f : (amax > 0x1p60f ? 0x1p-64f : 1.f);
+  s.c = 127.f * g;
+  s.a = amax * g;
+  s.ra = __frcp_rn(s.a);
+  s.scale = __fdiv_rn(amax, 127.f);
+  return s;
+}
+
+constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it leaves the nearest integer in the low byte
+
+// Low byte: q of one element.
+//  16-bit x: 127 x g is exact in fp32 and one correction step gives the
+//    quotient t to one unit in the last place, exactly where it is a tie.  With
+//    significands of 18 and 11 bits a t >= 1/4 that is not half-way between
+//    integers is at least 2^-20 t away from there, 16 times that error.
+//  fp32 x: f is an integer with f - eps <= t <= f + 1 + eps for the quotient t;
+//    the sign of 127 x g - a (f + 1/2), whose first term is held as yh + yl and
+//    whose fused difference is exact near zero, says whether t rounds to f + 1.
+template <typename T>
+__device__ __forceinline__ uint32_t quantize_one(float x, const RowScale& s) {
+  if constexpr (sizeof(T) == 2) {
+    const float y = x * s.c;
+    const float t = y * s.ra;
+    const float r = fmaf(-s.a, t, y);
+    return __float_as_uint(fmaf(r, s.ra, t) + kRound);
+  } else {
+    const float yh = x * s.c;
+    const float yl = fmaf(x, s.c, -yh);
+    const float m = fmaf(yh, s.ra, -0.5f) + kRound;
+    const float f = m - kRound;
+    const float d = fmaf(-s.a, f + 0.5f, yh) + yl;
+    const uint32_t q = __float_as_uint(m);
+    return q + ((d > 0.f || (d == 0.f && (q & 1u))) ? 1u : 0u);
+  }
+}
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// Largest |x| of a vector as fp32 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t abs_bits_to_f32(uint32_t h) {   // magnitude bits of T
+  if constexpr (sizeof(T) == 4) return h;
+  else {
+    const uint16_t u = (uint16_t)h;
+    T v;
+    __builtin_memcpy(&v, &u, 2);
+    return __float_as_uint(to_f32(v));
+  }
+}
+
+// ------------------------------------------------------------------ host checks
+inline int drop_resolve(const DropoutArgs& a, int64_t rows, int64_t cols, Drop& d, const char** why) {
+  d = Drop{};
+  if (!(a.p >= 0.0 && a.p <= 1.0)) { *why = "dropout p must be in [0, 1]"; return GEMM_ERR_CANNOT_IMPLEMENT; }
+  if (a.p == 0.0) return GEMM_OK;
+  if (a.row0 < 0 || a.col0 < 0) { *why = "dropout row0/col0 must be >= 0"; return GEMM_ERR_CANNOT_IMPLEMENT; }
+  if (a.row_elems < cols || a.col0 > a.row_elems - cols) {
+    *why = "dropout row_elems must be >= col0 + columns";
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  }
+  if (((__int128)a.row0 + rows) * a.row_elems > ((__int128)1 << 62)) {
+    *why = "dropout index beyond 2^62";
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  }
+  if (reinterpret_cast<uintptr_t>(a.seed_offset) & 7) {
+    *why = "dropout seed_offset must be 8-byte aligned";
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  }
+  d.on = 1;
+  d.seed_mix = a.seed + counter_rng::mix64(a.stream_id + counter_rng::kGolden);
+  d.seed_offset = a.seed_offset;
+  d.threshold = (uint64_t)std::llrint(a.p * 4294967296.0);
+  d.grow = a.p == 1.0 ? 0.f : (float)(1.0 / (1.0 - a.p));
+  d.row0 = a.row0; d.col0 = a.col0; d.row_elems = a.row_elems;
+  return GEMM_OK;
+}
+
+// Whether every row of a (base, stride in elements) matrix starts on a 16-byte boundary.
+inline bool rows_16b(const void* p, int64_t ld, int elem_bytes) {
+  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * elem_bytes)) & 15) == 0;
+}
+
+}  // namespace int8op

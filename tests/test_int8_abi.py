@@ -1,0 +1,162 @@
+"""CPU tests of the int8 operators' argument checks (no kernel launches): every
+refusal happens before any CUDA call, with a reason."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+def _gemm(pkg, **kw):
+    a = pkg.Int8GemmArgs()
+    a.struct_size = C.sizeof(pkg.Int8GemmArgs)
+    base = dict(d_type=0, m=64, n=128, k=256, a=0x10000, lda=256, b=0x20000, ldb=256, d=0x30000, ldd=128,
+                scale_a=0x40000, scale_b=0x50000)
+    base.update(kw)
+    for name, v in base.items():
+        if name.startswith("drop_"):
+            setattr(a.drop, name[5:], v)
+        else:
+            setattr(a, name, v)
+    return a
+
+
+def test_packed_layouts_match_the_structs(pkg):
+    import importlib
+    i8 = importlib.import_module("microbench_blackwell_b200.int8")
+    assert i8._GEMM_PACK.size == C.sizeof(pkg.Int8GemmArgs)
+    assert i8._QUANT_PACK.size == C.sizeof(pkg.Int8QuantArgs)
+    assert i8._DROPOUT_PACK.size == C.sizeof(pkg.DropoutOpArgs)
+    packed = i8._GEMM_PACK.pack(208, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18, 19, 20,
+                                0.5, 21, 22, 23, 24, 25, 26, 27, 28, 29)
+    s = pkg.Int8GemmArgs.from_buffer_copy(packed)
+    assert (s.struct_size, s.d_type, s.m, s.lda, s.ldc, s.bias_type, s.split_k) == (208, 2, 3, 7, 13, 17, 20)
+    assert (s.drop.p, s.drop.seed, s.drop.row_elems, s.status, s.timeout_ms, s.flags) == (0.5, 21, 26, 27, 28, 29)
+
+
+def test_a_plain_problem_is_accepted(pkg):
+    rc, info = pkg.query_int8(_gemm(pkg))
+    assert rc == pkg.OK and info.can_implement == 1
+
+
+@pytest.mark.parametrize("kw,rc,frag", [
+    (dict(struct_size=8), "bad", b"struct_size"),
+    (dict(a=None), "bad", b"null"),
+    (dict(d=None), "bad", b"null"),
+    (dict(d_type=3), "no", b"d_type"),
+    (dict(bias=0x60000, bias_type=7), "no", b"bias_type"),
+    (dict(k=0), "no", b"empty"),
+    (dict(m=-1), "no", b"empty"),
+    (dict(k=131072, lda=131072, ldb=131072), "no", b"131071"),
+    (dict(m=1 << 31), "no", b"too large"),
+    (dict(a=0x10008), "no", b"16-byte"),
+    (dict(lda=240), "no", b"lda"),
+    (dict(k=250, lda=250, ldb=256), "no", b"multiples of 16"),
+    (dict(ldd=127), "no", b"ldd"),
+    (dict(d=0x30001), "no", b"element"),
+    (dict(c=0x60000, ldc=100), "no", b"ldc"),
+    (dict(scale_a=0x40002), "no", b"scales"),
+    (dict(bias=0x60001), "no", b"bias"),
+    (dict(flags=2), "no", b"flags"),
+    (dict(drop_p=-0.1), "no", b"dropout p"),
+    (dict(drop_p=float("nan")), "no", b"dropout p"),
+    (dict(drop_p=0.5, drop_row_elems=127), "no", b"row_elems"),
+    (dict(drop_p=0.5, drop_row_elems=200, drop_col0=100), "no", b"row_elems"),
+    (dict(drop_p=0.5, drop_row_elems=128, drop_row0=-1), "no", b"row0"),
+    (dict(drop_p=0.5, drop_row_elems=128, drop_row0=1 << 60), "no", b"2^62"),
+    (dict(drop_p=0.5, drop_row_elems=128, drop_seed_offset=0x60004), "no", b"seed_offset"),
+])
+def test_refused_products(pkg, kw, rc, frag):
+    got, info = pkg.query_int8(_gemm(pkg, **kw))
+    assert got == (pkg.ERR_BAD_ARGS if rc == "bad" else pkg.ERR_CANNOT_IMPLEMENT)
+    assert frag in info.reason, info.reason
+    assert info.can_implement == 0
+    L = pkg.lib()
+    assert L.gemm_sm100a_int8_launch(bytes(_gemm(pkg, **kw)), None) == got
+    assert L.gemm_sm100a_int8_linear(bytes(_gemm(pkg, **kw)), C.c_void_p(0x70000), 0, 256, None) == got
+
+
+def test_null_argument_blocks(pkg):
+    L = pkg.lib()
+    assert L.gemm_sm100a_int8_launch(None, None) == pkg.ERR_BAD_ARGS
+    assert L.gemm_sm100a_quantize_int8(None, None) == pkg.ERR_BAD_ARGS
+    assert L.gemm_sm100a_dropout(None, None) == pkg.ERR_BAD_ARGS
+
+
+def test_empty_products_launch_nothing(pkg):
+    L = pkg.lib()
+    for kw in (dict(m=0), dict(n=0)):
+        assert L.gemm_sm100a_int8_launch(bytes(_gemm(pkg, **kw)), None) == pkg.OK
+        assert L.gemm_sm100a_int8_linear(bytes(_gemm(pkg, **kw)), C.c_void_p(0x70000), 0, 256, None) == pkg.OK
+
+
+@pytest.mark.parametrize("x,x_type,ldx", [(None, 0, 256), (0x70000, 5, 256), (0x70000, 0, 255), (0x70001, 0, 256)])
+def test_linear_refuses_bad_tokens(pkg, x, x_type, ldx):
+    assert pkg.lib().gemm_sm100a_int8_linear(bytes(_gemm(pkg)), C.c_void_p(x), x_type, ldx, None) in (
+        pkg.ERR_BAD_ARGS, pkg.ERR_CANNOT_IMPLEMENT)
+
+
+def _quant(pkg, **kw):
+    a = pkg.Int8QuantArgs()
+    a.struct_size = C.sizeof(pkg.Int8QuantArgs)
+    base = dict(x_type=0, rows=8, cols=32, x=0x10000, ldx=32, q=0x20000, ldq=32, scale=0x30000)
+    base.update(kw)
+    for name, v in base.items():
+        if name.startswith("drop_"):
+            setattr(a.drop, name[5:], v)
+        else:
+            setattr(a, name, v)
+    return a
+
+
+@pytest.mark.parametrize("kw", [
+    dict(struct_size=4), dict(x_type=3), dict(x_type=-1), dict(rows=-1), dict(cols=1 << 31), dict(x=None), dict(q=None),
+    dict(scale=None), dict(col_sums=0x40000), dict(ldx=31), dict(x=0x10001), dict(ldq=40), dict(ldq=16), dict(q=0x20008),
+    dict(scale=0x30002), dict(drop_p=2.0), dict(drop_p=0.5, drop_row_elems=31), dict(transpose=1, rows=40, ldq=32),
+])
+def test_refused_quantisations(pkg, kw):
+    rc = pkg.lib().gemm_sm100a_quantize_int8(bytes(_quant(pkg, **kw)), None)
+    assert rc in (pkg.ERR_BAD_ARGS, pkg.ERR_CANNOT_IMPLEMENT)
+
+
+def _drop(pkg, **kw):
+    a = pkg.DropoutOpArgs()
+    a.struct_size = C.sizeof(pkg.DropoutOpArgs)
+    base = dict(type=0, rows=8, cols=32, x=0x10000, ldx=32, y=0x20000, ldy=32, drop_p=0.5, drop_row_elems=32)
+    base.update(kw)
+    for name, v in base.items():
+        if name.startswith("drop_"):
+            setattr(a.drop, name[5:], v)
+        else:
+            setattr(a, name, v)
+    return a
+
+
+@pytest.mark.parametrize("kw", [
+    dict(struct_size=4), dict(type=3), dict(rows=-1), dict(x=None), dict(y=None), dict(ldx=31), dict(ldy=16),
+    dict(residual=0x30000, ldr=8), dict(residual=0x30001, ldr=32), dict(x=0x10001), dict(drop_p=1.5),
+    dict(drop_row_elems=16), dict(drop_col0=-2), dict(drop_seed_offset=0x50001),
+])
+def test_refused_dropouts(pkg, kw):
+    rc = pkg.lib().gemm_sm100a_dropout(bytes(_drop(pkg, **kw)), None)
+    assert rc in (pkg.ERR_BAD_ARGS, pkg.ERR_CANNOT_IMPLEMENT)
+
+
+def test_python_helpers_refuse_host_tensors(pkg):
+    """There is no CPU path: a host tensor is an error, not a fallback."""
+    x = torch.zeros((4, 32))
+    q = torch.zeros((4, 32), dtype=torch.int8)
+    s = torch.ones(4)
+    with pytest.raises(ValueError):
+        pkg.quantize_int8(x)
+    with pytest.raises(ValueError):
+        pkg.gemm_int8(q, s, q, s)
+    with pytest.raises(ValueError):
+        pkg.linear_int8(x, q, s)
+    with pytest.raises(ValueError):
+        pkg.linear_int8_backward(x, x, q, s)
+    with pytest.raises(ValueError):
+        pkg.dropout(x, pkg.Dropout(0.5))
+    with pytest.raises(ValueError):
+        pkg.quantize_int8(x.to(torch.float64))
+    with pytest.raises(ValueError):
+        pkg.quantize_int8(x[0])
