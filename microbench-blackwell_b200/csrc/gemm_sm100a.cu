@@ -42,13 +42,12 @@
 #include "gemm_sm100a.h"
 #include "sm100_ptx.cuh"
 #include "device_guard.cuh"
+#include "bounded_wait.cuh"
+#include "tensor_map.cuh"
 
 using namespace sm100;
 
 // Tuning switches (compile time).
-#ifndef GEMM_L2_PROMOTION
-#define GEMM_L2_PROMOTION CU_TENSOR_MAP_L2_PROMOTION_L2_256B
-#endif
 #ifndef GEMM_TMA_CACHE_HINT
 #define GEMM_TMA_CACHE_HINT 1   // 1: loads carry an L2 evict_normal policy; 0: no hint
 #endif
@@ -100,8 +99,6 @@ constexpr int kMinSmemPerCta = 120 * 1024;  // > half of the SM's 228 KiB: at mo
 #define GEMM_ACC_OVERLAP 64     // overlapped accumulator positions for 256-wide NVFP4 tiles (columns; 0 = off)
 #endif
 constexpr int kAccOverlap = GEMM_ACC_OVERLAP;
-
-enum Role : uint32_t { ROLE_PRODUCER = 1, ROLE_MMA = 2, ROLE_EPILOGUE = 3, ROLE_DRAIN = 4 };
 
 struct KernelParams {
   int32_t m, n, k;
@@ -171,55 +168,6 @@ __host__ __device__ constexpr uint32_t make_idesc(int dt, int mma_m, int mma_n) 
     d |= (uint32_t)(mma_m >> 4) << 24;
   }
   return d;
-}
-
-struct SharedCtl {
-  uint32_t abort_addr;     // local abort flag (shared::cta address)
-  uint32_t abort_peer;     // the pair peer's abort flag (shared::cluster), 0 if none
-  uint64_t timeout_ns;
-  int32_t* status;
-};
-
-__device__ __noinline__ void raise_abort(const SharedCtl& c, uint32_t role, uint32_t idx) {
-  if (c.status) {
-    const int32_t code = (int32_t)(0x3u | (role << 8) | ((idx & 0xFFu) << 12) | ((blockIdx.x & 0x7FFu) << 20));
-    atomicCAS(c.status, 0, code);
-  }
-  st_shared_u32(c.abort_addr, 1u);
-  if (c.abort_peer) st_shared_cluster_u32(c.abort_peer, 1u);
-}
-
-// Bounded wait for phase `parity` of mbarrier `bar`; false when aborted.
-// The probes are plain try_wait (no suspend-time hint: resuming a suspended
-// thread added latency to every pipeline round trip); the abort flag is
-// checked after every probe and the timer every 8 probes.
-template <bool kCluster>
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const SharedCtl& c,
-                                         uint32_t role, uint32_t idx) {
-  if (kCluster ? mbar_test_wait_cluster(bar, parity) : mbar_test_wait(bar, parity)) return true;
-  uint64_t t0 = 0;
-  for (uint32_t probe = 1;; ++probe) {
-    if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))
-      return true;
-    if (ld_shared_volatile_u32(c.abort_addr)) return false;
-    if ((probe & 7u) == 1u) {
-      const uint64_t now = globaltimer_ns();
-      if (t0 == 0) {
-        t0 = now;
-      } else if (now - t0 > c.timeout_ns) {
-        raise_abort(c, role, idx);
-        return false;
-      }
-    }
-  }
-}
-
-// Wait with a short fixed budget during abort drains; never raises.
-__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity, uint64_t budget_ns) {
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - t0 > budget_ns) break;
-  }
 }
 
 // Output-tile rasterisation.  raster_group G > 0: groups of G M-tiles, M
@@ -884,20 +832,6 @@ gemm_sm100a_kernel(const __grid_constant__ CUtensorMap tmap_a,
 // ----------------------------------------------------------------------------
 // Host side
 // ----------------------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-std::once_flag g_encode_once;
-
-bool get_encode() {
-  std::call_once(g_encode_once, [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-  });
-  return g_encode != nullptr;
-}
-
 struct Resolved {
   int dt, cg, bm, bn, tile_k, atoms, stages, max_stages, cluster_m;
   uint32_t a_atom_bytes, b_atom_bytes, sf_stage_bytes, stage_bytes;
@@ -1082,21 +1016,6 @@ int resolve(const GemmArgs* a, Resolved& r) {
   return GEMM_OK;
 }
 #undef FAIL
-
-bool encode_2d(CUtensorMap* m, const void* ptr, CUtensorMapDataType t, uint64_t inner, uint64_t outer,
-               uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, uint32_t swizzle_bytes) {
-  const CUtensorMapSwizzle swz = swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                               : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                               : swizzle_bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE;
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {row_bytes};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult res = g_encode(m, t, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                          GEMM_L2_PROMOTION, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return res == CUDA_SUCCESS;
-}
 
 // Scale-factor tensor map: dims (128 x uint32 = one 512-byte atom, K/64 atoms,
 // row blocks of 128), no swizzle; box (128, nsf atoms, row blocks).

@@ -279,6 +279,50 @@ def test_product_writes_only_its_output(pkg, cuda, dtype, m, n):
         assert (buf == 123.0).all()
 
 
+VARIANTS = ([dict(cta_group=1, tile_n=bn, split_k=s) for bn in (16, 32, 64, 128) for s in (1, 2, 4, 8)]
+            + [dict(cta_group=2, tile_n=bn) for bn in (128, 256)])
+
+
+@pytest.mark.parametrize("knobs", VARIANTS, ids=lambda v: "-".join(str(x) for x in v.values()))
+def test_every_tile_and_split_gives_the_same_bits(pkg, cuda, knobs):
+    """Each variant on ragged problems, with and without TMA stores (odd n), every epilogue term."""
+    for m, n, k, dtype in ((1, 200, 1100, torch.bfloat16), (75, 333, 2000, torch.float16), (301, 648, 1024, torch.float32),
+                           (530, 1100, 1500, torch.bfloat16)):
+        a, b, sa, sb = int8s(pkg, m, k, 1), int8s(pkg, n, k, 2), scales(m, 3) * 0.01, scales(n, 4)
+        bias, residual = normal((n,), 5, dtype), normal((m, n), 6, dtype)
+        drop = pkg.Dropout(0.3, seed=3)
+        for kw in (dict(), dict(bias=bias, residual=residual, dropout=drop)):
+            want = pkg.gemm_int8(a, sa, b, sb, out_dtype=dtype, **kw)
+            status = torch.zeros(1, dtype=torch.int32, device="cuda")
+            out = torch.full((m + 2, n), 77.0, dtype=dtype, device="cuda")
+            pkg.gemm_int8(a, sa, b, sb, out=out[1:m + 1], status=status, **kw, **knobs)
+            assert status.item() == 0
+            assert torch.equal(out[1:m + 1], want)
+            assert (out[0] == 77.0).all() and (out[m + 1] == 77.0).all()
+
+
+def test_refused_knobs(pkg, cuda):
+    a, b, sa, sb = int8s(pkg, 4, 512, 1), int8s(pkg, 6, 512, 2), scales(4, 3), scales(6, 4)
+    for knobs in (dict(tile_n=48), dict(cta_group=3), dict(cta_group=2, tile_n=64), dict(split_k=3),
+                  dict(cta_group=2, tile_n=256, split_k=2), dict(split_k=8)):       # 4 K blocks, 8 CTAs
+        with pytest.raises(pkg.GemmError):
+            pkg.gemm_int8(a, sa, b, sb, **knobs)
+
+
+def test_a_stalled_load_ends_with_a_status(pkg, cuda):
+    """The injected stall makes every wait run out: the status says so, nothing hangs, and the next
+    product is right."""
+    a, b, sa, sb = int8s(pkg, 300, 1024, 1), int8s(pkg, 600, 1024, 2), scales(300, 3), scales(600, 4)
+    want = pkg.gemm_int8(a, sa, b, sb)
+    for knobs in (dict(cta_group=1, tile_n=64, split_k=1), dict(cta_group=1, tile_n=64, split_k=4),
+                  dict(cta_group=2, tile_n=256)):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        pkg.gemm_int8(a, sa, b, sb, status=status, timeout_ms=20, flags=pkg.FLAG_INJECT_STALL, **knobs)
+        rc, detail = pkg.read_status(status.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == pkg.ERR_TIMEOUT and detail != 0
+        assert torch.equal(pkg.gemm_int8(a, sa, b, sb, **knobs), want)
+
+
 def test_product_extreme_sums(pkg, cuda):
     """The largest sums of 8-bit products, at the longest K: -128 * -128 * 131071 < 2^31."""
     k = pkg.MAX_INT8_K
