@@ -342,7 +342,10 @@ int gemm_sm100a_int8_launch(const Int8GemmArgs* args, void* stream);
  * Quantise the rows of X (m x k of x_type, row stride ldx elements) and multiply:
  * gemm_sm100a_quantize_int8 followed by gemm_sm100a_int8_launch, bit for bit, in one
  * or two launches.  args->a and args->scale_a are workspace of the caller
- * (m * lda bytes and m floats; their content afterwards is unspecified).
+ * (m * lda bytes and m floats; their content afterwards is unspecified).  They
+ * may be NULL for a few tokens, which one launch quantises and multiplies: with
+ * no tile knob set, n <= 262144 and p * k <= 65536 for the smallest power of two
+ * p >= m, p <= 4.
  */
 int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream);
 

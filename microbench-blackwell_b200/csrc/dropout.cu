@@ -9,6 +9,7 @@
 #include "device_guard.cuh"
 #include "gemm_sm100a.h"
 #include "int8_common.cuh"
+#include "sm100_ptx.cuh"
 
 using namespace int8op;
 
@@ -29,6 +30,8 @@ template <typename T, bool RES>
 __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
   constexpr int V = Vec<T>::N;
   const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
+  sm100::grid_dependency_wait();
+  sm100::grid_launch_dependents();
   if (c >= p.cols) return;
   const int n = (int)min((int64_t)V, p.cols - c);
   const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
@@ -60,9 +63,7 @@ cudaError_t launch(const DropoutParams& p, cudaStream_t st) {
   int64_t gy = (p.rows + ty - 1) / ty;
   if (gy > 65535) gy = 65535;
   const dim3 grid((unsigned)gx, (unsigned)gy), block((unsigned)tx, (unsigned)ty);
-  if (p.res) dropout_kernel<T, true><<<grid, block, 0, st>>>(p);
-  else dropout_kernel<T, false><<<grid, block, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_overlapped(p.res ? dropout_kernel<T, true> : dropout_kernel<T, false>, grid, block, 0, 1, st, p);
 }
 
 }  // namespace

@@ -31,6 +31,17 @@ __device__ __forceinline__ float load_as_f32(const void* p, int t, int64_t i) {
   return to_f32(static_cast<const __half*>(p)[i]);
 }
 
+__device__ __forceinline__ void store_as(void* p, int t, int64_t i, float v) {
+  if (t == GEMM_TYPE_FP32) static_cast<float*>(p)[i] = v;
+  else if (t == GEMM_TYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
+  else static_cast<__half*>(p)[i] = from_f32<__half>(v);
+}
+
+// One output of the product from its exact sum, before dropout and residual.
+__device__ __forceinline__ float finish(int32_t acc, float sa, float sb, float bias) {
+  return fmaf(__int2float_rn(acc) * sa, sb, bias);
+}
+
 // 16 bytes of T as registers; element access is compile-time indexed.
 template <typename T>
 struct Vec {
@@ -210,7 +221,28 @@ __device__ __forceinline__ uint32_t abs_bits_to_f32(uint32_t h) {   // magnitude
   }
 }
 
-// ------------------------------------------------------------------ host checks
+// ------------------------------------------------------------------ host
+// Launch a kernel that begins with grid_dependency_wait(): its launch latency
+// overlaps the end of the kernel before it.
+template <typename... P, typename... A>
+cudaError_t launch_overlapped(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
 inline int drop_resolve(const DropoutArgs& a, int64_t rows, int64_t cols, Drop& d, const char** why) {
   d = Drop{};
   if (!(a.p >= 0.0 && a.p <= 1.0)) { *why = "dropout p must be in [0, 1]"; return GEMM_ERR_CANNOT_IMPLEMENT; }

@@ -31,6 +31,7 @@
 #include "bounded_wait.cuh"
 #include "device_guard.cuh"
 #include "int8_common.cuh"
+#include "int8_gemv.cuh"
 #include "tensor_map.cuh"
 
 using namespace sm100;
@@ -44,6 +45,7 @@ constexpr int kBarrierBytes = 1024;
 constexpr int kMaxStages = 32;
 constexpr int kAtom = 128;              // bytes (= K elements) of one swizzled K atom
 constexpr int kChannels = 128;          // channels per CTA
+constexpr int kMaxSplit = 8;            // CTAs that may share a tile's K (portable cluster size)
 
 struct Int8Params {
   void* d; int64_t ldd;
@@ -67,6 +69,7 @@ struct Int8Params {
   int32_t* status;
   uint64_t timeout_ns;
   uint32_t flags;
+  int32_t weights_ready;                // the kernel before this one does not write the weights
 };
 
 // kind::i8: [4,6) D format (2 = S32), [7,10) and [10,13) A and B format (1 = signed
@@ -83,11 +86,6 @@ __device__ __forceinline__ void tile_coords(int u, const Int8Params& p, int& cb,
   const int r = u - g * per_group;
   cb = first + r % rows;
   tb = r / rows;
-}
-
-// One output from its exact sum.
-__device__ __forceinline__ float finish(int32_t acc, float sa, float sb, float bias) {
-  return fmaf(__int2float_rn(acc) * sa, sb, bias);
 }
 
 template <int CG, int BN, typename T>
@@ -156,9 +154,20 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
   ctl.timeout_ns = p.timeout_ns;
   ctl.status = p.status;
 
+  // Until here nothing of this launch depended on the kernels before it.  In the
+  // linear layer only the tokens do (the weights were complete before the
+  // quantisation of the tokens began): the producer then fetches the first
+  // weights before it waits.
+  if (!(warp == 0 && p.weights_ready)) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+  }
+
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (!(p.flags & GEMM_FLAG_INJECT_STALL)) {
+    if (p.flags & GEMM_FLAG_INJECT_STALL) {
+      if (p.weights_ready) grid_dependency_wait();
+    } else {
       const uint32_t issue = elect_one() ? 1u : 0u;
       const uint64_t policy = policy_evict_normal();
       const uint32_t leader_full = CG == 2 ? mapa_shared(full_bar, 0) : full_bar;
@@ -166,6 +175,24 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       int stage = 0;
       uint32_t phase = 0, issued_mask = 0, issued_parity = 0;
       bool ok = true;
+      int ahead = 0;      // k-blocks of the first tile whose weights are on their way
+      if (p.weights_ready) {
+        int cb, tb;
+        tile_coords(slot0, p, cb, tb);
+        const int32_t c0 = (cb * CG + (int32_t)(CG == 2 ? rank : 0u)) * kChannels;
+        ahead = min(p.stages, kb_end - kb_begin);
+        for (int s = 0; s < ahead; ++s) {
+          if (CG == 1 || issue) {
+            mbar_arrive_expect_tx(full_bar + 8u * s, tx_bytes, leader ? issue : 0u);
+            const uint32_t w_dst = base + (uint32_t)s * p.stage_bytes, target = leader_full + 8u * s;
+            if constexpr (CG == 2) tma_load_2d_pair(w_dst, &tmap_w, target, (kb_begin + s) * kAtom, c0, policy, issue);
+            else tma_load_2d(w_dst, &tmap_w, target, (kb_begin + s) * kAtom, c0, policy, issue);
+          }
+        }
+        __syncwarp();
+        grid_dependency_wait();
+        grid_launch_dependents();
+      }
       for (int u = slot0; u < p.num_units && ok; u += slots) {
         int cb, tb;
         tile_coords(u, p, cb, tb);
@@ -180,15 +207,17 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
           const uint32_t t_dst = w_dst + p.a_bytes;
           const uint32_t target = leader_full + 8u * stage;
           if (CG == 1 || issue) {
-            mbar_arrive_expect_tx(full_bar + 8u * stage, tx_bytes, leader ? issue : 0u);
+            const uint32_t weights = ahead == 0 ? issue : 0u;
+            mbar_arrive_expect_tx(full_bar + 8u * stage, tx_bytes, leader ? weights : 0u);
             if constexpr (CG == 2) {
-              tma_load_2d_pair(w_dst, &tmap_w, target, kb * kAtom, c0, policy, issue);
+              tma_load_2d_pair(w_dst, &tmap_w, target, kb * kAtom, c0, policy, weights);
               tma_load_2d_pair(t_dst, &tmap_t, target, kb * kAtom, t0, policy, issue);
             } else {
-              tma_load_2d(w_dst, &tmap_w, target, kb * kAtom, c0, policy, issue);
+              tma_load_2d(w_dst, &tmap_w, target, kb * kAtom, c0, policy, weights);
               tma_load_2d(t_dst, &tmap_t, target, kb * kAtom, t0, policy, issue);
             }
           }
+          if (ahead > 0) --ahead;
           issued_mask |= 1u << stage;
           issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
           if (++stage == p.stages) { stage = 0; phase ^= 1u; }
@@ -368,26 +397,39 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     cluster_arrive();
     cluster_wait();
     if (warp >= 2) {
-      // CTA `rank` finishes its share of the tokens: thread = channel.
+      // CTA `rank` finishes its share of the tokens: a warp takes a token, a lane
+      // four channels, with every peer's 16 bytes in flight at once.
       int cb, tb;
       tile_coords(slot0, p, cb, tb);
-      const int row = (int)(32u * (warp & 3u) + lane);
-      const int ch = cb * kChannels + row, t0 = tb * BN;
+      const int ch0 = cb * kChannels + 4 * (int)lane, t0 = tb * BN;
       const int per = BN / p.split;
-      if (ch < p.n) {
-        const float sb = p.sb ? p.sb[ch] : 1.f;
-        const float bias = p.bias ? load_as_f32(p.bias, p.bias_type, ch) : 0.f;
-        const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
-        for (int j = (int)rank * per; j < (int)(rank + 1) * per; ++j) {
-          const int t = t0 + j;
-          if (t >= p.m) break;
-          int32_t sum = 0;
-          for (int s = 0; s < p.split; ++s)
-            sum += (int32_t)ld_shared_cluster_u32(mapa_shared(base + (uint32_t)((j * kChannels + row) * 4), (uint32_t)s));
-          float v = finish(sum, p.sa ? p.sa[t] : 1.f, sb, bias);
-          if (p.drop.on) v = drop_keeps(key, p.drop.threshold, drop_index(p.drop, t, ch)) ? v * p.drop.grow : 0.f;
-          if (p.c) v += to_f32(static_cast<const T*>(p.c)[(int64_t)t * p.ldc + ch]);
-          static_cast<T*>(p.d)[(int64_t)t * p.ldd + ch] = from_f32<T>(v);
+      float sb[4], bias[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = ch0 + e < p.n;
+        sb[e] = in && p.sb ? p.sb[ch0 + e] : 1.f;
+        bias[e] = in && p.bias ? load_as_f32(p.bias, p.bias_type, ch0 + e) : 0.f;
+      }
+      const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
+      for (int j = (int)rank * per + (int)warp - 2; j < (int)(rank + 1) * per; j += 4) {
+        const int t = t0 + j;
+        if (t >= p.m) break;
+        const uint32_t at = base + (uint32_t)((j * kChannels + 4 * (int)lane) * 4);
+        uint4 part[kMaxSplit];
+#pragma unroll
+        for (int s = 0; s < kMaxSplit; ++s) part[s] = s < p.split ? ld_shared_cluster_v4(mapa_shared(at, (uint32_t)s)) : make_uint4(0, 0, 0, 0);
+        uint32_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < kMaxSplit; ++s) { sum[0] += part[s].x; sum[1] += part[s].y; sum[2] += part[s].z; sum[3] += part[s].w; }
+        const float sa = p.sa ? p.sa[t] : 1.f;
+        T* const d = static_cast<T*>(p.d) + (int64_t)t * p.ldd + ch0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (ch0 + e >= p.n) break;
+          float v = finish((int32_t)sum[e], sa, sb[e], bias[e]);
+          if (p.drop.on) v = drop_keeps(key, p.drop.threshold, drop_index(p.drop, t, ch0 + e)) ? v * p.drop.grow : 0.f;
+          if (p.c) v += to_f32(static_cast<const T*>(p.c)[(int64_t)t * p.ldc + ch0 + e]);
+          d[e] = from_f32<T>(v);
         }
       }
       __syncwarp();
@@ -418,7 +460,8 @@ struct Resolved {
 #define FAIL(...) do { snprintf(r.reason, sizeof(r.reason), __VA_ARGS__); return GEMM_ERR_CANNOT_IMPLEMENT; } while (0)
 #define BAD(...) do { snprintf(r.reason, sizeof(r.reason), __VA_ARGS__); return GEMM_ERR_BAD_ARGS; } while (0)
 
-int check(const Int8GemmArgs* a, Resolved& r) {
+// `tokens`: A and its scales are read or written (not by the few-token form of the linear layer).
+int check(const Int8GemmArgs* a, bool tokens, Resolved& r) {
   if (!a) BAD("null args");
   if (a->struct_size != sizeof(Int8GemmArgs)) BAD("Int8GemmArgs.struct_size %u != %zu", a->struct_size, sizeof(Int8GemmArgs));
   if (!type_ok(a->d_type)) FAIL("unknown d_type %d", a->d_type);
@@ -430,10 +473,12 @@ int check(const Int8GemmArgs* a, Resolved& r) {
   const char* why = "";
   if (drop_resolve(a->drop, a->m, a->n, r.p.drop, &why) != GEMM_OK) FAIL("%s", why);
   if (a->m > 0 && a->n > 0) {
-    if (!a->a || !a->b || !a->d) BAD("null A/B/D pointer");
-    if ((reinterpret_cast<uintptr_t>(a->a) | reinterpret_cast<uintptr_t>(a->b)) & 15) FAIL("A/B must be 16-byte aligned");
-    if (a->lda < a->k || a->ldb < a->k) FAIL("lda/ldb must be >= k");
-    if ((a->lda | a->ldb) & 15) FAIL("lda/ldb must be multiples of 16");
+    if ((tokens && !a->a) || !a->b || !a->d) BAD("null A/B/D pointer");
+    const uintptr_t pa = tokens ? reinterpret_cast<uintptr_t>(a->a) : 0;
+    const int64_t lda = tokens ? a->lda : a->ldb;
+    if ((pa | reinterpret_cast<uintptr_t>(a->b)) & 15) FAIL("A/B must be 16-byte aligned");
+    if (lda < a->k || a->ldb < a->k) FAIL("lda/ldb must be >= k");
+    if ((lda | a->ldb) & 15) FAIL("lda/ldb must be multiples of 16");
     const uintptr_t e = (uintptr_t)type_bytes(a->d_type);
     if ((reinterpret_cast<uintptr_t>(a->d) | reinterpret_cast<uintptr_t>(a->c)) % e) FAIL("D/C must be aligned to their element");
     if (a->ldd < a->n) FAIL("ldd must be >= n");
@@ -446,6 +491,15 @@ int check(const Int8GemmArgs* a, Resolved& r) {
 
 bool supported(int cg, int bn) {
   return cg == 1 ? (bn == 16 || bn == 32 || bn == 64 || bn == 128) : (bn == 128 || bn == 256);
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    sms = 148;
+  }
+  return sms;
 }
 
 // Tile and split from the sizes.
@@ -468,14 +522,9 @@ void choose(const Int8GemmArgs* a, int num_sms, int& cg, int& bn, int& split) {
 
 int resolve(const Int8GemmArgs* a, Resolved& r) {
   memset(&r, 0, sizeof(r));
-  const int rc = check(a, r);
+  const int rc = check(a, true, r);
   if (rc != GEMM_OK) return rc;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&r.num_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    r.num_sms = 148;
-    cudaGetLastError();
-  }
+  r.num_sms = sm_count();
   r.cg = a->cta_group; r.bn = a->tile_n; r.split = a->split_k;
   choose(a, r.num_sms, r.cg, r.bn, r.split);
   if (r.cg != 1 && r.cg != 2) FAIL("cta_group must be 1 or 2");
@@ -565,8 +614,34 @@ bool ensure_smem_attr(KernelFn fn, int dev) {
   return true;
 }
 
-// One product; the device of D is current.
-int launch_product(const Int8GemmArgs& a, cudaStream_t st, int dev) {
+// Few tokens and no tile asked for: one launch without tensor cores.
+bool use_gemv(const Int8GemmArgs& a, int num_sms) {
+  return !a.tile_n && !a.cta_group && !a.split_k && !a.flags && gemv_fits(a.m, a.n, a.k, num_sms);
+}
+
+int launch_gemv(const Int8GemmArgs& a, const void* x, int32_t x_type, int64_t ldx, int num_sms, cudaStream_t st) {
+  GemvParams g;
+  memset(&g, 0, sizeof(g));
+  const char* why = "";
+  if (drop_resolve(a.drop, a.m, a.n, g.drop, &why) != GEMM_OK) return GEMM_ERR_CANNOT_IMPLEMENT;
+  g.x = x; g.ldx = ldx; g.x_type = x_type;
+  g.b = static_cast<const int8_t*>(a.b); g.ldb = a.ldb;
+  g.d = a.d; g.ldd = a.ldd; g.d_type = a.d_type; g.c = a.c; g.ldc = a.ldc;
+  g.sa = a.scale_a; g.sb = a.scale_b; g.bias = a.bias; g.bias_type = a.bias_type;
+  g.m = (int32_t)a.m; g.n = (int32_t)a.n; g.k = (int32_t)a.k;
+  g.status = a.status;
+  g.timeout_ns = (uint64_t)(a.timeout_ms ? a.timeout_ms : 4000u) * 1000000ull;
+  g.wide = x_type != kTypeInt8 && rows_16b(x, ldx, type_bytes(x_type));
+  if (gemv_launch(g, num_sms, st) != cudaSuccess) {
+    cudaGetLastError();
+    return GEMM_ERR_LAUNCH;
+  }
+  return GEMM_OK;
+}
+
+// One product; the device of D is current.  `weights_ready`: the kernel launched
+// just before on this stream writes neither the weights nor anything they depend on.
+int launch_product(const Int8GemmArgs& a, bool weights_ready, cudaStream_t st, int dev) {
   Resolved r;
   const int rc = resolve(&a, r);
   if (rc != GEMM_OK) return rc;
@@ -587,20 +662,9 @@ int launch_product(const Int8GemmArgs& a, cudaStream_t st, int dev) {
   KernelFn fn = a.d_type == GEMM_TYPE_BF16 ? pick<__nv_bfloat16>(r.cg, r.bn)
               : a.d_type == GEMM_TYPE_FP16 ? pick<__half>(r.cg, r.bn) : pick<float>(r.cg, r.bn);
   if (!ensure_smem_attr(fn, dev)) return GEMM_ERR_LAUNCH;
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)r.grid);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)r.smem_bytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)(r.split > 1 ? r.split : r.cg);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, fn, tw, tt, td, r.p) != cudaSuccess) {
+  r.p.weights_ready = weights_ready ? 1 : 0;
+  if (launch_overlapped(fn, dim3((unsigned)r.grid), dim3(kThreads), (size_t)r.smem_bytes, r.split > 1 ? r.split : r.cg, st,
+                        tw, tt, td, r.p) != cudaSuccess) {
     cudaGetLastError();
     return GEMM_ERR_LAUNCH;
   }
@@ -629,25 +693,37 @@ extern "C" int gemm_sm100a_int8_query(const Int8GemmArgs* args, GemmInfo* info) 
 extern "C" int gemm_sm100a_int8_launch(const Int8GemmArgs* args, void* stream) {
   Resolved r;
   memset(&r, 0, sizeof(r));
-  const int rc = check(args, r);
+  const int rc = check(args, true, r);
   if (rc != GEMM_OK) return rc;
   if (args->m == 0 || args->n == 0) return GEMM_OK;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   PointerDeviceGuard guard(args->d);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
-  return launch_product(*args, reinterpret_cast<cudaStream_t>(stream), guard.dev);
+  const int sms = sm_count();
+  if (use_gemv(*args, sms)) return launch_gemv(*args, args->a, kTypeInt8, args->lda, sms, st);
+  return launch_product(*args, false, st, guard.dev);
 }
 
 extern "C" int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream) {
   Resolved r;
   memset(&r, 0, sizeof(r));
-  const int rc = check(args, r);
+  const int sms = sm_count();
+  const bool few = args && args->struct_size == sizeof(Int8GemmArgs) && use_gemv(*args, sms);
+  const int rc = check(args, !few, r);
   if (rc != GEMM_OK) return rc;
   if (args->m == 0 || args->n == 0) return GEMM_OK;
+  if (!type_ok(x_type)) return GEMM_ERR_CANNOT_IMPLEMENT;
+  if (!x || (!few && !args->scale_a)) return GEMM_ERR_BAD_ARGS;
+  if (ldx < args->k || reinterpret_cast<uintptr_t>(x) % type_bytes(x_type)) return GEMM_ERR_CANNOT_IMPLEMENT;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  PointerDeviceGuard guard(args->d);
+  if (!guard.ok) return GEMM_ERR_LAUNCH;
+  if (few) return launch_gemv(*args, x, x_type, ldx, sms, st);
   Int8QuantArgs q;
   memset(&q, 0, sizeof(q));
   q.struct_size = sizeof(q);
   q.x_type = x_type; q.rows = args->m; q.cols = args->k; q.x = x; q.ldx = ldx;
   q.q = const_cast<void*>(args->a); q.ldq = args->lda; q.scale = const_cast<float*>(args->scale_a);
   const int rq = gemm_sm100a_quantize_int8(&q, stream);
-  return rq != GEMM_OK ? rq : gemm_sm100a_int8_launch(args, stream);
+  return rq != GEMM_OK ? rq : launch_product(*args, true, st, guard.dev);
 }

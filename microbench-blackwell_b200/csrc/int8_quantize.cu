@@ -14,6 +14,7 @@
 #include "device_guard.cuh"
 #include "gemm_sm100a.h"
 #include "int8_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace cg = cooperative_groups;
 using namespace int8op;
@@ -46,6 +47,8 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const __grid_consta
   const int nvec = (int)((p.cols + V - 1) / V);
   const int per_chunk = NV * TX;
   const int chunks = (nvec + per_chunk - 1) / per_chunk;
+  sm100::grid_dependency_wait();
+  sm100::grid_launch_dependents();
   const uint64_t key = DROP ? drop_key(p.drop) : 0;
   for (int64_t row0 = (int64_t)blockIdx.x * blockDim.y; row0 < p.rows; row0 += (int64_t)gridDim.x * blockDim.y) {
     const int64_t row = row0 + threadIdx.y;
@@ -144,6 +147,8 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
   const int64_t col0 = (int64_t)(blockIdx.x / peers) * kStrip;
   const int64_t row0 = (int64_t)rank * p.row_chunk;
   const int n_rows = (int)max((int64_t)0, min((int64_t)p.row_chunk, p.rows - row0));
+  sm100::grid_dependency_wait();
+  sm100::grid_launch_dependents();
   const uint64_t key = DROP ? drop_key(p.drop) : 0;
 
   const int lane_c = threadIdx.x % LANES, lane_r = threadIdx.x / LANES;
@@ -279,9 +284,8 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
   int64_t blocks = (p.rows + ry - 1) / ry;
   if (blocks > 0x7FFFFFFF) blocks = 0x7FFFFFFF;
   const dim3 block((unsigned)tx, (unsigned)ry);
-  if (p.drop.on) quantize_rows_kernel<T, NV, true><<<(unsigned)blocks, block, 0, st>>>(p);
-  else quantize_rows_kernel<T, NV, false><<<(unsigned)blocks, block, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_overlapped(p.drop.on ? quantize_rows_kernel<T, NV, true> : quantize_rows_kernel<T, NV, false>,
+                           dim3((unsigned)blocks), block, 0, 1, st, p);
 }
 
 template <typename T>
@@ -296,18 +300,8 @@ cudaError_t launch_cols(QuantParams p, cudaStream_t st) {
   auto fn = p.drop.on ? quantize_cols_kernel<T, true> : quantize_cols_kernel<T, false>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kHeldBytes);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)(strips * peers));
-  cfg.blockDim = dim3(kColThreads);
-  cfg.dynamicSmemBytes = (size_t)(p.rows_held * (int64_t)(kStrip * sizeof(T)));
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)peers; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, p);
+  return launch_overlapped(fn, dim3((unsigned)(strips * peers)), dim3(kColThreads),
+                           (size_t)(p.rows_held * (int64_t)(kStrip * sizeof(T))), peers, st, p);
 }
 
 }  // namespace

@@ -113,15 +113,15 @@ def _drop_fields(drop: Dropout | None, cols: int, device: torch.device):
 
 def _matrix(t: torch.Tensor, name: str, dtype=None, shape=None, device=None) -> int:
     """Check one operand and return its row stride in elements."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+    if not isinstance(t, torch.Tensor) or len(t.shape) != 2:
         raise ValueError(f"{name} must be a 2-D tensor")
     if not t.is_cuda or (device is not None and t.device != device):
         raise ValueError(f"{name} must be on the operands' CUDA device")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     rows, cols = t.shape
-    if shape is not None and (rows, cols) != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {(rows, cols)}")
     ld, inner = t.stride()
     if cols > 1 and inner != 1:
         raise ValueError(f"{name} must have unit stride along its last axis")
@@ -158,13 +158,17 @@ def _pad16(n: int) -> int:
     return (n + 15) & ~15
 
 
-def _raw_stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# The current stream's handle; the Stream object that torch.cuda.current_stream builds costs
+# 2 us, as much as a launch.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def empty_int8(rows: int, cols: int, device) -> torch.Tensor:
     """An int8 matrix whose row stride is a multiple of 16 bytes."""
-    return torch.empty((rows, _pad16(max(cols, 1))), dtype=torch.int8, device=device)[:, :cols]
+    ld = _pad16(max(cols, 1))
+    q = torch.empty((rows, ld), dtype=torch.int8, device=device)
+    return q if ld == cols else q[:, :cols]
 
 
 def quantize_int8(x: torch.Tensor, *, transpose: bool = False, dropout: Dropout | None = None,
@@ -182,30 +186,39 @@ def quantize_int8(x: torch.Tensor, *, transpose: bool = False, dropout: Dropout 
     if column_sums and not transpose:
         raise ValueError("column_sums needs transpose=True")
     q = empty_int8(cols, rows, x.device) if transpose else empty_int8(rows, cols, x.device)
-    scale = torch.empty((cols if transpose else rows,), dtype=torch.float32, device=x.device)
-    sums = torch.empty((cols,), dtype=torch.float32, device=x.device) if column_sums else None
-    if scale.numel():
+    scale = x.new_empty((cols if transpose else rows,), dtype=torch.float32)
+    sums = x.new_empty((cols,), dtype=torch.float32) if column_sums else None
+    if scale.shape[0]:
         if not transpose and cols == 0:
             raise ValueError("x has no columns")
         args = _QUANT_PACK.pack(_QUANT_PACK.size, code, rows, cols, x.data_ptr(), ldx, q.data_ptr(), q.stride(0),
                                 scale.data_ptr(), 0 if sums is None else sums.data_ptr(), int(transpose), 0,
                                 *_drop_fields(dropout, cols, x.device))
-        rc = lib().gemm_sm100a_quantize_int8(args, _raw_stream(x.device))
+        rc = lib().gemm_sm100a_quantize_int8(args, _raw_stream(x.device.index))
         if rc != OK:
             raise GemmError(rc, "gemm_sm100a_quantize_int8")
     return (q, scale) if sums is None else (q, scale, sums)
 
 
-def _output(out, m, n, dtype, device) -> torch.Tensor:
+def _output(out, m, n, dtype, like) -> torch.Tensor:
     if out is None:
-        return torch.empty((m, n), dtype=dtype, device=device)
-    _matrix(out, "out", dtype, (m, n), device)
+        return like.new_empty((m, n), dtype=dtype)
+    _matrix(out, "out", dtype, (m, n), like.device)
     return out
+
+
+_KNOBS = {"tile_n", "cta_group", "split_k", "timeout_ms", "flags"}
+
+
+def _tiles(knobs):
+    if not _KNOBS.issuperset(knobs):
+        raise TypeError(f"unknown knobs {sorted(set(knobs) - _KNOBS)}")
+    return knobs.get("tile_n", 0), knobs.get("cta_group", 0), knobs.get("split_k", 0)
 
 
 def _pack_gemm(code, m, n, k, a, lda, b, ldb, d, residual, a_scale, b_scale, bias, dropout, status, knobs):
     device = d.device
-    ldd = _matrix(d, "out")
+    ldd = d.stride(0) if m > 1 else max(n, 1)
     c = ldc = 0
     if residual is not None:
         ldc = _matrix(residual, "residual", d.dtype, (m, n), device)
@@ -215,10 +228,9 @@ def _pack_gemm(code, m, n, k, a, lda, b, ldb, d, residual, a_scale, b_scale, bia
         bias_code = _floating(bias, "bias")
         bias_ptr = _vector(bias, "bias", n, device, None)
     return _GEMM_PACK.pack(_GEMM_PACK.size, code, m, n, k, a, lda, b, ldb, d.data_ptr(), ldd, c, ldc, a_scale, b_scale,
-                           bias_ptr, bias_code, knobs.pop("tile_n", 0), knobs.pop("cta_group", 0),
-                           knobs.pop("split_k", 0), *_drop_fields(dropout, n, device),
-                           0 if status is None else status.data_ptr(), knobs.pop("timeout_ms", 0),
-                           knobs.pop("flags", 0))
+                           bias_ptr, bias_code, *(_tiles(knobs) if knobs else (0, 0, 0)),
+                           *_drop_fields(dropout, n, device), 0 if status is None else status.data_ptr(),
+                           knobs.get("timeout_ms", 0), knobs.get("flags", 0))
 
 
 def _raise(rc, args, what):
@@ -242,7 +254,7 @@ def gemm_int8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor, b_
     ``a`` (m, k) and ``b`` (n, k) int8, ``a_scale`` (m) and ``b_scale`` (n) fp32 (None = 1);
     ``residual`` and ``out`` (which may be the residual) of ``out_dtype``.  The sum over k is
     exact, so the result does not depend on the batch or the tile.  ``status``: optional int32
-    device word, as in ``gemm_into``.  Knobs: tile_n, cta_group, split_k, timeout_ms."""
+    device word, as in ``gemm_into``.  Knobs: tile_n, cta_group, split_k, timeout_ms, flags."""
     lda = _int8(a, "a")
     device = a.device
     ldb = _int8(b, "b", (b.shape[0], a.shape[1]) if isinstance(b, torch.Tensor) and b.dim() == 2 else None, device)
@@ -253,14 +265,12 @@ def gemm_int8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor, b_
     code = _TYPES.get(out_dtype)
     if code is None:
         raise ValueError("out_dtype must be bfloat16, float16 or float32")
-    d = _output(out, m, n, out_dtype, device)
+    d = _output(out, m, n, out_dtype, a)
     sa = 0 if a_scale is None else _vector(a_scale, "a_scale", m, device)
     sb = 0 if b_scale is None else _vector(b_scale, "b_scale", n, device)
     args = _pack_gemm(code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, d, residual, sa, sb, bias, dropout,
                       status, knobs)
-    if knobs:
-        raise TypeError(f"unknown knobs {sorted(knobs)}")
-    rc = lib().gemm_sm100a_int8_launch(args, _raw_stream(device))
+    rc = lib().gemm_sm100a_int8_launch(args, _raw_stream(device.index))
     if rc != OK:
         _raise(rc, args, "gemm_sm100a_int8_launch")
     return d
@@ -280,15 +290,15 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
     ldw = _int8(w, "w", (w.shape[0], k) if isinstance(w, torch.Tensor) and w.dim() == 2 else None, device)
     n = w.shape[0]
     sb = _vector(w_scale, "w_scale", n, device)
-    d = _output(out, m, n, x.dtype, device)
+    d = _output(out, m, n, x.dtype, x)
     lda = _pad16(max(k, 1))
-    work = torch.empty((m * (lda + 4) + 16,), dtype=torch.uint8, device=device)   # int8 tokens, then their scales
-    q = work.data_ptr()
-    args = _pack_gemm(code, m, n, k, q, lda, w.data_ptr(), ldw, d, residual, q + m * lda, sb, bias, dropout,
-                      status, knobs)
-    if knobs:
-        raise TypeError(f"unknown knobs {sorted(knobs)}")
-    rc = lib().gemm_sm100a_int8_linear(args, x.data_ptr(), code, ldx, _raw_stream(device))
+    q = sa = 0
+    if m > 4 or knobs or n > 262144 or k << (m - 1).bit_length() > 65536:   # else no workspace is needed
+        work = x.new_empty((m * (lda + 4) + 16,), dtype=torch.uint8)          # int8 tokens, then their scales
+        q = work.data_ptr()
+        sa = q + m * lda
+    args = _pack_gemm(code, m, n, k, q, lda, w.data_ptr(), ldw, d, residual, sa, sb, bias, dropout, status, knobs)
+    rc = lib().gemm_sm100a_int8_linear(args, x.data_ptr(), code, ldx, _raw_stream(device.index))
     if rc != OK:
         _raise(rc, args, "gemm_sm100a_int8_linear")
     return d
@@ -336,15 +346,15 @@ def dropout(x: torch.Tensor, drop: Dropout, *, residual: torch.Tensor | None = N
     code = _floating(x, "x")
     ldx = _matrix(x, "x")
     rows, cols = x.shape
-    y = _output(out, rows, cols, x.dtype, x.device)
-    ldy = _matrix(y, "out")
+    y = _output(out, rows, cols, x.dtype, x)
+    ldy = y.stride(0) if rows > 1 else max(cols, 1)
     r = ldr = 0
     if residual is not None:
         ldr = _matrix(residual, "residual", x.dtype, (rows, cols), x.device)
         r = residual.data_ptr()
     args = _DROPOUT_PACK.pack(_DROPOUT_PACK.size, code, rows, cols, x.data_ptr(), ldx, r, ldr, y.data_ptr(), ldy,
                               *_drop_fields(drop, cols, x.device))
-    rc = lib().gemm_sm100a_dropout(args, _raw_stream(x.device))
+    rc = lib().gemm_sm100a_dropout(args, _raw_stream(x.device.index))
     if rc != OK:
         raise GemmError(rc, "gemm_sm100a_dropout")
     return y
