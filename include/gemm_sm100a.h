@@ -343,9 +343,8 @@ int gemm_sm100a_int8_launch(const Int8GemmArgs* args, void* stream);
  * gemm_sm100a_quantize_int8 followed by gemm_sm100a_int8_launch, bit for bit, in one
  * or two launches.  args->a and args->scale_a are workspace of the caller
  * (m * lda bytes and m floats; their content afterwards is unspecified).  They
- * may be NULL for a few tokens, which one launch quantises and multiplies: with
- * no tile knob set, n <= 262144 and p * k <= 65536 for the smallest power of two
- * p >= m, p <= 4.
+ * may be NULL where one launch quantises and multiplies: x_type equal to d_type,
+ * m <= 8, m * k <= 16384 and no knob or flag set.
  */
 int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream);
 

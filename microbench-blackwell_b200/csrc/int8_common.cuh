@@ -31,12 +31,6 @@ __device__ __forceinline__ float load_as_f32(const void* p, int t, int64_t i) {
   return to_f32(static_cast<const __half*>(p)[i]);
 }
 
-__device__ __forceinline__ void store_as(void* p, int t, int64_t i, float v) {
-  if (t == GEMM_TYPE_FP32) static_cast<float*>(p)[i] = v;
-  else if (t == GEMM_TYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
-  else static_cast<__half*>(p)[i] = from_f32<__half>(v);
-}
-
 // One output of the product from its exact sum, before dropout and residual.
 __device__ __forceinline__ float finish(int32_t acc, float sa, float sb, float bias) {
   return fmaf(__int2float_rn(acc) * sa, sb, bias);
@@ -209,15 +203,38 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Largest |x| of a vector as fp32 bits.
+// Magnitude bits of a T as fp32 bits.
 template <typename T>
-__device__ __forceinline__ uint32_t abs_bits_to_f32(uint32_t h) {   // magnitude bits of T
+__device__ __forceinline__ uint32_t abs_bits_to_f32(uint32_t h) {
   if constexpr (sizeof(T) == 4) return h;
   else {
     const uint16_t u = (uint16_t)h;
     T v;
     __builtin_memcpy(&v, &u, 2);
     return __float_as_uint(to_f32(v));
+  }
+}
+
+// Largest |x| of a vector as fp32 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t vec_magnitude(const Vec<T>& v) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) m = max(m, v.w[j] & 0x7FFFFFFFu);
+    else m = __vmaxu2(m, v.w[j] & 0x7FFF7FFFu);
+  }
+  if constexpr (sizeof(T) == 2) m = abs_bits_to_f32<T>(max(m & 0xFFFFu, m >> 16));
+  return m;
+}
+// The int8 values of a vector, four to a word.
+template <typename T>
+__device__ __forceinline__ void quantize_vec(const Vec<T>& v, const RowScale& s, uint32_t (&w)[Vec<T>::N / 4]) {
+#pragma unroll
+  for (int j = 0; j < Vec<T>::N / 4; ++j) {
+    w[j] = pack4(quantize_one<T>(v.get(4 * j), s), quantize_one<T>(v.get(4 * j + 1), s),
+                 quantize_one<T>(v.get(4 * j + 2), s), quantize_one<T>(v.get(4 * j + 3), s));
+    if (s.c == 0.f) w[j] = 0u;
   }
 }
 

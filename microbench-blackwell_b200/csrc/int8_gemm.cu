@@ -17,6 +17,10 @@
 //   split-K form   for few tiles: the CTAs of a cluster share one tile's K and
 //                  add their int32 partial tiles through distributed shared
 //                  memory (exact, so the order does not matter); no workspace.
+//   fused form     for a linear layer of at most 8 tokens, in one launch: while the
+//                  ring fills with weights, 12 warps find the tokens' maxima and
+//                  quantise the CTA's part of them straight into the swizzled
+//                  operand, which stays in shared memory for all of its tiles.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -31,7 +35,6 @@
 #include "bounded_wait.cuh"
 #include "device_guard.cuh"
 #include "int8_common.cuh"
-#include "int8_gemv.cuh"
 #include "tensor_map.cuh"
 
 using namespace sm100;
@@ -39,11 +42,17 @@ using namespace int8op;
 
 namespace {
 
-constexpr int kThreads = 192;
+constexpr int kFusedTokens = 8;         // most tokens of the fused form: one 8-row group of the swizzle
+constexpr int kFusedBN = 16;            // its MMA N, the smallest there is for 128 channels
+constexpr int kStageWarps = 12;         // warps of the fused form that quantise tokens (the epilogue's four among them)
+constexpr int kFusedElems = 16384;      // most tokens x K of the fused form (at most 128 KB of shared memory)
+__host__ __device__ constexpr int threads_for(bool fuse) { return fuse ? 64 + 32 * kStageWarps : 192; }
 constexpr int kSmemLimit = 232448;      // 227 KiB of opt-in dynamic shared memory per CTA
 constexpr int kBarrierBytes = 1024;
+constexpr int kStaticSmem = 512;        // bound of the static shared memory of the fused form
 constexpr int kMaxStages = 32;
 constexpr int kAtom = 128;              // bytes (= K elements) of one swizzled K atom
+constexpr uint32_t kTokAtom = 8 * kAtom;  // fused form: bytes of one K atom of the tokens
 constexpr int kChannels = 128;          // channels per CTA
 constexpr int kMaxSplit = 8;            // CTAs that may share a tile's K (portable cluster size)
 
@@ -69,7 +78,9 @@ struct Int8Params {
   int32_t* status;
   uint64_t timeout_ns;
   uint32_t flags;
-  int32_t weights_ready;                // the kernel before this one does not write the weights
+  const void* x; int64_t ldx;           // fused form: tokens before quantisation
+  int32_t x_wide, k;
+  uint32_t tok_offset;                  // fused form: quantised tokens, kTokAtom bytes per K atom
 };
 
 // kind::i8: [4,6) D format (2 = S32), [7,10) and [10,13) A and B format (1 = signed
@@ -88,8 +99,74 @@ __device__ __forceinline__ void tile_coords(int u, const Int8Params& p, int& cb,
   tb = r / rows;
 }
 
-template <int CG, int BN, typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+// Fused form: all staging warps, `tid` in [0, 32 * kStageWarps).  x's rows are
+// read twice (the second time from L1); atoms [kb_begin, kb_end) of the quantised
+// rows go to `tok`, 128-byte rows in the 128-byte swizzle, their scales to `sa_s`.
+// Rows from m on and bytes beyond K stay undefined: those accumulator columns
+// are not read, and the weights beyond K are zeros.  (Rows 8 to 15 of the MMA's
+// operand are the next K atom's, after the last one the 1 KB behind it.)
+template <typename X>
+__device__ __forceinline__ void stage_tokens(const Int8Params& p, uint32_t tok, uint32_t sa_s, RowScale* rows, uint32_t* top,
+                                             int kb_begin, int kb_end, int tid) {
+  constexpr int V = Vec<X>::N, N = 32 * kStageWarps;
+  constexpr int UN = 4;               // vectors in flight per thread, of whichever tokens they are
+  const X* const x = static_cast<const X*>(p.x);
+  const int nvec = (p.k + V - 1) / V;
+  // Thread `tid` takes vectors tid, tid + N, ... of the m x `width` vectors from `first`.
+  auto walk = [&](int first, int width, auto&& body) {
+    const int total = p.m * width;
+    const int dt = N / width, de = N - dt * width;
+    int t = tid / width, e = tid - t * width;
+    for (int i0 = tid & ~31; i0 < total; i0 += UN * N) {        // whole warps
+      Vec<X> v[UN];
+      int tt[UN], ee[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        tt[u] = t;
+        ee[u] = first + e;
+        v[u] = load_vec<X>(x + t * p.ldx + ee[u] * V, t < p.m ? p.k - ee[u] * V : 0, p.x_wide);
+        t += dt;
+        e += de;
+        if (e >= width) { e -= width; ++t; }
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+        if (i0 + u * N < total) body(tt[u], ee[u], v[u]);
+    }
+  };
+  if (tid < kFusedTokens) top[tid] = 0u;
+  named_bar_sync(2, N);
+  walk(0, nvec, [&](int t, int e, const Vec<X>& v) {
+    // One shared atomic per warp where its vectors are of one token.
+    uint32_t m = vec_magnitude<X>(v);
+    t = min(t, p.m - 1);
+    if (__all_sync(0xFFFFFFFFu, t == __shfl_sync(0xFFFFFFFFu, t, 0))) {
+      m = __reduce_max_sync(0xFFFFFFFFu, m);
+      if ((tid & 31) == 0) atomicMax(&top[t], m);
+    } else {
+      atomicMax(&top[t], m);
+    }
+  });
+  named_bar_sync(2, N);
+  if (tid < p.m) {
+    rows[tid] = row_scale(top[tid]);
+    st_shared_u32(sa_s + 4u * tid, __float_as_uint(rows[tid].scale));
+  }
+  named_bar_sync(2, N);
+  const int e0 = kb_begin * (kAtom / V), e1 = min(nvec, kb_end * (kAtom / V));
+  walk(e0, e1 - e0, [&](int t, int e, const Vec<X>& v) {
+    if (t >= p.m) return;
+    uint32_t w[V / 4];
+    quantize_vec<X>(v, rows[t], w);
+    const uint32_t b = (uint32_t)(e - e0) * V;                         // byte of the CTA's part of the row
+    const uint32_t at = tok + (uint32_t)t * 128u + (b >> 7) * kTokAtom + ((((b >> 4) & 7u) ^ (uint32_t)t) << 4) + (b & 15u);
+    if constexpr (V == 8) st_shared_v2(at, w[0], w[1]);
+    else st_shared_u32(at, w[0]);
+  });
+}
+
+template <int CG, int BN, typename T, bool FUSE>
+__global__ void __launch_bounds__(threads_for(FUSE), 1)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channels x K
                  const __grid_constant__ CUtensorMap tmap_t,   // tokens x K
                  const __grid_constant__ CUtensorMap tmap_d,   // D, for the staged epilogue
@@ -111,6 +188,9 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
   const uint32_t drain_bar = tempty_bar + 16u;
   const uint32_t tmem_slot = drain_bar + 8u;
   const uint32_t abort_flag = tmem_slot + 4u;
+  const uint32_t tok_bar = abort_flag + 4u;              // fused form: the tokens are in place
+  __shared__ RowScale tok_rows[FUSE ? kFusedTokens : 1];
+  __shared__ uint32_t tok_top[FUSE ? kFusedTokens : 1];
 
   const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const uint32_t lane = threadIdx.x & 31u;
@@ -135,6 +215,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       mbar_init(tempty_bar + 8u * a, 4 * CG);
     }
     mbar_init(drain_bar, 1);
+    mbar_init(tok_bar, kStageWarps);
     st_shared_u32(abort_flag, 0u);
     fence_mbar_init();
   }
@@ -154,20 +235,13 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
   ctl.timeout_ns = p.timeout_ns;
   ctl.status = p.status;
 
-  // Until here nothing of this launch depended on the kernels before it.  In the
-  // linear layer only the tokens do (the weights were complete before the
-  // quantisation of the tokens began): the producer then fetches the first
-  // weights before it waits.
-  if (!(warp == 0 && p.weights_ready)) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-  }
+  // Until here nothing of this launch depended on the kernels before it.
+  grid_dependency_wait();
+  grid_launch_dependents();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (p.flags & GEMM_FLAG_INJECT_STALL) {
-      if (p.weights_ready) grid_dependency_wait();
-    } else {
+    if (!(p.flags & GEMM_FLAG_INJECT_STALL)) {
       const uint32_t issue = elect_one() ? 1u : 0u;
       const uint64_t policy = policy_evict_normal();
       const uint32_t leader_full = CG == 2 ? mapa_shared(full_bar, 0) : full_bar;
@@ -175,24 +249,6 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       int stage = 0;
       uint32_t phase = 0, issued_mask = 0, issued_parity = 0;
       bool ok = true;
-      int ahead = 0;      // k-blocks of the first tile whose weights are on their way
-      if (p.weights_ready) {
-        int cb, tb;
-        tile_coords(slot0, p, cb, tb);
-        const int32_t c0 = (cb * CG + (int32_t)(CG == 2 ? rank : 0u)) * kChannels;
-        ahead = min(p.stages, kb_end - kb_begin);
-        for (int s = 0; s < ahead; ++s) {
-          if (CG == 1 || issue) {
-            mbar_arrive_expect_tx(full_bar + 8u * s, tx_bytes, leader ? issue : 0u);
-            const uint32_t w_dst = base + (uint32_t)s * p.stage_bytes, target = leader_full + 8u * s;
-            if constexpr (CG == 2) tma_load_2d_pair(w_dst, &tmap_w, target, (kb_begin + s) * kAtom, c0, policy, issue);
-            else tma_load_2d(w_dst, &tmap_w, target, (kb_begin + s) * kAtom, c0, policy, issue);
-          }
-        }
-        __syncwarp();
-        grid_dependency_wait();
-        grid_launch_dependents();
-      }
       for (int u = slot0; u < p.num_units && ok; u += slots) {
         int cb, tb;
         tile_coords(u, p, cb, tb);
@@ -207,17 +263,15 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
           const uint32_t t_dst = w_dst + p.a_bytes;
           const uint32_t target = leader_full + 8u * stage;
           if (CG == 1 || issue) {
-            const uint32_t weights = ahead == 0 ? issue : 0u;
-            mbar_arrive_expect_tx(full_bar + 8u * stage, tx_bytes, leader ? weights : 0u);
+            mbar_arrive_expect_tx(full_bar + 8u * stage, tx_bytes, leader ? issue : 0u);
             if constexpr (CG == 2) {
-              tma_load_2d_pair(w_dst, &tmap_w, target, kb * kAtom, c0, policy, weights);
+              tma_load_2d_pair(w_dst, &tmap_w, target, kb * kAtom, c0, policy, issue);
               tma_load_2d_pair(t_dst, &tmap_t, target, kb * kAtom, t0, policy, issue);
             } else {
-              tma_load_2d(w_dst, &tmap_w, target, kb * kAtom, c0, policy, weights);
-              tma_load_2d(t_dst, &tmap_t, target, kb * kAtom, t0, policy, issue);
+              tma_load_2d(w_dst, &tmap_w, target, kb * kAtom, c0, policy, issue);
+              if constexpr (!FUSE) tma_load_2d(t_dst, &tmap_t, target, kb * kAtom, t0, policy, issue);
             }
           }
-          if (ahead > 0) --ahead;
           issued_mask |= 1u << stage;
           issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
           if (++stage == p.stages) { stage = 0; phase ^= 1u; }
@@ -241,6 +295,10 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true, issued = false;
+      if constexpr (FUSE) {
+        const bool wt = wait_bar<false>(tok_bar, 0, ctl, ROLE_MMA, 0x90u);
+        ok = __all_sync(0xffffffffu, wt);
+      }
       for (int u = slot0; u < p.num_units && ok; u += slots) {
         const bool wt = wait_bar<CG == 2>(tempty_bar + 8u * acc, acc_phase ^ 1u, ctl, ROLE_MMA, 0x80u | acc);
         if (!__all_sync(0xffffffffu, wt)) { ok = false; break; }
@@ -253,7 +311,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
           tc_fence_after();
           const uint32_t w_src = base + (uint32_t)stage * p.stage_bytes;
           if (CG == 1 || issue) {
-            const uint64_t wd = sw128_kmajor_desc(w_src), td = sw128_kmajor_desc(w_src + p.a_bytes);
+            const uint64_t wd = sw128_kmajor_desc(w_src);
+            const uint64_t td = sw128_kmajor_desc(FUSE ? base + p.tok_offset + (uint32_t)(kb - kb_begin) * kTokAtom : w_src + p.a_bytes);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               mma_i8<CG>(d_tmem, wd + 2u * kk, td + 2u * kk, p.idesc, (kb != kb_begin || kk) ? 1u : 0u, issue);
@@ -278,13 +337,20 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       }
     }
   } else {
+    if constexpr (FUSE) {
+      stage_tokens<T>(p, base + p.tok_offset, base + p.sa_offset, tok_rows, tok_top, kb_begin, kb_end, (int)threadIdx.x - 64);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tok_bar);
+    }
+    if (!FUSE || warp < 6) {
     // ------------------------------------------------------------ epilogue
     const uint32_t q = warp & 3u;                        // TMEM lane quadrant
     const int row = (int)(32u * q + lane);               // channel within the CTA's 128
     const uint32_t gtid = (warp - 2u) * 32u + lane;
     const bool issuer = gtid == 0;
     const uint32_t stg = base + p.stg_offset;
-    const uint32_t sa_s = base + p.sa_offset + q * (uint32_t)(BN * 4);   // this warp's copy of the token scales
+    const uint32_t sa_s = base + p.sa_offset + (FUSE ? 0u : q * (uint32_t)(BN * 4));   // this warp's copy of the token scales
     const uint32_t leader_tempty = CG == 2 ? mapa_shared(tempty_bar, 0) : tempty_bar;
     const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
     uint32_t chunk_no = 0;
@@ -299,13 +365,15 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       const bool ch_ok = ch < p.n;
       const float sb = ch_ok ? (p.sb ? p.sb[ch] : 1.f) : 0.f;
       const float bias = ch_ok && p.bias ? load_as_f32(p.bias, p.bias_type, ch) : 0.f;
-      __syncwarp();
+      if constexpr (!FUSE) {
+        __syncwarp();
 #pragma unroll
-      for (int i = 0; i < (BN + 31) / 32; ++i) {
-        const int t = i * 32 + (int)lane;
-        if (t < BN) st_shared_u32(sa_s + 4u * t, __float_as_uint(t0 + t < p.m ? (p.sa ? p.sa[t0 + t] : 1.f) : 0.f));
+        for (int i = 0; i < (BN + 31) / 32; ++i) {
+          const int t = i * 32 + (int)lane;
+          if (t < BN) st_shared_u32(sa_s + 4u * t, __float_as_uint(t0 + t < p.m ? (p.sa ? p.sa[t0 + t] : 1.f) : 0.f));
+        }
+        __syncwarp();
       }
-      __syncwarp();
       const bool ok = wait_bar<false>(tfull_bar + 8u * acc, acc_phase, ctl, ROLE_EPILOGUE, acc);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
@@ -388,6 +456,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       if (++acc == p.num_acc) { acc = 0; acc_phase ^= 1u; }
     }
     if (issuer && p.stg_bufs > 0) bulk_wait_group<0>();
+    }
   }
 
   // ------------------------------------------------------------ split-K sum and teardown
@@ -396,7 +465,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
   if (split) {
     cluster_arrive();
     cluster_wait();
-    if (warp >= 2) {
+    if (warp >= 2 && warp < 6) {
       // CTA `rank` finishes its share of the tokens: a warp takes a token, a lane
       // four channels, with every peer's 16 bytes in flight at once.
       int cb, tb;
@@ -421,7 +490,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         uint32_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < kMaxSplit; ++s) { sum[0] += part[s].x; sum[1] += part[s].y; sum[2] += part[s].z; sum[3] += part[s].w; }
-        const float sa = p.sa ? p.sa[t] : 1.f;
+        const float sa = FUSE ? tok_rows[FUSE ? t : 0].scale : (p.sa ? p.sa[t] : 1.f);
         T* const d = static_cast<T*>(p.d) + (int64_t)t * p.ldd + ch0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -502,6 +571,17 @@ int sm_count() {
   return sms;
 }
 
+// CTAs that share a tile of 128 channels, for few tiles.  One SM pulls some 75 of
+// HBM's 6500 bytes per ns, so 64 to 128 CTAs stream at full rate; more than one
+// wave of them, or clusters of 8 (of which the GPU holds 16 at a time or fewer),
+// cost more than they give.  16 tokens, 8192 x 8192: 14.3 us whole, 14.3 split in 2,
+// 18.0 in 4, 29.7 in 8; 2048 x 16384: 17.0 whole, 10.5 split in 4, 13.7 in 8.
+int split_for(int64_t tiles, int64_t kb, int64_t most_ctas, int64_t least_kb) {
+  int s = 1;
+  while (s < 4 && tiles * s * 2 <= most_ctas && kb >= 2 * s * least_kb) s *= 2;
+  return s;
+}
+
 // Tile and split from the sizes.
 void choose(const Int8GemmArgs* a, int num_sms, int& cg, int& bn, int& split) {
   const int64_t cb = (a->n + 127) / 128;
@@ -512,20 +592,18 @@ void choose(const Int8GemmArgs* a, int num_sms, int& cg, int& bn, int& split) {
   if (!bn) bn = cg == 2 ? 256 : a->m <= 16 ? 16 : a->m <= 32 ? 32 : a->m <= 64 ? 64 : 128;
   if (!split) {
     split = 1;
-    if (cg == 1) {
-      const int64_t tiles = cb * ((a->m + bn - 1) / bn);
-      const int64_t kb = (a->k + kAtom - 1) / kAtom;
-      while (split < 8 && tiles * split * 2 <= 2 * num_sms && kb >= split * 2 * 4) split *= 2;
-    }
+    if (cg == 1) split = split_for(cb * ((a->m + bn - 1) / bn), (a->k + kAtom - 1) / kAtom, 64, 32);
   }
 }
 
-int resolve(const Int8GemmArgs* a, Resolved& r) {
+// `fused`: the fused form of the linear layer is wanted (the caller has checked that it applies).
+int resolve(const Int8GemmArgs* a, bool fused, Resolved& r) {
   memset(&r, 0, sizeof(r));
-  const int rc = check(a, true, r);
+  const int rc = check(a, !fused, r);
   if (rc != GEMM_OK) return rc;
   r.num_sms = sm_count();
   r.cg = a->cta_group; r.bn = a->tile_n; r.split = a->split_k;
+  if (fused) { r.cg = 1; r.bn = kFusedBN; r.split = split_for((a->n + kChannels - 1) / kChannels, (a->k + kAtom - 1) / kAtom, 128, 16); }
   choose(a, r.num_sms, r.cg, r.bn, r.split);
   if (r.cg != 1 && r.cg != 2) FAIL("cta_group must be 1 or 2");
   if (!supported(r.cg, r.bn)) FAIL("tile_n %d unsupported for cta_group %d", r.bn, r.cg);
@@ -546,7 +624,7 @@ int resolve(const Int8GemmArgs* a, Resolved& r) {
   p.num_units = p.num_cb * p.num_tb;
   p.raster = p.num_cb < 4 ? (p.num_cb > 0 ? p.num_cb : 1) : 4;
   p.a_bytes = kChannels * kAtom;
-  p.stage_bytes = p.a_bytes + (uint32_t)(r.bn / r.cg) * kAtom;
+  p.stage_bytes = p.a_bytes + (fused ? 0u : (uint32_t)(r.bn / r.cg) * kAtom);
   p.num_acc = r.split > 1 ? 1 : 2;
   int cols = 32;
   while (cols < p.num_acc * r.bn) cols *= 2;
@@ -558,10 +636,11 @@ int resolve(const Int8GemmArgs* a, Resolved& r) {
   p.stg_bytes = (uint32_t)(cw * kChannels * e);
   // (A TMA store whose row extent ends inside 16 bytes writes the rest of them too.)
   p.stg_bufs = r.split == 1 && a->m > 0 && rows_16b(a->d, a->ldd, e) && (a->n * e) % 16 == 0 ? 2 : 0;
-  const int64_t fixed = 1024 + kBarrierBytes + (int64_t)p.stg_bufs * p.stg_bytes + 4 * r.bn * 4;
+  const int kb_cta = (p.num_kb + r.split - 1) / r.split;
+  const int64_t tok_bytes = fused ? (int64_t)kb_cta * kTokAtom + kTokAtom : 0;
+  const int64_t fixed = 1024 + kBarrierBytes + (int64_t)p.stg_bufs * p.stg_bytes + 4 * r.bn * 4 + tok_bytes + kStaticSmem;
   r.max_stages = (int)((kSmemLimit - fixed) / p.stage_bytes);
   if (r.max_stages > 12) r.max_stages = 12;
-  const int kb_cta = (p.num_kb + r.split - 1) / r.split;
   r.stages = r.max_stages;
   if (r.split > 1) {
     if (r.stages > kb_cta) r.stages = kb_cta;
@@ -569,7 +648,9 @@ int resolve(const Int8GemmArgs* a, Resolved& r) {
   }
   p.stages = r.stages;
   p.bars_offset = (uint32_t)r.stages * p.stage_bytes;
-  p.stg_offset = p.bars_offset + kBarrierBytes;
+  p.tok_offset = p.bars_offset + kBarrierBytes;
+  p.stg_offset = p.tok_offset + (uint32_t)tok_bytes;
+  p.k = (int32_t)a->k;
   p.sa_offset = p.stg_offset + (uint32_t)p.stg_bufs * p.stg_bytes;
   r.smem_bytes = 1024 + (int64_t)p.sa_offset + 4 * r.bn * 4;
   p.status = a->status;
@@ -585,16 +666,17 @@ int resolve(const Int8GemmArgs* a, Resolved& r) {
 using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, Int8Params);
 
 template <typename T>
-KernelFn pick(int cg, int bn) {
+KernelFn pick(int cg, int bn, bool fused) {
+  if (fused) return int8_gemm_kernel<1, kFusedBN, T, true>;
   if (cg == 1) {
     switch (bn) {
-      case 16: return int8_gemm_kernel<1, 16, T>;
-      case 32: return int8_gemm_kernel<1, 32, T>;
-      case 64: return int8_gemm_kernel<1, 64, T>;
-      default: return int8_gemm_kernel<1, 128, T>;
+      case 16: return int8_gemm_kernel<1, 16, T, false>;
+      case 32: return int8_gemm_kernel<1, 32, T, false>;
+      case 64: return int8_gemm_kernel<1, 64, T, false>;
+      default: return int8_gemm_kernel<1, 128, T, false>;
     }
   }
-  return bn == 128 ? int8_gemm_kernel<2, 128, T> : int8_gemm_kernel<2, 256, T>;
+  return bn == 128 ? int8_gemm_kernel<2, 128, T, false> : int8_gemm_kernel<2, 256, T, false>;
 }
 
 std::mutex g_attr_mu;
@@ -602,11 +684,11 @@ struct AttrSet { KernelFn fn; int dev; };
 AttrSet g_attr_set[512];
 int g_attr_n = 0;
 
-bool ensure_smem_attr(KernelFn fn, int dev) {
+bool ensure_smem_attr(KernelFn fn, int dev, int bytes) {
   std::lock_guard<std::mutex> lock(g_attr_mu);
   for (int i = 0; i < g_attr_n; ++i)
     if (g_attr_set[i].fn == fn && g_attr_set[i].dev == dev) return true;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit) != cudaSuccess) {
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
     cudaGetLastError();
     return false;
   }
@@ -614,44 +696,30 @@ bool ensure_smem_attr(KernelFn fn, int dev) {
   return true;
 }
 
-// Few tokens and no tile asked for: one launch without tensor cores.
-bool use_gemv(const Int8GemmArgs& a, int num_sms) {
-  return !a.tile_n && !a.cta_group && !a.split_k && !a.flags && gemv_fits(a.m, a.n, a.k, num_sms);
-}
+struct Tokens {        // floating tokens of the fused form
+  const void* x;
+  int64_t ldx;
+};
 
-int launch_gemv(const Int8GemmArgs& a, const void* x, int32_t x_type, int64_t ldx, int num_sms, cudaStream_t st) {
-  GemvParams g;
-  memset(&g, 0, sizeof(g));
-  const char* why = "";
-  if (drop_resolve(a.drop, a.m, a.n, g.drop, &why) != GEMM_OK) return GEMM_ERR_CANNOT_IMPLEMENT;
-  g.x = x; g.ldx = ldx; g.x_type = x_type;
-  g.b = static_cast<const int8_t*>(a.b); g.ldb = a.ldb;
-  g.d = a.d; g.ldd = a.ldd; g.d_type = a.d_type; g.c = a.c; g.ldc = a.ldc;
-  g.sa = a.scale_a; g.sb = a.scale_b; g.bias = a.bias; g.bias_type = a.bias_type;
-  g.m = (int32_t)a.m; g.n = (int32_t)a.n; g.k = (int32_t)a.k;
-  g.status = a.status;
-  g.timeout_ns = (uint64_t)(a.timeout_ms ? a.timeout_ms : 4000u) * 1000000ull;
-  g.wide = x_type != kTypeInt8 && rows_16b(x, ldx, type_bytes(x_type));
-  if (gemv_launch(g, num_sms, st) != cudaSuccess) {
-    cudaGetLastError();
-    return GEMM_ERR_LAUNCH;
-  }
-  return GEMM_OK;
-}
-
-// One product; the device of D is current.  `weights_ready`: the kernel launched
-// just before on this stream writes neither the weights nor anything they depend on.
-int launch_product(const Int8GemmArgs& a, bool weights_ready, cudaStream_t st, int dev) {
+// One product; the device of D is current.
+int launch_product(const Int8GemmArgs& a, const Tokens* tokens, cudaStream_t st, int dev) {
   Resolved r;
-  const int rc = resolve(&a, r);
+  const int rc = resolve(&a, tokens != nullptr, r);
   if (rc != GEMM_OK) return rc;
   if (!get_encode()) return GEMM_ERR_LAUNCH;
   CUtensorMap tw, tt, td;
-  if (!encode_2d(&tw, a.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.ldb, kAtom, kChannels, 128) ||
-      !encode_2d(&tt, a.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.m, (uint64_t)a.lda, kAtom,
-                 (uint32_t)(r.bn / r.cg), 128))
-    return GEMM_ERR_CANNOT_IMPLEMENT;
+  memset(&tt, 0, sizeof(tt));
   memset(&td, 0, sizeof(td));
+  if (!encode_2d(&tw, a.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.ldb, kAtom, kChannels, 128))
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  if (tokens) {
+    r.p.x = tokens->x;
+    r.p.ldx = tokens->ldx;
+    r.p.x_wide = rows_16b(tokens->x, tokens->ldx, type_bytes(a.d_type)) ? 1 : 0;
+  } else if (!encode_2d(&tt, a.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.m, (uint64_t)a.lda, kAtom,
+                        (uint32_t)(r.bn / r.cg), 128)) {
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  }
   if (r.p.stg_bufs > 0) {
     const CUtensorMapDataType t = a.d_type == GEMM_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                 : a.d_type == GEMM_TYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
@@ -659,23 +727,31 @@ int launch_product(const Int8GemmArgs& a, bool weights_ready, cudaStream_t st, i
                    (uint32_t)(r.bn < 32 ? r.bn : 32), 0))
       return GEMM_ERR_CANNOT_IMPLEMENT;
   }
-  KernelFn fn = a.d_type == GEMM_TYPE_BF16 ? pick<__nv_bfloat16>(r.cg, r.bn)
-              : a.d_type == GEMM_TYPE_FP16 ? pick<__half>(r.cg, r.bn) : pick<float>(r.cg, r.bn);
-  if (!ensure_smem_attr(fn, dev)) return GEMM_ERR_LAUNCH;
-  r.p.weights_ready = weights_ready ? 1 : 0;
-  if (launch_overlapped(fn, dim3((unsigned)r.grid), dim3(kThreads), (size_t)r.smem_bytes, r.split > 1 ? r.split : r.cg, st,
-                        tw, tt, td, r.p) != cudaSuccess) {
+  KernelFn fn = a.d_type == GEMM_TYPE_BF16 ? pick<__nv_bfloat16>(r.cg, r.bn, tokens != nullptr)
+              : a.d_type == GEMM_TYPE_FP16 ? pick<__half>(r.cg, r.bn, tokens != nullptr) : pick<float>(r.cg, r.bn, tokens != nullptr);
+  if (!ensure_smem_attr(fn, dev, tokens ? kSmemLimit - kStaticSmem : kSmemLimit)) return GEMM_ERR_LAUNCH;
+  if (launch_overlapped(fn, dim3((unsigned)r.grid), dim3(threads_for(tokens != nullptr)), (size_t)r.smem_bytes,
+                        r.split > 1 ? r.split : r.cg, st, tw, tt, td, r.p) != cudaSuccess) {
     cudaGetLastError();
     return GEMM_ERR_LAUNCH;
   }
   return GEMM_OK;
 }
 
+// Few tokens, no knob set and X of D's type: one launch.  Every CTA then quantises
+// the tokens for itself, which costs more than the launch it saves beyond some
+// 16384 of their elements: 8192 x 8192, 1 token 14.5 us against 16.9 in two
+// launches, 4 tokens 18.0 against 16.1.
+bool use_fused(const Int8GemmArgs& a, int32_t x_type) {
+  return a.m <= kFusedTokens && a.m * a.k <= kFusedElems && x_type == a.d_type && !a.tile_n && !a.cta_group && !a.split_k &&
+         !a.flags;
+}
+
 }  // namespace
 
 extern "C" int gemm_sm100a_int8_query(const Int8GemmArgs* args, GemmInfo* info) {
   Resolved r;
-  const int rc = resolve(args, r);
+  const int rc = resolve(args, false, r);
   if (info) {
     memset(info, 0, sizeof(*info));
     info->struct_size = sizeof(GemmInfo);
@@ -696,19 +772,15 @@ extern "C" int gemm_sm100a_int8_launch(const Int8GemmArgs* args, void* stream) {
   const int rc = check(args, true, r);
   if (rc != GEMM_OK) return rc;
   if (args->m == 0 || args->n == 0) return GEMM_OK;
-  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   PointerDeviceGuard guard(args->d);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
-  const int sms = sm_count();
-  if (use_gemv(*args, sms)) return launch_gemv(*args, args->a, kTypeInt8, args->lda, sms, st);
-  return launch_product(*args, false, st, guard.dev);
+  return launch_product(*args, nullptr, reinterpret_cast<cudaStream_t>(stream), guard.dev);
 }
 
 extern "C" int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream) {
   Resolved r;
   memset(&r, 0, sizeof(r));
-  const int sms = sm_count();
-  const bool few = args && args->struct_size == sizeof(Int8GemmArgs) && use_gemv(*args, sms);
+  const bool few = args && args->struct_size == sizeof(Int8GemmArgs) && use_fused(*args, x_type);
   const int rc = check(args, !few, r);
   if (rc != GEMM_OK) return rc;
   if (args->m == 0 || args->n == 0) return GEMM_OK;
@@ -718,12 +790,15 @@ extern "C" int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, 
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   PointerDeviceGuard guard(args->d);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
-  if (few) return launch_gemv(*args, x, x_type, ldx, sms, st);
+  if (few) {
+    const Tokens tokens = {x, ldx};
+    return launch_product(*args, &tokens, st, guard.dev);
+  }
   Int8QuantArgs q;
   memset(&q, 0, sizeof(q));
   q.struct_size = sizeof(q);
   q.x_type = x_type; q.rows = args->m; q.cols = args->k; q.x = x; q.ldx = ldx;
   q.q = const_cast<void*>(args->a); q.ldq = args->lda; q.scale = const_cast<float*>(args->scale_a);
   const int rq = gemm_sm100a_quantize_int8(&q, stream);
-  return rq != GEMM_OK ? rq : launch_product(*args, true, st, guard.dev);
+  return rq != GEMM_OK ? rq : launch_product(*args, nullptr, st, guard.dev);
 }

@@ -102,12 +102,7 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const __grid_consta
         const int e = (c * per_chunk + i * TX + tx) * V;
         if (!live || e >= p.cols) continue;
         uint32_t w[V / 4];
-#pragma unroll
-        for (int j = 0; j < V / 4; ++j) {
-          w[j] = pack4(quantize_one<T>(v[i].get(4 * j), s), quantize_one<T>(v[i].get(4 * j + 1), s),
-                       quantize_one<T>(v[i].get(4 * j + 2), s), quantize_one<T>(v[i].get(4 * j + 3), s));
-          if (s.c == 0.f) w[j] = 0u;
-        }
+        quantize_vec<T>(v[i], s, w);
         uint8_t* q = p.q + row * p.ldq + e;
         if (p.cols - e >= V) {
           if constexpr (V == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);

@@ -293,7 +293,7 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
     d = _output(out, m, n, x.dtype, x)
     lda = _pad16(max(k, 1))
     q = sa = 0
-    if m > 4 or knobs or n > 262144 or k << (m - 1).bit_length() > 65536:   # else no workspace is needed
+    if m > 8 or knobs or m * k > 16384:   # else no workspace is needed
         work = x.new_empty((m * (lda + 4) + 16,), dtype=torch.uint8)          # int8 tokens, then their scales
         q = work.data_ptr()
         sa = q + m * lda
