@@ -40,12 +40,13 @@ __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ Dr
     const Vec<T> v = load_vec<T>(static_cast<const T*>(p.x) + r * p.ldx + c, n, p.wide);
     Vec<T> b = {};
     if constexpr (RES) b = load_vec<T>(static_cast<const T*>(p.res) + r * p.ldr + c, n, p.wide);
-    const uint32_t keep = p.drop.on ? drop_mask<V>(key, p.drop.threshold, drop_index(p.drop, r, c)) : 0xFFFFFFFFu;
+    uint32_t w[V];
+    if (p.drop.on) drop_words<V>(key, drop_index(p.drop, r, c), w);
     Vec<T> o;
     o.w[0] = o.w[1] = o.w[2] = o.w[3] = 0u;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float f = keep >> j & 1u ? v.get(j) * grow : 0.f;
+      float f = !p.drop.on || word_keeps(p.drop, w[j]) ? v.get(j) * grow : 0.f;
       if constexpr (RES) f += b.get(j);
       o.set(j, f);
     }

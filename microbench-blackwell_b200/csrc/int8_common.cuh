@@ -108,9 +108,10 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T>& v, int n, bool wid
 struct Drop {
   uint64_t seed_mix;            // seed + mix64(stream_id + golden)
   const uint64_t* seed_offset;
-  uint64_t threshold;           // rint(p * 2^32): a word below it is dropped
+  uint32_t threshold;           // a word below rint(p * 2^32) is dropped (p = 1: see drop_keeps)
   float grow;                   // 1 / (1 - p), 0 for p = 1
   int32_t on;
+  uint32_t all;                 // all ones where p rounds to 1 in 2^32 steps: every word is dropped
   int64_t row0, col0, row_elems;
 };
 
@@ -120,29 +121,40 @@ __device__ __forceinline__ uint64_t drop_key(const Drop& d) {
 __device__ __forceinline__ int64_t drop_index(const Drop& d, int64_t r, int64_t c) {
   return (d.row0 + r) * d.row_elems + d.col0 + c;
 }
-__device__ __forceinline__ bool drop_keeps(uint64_t key, uint64_t threshold, int64_t index) {
+// A word at or above 2^32 does not exist, so for p = 1 words are cleared first.
+__device__ __forceinline__ bool word_keeps(const Drop& d, uint32_t word) { return (word & ~d.all) >= d.threshold; }
+__device__ __forceinline__ bool drop_keeps(const Drop& d, uint64_t key, int64_t index) {
   const uint64_t h = counter_rng::draw(key, (uint64_t)index >> 1);
-  return (index & 1 ? h >> 32 : h & 0xFFFFFFFFull) >= threshold;
+  return word_keeps(d, (uint32_t)(index & 1 ? h >> 32 : h));
 }
-// Bit e of the result: element `index` + e is kept, e < N (N even).  One draw
-// serves the two elements of an aligned pair.
+// The words of elements `index` .. + N - 1 (N even).  One draw serves the two
+// elements of an aligned pair.
 template <int N>
-__device__ __forceinline__ uint32_t drop_mask(uint64_t key, uint64_t threshold, int64_t index) {
-  const uint64_t first = (uint64_t)index >> 1;
-  uint32_t m = 0;
+__device__ __forceinline__ void drop_words(uint64_t key, int64_t index, uint32_t (&w)[N]) {
+  uint64_t z = key + (((uint64_t)index >> 1) + 1) * counter_rng::kGolden;
 #pragma unroll
-  for (int j = 0; j < N / 2; ++j) {
-    const uint64_t h = counter_rng::draw(key, first + j);
-    m |= ((h & 0xFFFFFFFFull) >= threshold ? 1u : 0u) << (2 * j);
-    m |= ((h >> 32) >= threshold ? 1u : 0u) << (2 * j + 1);
+  for (int j = 0; j < N / 2; ++j, z += counter_rng::kGolden) {
+    const uint64_t h = counter_rng::mix64(z);
+    w[2 * j] = (uint32_t)h;
+    w[2 * j + 1] = (uint32_t)(h >> 32);
   }
   if (index & 1) {
-    const uint64_t h = counter_rng::draw(key, first + N / 2);
-    m = (m >> 1) | (((h & 0xFFFFFFFFull) >= threshold ? 1u : 0u) << (N - 1));
+    const uint64_t h = counter_rng::mix64(z);
+#pragma unroll
+    for (int j = 0; j + 1 < N; ++j) w[j] = w[j + 1];
+    w[N - 1] = (uint32_t)h;
   }
-  return m;
 }
 
+// Zeroes the dropped elements of a vector that starts at element `index`.
+template <typename T>
+__device__ __forceinline__ void drop_vec(const Drop& d, uint64_t key, int64_t index, Vec<T>& v) {
+  uint32_t w[Vec<T>::N];
+  drop_words<Vec<T>::N>(key, index, w);
+#pragma unroll
+  for (int j = 0; j < Vec<T>::N; ++j)
+    if (!word_keeps(d, w[j])) v.zero(j);
+}
 // ------------------------------------------------------------------ int8 rounding
 // q = 127 * x / amax to the nearest integer, ties to even, decided exactly.
 // Everything is scaled by a power of two g so that neither the products nor
@@ -280,7 +292,9 @@ inline int drop_resolve(const DropoutArgs& a, int64_t rows, int64_t cols, Drop& 
   d.on = 1;
   d.seed_mix = a.seed + counter_rng::mix64(a.stream_id + counter_rng::kGolden);
   d.seed_offset = a.seed_offset;
-  d.threshold = (uint64_t)std::llrint(a.p * 4294967296.0);
+  const uint64_t threshold = (uint64_t)std::llrint(a.p * 4294967296.0);
+  d.all = threshold >> 32 ? 0xFFFFFFFFu : 0u;
+  d.threshold = d.all ? 1u : (uint32_t)threshold;
   d.grow = a.p == 1.0 ? 0.f : (float)(1.0 / (1.0 - a.p));
   d.row0 = a.row0; d.col0 = a.col0; d.row_elems = a.row_elems;
   return GEMM_OK;

@@ -411,7 +411,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
           const int64_t index = drop_index(p.drop, tc, ch);
 #pragma unroll
           for (int j = 0; j < CW; ++j)
-            v[j] = drop_keeps(key, p.drop.threshold, index + j * p.drop.row_elems) ? v[j] * p.drop.grow : 0.f;
+            v[j] = drop_keeps(p.drop, key, index + j * p.drop.row_elems) ? v[j] * p.drop.grow : 0.f;
         }
         if (p.c && ch_ok) {
           const T* c = static_cast<const T*>(p.c) + (int64_t)tc * p.ldc + ch;
@@ -496,7 +496,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         for (int e = 0; e < 4; ++e) {
           if (ch0 + e >= p.n) break;
           float v = finish((int32_t)sum[e], sa, sb[e], bias[e]);
-          if (p.drop.on) v = drop_keeps(key, p.drop.threshold, drop_index(p.drop, t, ch0 + e)) ? v * p.drop.grow : 0.f;
+          if (p.drop.on) v = drop_keeps(p.drop, key, drop_index(p.drop, t, ch0 + e)) ? v * p.drop.grow : 0.f;
           if (p.c) v += to_f32(static_cast<const T*>(p.c)[(int64_t)t * p.ldc + ch0 + e]);
           d[e] = from_f32<T>(v);
         }

@@ -31,16 +31,18 @@ struct QuantParams {
   Drop drop;
   int32_t wide;         // every row of X starts on a 16-byte boundary
   int32_t row_chunk;    // columns kernel: rows of one CTA of the cluster
-  int32_t rows_held;    // columns kernel: how many of them stay in shared memory
+  int32_t rows_held;    // columns kernel: how many of them are in shared memory at a time (a multiple of 16)
 };
 
 // ----------------------------------------------------------------- rows
+constexpr int kRowThreads = 512;
+
 // A row belongs to blockDim.x threads (a block holds blockDim.y rows); each
 // keeps NV 16-byte vectors in registers between the maximum and the rounding,
 // so X is read once.  Rows longer than NV * blockDim.x vectors are read again
 // (from L2) chunk by chunk.
 template <typename T, int NV, bool DROP>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(const __grid_constant__ QuantParams p) {
+__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const __grid_constant__ QuantParams p) {
   constexpr int V = Vec<T>::N;
   __shared__ uint32_t warp_max[32];
   const int tx = threadIdx.x, TX = blockDim.x;
@@ -65,10 +67,7 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           const int64_t e = (int64_t)(chunk * per_chunk + i * TX + tx) * V;
-          const uint32_t keep = drop_mask<V>(key, p.drop.threshold, drop_index(p.drop, row, e));
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (!(keep >> j & 1u)) v[i].zero(j);
+          drop_vec<T>(p.drop, key, drop_index(p.drop, row, e), v[i]);
         }
       }
     };
@@ -118,151 +117,206 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const __grid_consta
 }
 
 // ----------------------------------------------------------------- columns
-// A cluster owns a strip of 64 columns; its CTAs split the rows.  Each CTA
-// reads its rows once, keeps them in shared memory and finds the column
-// maxima (and sums); the cluster combines them through distributed shared
-// memory; then every thread rounds 32 rows of two columns and writes two
-// whole 32-byte sectors of the transposed result.
-constexpr int kStrip = 64;
+// A cluster owns a strip of columns, 64 bytes of each row; its CTAs split the
+// rows.  Each CTA copies its rows to shared memory with every load in flight at
+// once, finds the column maxima (and sums) there, combines them with its peers
+// through distributed shared memory, and rounds 16 rows of two columns per
+// thread into 16-byte stores (whole 32-byte sectors per column) of the transposed
+// result.  1024 rows (64 KB) at a time leave room for three CTAs per SM, whose
+// phases overlap; X is read once, and a column of more than 8 x 1024 rows a second
+// time from L2 (the strips at work at one time are smaller than it).
+constexpr int kStripBytes = 64;
 constexpr int kColThreads = 256;
+constexpr int kRowsHeld = 1024;                // rows of a CTA in shared memory at a time
+constexpr int kColWarps = kColThreads / 32;
+
+// Byte of row r in the held strip: a 64-byte gap after every 16 rows puts rows 16
+// apart, which the lanes of a warp read together, in different banks.
+__device__ __forceinline__ int held_at(int r) { return (r + (r >> 4)) * kStripBytes; }
 
 template <typename T, bool DROP>
 __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid_constant__ QuantParams p) {
   constexpr int V = Vec<T>::N;
-  constexpr int LANES = kStrip / V;            // threads that cover one row of the strip
-  constexpr int RPP = kColThreads / LANES;     // rows read per pass
-  extern __shared__ __align__(16) uint8_t smem[];
-  T* const held = reinterpret_cast<T*>(smem);  // [rows_held][kStrip]
-  __shared__ uint32_t part_max[RPP][kStrip];
-  __shared__ float part_sum[RPP][kStrip];
-  __shared__ uint32_t cta_max[kStrip];
-  __shared__ float cta_sum[kStrip];
+  constexpr int COLS = kStripBytes / (int)sizeof(T);
+  constexpr int LANES = kStripBytes / 16;      // threads that cover one row of the strip
+  constexpr int RPP = kColThreads / LANES;     // rows per pass of the block
+  constexpr int PAIRS = COLS / 2;              // lanes that cover the strip two columns each
+  constexpr int SETS = 32 / PAIRS;             // 16-row sets a warp rounds at once
+  extern __shared__ __align__(16) uint8_t held[];
+  __shared__ uint32_t part_max[kColWarps][COLS];
+  __shared__ float part_sum[kColWarps][COLS];
+  __shared__ uint32_t cta_max[COLS];
+  __shared__ float cta_sum[COLS];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), peers = (int)cluster.num_blocks();
-  const int64_t col0 = (int64_t)(blockIdx.x / peers) * kStrip;
+  const int64_t col0 = (int64_t)(blockIdx.x / peers) * COLS;
   const int64_t row0 = (int64_t)rank * p.row_chunk;
   const int n_rows = (int)max((int64_t)0, min((int64_t)p.row_chunk, p.rows - row0));
   sm100::grid_dependency_wait();
   sm100::grid_launch_dependents();
   const uint64_t key = DROP ? drop_key(p.drop) : 0;
 
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int lane_c = threadIdx.x % LANES, lane_r = threadIdx.x / LANES;
   const int64_t c = col0 + lane_c * V;
   const int n_valid = (int)max((int64_t)0, min((int64_t)V, p.cols - c));
-  const T* const x = static_cast<const T*>(p.x);
-  uint32_t top[V];
+  const T* const x = static_cast<const T*>(p.x) + row0 * p.ldx;
+  const uint32_t held_s = sm100::smem_u32(held);
+  // Rows [b * rows_held, ..) of this CTA into shared memory; every thread waits for
+  // what it has copied itself, and masks it.
+  auto fetch = [&](int b) {
+    const int first = b * p.rows_held, n = min(n_rows - first, p.rows_held);
+    for (int r = lane_r; r < n; r += RPP) {
+      const uint32_t dst = held_s + (uint32_t)(held_at(r) + lane_c * 16);
+      const T* src = x + (int64_t)(first + r) * p.ldx + c;
+      if (p.wide) {
+        sm100::cp_async_16(dst, n_valid > 0 ? src : x, (uint32_t)(n_valid * (int)sizeof(T)));
+      } else {
+        const Vec<T> v = load_vec<T>(src, n_valid, false);
+        sm100::st_shared_v4(dst, v.w[0], v.w[1], v.w[2], v.w[3]);
+      }
+    }
+    sm100::cp_async_wait_all();
+    if constexpr (DROP) {
+      for (int r = lane_r; r < n; r += RPP) {
+        const uint32_t at = held_s + (uint32_t)(held_at(r) + lane_c * 16);
+        const uint4 u = sm100::ld_shared_v4(at);
+        Vec<T> v;
+        v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
+        drop_vec<T>(p.drop, key, drop_index(p.drop, row0 + first + r, c), v);
+        sm100::st_shared_v4(at, v.w[0], v.w[1], v.w[2], v.w[3]);
+      }
+    }
+  };
+
+  // Maxima and sums of this thread's V columns over the rows it has copied itself.
+  uint32_t top[4];
   float sum[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) { top[j] = 0u; sum[j] = 0.f; }
-  constexpr int UN = 4;   // rows in flight per thread
-  for (int r = lane_r; r < n_rows; r += UN * RPP) {
-    Vec<T> v[UN];
+  for (int j = 0; j < 4; ++j) top[j] = 0u;
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int rr = r + u * RPP;
-      v[u] = load_vec<T>(x + (row0 + rr) * p.ldx + c, rr < n_rows ? n_valid : 0, p.wide);
-    }
+  for (int j = 0; j < V; ++j) sum[j] = 0.f;
+  const int batches = max(1, (n_rows + p.rows_held - 1) / max(1, p.rows_held));
+  for (int b = 0; b < batches; ++b) {
+    fetch(b);
+    const int n = min(n_rows - b * p.rows_held, p.rows_held);
+    for (int r = lane_r; r < n; r += RPP) {
+      const uint4 u = sm100::ld_shared_v4(held_s + (uint32_t)(held_at(r) + lane_c * 16));
+      Vec<T> v;
+      v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
 #pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int rr = r + u * RPP;
-      if (rr >= n_rows) break;
-      if constexpr (DROP) {
-        const uint32_t keep = drop_mask<V>(key, p.drop.threshold, drop_index(p.drop, row0 + rr, c));
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (!(keep >> j & 1u)) v[u].zero(j);
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) top[j] = max(top[j], v.w[j] & 0x7FFFFFFFu);
+        else top[j] = __vmaxu2(top[j], v.w[j] & 0x7FFF7FFFu);
       }
+      if (p.col_sums) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float f = v[u].get(j);
-        top[j] = max(top[j], __float_as_uint(f) & 0x7FFFFFFFu);
-        sum[j] += f;
+        for (int j = 0; j < V; ++j) sum[j] += v.get(j);
       }
-      if (rr < p.rows_held)
-        *reinterpret_cast<uint4*>(held + rr * kStrip + lane_c * V) = make_uint4(v[u].w[0], v[u].w[1], v[u].w[2], v[u].w[3]);
     }
   }
+  // Lanes lane % LANES of a warp hold the same columns.
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    part_max[lane_r][lane_c * V + j] = top[j];
-    part_sum[lane_r][lane_c * V + j] = sum[j];
+  for (int s = LANES; s < 32; s *= 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t o = __shfl_xor_sync(0xFFFFFFFFu, top[j], s);
+      top[j] = sizeof(T) == 4 ? max(top[j], o) : __vmaxu2(top[j], o);
+    }
+    if (p.col_sums) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += __shfl_xor_sync(0xFFFFFFFFu, sum[j], s);
+    }
+  }
+  if (lane < LANES) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      part_max[warp][lane * V + j] =
+          sizeof(T) == 4 ? top[j & 3] : abs_bits_to_f32<T>(j & 1 ? top[(j / 2) & 3] >> 16 : top[(j / 2) & 3] & 0xFFFFu);
+      part_sum[warp][lane * V + j] = sum[j];
+    }
   }
   __syncthreads();
-  if (threadIdx.x < kStrip) {
+  if (threadIdx.x < COLS) {
     uint32_t m = 0;
     float s = 0.f;
-    for (int r = 0; r < RPP; ++r) {
-      m = max(m, part_max[r][threadIdx.x]);
-      s += part_sum[r][threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < kColWarps; ++w) {
+      m = max(m, part_max[w][threadIdx.x]);
+      s += part_sum[w][threadIdx.x];
     }
     cta_max[threadIdx.x] = m;
     cta_sum[threadIdx.x] = s;
   }
   cluster.sync();
-  // Every thread of warp w works on columns 2 * lane and 2 * lane + 1.
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pair = lane % PAIRS, set = lane / PAIRS;
   uint32_t m0 = 0, m1 = 0;
   float s0 = 0.f, s1 = 0.f;
+  const bool writer = rank == 0 && warp == 0 && set == 0;
   for (int i = 0; i < peers; ++i) {
     const uint32_t* pm = cluster.map_shared_rank(cta_max, i);
-    m0 = max(m0, pm[2 * lane]);
-    m1 = max(m1, pm[2 * lane + 1]);
-    if (rank == 0 && warp == 0 && p.col_sums) {
+    m0 = max(m0, pm[2 * pair]);
+    m1 = max(m1, pm[2 * pair + 1]);
+    if (writer && p.col_sums) {
       const float* ps = cluster.map_shared_rank(cta_sum, i);
-      s0 += ps[2 * lane];
-      s1 += ps[2 * lane + 1];
+      s0 += ps[2 * pair];
+      s1 += ps[2 * pair + 1];
     }
   }
   const RowScale q0 = row_scale(m0), q1 = row_scale(m1);
-  const int64_t c0 = col0 + 2 * lane;
-  if (rank == 0 && warp == 0) {
+  const int64_t c0 = col0 + 2 * pair;
+  if (writer) {
     const float grow = DROP ? p.drop.grow : 1.f;
     if (c0 < p.cols) { p.scale[c0] = q0.scale * grow; if (p.col_sums) p.col_sums[c0] = s0 * grow; }
     if (c0 + 1 < p.cols) { p.scale[c0 + 1] = q1.scale * grow; if (p.col_sums) p.col_sums[c0 + 1] = s1 * grow; }
   }
-  auto value = [&](int r, int64_t col) -> float {   // a row that did not fit: read and masked again
-    if (col >= p.cols) return 0.f;
-    if (DROP && !drop_keeps(key, p.drop.threshold, drop_index(p.drop, row0 + r, col))) return 0.f;
-    return to_f32(x[(row0 + r) * p.ldx + col]);
-  };
-  for (int g = warp * 32; g < n_rows; g += (kColThreads / 32) * 32) {
-    uint32_t w0[8], w1[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t b0[4], b1[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = g + 4 * k + j;
-        float f0 = 0.f, f1 = 0.f;
-        if (r < n_rows) {
-          if (r < p.rows_held) {
-            f0 = to_f32(held[r * kStrip + 2 * lane]);
-            f1 = to_f32(held[r * kStrip + 2 * lane + 1]);
-          } else {
-            f0 = value(r, c0);
-            f1 = value(r, c0 + 1);
-          }
-        }
-        b0[j] = quantize_one<T>(f0, q0);
-        b1[j] = quantize_one<T>(f1, q1);
-      }
-      w0[k] = q0.c == 0.f ? 0u : pack4(b0[0], b0[1], b0[2], b0[3]);
-      w1[k] = q1.c == 0.f ? 0u : pack4(b1[0], b1[1], b1[2], b1[3]);
+  // The last batch is still in shared memory; earlier ones are read again (from L2).
+  for (int b = batches - 1; b >= 0; --b) {
+    const int first = b * p.rows_held, n = min(n_rows - first, p.rows_held);
+    if (b + 1 < batches) {
+      __syncthreads();
+      fetch(b);
+      __syncthreads();
     }
-    auto store = [&](int64_t col, const uint32_t (&w)[8]) {
-      if (col >= p.cols) return;
-      uint8_t* q = p.q + col * p.ldq + row0 + g;
-      if (n_rows - g >= 32) {
-        reinterpret_cast<uint4*>(q)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        reinterpret_cast<uint4*>(q)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      } else {
+    for (int g = (warp * SETS + set) * 16; g < n; g += kColWarps * SETS * 16) {
+      uint32_t w0[4], w1[4];
+      const uint32_t at = held_s + (uint32_t)(held_at(g) + pair * 2 * (int)sizeof(T));
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (g + j < n_rows) q[j] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
+      for (int k = 0; k < 4; ++k) {
+        uint32_t b0[4], b1[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float f0, f1;
+          if constexpr (sizeof(T) == 4) {
+            const uint2 u = sm100::ld_shared_v2(at + (uint32_t)((4 * k + j) * kStripBytes));
+            f0 = __uint_as_float(u.x);
+            f1 = __uint_as_float(u.y);
+          } else {
+            Vec<T> v;
+            v.w[0] = sm100::ld_shared_u32(at + (uint32_t)((4 * k + j) * kStripBytes));
+            f0 = v.get(0);
+            f1 = v.get(1);
+          }
+          b0[j] = quantize_one<T>(f0, q0);
+          b1[j] = quantize_one<T>(f1, q1);
+        }
+        w0[k] = q0.c == 0.f ? 0u : pack4(b0[0], b0[1], b0[2], b0[3]);
+        w1[k] = q1.c == 0.f ? 0u : pack4(b1[0], b1[1], b1[2], b1[3]);
       }
-    };
-    store(c0, w0);
-    store(c0 + 1, w1);
+      auto store = [&](int64_t col, const uint32_t (&w)[4]) {
+        if (col >= p.cols) return;
+        uint8_t* q = p.q + col * p.ldq + row0 + first + g;
+        if (n - g >= 16) {
+          *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (g + j < n) q[j] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
+        }
+      };
+      store(c0, w0);
+      store(c0 + 1, w1);
+    }
   }
   cluster.sync();   // peers may still read this CTA's maxima
 }
@@ -270,12 +324,12 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
 // ----------------------------------------------------------------- host
 template <typename T>
 cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
-  constexpr int NV = 4;
+  constexpr int NV = 8;
   const int64_t nvec = (p.cols + Vec<T>::N - 1) / Vec<T>::N;
   int64_t tx = (nvec + NV - 1) / NV;
   tx = (tx + 31) / 32 * 32;
-  if (tx > 1024) tx = 1024;
-  const int ry = tx >= 256 ? 1 : (int)(256 / tx);
+  if (tx > kRowThreads) tx = kRowThreads;
+  const int ry = tx >= 128 ? 1 : (int)(128 / tx);
   int64_t blocks = (p.rows + ry - 1) / ry;
   if (blocks > 0x7FFFFFFF) blocks = 0x7FFFFFFF;
   const dim3 block((unsigned)tx, (unsigned)ry);
@@ -285,18 +339,17 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_cols(QuantParams p, cudaStream_t st) {
-  constexpr int64_t kHeldBytes = 192 * 1024;
+  constexpr int kCols = kStripBytes / (int)sizeof(T);
   int peers = (int)((p.rows + 255) / 256);
   peers = peers < 1 ? 1 : (peers > 8 ? 8 : peers);
-  p.row_chunk = (int32_t)(((p.rows + peers - 1) / peers + 31) / 32 * 32);
-  const int64_t fit = kHeldBytes / (kStrip * (int64_t)sizeof(T));
-  p.rows_held = (int32_t)(p.row_chunk < fit ? p.row_chunk : fit);
-  const int64_t strips = (p.cols + kStrip - 1) / kStrip;
+  p.row_chunk = (int32_t)(((p.rows + peers - 1) / peers + 15) / 16 * 16);
+  p.rows_held = p.row_chunk < kRowsHeld ? p.row_chunk : kRowsHeld;
+  const int64_t strips = (p.cols + kCols - 1) / kCols;
   auto fn = p.drop.on ? quantize_cols_kernel<T, true> : quantize_cols_kernel<T, false>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kHeldBytes);
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsHeld / 16 * 17 * kStripBytes);
   if (e != cudaSuccess) return e;
   return launch_overlapped(fn, dim3((unsigned)(strips * peers)), dim3(kColThreads),
-                           (size_t)(p.rows_held * (int64_t)(kStrip * sizeof(T))), peers, st, p);
+                           (size_t)(p.rows_held / 16 * 17 * kStripBytes), peers, st, p);
 }
 
 }  // namespace
