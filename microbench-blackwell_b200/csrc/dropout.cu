@@ -25,32 +25,48 @@ struct DropoutParams {
 };
 
 // One 16-byte vector per thread and row; blockDim.x threads cover a segment of
-// the row, blockDim.y rows.
-template <typename T, bool RES>
+// the row, blockDim.y rows.  A thread walks down its column of vectors two rows
+// at a time, so the key, the pointers and the addresses cost little per vector:
+// drawing the mask (two 64-bit products per pair of elements) is what bounds the
+// kernel next to the bytes.
+template <typename T, bool RES, bool ON>
 __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
-  constexpr int V = Vec<T>::N;
+  constexpr int V = Vec<T>::N, UN = 2;
   const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
   sm100::grid_dependency_wait();
   sm100::grid_launch_dependents();
   if (c >= p.cols) return;
   const int n = (int)min((int64_t)V, p.cols - c);
-  const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
-  const float grow = p.drop.on ? p.drop.grow : 1.f;
-  for (int64_t r = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r < p.rows; r += (int64_t)gridDim.y * blockDim.y) {
-    const Vec<T> v = load_vec<T>(static_cast<const T*>(p.x) + r * p.ldx + c, n, p.wide);
-    Vec<T> b = {};
-    if constexpr (RES) b = load_vec<T>(static_cast<const T*>(p.res) + r * p.ldr + c, n, p.wide);
-    uint32_t w[V];
-    if (p.drop.on) drop_words<V>(key, drop_index(p.drop, r, c), w);
-    Vec<T> o;
-    o.w[0] = o.w[1] = o.w[2] = o.w[3] = 0u;
+  const uint64_t key = ON ? drop_key(p.drop) : 0;
+  const float grow = ON ? p.drop.grow : 1.f;
+  const uint32_t threshold = p.drop.threshold;
+  const int64_t step = (int64_t)gridDim.y * blockDim.y;
+  for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < p.rows; r0 += UN * step) {
+    Vec<T> v[UN], b[UN];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float f = !p.drop.on || word_keeps(p.drop, w[j]) ? v.get(j) * grow : 0.f;
-      if constexpr (RES) f += b.get(j);
-      o.set(j, f);
+    for (int u = 0; u < UN; ++u) {
+      const int64_t r = r0 + u * step;
+      const int nn = r < p.rows ? n : 0;
+      v[u] = load_vec<T>(static_cast<const T*>(p.x) + r * p.ldx + c, nn, p.wide);
+      if constexpr (RES) b[u] = load_vec<T>(static_cast<const T*>(p.res) + r * p.ldr + c, nn, p.wide);
     }
-    store_vec<T>(static_cast<T*>(p.y) + r * p.ldy + c, o, n, p.wide);
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int64_t r = r0 + u * step;
+      if (r >= p.rows) break;
+      uint32_t w[V];
+      if constexpr (ON) drop_words<V>(p.drop, key, drop_index(p.drop, r, c), w);
+      Vec<T> o;
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        f[j] = !ON || w[j] >= threshold ? v[u].get(j) * grow : 0.f;
+        if constexpr (RES) f[j] += b[u].get(j);
+      }
+#pragma unroll
+      for (int j = 0; j < V; j += 2) o.set2(j, f[j], f[j + 1]);
+      store_vec<T>(static_cast<T*>(p.y) + r * p.ldy + c, o, n, p.wide);
+    }
   }
 }
 
@@ -62,9 +78,12 @@ cudaError_t launch(const DropoutParams& p, cudaStream_t st) {
   const int ty = 256 / tx;
   const int64_t gx = (nvec + tx - 1) / tx;
   int64_t gy = (p.rows + ty - 1) / ty;
-  if (gy > 65535) gy = 65535;
+  const int64_t most = (148 * 16 + gx - 1) / gx;      // two waves of blocks and more rows per thread
+  if (gy > most) gy = most;
   const dim3 grid((unsigned)gx, (unsigned)gy), block((unsigned)tx, (unsigned)ty);
-  return launch_overlapped(p.res ? dropout_kernel<T, true> : dropout_kernel<T, false>, grid, block, 0, 1, st, p);
+  void (*fn)(DropoutParams) = p.drop.on ? (p.res ? dropout_kernel<T, true, true> : dropout_kernel<T, false, true>)
+                                        : (p.res ? dropout_kernel<T, true, false> : dropout_kernel<T, false, false>);
+  return launch_overlapped(fn, grid, block, 0, 1, st, p);
 }
 
 }  // namespace

@@ -7,6 +7,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "counter_rng.cuh"
 #include "gemm_sm100a.h"
@@ -36,6 +37,22 @@ __device__ __forceinline__ float finish(int32_t acc, float sa, float sb, float b
   return fmaf(__int2float_rn(acc) * sa, sb, bias);
 }
 
+// Two 16-bit values, rounded, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float f0, float f1) {
+  uint32_t u;
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(f0, f1);
+      __builtin_memcpy(&u, &h, 4);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f0, f1);
+      __builtin_memcpy(&u, &h, 4);
+    }
+  }
+  return u;
+}
+
 // 16 bytes of T as registers; element access is compile-time indexed.
 template <typename T>
 struct Vec {
@@ -51,14 +68,13 @@ struct Vec {
       return to_f32(v);
     }
   }
-  __device__ __forceinline__ void set(int i, float f) {
+  // Elements i and i + 1 (i even), rounded.
+  __device__ __forceinline__ void set2(int i, float f0, float f1) {
     if constexpr (sizeof(T) == 4) {
-      w[i] = __float_as_uint(f);
+      w[i] = __float_as_uint(f0);
+      w[i + 1] = __float_as_uint(f1);
     } else {
-      const T v = from_f32<T>(f);
-      uint16_t h;
-      __builtin_memcpy(&h, &v, 2);
-      w[i / 2] = i & 1 ? (w[i / 2] & 0xFFFFu) | ((uint32_t)h << 16) : (w[i / 2] & 0xFFFF0000u) | h;
+      w[i / 2] = pack2<T>(f0, f1);
     }
   }
   __device__ __forceinline__ void zero(int i) {
@@ -108,10 +124,10 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T>& v, int n, bool wid
 struct Drop {
   uint64_t seed_mix;            // seed + mix64(stream_id + golden)
   const uint64_t* seed_offset;
-  uint32_t threshold;           // a word below rint(p * 2^32) is dropped (p = 1: see drop_keeps)
+  uint32_t threshold;           // a word below rint(p * 2^32) is dropped (unless `all`: at least 1)
   float grow;                   // 1 / (1 - p), 0 for p = 1
   int32_t on;
-  uint32_t all;                 // all ones where p rounds to 1 in 2^32 steps: every word is dropped
+  int32_t all;                  // p rounds to 1 in steps of 2^-32: every element is dropped
   int64_t row0, col0, row_elems;
 };
 
@@ -121,16 +137,14 @@ __device__ __forceinline__ uint64_t drop_key(const Drop& d) {
 __device__ __forceinline__ int64_t drop_index(const Drop& d, int64_t r, int64_t c) {
   return (d.row0 + r) * d.row_elems + d.col0 + c;
 }
-// A word at or above 2^32 does not exist, so for p = 1 words are cleared first.
-__device__ __forceinline__ bool word_keeps(const Drop& d, uint32_t word) { return (word & ~d.all) >= d.threshold; }
 __device__ __forceinline__ bool drop_keeps(const Drop& d, uint64_t key, int64_t index) {
   const uint64_t h = counter_rng::draw(key, (uint64_t)index >> 1);
-  return word_keeps(d, (uint32_t)(index & 1 ? h >> 32 : h));
+  return !d.all && (uint32_t)(index & 1 ? h >> 32 : h) >= d.threshold;
 }
-// The words of elements `index` .. + N - 1 (N even).  One draw serves the two
-// elements of an aligned pair.
+// The words of elements `index` .. + N - 1 (N even); zeros where all are dropped.
+// One draw serves the two elements of an aligned pair.
 template <int N>
-__device__ __forceinline__ void drop_words(uint64_t key, int64_t index, uint32_t (&w)[N]) {
+__device__ __forceinline__ void drop_words(const Drop& d, uint64_t key, int64_t index, uint32_t (&w)[N]) {
   uint64_t z = key + (((uint64_t)index >> 1) + 1) * counter_rng::kGolden;
 #pragma unroll
   for (int j = 0; j < N / 2; ++j, z += counter_rng::kGolden) {
@@ -144,16 +158,21 @@ __device__ __forceinline__ void drop_words(uint64_t key, int64_t index, uint32_t
     for (int j = 0; j + 1 < N; ++j) w[j] = w[j + 1];
     w[N - 1] = (uint32_t)h;
   }
+  if (d.all) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = 0u;
+  }
 }
 
 // Zeroes the dropped elements of a vector that starts at element `index`.
 template <typename T>
 __device__ __forceinline__ void drop_vec(const Drop& d, uint64_t key, int64_t index, Vec<T>& v) {
   uint32_t w[Vec<T>::N];
-  drop_words<Vec<T>::N>(key, index, w);
+  drop_words<Vec<T>::N>(d, key, index, w);
+  const uint32_t threshold = d.threshold;
 #pragma unroll
   for (int j = 0; j < Vec<T>::N; ++j)
-    if (!word_keeps(d, w[j])) v.zero(j);
+    if (w[j] < threshold) v.zero(j);
 }
 // ------------------------------------------------------------------ int8 rounding
 // q = 127 * x / amax to the nearest integer, ties to even, decided exactly.
@@ -293,7 +312,7 @@ inline int drop_resolve(const DropoutArgs& a, int64_t rows, int64_t cols, Drop& 
   d.seed_mix = a.seed + counter_rng::mix64(a.stream_id + counter_rng::kGolden);
   d.seed_offset = a.seed_offset;
   const uint64_t threshold = (uint64_t)std::llrint(a.p * 4294967296.0);
-  d.all = threshold >> 32 ? 0xFFFFFFFFu : 0u;
+  d.all = threshold >> 32 ? 1 : 0;
   d.threshold = d.all ? 1u : (uint32_t)threshold;
   d.grow = a.p == 1.0 ? 0.f : (float)(1.0 / (1.0 - a.p));
   d.row0 = a.row0; d.col0 = a.col0; d.row_elems = a.row_elems;
