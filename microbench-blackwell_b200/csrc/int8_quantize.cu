@@ -35,14 +35,15 @@ struct QuantParams {
 };
 
 // ----------------------------------------------------------------- rows
-constexpr int kRowThreads = 512;
+// Most threads of a row that keep nv vectors each (32768 16-bit values in all).
+__host__ __device__ constexpr int row_threads(int nv) { return 4096 / nv; }
 
 // A row belongs to blockDim.x threads (a block holds blockDim.y rows); each
 // keeps NV 16-byte vectors in registers between the maximum and the rounding,
 // so X is read once.  Rows longer than NV * blockDim.x vectors are read again
 // (from L2) chunk by chunk.
 template <typename T, int NV, bool DROP>
-__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const __grid_constant__ QuantParams p) {
+__global__ void __launch_bounds__(row_threads(NV)) quantize_rows_kernel(const __grid_constant__ QuantParams p) {
   constexpr int V = Vec<T>::N;
   __shared__ uint32_t warp_max[32];
   const int tx = threadIdx.x, TX = blockDim.x;
@@ -122,12 +123,15 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const __grid
 // once, finds the column maxima (and sums) there, combines them with its peers
 // through distributed shared memory, and rounds 16 rows of two columns per
 // thread into 16-byte stores (whole 32-byte sectors per column) of the transposed
-// result.  1024 rows (64 KB) at a time leave room for three CTAs per SM, whose
-// phases overlap; X is read once, and a column of more than 8 x 1024 rows a second
-// time from L2 (the strips at work at one time are smaller than it).
+// result.  A strip of 512 or 1024 rows at a time leaves room for several CTAs per SM,
+// whose phases overlap; the rows before the last such batch are read a second time,
+// from L2 (the strips at work at one time are smaller than it).
 constexpr int kStripBytes = 64;
 constexpr int kColThreads = 256;
-constexpr int kRowsHeld = 1024;                // rows of a CTA in shared memory at a time
+// Rows of a CTA in shared memory at a time: with fewer, more CTAs overlap their
+// phases, but more rows are read (and masked) twice.  8192 x 28672 bf16: 200 us
+// with 512, 218 with 1024; with dropout and sums 436 and 364.
+constexpr int rows_held(bool drop) { return drop ? 1024 : 512; }
 constexpr int kColWarps = kColThreads / 32;
 
 // Byte of row r in the held strip: a 64-byte gap after every 16 rows puts rows 16
@@ -147,6 +151,7 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
   __shared__ float part_sum[kColWarps][COLS];
   __shared__ uint32_t cta_max[COLS];
   __shared__ float cta_sum[COLS];
+  __shared__ RowScale scales[COLS];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), peers = (int)cluster.num_blocks();
   const int64_t col0 = (int64_t)(blockIdx.x / peers) * COLS;
@@ -249,27 +254,28 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
     cta_sum[threadIdx.x] = s;
   }
   cluster.sync();
-  const int pair = lane % PAIRS, set = lane / PAIRS;
-  uint32_t m0 = 0, m1 = 0;
-  float s0 = 0.f, s1 = 0.f;
-  const bool writer = rank == 0 && warp == 0 && set == 0;
-  for (int i = 0; i < peers; ++i) {
-    const uint32_t* pm = cluster.map_shared_rank(cta_max, i);
-    m0 = max(m0, pm[2 * pair]);
-    m1 = max(m1, pm[2 * pair + 1]);
-    if (writer && p.col_sums) {
-      const float* ps = cluster.map_shared_rank(cta_sum, i);
-      s0 += ps[2 * pair];
-      s1 += ps[2 * pair + 1];
+  // One thread per column combines the peers' results.
+  if (threadIdx.x < COLS) {
+    uint32_t m = 0;
+    float s = 0.f;
+    for (int i = 0; i < peers; ++i) {
+      m = max(m, cluster.map_shared_rank(cta_max, i)[threadIdx.x]);
+      if (rank == 0 && p.col_sums) s += cluster.map_shared_rank(cta_sum, i)[threadIdx.x];
+    }
+    const RowScale q = row_scale(m);
+    scales[threadIdx.x] = q;
+    const int64_t col = col0 + threadIdx.x;
+    if (rank == 0 && col < p.cols) {
+      const float grow = DROP ? p.drop.grow : 1.f;
+      p.scale[col] = q.scale * grow;
+      if (p.col_sums) p.col_sums[col] = s * grow;
     }
   }
-  const RowScale q0 = row_scale(m0), q1 = row_scale(m1);
+  __syncthreads();
+  sm100::cluster_arrive_relaxed();   // this CTA has read its peers' results; waited for at the end
+  const int pair = lane % PAIRS, set = lane / PAIRS;
+  const RowScale q0 = scales[2 * pair], q1 = scales[2 * pair + 1];
   const int64_t c0 = col0 + 2 * pair;
-  if (writer) {
-    const float grow = DROP ? p.drop.grow : 1.f;
-    if (c0 < p.cols) { p.scale[c0] = q0.scale * grow; if (p.col_sums) p.col_sums[c0] = s0 * grow; }
-    if (c0 + 1 < p.cols) { p.scale[c0 + 1] = q1.scale * grow; if (p.col_sums) p.col_sums[c0 + 1] = s1 * grow; }
-  }
   // The last batch is still in shared memory; earlier ones are read again (from L2).
   for (int b = batches - 1; b >= 0; --b) {
     const int first = b * p.rows_held, n = min(n_rows - first, p.rows_held);
@@ -318,23 +324,25 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
       store(c0 + 1, w1);
     }
   }
-  cluster.sync();   // peers may still read this CTA's maxima
+  sm100::cluster_wait();             // until the peers have read this CTA's
 }
 
 // ----------------------------------------------------------------- host
-template <typename T>
+template <typename T, int NV, bool DROP>
 cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
-  constexpr int NV = 8;
   const int64_t nvec = (p.cols + Vec<T>::N - 1) / Vec<T>::N;
   int64_t tx = (nvec + NV - 1) / NV;
   tx = (tx + 31) / 32 * 32;
-  if (tx > kRowThreads) tx = kRowThreads;
+  if (tx > row_threads(NV)) tx = row_threads(NV);
   const int ry = tx >= 128 ? 1 : (int)(128 / tx);
   int64_t blocks = (p.rows + ry - 1) / ry;
   if (blocks > 0x7FFFFFFF) blocks = 0x7FFFFFFF;
-  const dim3 block((unsigned)tx, (unsigned)ry);
-  return launch_overlapped(p.drop.on ? quantize_rows_kernel<T, NV, true> : quantize_rows_kernel<T, NV, false>,
-                           dim3((unsigned)blocks), block, 0, 1, st, p);
+  return launch_overlapped(quantize_rows_kernel<T, NV, DROP>, dim3((unsigned)blocks), dim3((unsigned)tx, (unsigned)ry), 0, 1, st, p);
+}
+// The mask's words need registers: half as many vectors per thread with it.
+template <typename T>
+cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
+  return p.drop.on ? launch_rows<T, 4, true>(p, st) : launch_rows<T, 8, false>(p, st);
 }
 
 template <typename T>
@@ -343,10 +351,11 @@ cudaError_t launch_cols(QuantParams p, cudaStream_t st) {
   int peers = (int)((p.rows + 255) / 256);
   peers = peers < 1 ? 1 : (peers > 8 ? 8 : peers);
   p.row_chunk = (int32_t)(((p.rows + peers - 1) / peers + 15) / 16 * 16);
-  p.rows_held = p.row_chunk < kRowsHeld ? p.row_chunk : kRowsHeld;
+  const int held = rows_held(p.drop.on);
+  p.rows_held = p.row_chunk < held ? p.row_chunk : held;
   const int64_t strips = (p.cols + kCols - 1) / kCols;
   auto fn = p.drop.on ? quantize_cols_kernel<T, true> : quantize_cols_kernel<T, false>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsHeld / 16 * 17 * kStripBytes);
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, held / 16 * 17 * kStripBytes);
   if (e != cudaSuccess) return e;
   return launch_overlapped(fn, dim3((unsigned)(strips * peers)), dim3(kColThreads),
                            (size_t)(p.rows_held / 16 * 17 * kStripBytes), peers, st, p);
