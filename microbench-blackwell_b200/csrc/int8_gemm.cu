@@ -51,6 +51,8 @@ constexpr int kSmemLimit = 232448;      // 227 KiB of opt-in dynamic shared memo
 constexpr int kBarrierBytes = 1024;
 constexpr int kStaticSmem = 512;        // bound of the static shared memory of the fused form
 constexpr int kMaxStages = 32;
+constexpr int kCBufs = 4;               // staging buffers of an epilogue that reads C by TMA
+constexpr int kCAhead = 2;              // chunks of C on their way ahead of the one in work
 constexpr int kAtom = 128;              // bytes (= K elements) of one swizzled K atom
 constexpr uint32_t kTokAtom = 8 * kAtom;  // fused form: bytes of one K atom of the tokens
 constexpr int kChannels = 128;          // channels per CTA
@@ -72,6 +74,7 @@ struct Int8Params {
   uint32_t stage_bytes, a_bytes;        // per CTA: weights, then tokens
   uint32_t bars_offset, stg_offset, sa_offset, stg_bytes;
   int32_t stg_bufs;                     // staging buffers (0 = direct stores)
+  int32_t c_staged;                     // chunks of C are fetched into the staging buffers (kCBufs of them)
   int32_t tmem_cols, num_acc;
   int32_t raster;                       // channel blocks per raster group
   uint32_t idesc;
@@ -165,11 +168,25 @@ __device__ __forceinline__ void stage_tokens(const Int8Params& p, uint32_t tok, 
   });
 }
 
+// One element of a staged chunk.
+template <typename T>
+__device__ __forceinline__ float staged(uint32_t addr) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(ld_shared_u32(addr));
+  } else {
+    const uint16_t h = ld_shared_u16(addr);
+    T v;
+    __builtin_memcpy(&v, &h, 2);
+    return to_f32(v);
+  }
+}
+
 template <int CG, int BN, typename T, bool FUSE>
 __global__ void __launch_bounds__(threads_for(FUSE), 1)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channels x K
                  const __grid_constant__ CUtensorMap tmap_t,   // tokens x K
                  const __grid_constant__ CUtensorMap tmap_d,   // D, for the staged epilogue
+                 const __grid_constant__ CUtensorMap tmap_c,   // C, where it is staged too
                  const __grid_constant__ Int8Params p) {
   constexpr int TROWS = BN / CG;                    // token rows each CTA of a pair loads
   constexpr int CW = BN < 32 ? BN : 32;             // tokens per epilogue chunk
@@ -189,6 +206,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
   const uint32_t tmem_slot = drain_bar + 8u;
   const uint32_t abort_flag = tmem_slot + 4u;
   const uint32_t tok_bar = abort_flag + 4u;              // fused form: the tokens are in place
+  const uint32_t c_bar = tok_bar + 8u;                   // [kCBufs]: a chunk of C is in its buffer
+  const uint32_t lost_flag = c_bar + 8u * kCBufs;        // an epilogue warp has given up a wait
   __shared__ RowScale tok_rows[FUSE ? kFusedTokens : 1];
   __shared__ uint32_t tok_top[FUSE ? kFusedTokens : 1];
 
@@ -216,7 +235,9 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     }
     mbar_init(drain_bar, 1);
     mbar_init(tok_bar, kStageWarps);
+    for (int b = 0; b < kCBufs; ++b) mbar_init(c_bar + 8u * b, 1);
     st_shared_u32(abort_flag, 0u);
+    st_shared_u32(lost_flag, 0u);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -353,7 +374,32 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     const uint32_t sa_s = base + p.sa_offset + (FUSE ? 0u : q * (uint32_t)(BN * 4));   // this warp's copy of the token scales
     const uint32_t leader_tempty = CG == 2 ? mapa_shared(tempty_bar, 0) : tempty_bar;
     const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
+    // Rows of an even length that begin at an even index: even channels are the first of a draw's pair.
+    const bool drop_pairs = p.drop.on && !p.drop.all && !((p.drop.row_elems | p.drop.col0) & 1);
+    const uint64_t drop_step = (uint64_t)p.drop.row_elems * counter_rng::kGolden;   // two tokens on
+    const uint32_t drop_thr = p.drop.threshold;
+    const float drop_grow = p.drop.grow;
     uint32_t chunk_no = 0;
+    // C staged: chunk x of this CTA (over all its tiles) goes through buffer x % kCBufs, is
+    // replaced there by D, element by element in the same thread, and stored from it.  One
+    // thread fetches kCAhead chunks ahead, also across tiles.
+    int c_u = slot0, c_i = 0;
+    uint32_t c_no = 0;
+    const uint64_t c_policy = policy_evict_normal();
+    auto fetch_c = [&]() {
+      if (c_u >= p.num_units) return;
+      int cb, tb;
+      tile_coords(c_u, p, cb, tb);
+      const int buf = (int)(c_no % kCBufs);
+      mbar_arrive_expect_tx(c_bar + 8u * buf, p.stg_bytes);
+      tma_load_2d(stg + (uint32_t)buf * p.stg_bytes, &tmap_c, c_bar + 8u * buf,
+                  (cb * CG + (int)(CG == 2 ? rank : 0u)) * kChannels, tb * BN + c_i * CW, c_policy);
+      ++c_no;
+      if (++c_i == NCH) { c_i = 0; c_u += slots; }
+    };
+    if (p.c_staged && issuer) {
+      for (int b = 0; b < kCAhead; ++b) fetch_c();
+    }
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int u = slot0; u < p.num_units; u += slots) {
@@ -374,8 +420,19 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         }
         __syncwarp();
       }
-      const bool ok = wait_bar<false>(tfull_bar + 8u * acc, acc_phase, ctl, ROLE_EPILOGUE, acc);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      const bool ok = __all_sync(0xffffffffu, wait_bar<false>(tfull_bar + 8u * acc, acc_phase, ctl, ROLE_EPILOGUE, acc));
+      if (p.stg_bufs > 0) {
+        // The warps meet at named barriers below, so after an abort all four leave, or none:
+        // whichever gave up (here or on a chunk of C) says so before the first barrier, and
+        // none can say so again before all have looked.
+        if (!ok && lane == 0) st_shared_u32(lost_flag, 1u);
+        named_bar_sync(1, 128);
+        const bool lost = ld_shared_volatile_u32(lost_flag) != 0u;
+        named_bar_sync(1, 128);
+        if (lost) break;
+      } else if (!ok) {
+        break;
+      }
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((32u * q) << 16) + (uint32_t)(acc * BN);
       if (split) {
@@ -406,14 +463,36 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         const int tc = t0 + i * CW;
         float v[CW];
 #pragma unroll
-        for (int j = 0; j < CW; ++j) v[j] = finish((int32_t)r[j], ld_shared_f32(sa_s + 4u * (uint32_t)(i * CW + j)), sb, bias);
+        for (int j = 0; j < CW; j += 4) {
+          const uint4 sa = ld_shared_v4(sa_s + 4u * (uint32_t)(i * CW + j));
+          v[j] = finish((int32_t)r[j], __uint_as_float(sa.x), sb, bias);
+          v[j + 1] = finish((int32_t)r[j + 1], __uint_as_float(sa.y), sb, bias);
+          v[j + 2] = finish((int32_t)r[j + 2], __uint_as_float(sa.z), sb, bias);
+          v[j + 3] = finish((int32_t)r[j + 3], __uint_as_float(sa.w), sb, bias);
+        }
         if (p.drop.on) {
           const int64_t index = drop_index(p.drop, tc, ch);
+          if (drop_pairs) {
+            // Lanes 2 i and 2 i + 1 hold the two elements of a draw: the even lane draws for
+            // token j, the odd one for token j + 1, and each passes on the other's word.
+            const bool odd = lane & 1u;
+            const uint64_t first = (uint64_t)(index + (odd ? p.drop.row_elems : 0)) >> 1;
+            uint64_t z = key + (first + 1) * counter_rng::kGolden;
 #pragma unroll
-          for (int j = 0; j < CW; ++j)
-            v[j] = drop_keeps(p.drop, key, index + j * p.drop.row_elems) ? v[j] * p.drop.grow : 0.f;
+            for (int j = 0; j < CW; j += 2, z += drop_step) {
+              const uint64_t h = counter_rng::mix64(z);
+              const uint32_t lo = (uint32_t)h, hi = (uint32_t)(h >> 32);
+              const uint32_t other = __shfl_xor_sync(0xFFFFFFFFu, odd ? lo : hi, 1);
+              v[j] = (odd ? other : lo) >= drop_thr ? v[j] * drop_grow : 0.f;
+              v[j + 1] = (odd ? hi : other) >= drop_thr ? v[j + 1] * drop_grow : 0.f;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < CW; ++j)
+              v[j] = drop_keeps(p.drop, key, index + j * p.drop.row_elems) ? v[j] * drop_grow : 0.f;
+          }
         }
-        if (p.c && ch_ok) {
+        if (p.c && ch_ok && !p.c_staged) {
           const T* c = static_cast<const T*>(p.c) + (int64_t)tc * p.ldc + ch;
           float cv[CW];
 #pragma unroll
@@ -422,21 +501,35 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
           for (int j = 0; j < CW; ++j) v[j] += cv[j];
         }
         if (p.stg_bufs > 0) {
-          const uint32_t buf = stg + (p.stg_bufs == 2 ? (chunk_no & 1u) : 0u) * p.stg_bytes;
-          if (issuer) {
-            if (p.stg_bufs == 2) bulk_wait_group_read<1>(); else bulk_wait_group_read<0>();
+          const uint32_t b = p.c_staged ? chunk_no % kCBufs : chunk_no & 1u;
+          const uint32_t buf = stg + b * p.stg_bytes;
+          if (p.c_staged) {
+            if (issuer) {
+              bulk_wait_group_read<kCBufs - kCAhead - 1>();     // the buffer that fetch_c takes has been stored
+              fetch_c();
+            }
+            __syncwarp();
+            const bool c_ok = wait_bar<false>(c_bar + 8u * b, (chunk_no / kCBufs) & 1u, ctl, ROLE_EPILOGUE, 0xC0u | b);
+            if (!c_ok) st_shared_u32(lost_flag, 1u);
+            __syncwarp();
+          } else {
+            if (issuer) bulk_wait_group_read<1>();
+            named_bar_sync(1, 128);
           }
-          named_bar_sync(1, 128);
+          if (p.c_staged) {
 #pragma unroll
-          for (int j = 0; j < CW; ++j) {
-            const T o = from_f32<T>(v[j]);
-            const uint32_t at = buf + (uint32_t)((j * kChannels + row) * (int)sizeof(T));
+            for (int j = 0; j < CW; ++j) v[j] += staged<T>(buf + (uint32_t)((j * kChannels + row) * (int)sizeof(T)));
+          }
+          const uint32_t at = buf + (uint32_t)(row * (int)sizeof(T));
+#pragma unroll
+          for (int j = 0; j < CW; j += 2) {
             if constexpr (sizeof(T) == 4) {
-              st_shared_u32(at, __float_as_uint(v[j]));
+              st_shared_u32(at + (uint32_t)(j * kChannels * 4), __float_as_uint(v[j]));
+              st_shared_u32(at + (uint32_t)((j + 1) * kChannels * 4), __float_as_uint(v[j + 1]));
             } else {
-              uint16_t h;
-              __builtin_memcpy(&h, &o, 2);
-              st_shared_u16(at, h);
+              const uint32_t h = pack2<T>(v[j], v[j + 1]);
+              st_shared_u16(at + (uint32_t)(j * kChannels * 2), (uint16_t)h);
+              st_shared_u16(at + (uint32_t)((j + 1) * kChannels * 2), (uint16_t)(h >> 16));
             }
           }
           fence_proxy_async_shared();
@@ -454,6 +547,10 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         }
       }
       if (++acc == p.num_acc) { acc = 0; acc_phase ^= 1u; }
+    }
+    if (issuer && p.c_staged) {
+      // Chunks fetched but not used (only after an abort) must land before the CTA exits.
+      for (uint32_t x = chunk_no; x < c_no; ++x) drain_wait(c_bar + 8u * (x % kCBufs), (x / kCBufs) & 1u, 100000000ull);
     }
     if (issuer && p.stg_bufs > 0) bulk_wait_group<0>();
     }
@@ -636,6 +733,8 @@ int resolve(const Int8GemmArgs* a, bool fused, Resolved& r) {
   p.stg_bytes = (uint32_t)(cw * kChannels * e);
   // (A TMA store whose row extent ends inside 16 bytes writes the rest of them too.)
   p.stg_bufs = r.split == 1 && a->m > 0 && rows_16b(a->d, a->ldd, e) && (a->n * e) % 16 == 0 ? 2 : 0;
+  p.c_staged = p.stg_bufs > 0 && a->c && rows_16b(a->c, a->ldc, e) ? 1 : 0;
+  if (p.c_staged) p.stg_bufs = kCBufs;
   const int kb_cta = (p.num_kb + r.split - 1) / r.split;
   const int64_t tok_bytes = fused ? (int64_t)kb_cta * kTokAtom + kTokAtom : 0;
   const int64_t fixed = 1024 + kBarrierBytes + (int64_t)p.stg_bufs * p.stg_bytes + 4 * r.bn * 4 + tok_bytes + kStaticSmem;
@@ -663,7 +762,7 @@ int resolve(const Int8GemmArgs* a, bool fused, Resolved& r) {
 #undef FAIL
 #undef BAD
 
-using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, Int8Params);
+using KernelFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, Int8Params);
 
 template <typename T>
 KernelFn pick(int cg, int bn, bool fused) {
@@ -707,9 +806,10 @@ int launch_product(const Int8GemmArgs& a, const Tokens* tokens, cudaStream_t st,
   const int rc = resolve(&a, tokens != nullptr, r);
   if (rc != GEMM_OK) return rc;
   if (!get_encode()) return GEMM_ERR_LAUNCH;
-  CUtensorMap tw, tt, td;
+  CUtensorMap tw, tt, td, tc;
   memset(&tt, 0, sizeof(tt));
   memset(&td, 0, sizeof(td));
+  memset(&tc, 0, sizeof(tc));
   if (!encode_2d(&tw, a.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.ldb, kAtom, kChannels, 128))
     return GEMM_ERR_CANNOT_IMPLEMENT;
   if (tokens) {
@@ -723,15 +823,18 @@ int launch_product(const Int8GemmArgs& a, const Tokens* tokens, cudaStream_t st,
   if (r.p.stg_bufs > 0) {
     const CUtensorMapDataType t = a.d_type == GEMM_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                 : a.d_type == GEMM_TYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-    if (!encode_2d(&td, a.d, t, (uint64_t)a.n, (uint64_t)a.m, (uint64_t)(a.ldd * type_bytes(a.d_type)), kChannels,
-                   (uint32_t)(r.bn < 32 ? r.bn : 32), 0))
+    const uint32_t tokens_box = (uint32_t)(r.bn < 32 ? r.bn : 32);
+    if (!encode_2d(&td, a.d, t, (uint64_t)a.n, (uint64_t)a.m, (uint64_t)(a.ldd * type_bytes(a.d_type)), kChannels, tokens_box, 0))
+      return GEMM_ERR_CANNOT_IMPLEMENT;
+    if (r.p.c_staged &&
+        !encode_2d(&tc, a.c, t, (uint64_t)a.n, (uint64_t)a.m, (uint64_t)(a.ldc * type_bytes(a.d_type)), kChannels, tokens_box, 0))
       return GEMM_ERR_CANNOT_IMPLEMENT;
   }
   KernelFn fn = a.d_type == GEMM_TYPE_BF16 ? pick<__nv_bfloat16>(r.cg, r.bn, tokens != nullptr)
               : a.d_type == GEMM_TYPE_FP16 ? pick<__half>(r.cg, r.bn, tokens != nullptr) : pick<float>(r.cg, r.bn, tokens != nullptr);
   if (!ensure_smem_attr(fn, dev, tokens ? kSmemLimit - kStaticSmem : kSmemLimit)) return GEMM_ERR_LAUNCH;
   if (launch_overlapped(fn, dim3((unsigned)r.grid), dim3(threads_for(tokens != nullptr)), (size_t)r.smem_bytes,
-                        r.split > 1 ? r.split : r.cg, st, tw, tt, td, r.p) != cudaSuccess) {
+                        r.split > 1 ? r.split : r.cg, st, tw, tt, td, tc, r.p) != cudaSuccess) {
     cudaGetLastError();
     return GEMM_ERR_LAUNCH;
   }
