@@ -73,7 +73,8 @@ struct Int8Params {
   int32_t stages;
   uint32_t stage_bytes, a_bytes;        // per CTA: weights, then tokens
   uint32_t bars_offset, stg_offset, sa_offset, stg_bytes;
-  int32_t stg_bufs;                     // staging buffers (0 = direct stores)
+  int32_t stg_bufs;                     // staging buffers (0: D is written from registers)
+  int32_t tma_store;                    // D is written from them, by TMA
   int32_t c_staged;                     // chunks of C are fetched into the staging buffers (kCBufs of them)
   int32_t tmem_cols, num_acc;
   int32_t raster;                       // channel blocks per raster group
@@ -181,6 +182,27 @@ __device__ __forceinline__ float staged(uint32_t addr) {
   }
 }
 
+// A thread's column of a chunk, `tokens` rows of D from `d`, `step` bytes apart: for
+// a D that TMA cannot store.  With one warp per scheduler every instruction counts, hence the running
+// pointer and the paired conversions (777 x 5001 x 2048: 18.1 us through shared memory in
+// aligned 16-byte stores).
+template <typename T, int CW>
+__device__ __forceinline__ void store_column(uint8_t* d, int64_t step, const float (&v)[CW], int tokens) {
+#pragma unroll
+  for (int j = 0; j < CW; j += 2) {
+    uint8_t* const d1 = d + step;
+    if constexpr (sizeof(T) == 4) {
+      if (j < tokens) *reinterpret_cast<float*>(d) = v[j];
+      if (j + 1 < tokens) *reinterpret_cast<float*>(d1) = v[j + 1];
+    } else {
+      const uint32_t h = pack2<T>(v[j], v[j + 1]);
+      if (j < tokens) *reinterpret_cast<uint16_t*>(d) = (uint16_t)h;
+      if (j + 1 < tokens) *reinterpret_cast<uint16_t*>(d1) = (uint16_t)(h >> 16);
+    }
+    d = d1 + step;
+  }
+}
+
 template <int CG, int BN, typename T, bool FUSE>
 __global__ void __launch_bounds__(threads_for(FUSE), 1)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channels x K
@@ -224,7 +246,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
   if (threadIdx.x == 0) {
     prefetch_tmap(&tmap_w);
     prefetch_tmap(&tmap_t);
-    if (p.stg_bufs > 0) prefetch_tmap(&tmap_d);
+    if (p.tma_store) prefetch_tmap(&tmap_d);
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(full_bar + 8u * s, 1);
       mbar_init(empty_bar + 8u * s, 1);
@@ -421,7 +443,9 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         __syncwarp();
       }
       const bool ok = __all_sync(0xffffffffu, wait_bar<false>(tfull_bar + 8u * acc, acc_phase, ctl, ROLE_EPILOGUE, acc));
-      if (p.stg_bufs > 0) {
+      if (!p.tma_store) {
+        if (!ok) break;
+      } else {
         // The warps meet at named barriers below, so after an abort all four leave, or none:
         // whichever gave up (here or on a chunk of C) says so before the first barrier, and
         // none can say so again before all have looked.
@@ -430,8 +454,6 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         const bool lost = ld_shared_volatile_u32(lost_flag) != 0u;
         named_bar_sync(1, 128);
         if (lost) break;
-      } else if (!ok) {
-        break;
       }
       tc_fence_after();
       const uint32_t t_row = tmem_base + ((32u * q) << 16) + (uint32_t)(acc * BN);
@@ -496,13 +518,14 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
           const T* c = static_cast<const T*>(p.c) + (int64_t)tc * p.ldc + ch;
           float cv[CW];
 #pragma unroll
-          for (int j = 0; j < CW; ++j) cv[j] = tc + j < p.m ? to_f32(c[j * p.ldc]) : 0.f;
+          for (int j = 0; j < CW; ++j, c += p.ldc) cv[j] = tc + j < p.m ? to_f32(*c) : 0.f;
 #pragma unroll
           for (int j = 0; j < CW; ++j) v[j] += cv[j];
         }
-        if (p.stg_bufs > 0) {
+        if (p.tma_store) {
           const uint32_t b = p.c_staged ? chunk_no % kCBufs : chunk_no & 1u;
           const uint32_t buf = stg + b * p.stg_bytes;
+          const uint32_t at = buf + (uint32_t)(row * (int)sizeof(T));
           if (p.c_staged) {
             if (issuer) {
               bulk_wait_group_read<kCBufs - kCAhead - 1>();     // the buffer that fetch_c takes has been stored
@@ -512,15 +535,12 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
             const bool c_ok = wait_bar<false>(c_bar + 8u * b, (chunk_no / kCBufs) & 1u, ctl, ROLE_EPILOGUE, 0xC0u | b);
             if (!c_ok) st_shared_u32(lost_flag, 1u);
             __syncwarp();
+#pragma unroll
+            for (int j = 0; j < CW; ++j) v[j] += staged<T>(at + (uint32_t)(j * kChannels * (int)sizeof(T)));
           } else {
             if (issuer) bulk_wait_group_read<1>();
             named_bar_sync(1, 128);
           }
-          if (p.c_staged) {
-#pragma unroll
-            for (int j = 0; j < CW; ++j) v[j] += staged<T>(buf + (uint32_t)((j * kChannels + row) * (int)sizeof(T)));
-          }
-          const uint32_t at = buf + (uint32_t)(row * (int)sizeof(T));
 #pragma unroll
           for (int j = 0; j < CW; j += 2) {
             if constexpr (sizeof(T) == 4) {
@@ -540,10 +560,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
           }
           ++chunk_no;
         } else if (ch_ok) {
-          T* d = static_cast<T*>(p.d) + (int64_t)tc * p.ldd + ch;
-#pragma unroll
-          for (int j = 0; j < CW; ++j)
-            if (tc + j < p.m) d[j * p.ldd] = from_f32<T>(v[j]);
+          store_column<T, CW>(static_cast<uint8_t*>(p.d) + ((int64_t)tc * p.ldd + ch) * (int64_t)sizeof(T),
+                              p.ldd * (int64_t)sizeof(T), v, p.m - tc);
         }
       }
       if (++acc == p.num_acc) { acc = 0; acc_phase ^= 1u; }
@@ -552,7 +570,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       // Chunks fetched but not used (only after an abort) must land before the CTA exits.
       for (uint32_t x = chunk_no; x < c_no; ++x) drain_wait(c_bar + 8u * (x % kCBufs), (x / kCBufs) & 1u, 100000000ull);
     }
-    if (issuer && p.stg_bufs > 0) bulk_wait_group<0>();
+    if (issuer && p.tma_store) bulk_wait_group<0>();
     }
   }
 
@@ -668,7 +686,8 @@ int sm_count() {
   return sms;
 }
 
-// CTAs that share a tile of 128 channels, for few tiles.  One SM pulls some 75 of
+// CTAs that share a tile of 128 channels, for few tiles (at most `most_ctas` in all, at least
+// `least_kb` K atoms each).  One SM pulls some 75 of
 // HBM's 6500 bytes per ns, so 64 to 128 CTAs stream at full rate; more than one
 // wave of them, or clusters of 8 (of which the GPU holds 16 at a time or fewer),
 // cost more than they give.  16 tokens, 8192 x 8192: 14.3 us whole, 14.3 split in 2,
@@ -679,18 +698,32 @@ int split_for(int64_t tiles, int64_t kb, int64_t most_ctas, int64_t least_kb) {
   return s;
 }
 
-// Tile and split from the sizes.
+// Tile and split with the least estimated time, in SM cycles.  A K atom costs a CTA
+// what its tensor core needs (2 BN cycles at 8192 int8 multiply-adds a cycle; a pair
+// halves the tokens' rows but not this) or the bytes that it has to pull
+// from L2 at some 64 a cycle, whichever is more; the last tile's epilogue follows, 11
+// cycles a token; a split adds the exchange of the partial tiles.  The order of the
+// candidates' measured times agreed in 18 of 18 problems of 48 to 4096 tokens (512 x 8192
+// x 8192: pairs of 256 tokens 28.3 us, of 128 31.6, single CTAs of 128 37.7, of 64 50.9).
 void choose(const Int8GemmArgs* a, int num_sms, int& cg, int& bn, int& split) {
-  const int64_t cb = (a->n + 127) / 128;
-  if (!bn && !cg && a->m > 128 && ((a->n + 255) / 256) * ((a->m + 255) / 256) * 2 >= num_sms) {
-    cg = 2; bn = 256;
+  static const int kTiles[6][2] = {{1, 16}, {1, 32}, {1, 64}, {1, 128}, {2, 128}, {2, 256}};
+  const int64_t kb = (a->k + kAtom - 1) / kAtom;
+  int64_t best = INT64_MAX;
+  int best_cg = cg ? cg : 1, best_bn = bn ? bn : 128, best_split = split ? split : 1;
+  for (const auto& tile : kTiles) {
+    const int g = tile[0], w = tile[1];
+    if ((cg && g != cg) || (bn && w != bn)) continue;
+    const int64_t tiles = ((a->n + kChannels * g - 1) / (kChannels * g)) * ((a->m + w - 1) / w);
+    const int64_t tensor = 2 * w, load = (kChannels * kAtom + (int64_t)w / g * kAtom) / 64;
+    const int64_t atom = tensor > load ? tensor : load;
+    const int s = split ? split : (g == 1 ? split_for(tiles, kb, 64, 16) : 1);
+    const int64_t slots = num_sms / g, waves = s > 1 ? 1 : (tiles + slots - 1) / slots;
+    const int64_t time = waves * ((kb + s - 1) / s) * atom + 11 * w + (s > 1 ? 3000 : 0);
+    if (time < best) { best = time; best_cg = g; best_bn = w; best_split = s; }
   }
-  if (!cg) cg = 1;
-  if (!bn) bn = cg == 2 ? 256 : a->m <= 16 ? 16 : a->m <= 32 ? 32 : a->m <= 64 ? 64 : 128;
-  if (!split) {
-    split = 1;
-    if (cg == 1) split = split_for(cb * ((a->m + bn - 1) / bn), (a->k + kAtom - 1) / kAtom, 64, 32);
-  }
+  cg = best_cg;
+  bn = best_bn;
+  split = best_split;
 }
 
 // `fused`: the fused form of the linear layer is wanted (the caller has checked that it applies).
@@ -732,8 +765,9 @@ int resolve(const Int8GemmArgs* a, bool fused, Resolved& r) {
   const int cw = r.bn < 32 ? r.bn : 32;
   p.stg_bytes = (uint32_t)(cw * kChannels * e);
   // (A TMA store whose row extent ends inside 16 bytes writes the rest of them too.)
-  p.stg_bufs = r.split == 1 && a->m > 0 && rows_16b(a->d, a->ldd, e) && (a->n * e) % 16 == 0 ? 2 : 0;
-  p.c_staged = p.stg_bufs > 0 && a->c && rows_16b(a->c, a->ldc, e) ? 1 : 0;
+  p.tma_store = r.split == 1 && a->m > 0 && rows_16b(a->d, a->ldd, e) && (a->n * e) % 16 == 0 ? 1 : 0;
+  p.stg_bufs = p.tma_store ? 2 : 0;
+  p.c_staged = p.tma_store && a->c && rows_16b(a->c, a->ldc, e) ? 1 : 0;
   if (p.c_staged) p.stg_bufs = kCBufs;
   const int kb_cta = (p.num_kb + r.split - 1) / r.split;
   const int64_t tok_bytes = fused ? (int64_t)kb_cta * kTokAtom + kTokAtom : 0;
@@ -820,7 +854,7 @@ int launch_product(const Int8GemmArgs& a, const Tokens* tokens, cudaStream_t st,
                         (uint32_t)(r.bn / r.cg), 128)) {
     return GEMM_ERR_CANNOT_IMPLEMENT;
   }
-  if (r.p.stg_bufs > 0) {
+  if (r.p.tma_store) {
     const CUtensorMapDataType t = a.d_type == GEMM_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                 : a.d_type == GEMM_TYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     const uint32_t tokens_box = (uint32_t)(r.bn < 32 ? r.bn : 32);

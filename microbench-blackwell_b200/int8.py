@@ -164,9 +164,15 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _row_bytes(cols: int) -> int:
+    """Row stride of the int8 matrices made here: whole 128-byte lines, which a TMA row of an operand
+    then never straddles (777 x 5000 x 2056: 11.4 us with rows of 2176 bytes, 18.8 with 2064)."""
+    return (max(cols, 1) + 127) & ~127 if cols > 64 else _pad16(max(cols, 1))
+
+
 def empty_int8(rows: int, cols: int, device) -> torch.Tensor:
-    """An int8 matrix whose row stride is a multiple of 16 bytes."""
-    ld = _pad16(max(cols, 1))
+    """An int8 matrix whose row stride is a multiple of 16 bytes (of 128 for more than 64 columns)."""
+    ld = _row_bytes(cols)
     q = torch.empty((rows, ld), dtype=torch.int8, device=device)
     return q if ld == cols else q[:, :cols]
 
@@ -291,7 +297,7 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
     n = w.shape[0]
     sb = _vector(w_scale, "w_scale", n, device)
     d = _output(out, m, n, x.dtype, x)
-    lda = _pad16(max(k, 1))
+    lda = _row_bytes(k)
     q = sa = 0
     if m > 8 or knobs or m * k > 16384:   # else no workspace is needed
         work = x.new_empty((m * (lda + 4) + 16,), dtype=torch.uint8)          # int8 tokens, then their scales
