@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -81,8 +81,7 @@ _NO_DROP = (0.0, 0, 0, 0, 0, 0, 0)
 _U64 = (1 << 64) - 1
 
 
-@dataclass(frozen=True)
-class Dropout:
+class Dropout(NamedTuple):
     """Dropout with probability ``p`` of elements of a matrix with ``row_elems`` columns in
     all, of which the call sees the part that begins at (``row0``, ``col0``): the mask is a
     pure function of (seed, stream_id, (row0 + r) * row_elems + col0 + c), so a rank that owns a
@@ -99,35 +98,39 @@ class Dropout:
     row_elems: int | None = None
 
 
-def _drop_fields(drop: Dropout | None, cols: int, device: torch.device):
-    if drop is None or drop.p == 0.0:
+def _drop_fields(drop: Dropout | None, cols: int, index: int):
+    if drop is None:
         return _NO_DROP
-    seed, word = drop.seed, 0
+    p, seed, stream_id, row0, col0, row_elems = drop
+    if p == 0.0:
+        return _NO_DROP
+    word = 0
     if isinstance(seed, torch.Tensor):
-        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != device:
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.get_device() != index:
             raise ValueError("a seed tensor holds one int64 on the operands' device")
         seed, word = 0, seed.data_ptr()
-    row_elems = drop.col0 + cols if drop.row_elems is None else drop.row_elems
-    return (float(drop.p), seed & _U64, drop.stream_id & _U64, word, drop.row0, drop.col0, row_elems)
+    return (p, seed & _U64, stream_id & _U64, word, row0, col0, col0 + cols if row_elems is None else row_elems)
 
 
-def _matrix(t: torch.Tensor, name: str, dtype=None, shape=None, device=None) -> int:
-    """Check one operand and return its row stride in elements."""
-    if not isinstance(t, torch.Tensor) or len(t.shape) != 2:
-        raise ValueError(f"{name} must be a 2-D tensor")
-    if not t.is_cuda or (device is not None and t.device != device):
+def _matrix(t: torch.Tensor, name: str, dtype=None, shape=None, index: int | None = None) -> int:
+    """Check one operand and return its row stride in elements.  `index`: the device it must be on."""
+    try:
+        (rows, cols), (ld, inner), dev = t.shape, t.stride(), t.get_device()
+    except (AttributeError, ValueError):
+        raise ValueError(f"{name} must be a 2-D tensor") from None
+    if dev < 0 or (index is not None and dev != index):
         raise ValueError(f"{name} must be on the operands' CUDA device")
     if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    rows, cols = t.shape
-    ld, inner = t.stride()
-    if cols > 1 and inner != 1:
+    if shape is not None and (rows, cols) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {(rows, cols)}")
+    if inner != 1 and cols > 1:
         raise ValueError(f"{name} must have unit stride along its last axis")
-    if rows > 1 and ld < cols:
-        raise ValueError(f"{name} has overlapping rows")
-    return ld if rows > 1 else max(cols, 1)
+    if rows > 1:
+        if ld < cols:
+            raise ValueError(f"{name} has overlapping rows")
+        return ld
+    return cols or 1
 
 
 def _floating(t: torch.Tensor, name: str) -> int:
@@ -137,19 +140,23 @@ def _floating(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _int8(t: torch.Tensor, name: str, shape=None, device=None) -> int:
-    ld = _matrix(t, name, torch.int8, shape, device)
-    if t.shape[0] <= 1:
+def _int8(t: torch.Tensor, name: str, shape=None, index: int | None = None) -> int:
+    ld = _matrix(t, name, torch.int8, shape, index)
+    if ld & 15 and t.shape[0] <= 1:
         ld = _pad16(ld)
-    if ld % 16:
+    if ld & 15:
         raise ValueError(f"{name} must have a row stride that is a multiple of 16 bytes")
     return ld
 
 
-def _vector(t: torch.Tensor, name: str, n: int, device, dtype=torch.float32) -> int:
-    if not isinstance(t, torch.Tensor) or t.shape != (n,) or t.device != device or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be a contiguous vector of {n} elements on {device}")
-    if dtype is not None and t.dtype != dtype:
+def _vector(t: torch.Tensor, name: str, n: int, index: int, dtype=torch.float32) -> int:
+    try:
+        (size,), (step,), dev = t.shape, t.stride(), t.get_device()
+    except (AttributeError, ValueError):
+        size = -1
+    if size != n or dev != index or (step != 1 and n > 1):
+        raise ValueError(f"{name} must be a contiguous vector of {n} elements on the operands' device")
+    if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     return t.data_ptr()
 
@@ -172,9 +179,7 @@ def _row_bytes(cols: int) -> int:
 
 def empty_int8(rows: int, cols: int, device) -> torch.Tensor:
     """An int8 matrix whose row stride is a multiple of 16 bytes (of 128 for more than 64 columns)."""
-    ld = _row_bytes(cols)
-    q = torch.empty((rows, ld), dtype=torch.int8, device=device)
-    return q if ld == cols else q[:, :cols]
+    return torch.empty_strided((rows, cols), (_row_bytes(cols), 1), dtype=torch.int8, device=device)
 
 
 def quantize_int8(x: torch.Tensor, *, transpose: bool = False, dropout: Dropout | None = None,
@@ -199,8 +204,8 @@ def quantize_int8(x: torch.Tensor, *, transpose: bool = False, dropout: Dropout 
             raise ValueError("x has no columns")
         args = _QUANT_PACK.pack(_QUANT_PACK.size, code, rows, cols, x.data_ptr(), ldx, q.data_ptr(), q.stride(0),
                                 scale.data_ptr(), 0 if sums is None else sums.data_ptr(), int(transpose), 0,
-                                *_drop_fields(dropout, cols, x.device))
-        rc = lib().gemm_sm100a_quantize_int8(args, _raw_stream(x.device.index))
+                                *_drop_fields(dropout, cols, x.get_device()))
+        rc = lib().gemm_sm100a_quantize_int8(args, _raw_stream(x.get_device()))
         if rc != OK:
             raise GemmError(rc, "gemm_sm100a_quantize_int8")
     return (q, scale) if sums is None else (q, scale, sums)
@@ -209,7 +214,7 @@ def quantize_int8(x: torch.Tensor, *, transpose: bool = False, dropout: Dropout 
 def _output(out, m, n, dtype, like) -> torch.Tensor:
     if out is None:
         return like.new_empty((m, n), dtype=dtype)
-    _matrix(out, "out", dtype, (m, n), like.device)
+    _matrix(out, "out", dtype, (m, n), like.get_device())
     return out
 
 
@@ -222,20 +227,19 @@ def _tiles(knobs):
     return knobs.get("tile_n", 0), knobs.get("cta_group", 0), knobs.get("split_k", 0)
 
 
-def _pack_gemm(code, m, n, k, a, lda, b, ldb, d, residual, a_scale, b_scale, bias, dropout, status, knobs):
-    device = d.device
+def _pack_gemm(index, code, m, n, k, a, lda, b, ldb, d, residual, a_scale, b_scale, bias, dropout, status, knobs):
     ldd = d.stride(0) if m > 1 else max(n, 1)
     c = ldc = 0
     if residual is not None:
-        ldc = _matrix(residual, "residual", d.dtype, (m, n), device)
+        ldc = _matrix(residual, "residual", d.dtype, (m, n), index)
         c = residual.data_ptr()
     bias_ptr = bias_code = 0
     if bias is not None:
         bias_code = _floating(bias, "bias")
-        bias_ptr = _vector(bias, "bias", n, device, None)
+        bias_ptr = _vector(bias, "bias", n, index, None)
     return _GEMM_PACK.pack(_GEMM_PACK.size, code, m, n, k, a, lda, b, ldb, d.data_ptr(), ldd, c, ldc, a_scale, b_scale,
                            bias_ptr, bias_code, *(_tiles(knobs) if knobs else (0, 0, 0)),
-                           *_drop_fields(dropout, n, device), 0 if status is None else status.data_ptr(),
+                           *_drop_fields(dropout, n, index), 0 if status is None else status.data_ptr(),
                            knobs.get("timeout_ms", 0), knobs.get("flags", 0))
 
 
@@ -262,21 +266,23 @@ def gemm_int8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor, b_
     exact, so the result does not depend on the batch or the tile.  ``status``: optional int32
     device word, as in ``gemm_into``.  Knobs: tile_n, cta_group, split_k, timeout_ms, flags."""
     lda = _int8(a, "a")
-    device = a.device
-    ldb = _int8(b, "b", (b.shape[0], a.shape[1]) if isinstance(b, torch.Tensor) and b.dim() == 2 else None, device)
+    index = a.get_device()
     m, k = a.shape
-    n = b.shape[0]
+    ldb = _int8(b, "b", None, index)
+    n, bk = b.shape
+    if bk != k:
+        raise ValueError(f"b must have {k} columns, as a has, got {bk}")
     if out is not None:
         out_dtype = out.dtype
     code = _TYPES.get(out_dtype)
     if code is None:
         raise ValueError("out_dtype must be bfloat16, float16 or float32")
     d = _output(out, m, n, out_dtype, a)
-    sa = 0 if a_scale is None else _vector(a_scale, "a_scale", m, device)
-    sb = 0 if b_scale is None else _vector(b_scale, "b_scale", n, device)
-    args = _pack_gemm(code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, d, residual, sa, sb, bias, dropout,
+    sa = 0 if a_scale is None else _vector(a_scale, "a_scale", m, index)
+    sb = 0 if b_scale is None else _vector(b_scale, "b_scale", n, index)
+    args = _pack_gemm(index, code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, d, residual, sa, sb, bias, dropout,
                       status, knobs)
-    rc = lib().gemm_sm100a_int8_launch(args, _raw_stream(device.index))
+    rc = lib().gemm_sm100a_int8_launch(args, _raw_stream(index))
     if rc != OK:
         _raise(rc, args, "gemm_sm100a_int8_launch")
     return d
@@ -291,11 +297,13 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
     ``x`` (m, k); ``w`` (n, k) int8 and ``w_scale`` (n) as ``quantize_int8`` makes them."""
     code = _floating(x, "x")
     ldx = _matrix(x, "x")
-    device = x.device
+    index = x.get_device()
     m, k = x.shape
-    ldw = _int8(w, "w", (w.shape[0], k) if isinstance(w, torch.Tensor) and w.dim() == 2 else None, device)
-    n = w.shape[0]
-    sb = _vector(w_scale, "w_scale", n, device)
+    ldw = _int8(w, "w", None, index)
+    n, wk = w.shape
+    if wk != k:
+        raise ValueError(f"w must have {k} columns, as x has, got {wk}")
+    sb = _vector(w_scale, "w_scale", n, index)
     d = _output(out, m, n, x.dtype, x)
     lda = _row_bytes(k)
     q = sa = 0
@@ -303,8 +311,8 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
         work = x.new_empty((m * (lda + 4) + 16,), dtype=torch.uint8)          # int8 tokens, then their scales
         q = work.data_ptr()
         sa = q + m * lda
-    args = _pack_gemm(code, m, n, k, q, lda, w.data_ptr(), ldw, d, residual, sa, sb, bias, dropout, status, knobs)
-    rc = lib().gemm_sm100a_int8_linear(args, x.data_ptr(), code, ldx, _raw_stream(device.index))
+    args = _pack_gemm(index, code, m, n, k, q, lda, w.data_ptr(), ldw, d, residual, sa, sb, bias, dropout, status, knobs)
+    rc = lib().gemm_sm100a_int8_linear(args, x.data_ptr(), code, ldx, _raw_stream(index))
     if rc != OK:
         _raise(rc, args, "gemm_sm100a_int8_linear")
     return d
@@ -325,14 +333,14 @@ def linear_int8_backward(dy: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, wt
     _matrix(dy, "dy")
     _floating(x, "x")
     m, n = dy.shape
-    _matrix(x, "x", dy.dtype, (m, x.shape[1]) if x.dim() == 2 else None, dy.device)
+    _matrix(x, "x", dy.dtype, (m, x.shape[1]) if x.dim() == 2 else None, dy.get_device())
     k = x.shape[1]
     if m > MAX_INT8_K or n > MAX_INT8_K:
         raise GemmError(ERR_CANNOT_IMPLEMENT, f"linear_int8_backward: sums over m and n are exact up to {MAX_INT8_K}")
     if dw_dtype not in _TYPES:
         raise ValueError("dw_dtype must be bfloat16, float16 or float32")
-    _int8(wt, "wt", (k, n), dy.device)
-    _vector(wt_scale, "wt_scale", k, dy.device)
+    _int8(wt, "wt", (k, n), dy.get_device())
+    _vector(wt_scale, "wt_scale", k, dy.get_device())
     if m == 0:
         return (torch.empty((0, k), dtype=x.dtype, device=x.device),
                 torch.zeros((n, k), dtype=dw_dtype, device=x.device),
@@ -351,16 +359,17 @@ def dropout(x: torch.Tensor, drop: Dropout, *, residual: torch.Tensor | None = N
     is the same call on dy without the residual.  ``out`` may be x or residual."""
     code = _floating(x, "x")
     ldx = _matrix(x, "x")
+    index = x.get_device()
     rows, cols = x.shape
-    y = _output(out, rows, cols, x.dtype, x)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else _output(out, rows, cols, x.dtype, x)
     ldy = y.stride(0) if rows > 1 else max(cols, 1)
     r = ldr = 0
     if residual is not None:
-        ldr = _matrix(residual, "residual", x.dtype, (rows, cols), x.device)
+        ldr = _matrix(residual, "residual", x.dtype, (rows, cols), index)
         r = residual.data_ptr()
     args = _DROPOUT_PACK.pack(_DROPOUT_PACK.size, code, rows, cols, x.data_ptr(), ldx, r, ldr, y.data_ptr(), ldy,
-                              *_drop_fields(drop, cols, x.device))
-    rc = lib().gemm_sm100a_dropout(args, _raw_stream(x.device.index))
+                              *_drop_fields(drop, cols, index))
+    rc = lib().gemm_sm100a_dropout(args, _raw_stream(index))
     if rc != OK:
         raise GemmError(rc, "gemm_sm100a_dropout")
     return y
