@@ -379,6 +379,40 @@ typedef struct Int8QuantArgs {
 int gemm_sm100a_quantize_int8(const Int8QuantArgs* args, void* stream);
 
 /*
+ * Gradients of y = residual + dropout(x . w^T + bias) for dY, by int8 products (the
+ * straight-through gradient of the quantised layer):
+ *   dZ = dropout(dY), dX = dZ . W, dW = dZ^T . X, dbias = column sums of dZ (fp32)
+ * dY m x n, X and dX m x k of `type`; wt k x n int8 and wt_scale (k): W quantised
+ * with transpose = 1; dW n x k of dw_type.  dx, dw and dbias may each be NULL (not
+ * wanted; wt is read for dx only, x for dw only).  m, n <= 131071 (sums over them).
+ * workspace: gemm_sm100a_int8_backward_workspace(m, n, k) bytes, 16-byte aligned,
+ * of this call alone until it has run.  m = 0 sets dW and dbias to 0.  Refusals come before the first
+ * launch.  Asynchronous, capturable.
+ */
+typedef struct Int8BackwardArgs {
+  uint32_t struct_size;    /* sizeof(Int8BackwardArgs) */
+  int32_t  type;           /* GEMM_TYPE_*: dY, X and dX */
+  int64_t  m, n, k;
+  const void* dy;  int64_t lddy;
+  const void* x;   int64_t ldx;
+  const void* wt;  int64_t ldwt;
+  const float* wt_scale;
+  void*    dx;     int64_t lddx;
+  void*    dw;     int64_t lddw;
+  float*   dbias;
+  int32_t  dw_type;        /* GEMM_TYPE_* */
+  int32_t  reserved;       /* 0 */
+  void*    workspace;  int64_t workspace_bytes;
+  DropoutArgs drop;
+  int32_t* status;         /* optional, as in Int8GemmArgs */
+} Int8BackwardArgs;
+
+/* Bytes of workspace, -1 for sizes that are refused. */
+int64_t gemm_sm100a_int8_backward_workspace(int64_t m, int64_t n, int64_t k);
+
+int gemm_sm100a_int8_linear_backward(const Int8BackwardArgs* args, void* stream);
+
+/*
  * Y = residual + dropout(X), rows x cols row-major with their own row strides
  * (elements), all of one type, any alignment of that type; computed in fp32 and
  * rounded once.  Its gradient is the same call on dY without the residual.

@@ -71,6 +71,7 @@ EXPORTED = (
     "gemm_sm100a_generate", "gemm_sm100a_generate_nvfp4", "gemm_sm100a_umma_peak",
     "gemm_sm100a_tma_read_probe",
     "gemm_sm100a_int8_query", "gemm_sm100a_int8_launch", "gemm_sm100a_int8_linear",
+    "gemm_sm100a_int8_backward_workspace", "gemm_sm100a_int8_linear_backward",
     "gemm_sm100a_quantize_int8", "gemm_sm100a_dropout",
 )
 
@@ -120,6 +121,10 @@ def lib():
         L.gemm_sm100a_int8_launch.argtypes = [C.c_char_p, vp]
         L.gemm_sm100a_int8_linear.restype = C.c_int
         L.gemm_sm100a_int8_linear.argtypes = [C.c_char_p, vp, i32, i64, vp]
+        L.gemm_sm100a_int8_backward_workspace.restype = i64
+        L.gemm_sm100a_int8_backward_workspace.argtypes = [i64, i64, i64]
+        L.gemm_sm100a_int8_linear_backward.restype = C.c_int
+        L.gemm_sm100a_int8_linear_backward.argtypes = [C.c_char_p, vp]
         L.gemm_sm100a_quantize_int8.restype = C.c_int
         L.gemm_sm100a_quantize_int8.argtypes = [C.c_char_p, vp]
         L.gemm_sm100a_dropout.restype = C.c_int
@@ -301,5 +306,5 @@ def sf_bytes(rows: int, cols: int) -> int:
 
 
 from .torch_api import Operands, make_operands, gemm, gemm_into, flops  # noqa: E402,F401
-from .int8 import (Dropout, DropoutArgs, DropoutOpArgs, Int8GemmArgs, Int8QuantArgs, MAX_INT8_K,  # noqa: E402,F401
+from .int8 import (Dropout, DropoutArgs, DropoutOpArgs, Int8BackwardArgs, Int8GemmArgs, Int8QuantArgs, MAX_INT8_K,  # noqa: E402,F401
                    dropout, empty_int8, gemm_int8, linear_int8, linear_int8_backward, quantize_int8, query_int8)

@@ -60,6 +60,23 @@ class Int8QuantArgs(C.Structure):
     ]
 
 
+class Int8BackwardArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("type", C.c_int32),
+        ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64),
+        ("dy", C.c_void_p), ("lddy", C.c_int64),
+        ("x", C.c_void_p), ("ldx", C.c_int64),
+        ("wt", C.c_void_p), ("ldwt", C.c_int64),
+        ("wt_scale", C.c_void_p),
+        ("dx", C.c_void_p), ("lddx", C.c_int64),
+        ("dw", C.c_void_p), ("lddw", C.c_int64),
+        ("dbias", C.c_void_p), ("dw_type", C.c_int32), ("reserved", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("drop", DropoutArgs),
+        ("status", C.c_void_p),
+    ]
+
+
 class DropoutOpArgs(C.Structure):
     _fields_ = [
         ("struct_size", C.c_uint32), ("type", C.c_int32),
@@ -76,6 +93,7 @@ class DropoutOpArgs(C.Structure):
 _DROP = "dQQPqqq"
 _GEMM_PACK = struct.Struct("@IiqqqPqPqPqPqPPPiiii" + _DROP + "PII")
 _QUANT_PACK = struct.Struct("@IiqqPqPqPPii" + _DROP)
+_BACKWARD_PACK = struct.Struct("@IiqqqPqPqPqPPqPqPiiPq" + _DROP + "P")
 _DROPOUT_PACK = struct.Struct("@IiqqPqPqPq" + _DROP)
 _NO_DROP = (0.0, 0, 0, 0, 0, 0, 0)
 _U64 = (1 << 64) - 1
@@ -319,7 +337,8 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
 
 
 def linear_int8_backward(dy: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, wt_scale: torch.Tensor, *,
-                         dropout: Dropout | None = None, dw_dtype: torch.dtype = torch.float32):
+                         dropout: Dropout | None = None, dw_dtype: torch.dtype = torch.float32,
+                         status: torch.Tensor | None = None):
     """Gradients (dx, dw, dbias) of y = residual + dropout(x . w^T + bias) for ``dy`` (m, n), by
     int8 products (the straight-through gradient of the quantised layer):
 
@@ -329,27 +348,34 @@ def linear_int8_backward(dy: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, wt
     ``quantize_int8(w, transpose=True)``: the products contract over n and m, so the scales lie
     along the other axis.  dx has x's type, dw ``dw_dtype``, dbias is fp32.  The residual's
     gradient is dy.  m = 0 gives zeros for dw and dbias."""
-    _floating(dy, "dy")
-    _matrix(dy, "dy")
-    _floating(x, "x")
+    code = _floating(dy, "dy")
+    lddy = _matrix(dy, "dy")
+    index = dy.get_device()
     m, n = dy.shape
-    _matrix(x, "x", dy.dtype, (m, x.shape[1]) if x.dim() == 2 else None, dy.get_device())
-    k = x.shape[1]
-    if m > MAX_INT8_K or n > MAX_INT8_K:
-        raise GemmError(ERR_CANNOT_IMPLEMENT, f"linear_int8_backward: sums over m and n are exact up to {MAX_INT8_K}")
-    if dw_dtype not in _TYPES:
+    _floating(x, "x")
+    ldx = _matrix(x, "x", dy.dtype, None, index)
+    xm, k = x.shape
+    if xm != m:
+        raise ValueError(f"x must have {m} rows, as dy has, got {xm}")
+    dw_code = _TYPES.get(dw_dtype)
+    if dw_code is None:
         raise ValueError("dw_dtype must be bfloat16, float16 or float32")
-    _int8(wt, "wt", (k, n), dy.get_device())
-    _vector(wt_scale, "wt_scale", k, dy.get_device())
-    if m == 0:
-        return (torch.empty((0, k), dtype=x.dtype, device=x.device),
-                torch.zeros((n, k), dtype=dw_dtype, device=x.device),
-                torch.zeros((n,), dtype=torch.float32, device=x.device))
-    zt, zt_scale, dbias = quantize_int8(dy, transpose=True, dropout=dropout, column_sums=True)
-    z, z_scale = quantize_int8(dy, dropout=dropout)
-    dx = gemm_int8(z, z_scale, wt, wt_scale, out_dtype=x.dtype)
-    xt, xt_scale = quantize_int8(x, transpose=True)
-    dw = gemm_int8(zt, zt_scale, xt, xt_scale, out_dtype=dw_dtype)
+    ldwt = _int8(wt, "wt", (k, n), index)
+    scale = _vector(wt_scale, "wt_scale", k, index)
+    need = lib().gemm_sm100a_int8_backward_workspace(m, n, k)
+    if need < 0:
+        raise GemmError(ERR_CANNOT_IMPLEMENT, f"linear_int8_backward: sums over m and n are exact up to {MAX_INT8_K}")
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dw = x.new_empty((n, k), dtype=dw_dtype)
+    dbias = x.new_empty((n,), dtype=torch.float32)
+    work = x.new_empty((need,), dtype=torch.uint8)
+    args = _BACKWARD_PACK.pack(_BACKWARD_PACK.size, code, m, n, k, dy.data_ptr(), lddy, x.data_ptr(), ldx, wt.data_ptr(),
+                               ldwt, scale, dx.data_ptr(), k, dw.data_ptr(), k, dbias.data_ptr(), dw_code, 0,
+                               work.data_ptr(), need, *_drop_fields(dropout, n, index),
+                               0 if status is None else status.data_ptr())
+    rc = lib().gemm_sm100a_int8_linear_backward(args, _raw_stream(index))
+    if rc != OK:
+        raise GemmError(rc, "gemm_sm100a_int8_linear_backward")
     return dx, dw, dbias
 
 

@@ -26,6 +26,7 @@ def test_packed_layouts_match_the_structs(pkg):
     assert i8._GEMM_PACK.size == C.sizeof(pkg.Int8GemmArgs)
     assert i8._QUANT_PACK.size == C.sizeof(pkg.Int8QuantArgs)
     assert i8._DROPOUT_PACK.size == C.sizeof(pkg.DropoutOpArgs)
+    assert i8._BACKWARD_PACK.size == C.sizeof(pkg.Int8BackwardArgs)
     packed = i8._GEMM_PACK.pack(208, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18, 19, 20,
                                 0.5, 21, 22, 23, 24, 25, 26, 27, 28, 29)
     s = pkg.Int8GemmArgs.from_buffer_copy(packed)
@@ -80,6 +81,7 @@ def test_null_argument_blocks(pkg):
     assert L.gemm_sm100a_int8_launch(None, None) == pkg.ERR_BAD_ARGS
     assert L.gemm_sm100a_quantize_int8(None, None) == pkg.ERR_BAD_ARGS
     assert L.gemm_sm100a_dropout(None, None) == pkg.ERR_BAD_ARGS
+    assert L.gemm_sm100a_int8_linear_backward(None, None) == pkg.ERR_BAD_ARGS
 
 
 def test_empty_products_launch_nothing(pkg):
@@ -116,6 +118,44 @@ def _quant(pkg, **kw):
 def test_refused_quantisations(pkg, kw):
     rc = pkg.lib().gemm_sm100a_quantize_int8(bytes(_quant(pkg, **kw)), None)
     assert rc in (pkg.ERR_BAD_ARGS, pkg.ERR_CANNOT_IMPLEMENT)
+
+
+def _backward(pkg, **kw):
+    a = pkg.Int8BackwardArgs()
+    a.struct_size = C.sizeof(pkg.Int8BackwardArgs)
+    base = dict(type=0, m=8, n=32, k=48, dy=0x10000, lddy=32, x=0x20000, ldx=48, wt=0x30000, ldwt=32, wt_scale=0x40000,
+                dx=0x50000, lddx=48, dw=0x60000, lddw=48, dbias=0x70000, dw_type=2, workspace=0x80000,
+                workspace_bytes=1 << 20)
+    base.update(kw)
+    for name, v in base.items():
+        if name.startswith("drop_"):
+            setattr(a.drop, name[5:], v)
+        else:
+            setattr(a, name, v)
+    return a
+
+
+def test_backward_workspace(pkg):
+    size = pkg.lib().gemm_sm100a_int8_backward_workspace
+    assert size(8, 32, 48) >= 8 * 32 + 32 * 8 + 48 * 8 + 4 * (8 + 32 + 48)
+    assert size(131071, 131071, 1) > 0
+    assert size(131072, 1, 1) == -1 and size(1, 131072, 1) == -1 and size(-1, 1, 1) == -1
+
+
+@pytest.mark.parametrize("kw", [
+    dict(struct_size=4), dict(type=3), dict(dw_type=-1), dict(m=-1), dict(n=0), dict(k=0), dict(m=131072), dict(n=131072),
+    dict(dy=None), dict(x=None), dict(wt=None), dict(wt_scale=None), dict(workspace=None), dict(workspace_bytes=100),
+    dict(dy=0x10001), dict(x=0x20001), dict(wt=0x30008), dict(dx=0x50001), dict(dw=0x60002), dict(dbias=0x70002),
+    dict(workspace=0x80008), dict(lddy=31), dict(ldx=47), dict(ldwt=31), dict(ldwt=40), dict(lddx=47), dict(lddw=47),
+    dict(drop_p=1.5), dict(drop_p=0.5, drop_row_elems=8),
+])
+def test_refused_backward_passes(pkg, kw):
+    rc = pkg.lib().gemm_sm100a_int8_linear_backward(bytes(_backward(pkg, **kw)), None)
+    assert rc in (pkg.ERR_BAD_ARGS, pkg.ERR_CANNOT_IMPLEMENT)
+
+
+def test_a_backward_pass_of_nothing_launches_nothing(pkg):
+    assert pkg.lib().gemm_sm100a_int8_linear_backward(bytes(_backward(pkg, dx=None, dw=None, dbias=None)), None) == pkg.OK
 
 
 def _drop(pkg, **kw):

@@ -481,6 +481,35 @@ def test_backward_is_near_the_gradient_of_the_linear_map(pkg, cuda):
         assert abs(db[i].item() - (f(x, w, b) - f(x, w, -b)).item()) <= 100 * U32 * dy.abs().sum(0)[i]
 
 
+@pytest.mark.parametrize("wanted", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1)])
+def test_backward_of_some_gradients(pkg, cuda, wanted):
+    """NULL outputs are not computed; the others have the same bits, and nothing else is written."""
+    m, n, k = 50, 70, 90
+    dy, x = normal((m, n), 1), normal((m, k), 2)
+    wt, wts = pkg.quantize_int8(normal((n, k), 3, scale=0.02), transpose=True)
+    full = pkg.linear_int8_backward(dy, x, wt, wts)
+    out = [torch.full((m + 1, k + 3), 5.0, device="cuda"), torch.full((n + 1, k + 3), 5.0, device="cuda"),
+           torch.full((n + 1,), 5.0, device="cuda")]
+    need = pkg.lib().gemm_sm100a_int8_backward_workspace(m, n, k)
+    work = torch.full((need + 64,), 77, dtype=torch.uint8, device="cuda")
+    a = pkg.Int8BackwardArgs(struct_size=0, type=2, m=m, n=n, k=k, dy=dy.data_ptr(), lddy=n,
+                             x=x.data_ptr() if wanted[1] else None, ldx=k, wt=wt.data_ptr() if wanted[0] else None,
+                             ldwt=wt.stride(0), wt_scale=wts.data_ptr() if wanted[0] else None, lddx=k + 3, lddw=k + 3,
+                             dw_type=2, workspace=work.data_ptr(), workspace_bytes=need)
+    import ctypes
+    a.struct_size = ctypes.sizeof(a)
+    for name, want, o in zip(("dx", "dw", "dbias"), wanted, out):
+        setattr(a, name, o.data_ptr() if want else None)
+    assert pkg.lib().gemm_sm100a_int8_linear_backward(bytes(a), torch.cuda.current_stream().cuda_stream) == pkg.OK
+    for want, o, f in zip(wanted, out, full):
+        part = o[tuple(slice(0, s) for s in f.shape)]
+        if want:
+            assert torch.equal(part, f)
+            part.fill_(5.0)
+        assert (o == 5.0).all()
+    assert (work[need:] == 77).all()
+
+
 def test_backward_of_no_tokens(pkg, cuda):
     wt, wts = pkg.quantize_int8(normal((20, 30), 3), transpose=True)
     dx, dw, db = pkg.linear_int8_backward(torch.empty((0, 20), device="cuda"), torch.empty((0, 30), device="cuda"), wt, wts)
