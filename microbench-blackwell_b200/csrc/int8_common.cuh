@@ -205,7 +205,7 @@ __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
 
 constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it leaves the nearest integer in the low byte
 
-// Low byte: q of one element.
+// Low byte: q of an element.
 //  16-bit x: 127 x g is exact in fp32 and one correction step gives the
 //    quotient t to one unit in the last place, exactly where it is a tie.  With
 //    significands of 18 and 11 bits a t >= 1/4 that is not half-way between
@@ -213,21 +213,48 @@ constexpr float kRound = 12582912.f;   // 1.5 * 2^23: adding it leaves the neare
 //  fp32 x: f is an integer with f - eps <= t <= f + 1 + eps for the quotient t;
 //    the sign of 127 x g - a (f + 1/2), whose first term is held as yh + yl and
 //    whose fused difference is exact near zero, says whether t rounds to f + 1.
+// Two elements at a time, each with its row's scale, in packed fp32 operations.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ void get(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+struct RowScale2 {
+  F2 c, na, ra;   // 127 * g, -amax * g, 1 / (amax * g) of both
+  __device__ __forceinline__ RowScale2(const RowScale& s0, const RowScale& s1) : c(s0.c, s1.c), na(-s0.a, -s1.a), ra(s0.ra, s1.ra) {}
+};
+
 template <typename T>
-__device__ __forceinline__ uint32_t quantize_one(float x, const RowScale& s) {
+__device__ __forceinline__ void quantize_two(float x0, float x1, const RowScale2& s, uint32_t& q0, uint32_t& q1) {
+  const F2 x(x0, x1), round(kRound, kRound);
+  const F2 y = mul2(x, s.c);
+  float m0, m1;
   if constexpr (sizeof(T) == 2) {
-    const float y = x * s.c;
-    const float t = y * s.ra;
-    const float r = fmaf(-s.a, t, y);
-    return __float_as_uint(fmaf(r, s.ra, t) + kRound);
+    const F2 t = mul2(y, s.ra);
+    const F2 r = fma2(s.na, t, y);
+    add2(fma2(r, s.ra, t), round).get(m0, m1);
+    q0 = __float_as_uint(m0);
+    q1 = __float_as_uint(m1);
   } else {
-    const float yh = x * s.c;
-    const float yl = fmaf(x, s.c, -yh);
-    const float m = fmaf(yh, s.ra, -0.5f) + kRound;
-    const float f = m - kRound;
-    const float d = fmaf(-s.a, f + 0.5f, yh) + yl;
-    const uint32_t q = __float_as_uint(m);
-    return q + ((d > 0.f || (d == 0.f && (q & 1u))) ? 1u : 0u);
+    float y0, y1, d0, d1;
+    y.get(y0, y1);
+    const F2 yl = fma2(x, s.c, F2(-y0, -y1));
+    const F2 m = add2(fma2(y, s.ra, F2(-0.5f, -0.5f)), round);
+    const F2 f = add2(m, F2(-kRound, -kRound));
+    add2(fma2(s.na, add2(f, F2(0.5f, 0.5f)), y), yl).get(d0, d1);
+    m.get(m0, m1);
+    q0 = __float_as_uint(m0);
+    q1 = __float_as_uint(m1);
+    q0 += d0 > 0.f || (d0 == 0.f && (q0 & 1u)) ? 1u : 0u;
+    q1 += d1 > 0.f || (d1 == 0.f && (q1 & 1u)) ? 1u : 0u;
   }
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -261,11 +288,13 @@ __device__ __forceinline__ uint32_t vec_magnitude(const Vec<T>& v) {
 // The int8 values of a vector, four to a word.
 template <typename T>
 __device__ __forceinline__ void quantize_vec(const Vec<T>& v, const RowScale& s, uint32_t (&w)[Vec<T>::N / 4]) {
+  const RowScale2 s2(s, s);
 #pragma unroll
   for (int j = 0; j < Vec<T>::N / 4; ++j) {
-    w[j] = pack4(quantize_one<T>(v.get(4 * j), s), quantize_one<T>(v.get(4 * j + 1), s),
-                 quantize_one<T>(v.get(4 * j + 2), s), quantize_one<T>(v.get(4 * j + 3), s));
-    if (s.c == 0.f) w[j] = 0u;
+    uint32_t q[4];
+    quantize_two<T>(v.get(4 * j), v.get(4 * j + 1), s2, q[0], q[1]);
+    quantize_two<T>(v.get(4 * j + 2), v.get(4 * j + 3), s2, q[2], q[3]);
+    w[j] = s.c == 0.f ? 0u : pack4(q[0], q[1], q[2], q[3]);
   }
 }
 

@@ -167,24 +167,28 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
   const int n_valid = (int)max((int64_t)0, min((int64_t)V, p.cols - c));
   const T* const x = static_cast<const T*>(p.x) + row0 * p.ldx;
   const uint32_t held_s = sm100::smem_u32(held);
+  const uint32_t own_s = held_s + (uint32_t)(held_at(lane_r) + lane_c * 16);   // this thread's first 16 bytes
+  constexpr uint32_t kPass = (RPP + RPP / 16) * kStripBytes;                     // and RPP rows on
+  const int64_t pass_elems = RPP * p.ldx;
   // Rows [b * rows_held, ..) of this CTA into shared memory; every thread waits for
   // what it has copied itself, and masks it.
   auto fetch = [&](int b) {
     const int first = b * p.rows_held, n = min(n_rows - first, p.rows_held);
-    for (int r = lane_r; r < n; r += RPP) {
-      const uint32_t dst = held_s + (uint32_t)(held_at(r) + lane_c * 16);
-      const T* src = x + (int64_t)(first + r) * p.ldx + c;
-      if (p.wide) {
-        sm100::cp_async_16(dst, n_valid > 0 ? src : x, (uint32_t)(n_valid * (int)sizeof(T)));
-      } else {
+    const T* src = x + (int64_t)(first + lane_r) * p.ldx + (n_valid > 0 ? c : 0);
+    uint32_t dst = own_s;
+    if (p.wide) {
+      for (int r = lane_r; r < n; r += RPP, dst += kPass, src += pass_elems)
+        sm100::cp_async_16(dst, src, (uint32_t)(n_valid * (int)sizeof(T)));
+    } else {
+      for (int r = lane_r; r < n; r += RPP, dst += kPass, src += pass_elems) {
         const Vec<T> v = load_vec<T>(src, n_valid, false);
         sm100::st_shared_v4(dst, v.w[0], v.w[1], v.w[2], v.w[3]);
       }
     }
     sm100::cp_async_wait_all();
     if constexpr (DROP) {
-      for (int r = lane_r; r < n; r += RPP) {
-        const uint32_t at = held_s + (uint32_t)(held_at(r) + lane_c * 16);
+      uint32_t at = own_s;
+      for (int r = lane_r; r < n; r += RPP, at += kPass) {
         const uint4 u = sm100::ld_shared_v4(at);
         Vec<T> v;
         v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
@@ -205,8 +209,9 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
   for (int b = 0; b < batches; ++b) {
     fetch(b);
     const int n = min(n_rows - b * p.rows_held, p.rows_held);
-    for (int r = lane_r; r < n; r += RPP) {
-      const uint4 u = sm100::ld_shared_v4(held_s + (uint32_t)(held_at(r) + lane_c * 16));
+    uint32_t at = own_s;
+    for (int r = lane_r; r < n; r += RPP, at += kPass) {
+      const uint4 u = sm100::ld_shared_v4(at);
       Vec<T> v;
       v.w[0] = u.x; v.w[1] = u.y; v.w[2] = u.z; v.w[3] = u.w;
 #pragma unroll
@@ -275,6 +280,7 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
   sm100::cluster_arrive_relaxed();   // this CTA has read its peers' results; waited for at the end
   const int pair = lane % PAIRS, set = lane / PAIRS;
   const RowScale q0 = scales[2 * pair], q1 = scales[2 * pair + 1];
+  const RowScale2 q01(q0, q1);
   const int64_t c0 = col0 + 2 * pair;
   // The last batch is still in shared memory; earlier ones are read again (from L2).
   for (int b = batches - 1; b >= 0; --b) {
@@ -284,9 +290,11 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
       fetch(b);
       __syncthreads();
     }
-    for (int g = (warp * SETS + set) * 16; g < n; g += kColWarps * SETS * 16) {
+    constexpr int kStep = kColWarps * SETS * 16;     // rows that the block rounds at once
+    uint32_t at = held_s + (uint32_t)(held_at((warp * SETS + set) * 16) + pair * 2 * (int)sizeof(T));
+    uint8_t* qa = p.q + c0 * p.ldq + row0 + first + (warp * SETS + set) * 16;
+    for (int g = (warp * SETS + set) * 16; g < n; g += kStep, at += kStep / 16 * 17 * kStripBytes, qa += kStep) {
       uint32_t w0[4], w1[4];
-      const uint32_t at = held_s + (uint32_t)(held_at(g) + pair * 2 * (int)sizeof(T));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t b0[4], b1[4];
@@ -303,15 +311,13 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
             f0 = v.get(0);
             f1 = v.get(1);
           }
-          b0[j] = quantize_one<T>(f0, q0);
-          b1[j] = quantize_one<T>(f1, q1);
+          quantize_two<T>(f0, f1, q01, b0[j], b1[j]);
         }
         w0[k] = q0.c == 0.f ? 0u : pack4(b0[0], b0[1], b0[2], b0[3]);
         w1[k] = q1.c == 0.f ? 0u : pack4(b1[0], b1[1], b1[2], b1[3]);
       }
-      auto store = [&](int64_t col, const uint32_t (&w)[4]) {
+      auto store = [&](int64_t col, uint8_t* q, const uint32_t (&w)[4]) {
         if (col >= p.cols) return;
-        uint8_t* q = p.q + col * p.ldq + row0 + first + g;
         if (n - g >= 16) {
           *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
@@ -320,8 +326,8 @@ __global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid
             if (g + j < n) q[j] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
         }
       };
-      store(c0, w0);
-      store(c0 + 1, w1);
+      store(c0, qa, w0);
+      store(c0 + 1, qa + p.ldq, w1);
     }
   }
   sm100::cluster_wait();             // until the peers have read this CTA's
