@@ -262,25 +262,42 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     st_shared_u32(lost_flag, 0u);
     fence_mbar_init();
   }
+  if constexpr (CG == 2) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
+  // Until here nothing of this launch depended on the kernels before it, and it holds
+  // no tensor memory while it waits for them (one of them might still need some).
+  grid_dependency_wait();
+  uint32_t tmem_base = 0;
+  auto read_tmem_base = [&]() {
+    tmem_base = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(base_ptr + (tmem_slot - base)), 0);
+  };
   if (warp == 1) {
     tmem_alloc<CG>(tmem_slot, (uint32_t)p.tmem_cols);
     tmem_relinquish<CG>();
+    grid_launch_dependents();   // the next kernel's blocks come after this one's have their tensor memory
   }
-  tc_fence_before();
-  if constexpr (CG == 2) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
-  tc_fence_after();
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu,
-      *reinterpret_cast<volatile uint32_t*>(base_ptr + (tmem_slot - base)), 0);
+  if constexpr (CG == 2) {
+    tc_fence_before();
+    cluster_arrive();
+    cluster_wait();
+    tc_fence_after();
+    read_tmem_base();
+  } else if (warp == 1) {
+    // The loads are on their way meanwhile; only the epilogue waits for the address.
+    __syncwarp();
+    read_tmem_base();
+    tc_fence_before();
+    named_bar_arrive(3, 160);
+  } else if (warp >= 2 && warp < 6) {
+    named_bar_sync(3, 160);
+    tc_fence_after();
+    read_tmem_base();
+  }
 
   SharedCtl ctl;
   ctl.abort_addr = abort_flag;
   ctl.abort_peer = CG == 2 ? mapa_shared(abort_flag, rank ^ 1u) : 0u;
   ctl.timeout_ns = p.timeout_ns;
   ctl.status = p.status;
-
-  // Until here nothing of this launch depended on the kernels before it.
-  grid_dependency_wait();
-  grid_launch_dependents();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer

@@ -35,8 +35,8 @@ struct QuantParams {
 };
 
 // ----------------------------------------------------------------- rows
-// Most threads of a row that keep nv vectors each (32768 16-bit values in all).
-__host__ __device__ constexpr int row_threads(int nv) { return 4096 / nv; }
+// Most threads of a row that keep nv vectors each (32768 16-bit values in all; 16384 for nv = 2).
+__host__ __device__ constexpr int row_threads(int nv) { return nv < 4 ? 1024 : 4096 / nv; }
 
 // A row belongs to blockDim.x threads (a block holds blockDim.y rows); each
 // keeps NV 16-byte vectors in registers between the maximum and the rounding,
@@ -345,9 +345,14 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
   if (blocks > 0x7FFFFFFF) blocks = 0x7FFFFFFF;
   return launch_overlapped(quantize_rows_kernel<T, NV, DROP>, dim3((unsigned)blocks), dim3((unsigned)tx, (unsigned)ry), 0, 1, st, p);
 }
-// The mask's words need registers: half as many vectors per thread with it.
+// Many loads in flight per thread for large X; two where one wave of threads covers
+// it (333 x 1000 fp32 2.1 us, 3.7 with eight; 16384 x 8192 bf16 99 us, 71 with eight).  The
+// mask's words need registers: four with dropout.
 template <typename T>
 cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
+  const int64_t nvec = (p.cols + Vec<T>::N - 1) / Vec<T>::N;
+  if (p.rows * nvec <= 148 * 2048 && nvec <= 2 * row_threads(2))
+    return p.drop.on ? launch_rows<T, 2, true>(p, st) : launch_rows<T, 2, false>(p, st);
   return p.drop.on ? launch_rows<T, 4, true>(p, st) : launch_rows<T, 8, false>(p, st);
 }
 

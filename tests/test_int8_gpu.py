@@ -686,3 +686,123 @@ def test_two_streams_at_once(pkg, cuda):
                 outs.append(pkg.linear_int8(x, w, ws))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_each_call_sees_the_call_before_it(pkg, cuda):
+    """Launches overlap: every operand is written by the kernel just before the one that reads it
+    (weights, tokens, scales, residual, output read by torch), over and over in the same buffers."""
+    m, n, k = 24, 640, 768
+    w = torch.empty((n, k), device="cuda")
+    x = torch.empty((m, k), device="cuda", dtype=torch.bfloat16)
+    ws, xs, outs = [normal((n, k), 10 + i, scale=0.05) for i in range(6)], [normal((m, k), 20 + i, torch.bfloat16) for i in range(6)], []
+    for rows in (m, 2):
+        direct = []
+        for i in range(6):
+            q, s = pkg.quantize_int8(ws[i])
+            torch.cuda.synchronize()
+            y = pkg.linear_int8(xs[i][:rows], q, s)
+            torch.cuda.synchronize()
+            y = pkg.dropout(y, pkg.Dropout(0.5, seed=i))
+            z, zs = pkg.quantize_int8(y, transpose=True)
+            torch.cuda.synchronize()
+            direct.append((y.clone(), z.clone(), zs.clone()))
+        torch.cuda.synchronize()
+        outs = []
+        for _ in range(20):
+            for i in range(6):
+                w.copy_(ws[i])
+                x.copy_(xs[i])
+                q, s = pkg.quantize_int8(w)
+                y = pkg.linear_int8(x[:rows], q, s)
+                pkg.dropout(y, pkg.Dropout(0.5, seed=i), out=y)
+                z, zs = pkg.quantize_int8(y, transpose=True)
+                outs.append((y.clone(), z.clone(), zs.clone()))
+                del q, s, y, z, zs
+        for j, got in enumerate(outs):
+            for a, b in zip(got, direct[j % 6]):
+                assert torch.equal(a, b), (rows, j)
+
+
+def test_capture_across_streams(pkg, cuda):
+    """Calls captured on two streams that fork and join, and a graph whose nodes are other kernels
+    between them."""
+    x = normal((40, 512), 1, torch.bfloat16)
+    wq, ws = pkg.quantize_int8(normal((300, 512), 2, scale=0.05))
+    drop = pkg.Dropout(0.3, seed=1)
+
+    def step(side):
+        main = torch.cuda.current_stream()
+        a = pkg.linear_int8(x, wq, ws)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b = pkg.dropout(a, drop)
+            qb, sb = pkg.quantize_int8(b, transpose=True)
+        c = pkg.linear_int8(x[:3], wq, ws)
+        d = (a * 2).contiguous()
+        main.wait_stream(side)
+        e = pkg.dropout(d, drop, residual=b)
+        return a, b, qb, sb, c, e
+
+    side, stream = torch.cuda.Stream(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = [t.clone() for t in step(side)]
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = step(side)
+    for _ in range(3):
+        for t in out:
+            t.fill_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+    del graph
+
+
+def test_strides_beyond_32_bits(pkg, cuda):
+    """Rows 2^30 elements apart: offsets of 2^31 elements and more in every operand."""
+    m, n, k, far = 3, 150, 160, 2 ** 30
+    big = torch.empty((2 * far + 512,), dtype=torch.bfloat16, device="cuda")
+    big8 = torch.empty((2 * far + 512,), dtype=torch.int8, device="cuda")
+
+    def spread(t, store):
+        v = store.as_strided((t.shape[0], t.shape[1]), (far, 1))
+        v.copy_(t)
+        return v
+
+    x = normal((m, k), 1, torch.bfloat16)
+    q, s = pkg.quantize_int8(x)
+    qt, st = pkg.quantize_int8(x, transpose=True)
+    fx = spread(x, big)
+    for t, want, scale in ((False, q, s), (True, qt, st)):
+        got = pkg.quantize_int8(fx, transpose=t)
+        assert torch.equal(got[0], want) and torch.equal(got[1], scale)
+    drop = pkg.Dropout(0.4, seed=2, row_elems=far)
+    want = pkg.dropout(x, drop)
+    assert torch.equal(pkg.dropout(fx, drop), want)
+    pkg.dropout(fx, drop, out=fx)
+    assert torch.equal(fx, want)
+    w, ws = pkg.quantize_int8(normal((n, k), 3, scale=0.05))
+    y = pkg.gemm_int8(q, s, w, ws)
+    fq = spread(q, big8)
+    assert torch.equal(pkg.gemm_int8(fq, s, w, ws), y)
+    for kn in (dict(), dict(cta_group=2, tile_n=128), dict(cta_group=1, tile_n=16, split_k=2)):
+        out = spread(torch.zeros((m, n), dtype=torch.bfloat16, device="cuda"), big)
+        pkg.gemm_int8(q, s, w, ws, residual=out, out=out, **kn)
+        assert torch.equal(out, y), kn
+    assert torch.equal(pkg.linear_int8(spread(x, big), w, ws), pkg.linear_int8(x, w, ws))
+    w3, ws3 = w[:3], ws[:3]
+    assert torch.equal(pkg.gemm_int8(q, s, spread(w3, big8), ws3), y[:, :3])
+
+
+def test_host_memory_is_refused(pkg, cuda):
+    """A pointer to host memory is an error of the call, before any launch."""
+    L = pkg.lib()
+    host = torch.zeros((64,), dtype=torch.bfloat16)
+    x = normal((2, 16), 1, torch.bfloat16)
+    a = pkg.DropoutOpArgs(struct_size=128, type=0, rows=2, cols=16, x=x.data_ptr(), ldx=16, y=host.data_ptr(), ldy=16)
+    assert L.gemm_sm100a_dropout(bytes(a), torch.cuda.current_stream().cuda_stream) == pkg.ERR_LAUNCH
+    torch.cuda.synchronize()
+    assert torch.equal(pkg.dropout(x, pkg.Dropout(0.0)), x)
