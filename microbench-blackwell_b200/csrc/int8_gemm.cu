@@ -11,7 +11,14 @@
 // write 32 consecutive elements of a row of D.
 //
 // Warp 0 loads 128-byte K atoms by TMA into a ring, warp 1 issues the MMAs,
-// warps 2..5 run the epilogue (one TMEM lane quadrant each).
+// warps 2..5 run the epilogue (one TMEM lane quadrant each; in a pair with a short
+// main loop warps 6..9 take every other chunk).
+//
+// Measured on B200 (1000 W cap): 8192 x 8192 x 8192 in 326 us under ncu, tensor pipe
+// 96.5 % active, 3.37 PFLOP/s; 8192 x 28672 x 8192 back to back 1.39 ms, 2.77 PFLOP/s at the
+// clock that the power cap leaves.  One token x 8192 x 8192 in 14.5 us, 4.6 of
+// the 6.55 TB/s that a copy reaches; about 4 us of it are launch, first loads and last stores
+// (a 1024 x 1024 layer takes 4.7 us in all).
 //   whole-K form   persistent CTAs (CTA pairs for large problems), two
 //                  accumulators, so a tile's epilogue overlaps the next mainloop.
 //   split-K form   for few tiles: the CTAs of a cluster share one tile's K and
@@ -46,13 +53,17 @@ constexpr int kFusedTokens = 8;         // most tokens of the fused form: one 8-
 constexpr int kFusedBN = 16;            // its MMA N, the smallest there is for 128 channels
 constexpr int kStageWarps = 12;         // warps of the fused form that quantise tokens (the epilogue's four among them)
 constexpr int kFusedElems = 16384;      // most tokens x K of the fused form (at most 128 KB of shared memory)
-__host__ __device__ constexpr int threads_for(bool fuse) { return fuse ? 64 + 32 * kStageWarps : 192; }
+constexpr int kMaxGroups = 2;           // epilogue groups of a CTA pair's kernel (four warps each)
+// Most threads of a CTA.
+__host__ __device__ constexpr int threads_for(int cg, bool fuse) {
+  return 64 + (fuse ? 32 * kStageWarps : 128 * (cg == 2 ? kMaxGroups : 1));
+}
 constexpr int kSmemLimit = 232448;      // 227 KiB of opt-in dynamic shared memory per CTA
 constexpr int kBarrierBytes = 1024;
 constexpr int kStaticSmem = 512;        // bound of the static shared memory of the fused form
 constexpr int kMaxStages = 32;
-constexpr int kCBufs = 4;               // staging buffers of an epilogue that reads C by TMA
-constexpr int kCAhead = 2;              // chunks of C on their way ahead of the one in work
+constexpr int kCBufs = 4;               // most staging buffers of an epilogue group that reads C by TMA:
+                                        // all but two hold chunks of C on their way
 constexpr int kAtom = 128;              // bytes (= K elements) of one swizzled K atom
 constexpr uint32_t kTokAtom = 8 * kAtom;  // fused form: bytes of one K atom of the tokens
 constexpr int kChannels = 128;          // channels per CTA
@@ -75,7 +86,9 @@ struct Int8Params {
   uint32_t bars_offset, stg_offset, sa_offset, stg_bytes;
   int32_t stg_bufs;                     // staging buffers (0: D is written from registers)
   int32_t tma_store;                    // D is written from them, by TMA
-  int32_t c_staged;                     // chunks of C are fetched into the staging buffers (kCBufs of them)
+  int32_t groups;                       // epilogue groups: each takes every groups-th chunk of a tile
+  int32_t c_bufs;                       // staging buffers of a group where C is staged
+  int32_t c_staged;                     // chunks of C are fetched into the staging buffers (c_bufs per group)
   int32_t tmem_cols, num_acc;
   int32_t raster;                       // channel blocks per raster group
   uint32_t idesc;
@@ -204,7 +217,7 @@ __device__ __forceinline__ void store_column(uint8_t* d, int64_t step, const flo
 }
 
 template <int CG, int BN, typename T, bool FUSE>
-__global__ void __launch_bounds__(threads_for(FUSE), 1)
+__global__ void __launch_bounds__(threads_for(CG, FUSE), 1)
 int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channels x K
                  const __grid_constant__ CUtensorMap tmap_t,   // tokens x K
                  const __grid_constant__ CUtensorMap tmap_d,   // D, for the staged epilogue
@@ -228,8 +241,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
   const uint32_t tmem_slot = drain_bar + 8u;
   const uint32_t abort_flag = tmem_slot + 4u;
   const uint32_t tok_bar = abort_flag + 4u;              // fused form: the tokens are in place
-  const uint32_t c_bar = tok_bar + 8u;                   // [kCBufs]: a chunk of C is in its buffer
-  const uint32_t lost_flag = c_bar + 8u * kCBufs;        // an epilogue warp has given up a wait
+  const uint32_t c_bar = tok_bar + 8u;                   // [groups][kCBufs]: a chunk of C is in its buffer
+  const uint32_t lost_flag0 = c_bar + 8u * kCBufs * kMaxGroups;   // [groups]: a warp of the group has given up a wait
   __shared__ RowScale tok_rows[FUSE ? kFusedTokens : 1];
   __shared__ uint32_t tok_top[FUSE ? kFusedTokens : 1];
 
@@ -253,13 +266,13 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar + 8u * a, 1);
-      mbar_init(tempty_bar + 8u * a, 4 * CG);
+      mbar_init(tempty_bar + 8u * a, 4 * CG * p.groups);
     }
     mbar_init(drain_bar, 1);
     mbar_init(tok_bar, kStageWarps);
-    for (int b = 0; b < kCBufs; ++b) mbar_init(c_bar + 8u * b, 1);
+    for (int b = 0; b < kCBufs * kMaxGroups; ++b) mbar_init(c_bar + 8u * b, 1);
     st_shared_u32(abort_flag, 0u);
-    st_shared_u32(lost_flag, 0u);
+    for (int g = 0; g < kMaxGroups; ++g) st_shared_u32(lost_flag0 + 4u * g, 0u);
     fence_mbar_init();
   }
   if constexpr (CG == 2) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
@@ -407,10 +420,14 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     // ------------------------------------------------------------ epilogue
     const uint32_t q = warp & 3u;                        // TMEM lane quadrant
     const int row = (int)(32u * q + lane);               // channel within the CTA's 128
-    const uint32_t gtid = (warp - 2u) * 32u + lane;
-    const bool issuer = gtid == 0;
-    const uint32_t stg = base + p.stg_offset;
-    const uint32_t sa_s = base + p.sa_offset + (FUSE ? 0u : q * (uint32_t)(BN * 4));   // this warp's copy of the token scales
+    const uint32_t grp = CG == 2 ? (warp - 2u) >> 2 : 0u;
+    const int groups = CG == 2 ? p.groups : 1;
+    const bool issuer = ((warp - 2u) & 3u) * 32u + lane == 0;
+    const uint32_t bar_id = grp ? 4u : 1u;               // named barrier of the group
+    const uint32_t stg = base + p.stg_offset + grp * (uint32_t)p.stg_bufs * p.stg_bytes;
+    const uint32_t lost_flag = lost_flag0 + 4u * grp;
+    const uint32_t c_full = c_bar + grp * 8u * kCBufs;
+    const uint32_t sa_s = base + p.sa_offset + (FUSE ? 0u : (warp - 2u) * (uint32_t)(BN * 4));   // this warp's copy of the token scales
     const uint32_t leader_tempty = CG == 2 ? mapa_shared(tempty_bar, 0) : tempty_bar;
     const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
     // Rows of an even length that begin at an even index: even channels are the first of a draw's pair.
@@ -419,25 +436,26 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     const uint32_t drop_thr = p.drop.threshold;
     const float drop_grow = p.drop.grow;
     uint32_t chunk_no = 0;
-    // C staged: chunk x of this CTA (over all its tiles) goes through buffer x % kCBufs, is
+    // C staged: chunk x of this group (over all its tiles) goes through buffer x % c_bufs, is
     // replaced there by D, element by element in the same thread, and stored from it.  One
-    // thread fetches kCAhead chunks ahead, also across tiles.
-    int c_u = slot0, c_i = 0;
+    // thread fetches c_bufs - 2 chunks ahead, also across tiles.
+    const uint32_t c_bufs = (uint32_t)p.c_bufs;
+    int c_u = slot0, c_i = (int)grp;
     uint32_t c_no = 0;
     const uint64_t c_policy = policy_evict_normal();
     auto fetch_c = [&]() {
       if (c_u >= p.num_units) return;
       int cb, tb;
       tile_coords(c_u, p, cb, tb);
-      const int buf = (int)(c_no % kCBufs);
-      mbar_arrive_expect_tx(c_bar + 8u * buf, p.stg_bytes);
-      tma_load_2d(stg + (uint32_t)buf * p.stg_bytes, &tmap_c, c_bar + 8u * buf,
+      const uint32_t buf = c_no % c_bufs;
+      mbar_arrive_expect_tx(c_full + 8u * buf, p.stg_bytes);
+      tma_load_2d(stg + buf * p.stg_bytes, &tmap_c, c_full + 8u * buf,
                   (cb * CG + (int)(CG == 2 ? rank : 0u)) * kChannels, tb * BN + c_i * CW, c_policy);
       ++c_no;
-      if (++c_i == NCH) { c_i = 0; c_u += slots; }
+      if ((c_i += groups) >= NCH) { c_i = (int)grp; c_u += slots; }
     };
     if (p.c_staged && issuer) {
-      for (int b = 0; b < kCAhead; ++b) fetch_c();
+      for (uint32_t b = 2; b < c_bufs; ++b) fetch_c();
     }
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -467,9 +485,9 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         // whichever gave up (here or on a chunk of C) says so before the first barrier, and
         // none can say so again before all have looked.
         if (!ok && lane == 0) st_shared_u32(lost_flag, 1u);
-        named_bar_sync(1, 128);
+        named_bar_sync(bar_id, 128);
         const bool lost = ld_shared_volatile_u32(lost_flag) != 0u;
-        named_bar_sync(1, 128);
+        named_bar_sync(bar_id, 128);
         if (lost) break;
       }
       tc_fence_after();
@@ -488,11 +506,11 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         break;   // one tile per cluster; the sum follows the cluster barrier
       }
 #pragma unroll 1
-      for (int i = 0; i < NCH; ++i) {
+      for (int i = (int)grp; i < NCH; i += groups) {
         uint32_t r[CW];
         if constexpr (CW == 32) tmem_ld32(t_row + (uint32_t)(i * CW), r); else tmem_ld16(t_row + (uint32_t)(i * CW), r);
         tmem_ld_wait();
-        if (i == NCH - 1) {
+        if (i + groups >= NCH) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -540,23 +558,23 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
           for (int j = 0; j < CW; ++j) v[j] += cv[j];
         }
         if (p.tma_store) {
-          const uint32_t b = p.c_staged ? chunk_no % kCBufs : chunk_no & 1u;
+          const uint32_t b = p.c_staged ? chunk_no % c_bufs : chunk_no & 1u;
           const uint32_t buf = stg + b * p.stg_bytes;
           const uint32_t at = buf + (uint32_t)(row * (int)sizeof(T));
           if (p.c_staged) {
             if (issuer) {
-              bulk_wait_group_read<kCBufs - kCAhead - 1>();     // the buffer that fetch_c takes has been stored
+              bulk_wait_group_read<1>();     // the buffer that fetch_c takes has been stored
               fetch_c();
             }
             __syncwarp();
-            const bool c_ok = wait_bar<false>(c_bar + 8u * b, (chunk_no / kCBufs) & 1u, ctl, ROLE_EPILOGUE, 0xC0u | b);
+            const bool c_ok = wait_bar<false>(c_full + 8u * b, (chunk_no / c_bufs) & 1u, ctl, ROLE_EPILOGUE, 0xC0u | b);
             if (!c_ok) st_shared_u32(lost_flag, 1u);
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < CW; ++j) v[j] += staged<T>(at + (uint32_t)(j * kChannels * (int)sizeof(T)));
           } else {
             if (issuer) bulk_wait_group_read<1>();
-            named_bar_sync(1, 128);
+            named_bar_sync(bar_id, 128);
           }
 #pragma unroll
           for (int j = 0; j < CW; j += 2) {
@@ -570,7 +588,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
             }
           }
           fence_proxy_async_shared();
-          named_bar_sync(1, 128);
+          named_bar_sync(bar_id, 128);
           if (issuer) {
             if (tc < p.m && c0 < p.n) tma_store_2d(&tmap_d, buf, c0, tc);
             bulk_commit_group();
@@ -585,7 +603,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     }
     if (issuer && p.c_staged) {
       // Chunks fetched but not used (only after an abort) must land before the CTA exits.
-      for (uint32_t x = chunk_no; x < c_no; ++x) drain_wait(c_bar + 8u * (x % kCBufs), (x / kCBufs) & 1u, 100000000ull);
+      for (uint32_t x = chunk_no; x < c_no; ++x) drain_wait(c_full + 8u * (x % c_bufs), (x / c_bufs) & 1u, 100000000ull);
     }
     if (issuer && p.tma_store) bulk_wait_group<0>();
     }
@@ -785,10 +803,15 @@ int resolve(const Int8GemmArgs* a, bool fused, Resolved& r) {
   p.tma_store = r.split == 1 && a->m > 0 && rows_16b(a->d, a->ldd, e) && (a->n * e) % 16 == 0 ? 1 : 0;
   p.stg_bufs = p.tma_store ? 2 : 0;
   p.c_staged = p.tma_store && a->c && rows_16b(a->c, a->ldc, e) ? 1 : 0;
-  if (p.c_staged) p.stg_bufs = kCBufs;
+  p.c_bufs = e == 4 ? 3 : kCBufs;
+  if (p.c_staged) p.stg_bufs = p.c_bufs;
+  // A second epilogue group where the main loop is too short to hide one (4096 x 4096 x 1024: 18.8 us
+  // with two, 22.4 with one; with bias, dropout and residual 43 and 50); its staging buffers cost
+  // the ring a stage, which long main loops need.
+  p.groups = r.cg == 2 && p.num_kb < (p.drop.on || p.c ? 40 : 20) ? 2 : 1;
   const int kb_cta = (p.num_kb + r.split - 1) / r.split;
   const int64_t tok_bytes = fused ? (int64_t)kb_cta * kTokAtom + kTokAtom : 0;
-  const int64_t fixed = 1024 + kBarrierBytes + (int64_t)p.stg_bufs * p.stg_bytes + 4 * r.bn * 4 + tok_bytes + kStaticSmem;
+  const int64_t fixed = 1024 + kBarrierBytes + (int64_t)p.groups * p.stg_bufs * p.stg_bytes + p.groups * 4 * r.bn * 4 + tok_bytes + kStaticSmem;
   r.max_stages = (int)((kSmemLimit - fixed) / p.stage_bytes);
   if (r.max_stages > 12) r.max_stages = 12;
   r.stages = r.max_stages;
@@ -801,8 +824,8 @@ int resolve(const Int8GemmArgs* a, bool fused, Resolved& r) {
   p.tok_offset = p.bars_offset + kBarrierBytes;
   p.stg_offset = p.tok_offset + (uint32_t)tok_bytes;
   p.k = (int32_t)a->k;
-  p.sa_offset = p.stg_offset + (uint32_t)p.stg_bufs * p.stg_bytes;
-  r.smem_bytes = 1024 + (int64_t)p.sa_offset + 4 * r.bn * 4;
+  p.sa_offset = p.stg_offset + (uint32_t)(p.groups * p.stg_bufs) * p.stg_bytes;
+  r.smem_bytes = 1024 + (int64_t)p.sa_offset + p.groups * 4 * r.bn * 4;
   p.status = a->status;
   p.timeout_ns = (uint64_t)(a->timeout_ms ? a->timeout_ms : 4000u) * 1000000ull;
   p.flags = a->flags;
@@ -884,7 +907,7 @@ int launch_product(const Int8GemmArgs& a, const Tokens* tokens, cudaStream_t st,
   KernelFn fn = a.d_type == GEMM_TYPE_BF16 ? pick<__nv_bfloat16>(r.cg, r.bn, tokens != nullptr)
               : a.d_type == GEMM_TYPE_FP16 ? pick<__half>(r.cg, r.bn, tokens != nullptr) : pick<float>(r.cg, r.bn, tokens != nullptr);
   if (!ensure_smem_attr(fn, dev, tokens ? kSmemLimit - kStaticSmem : kSmemLimit)) return GEMM_ERR_LAUNCH;
-  if (launch_overlapped(fn, dim3((unsigned)r.grid), dim3(threads_for(tokens != nullptr)), (size_t)r.smem_bytes,
+  if (launch_overlapped(fn, dim3((unsigned)r.grid), dim3(tokens ? threads_for(1, true) : 64 + 128 * r.p.groups), (size_t)r.smem_bytes,
                         r.split > 1 ? r.split : r.cg, st, tw, tt, td, tc, r.p) != cudaSuccess) {
     cudaGetLastError();
     return GEMM_ERR_LAUNCH;
