@@ -306,7 +306,8 @@ typedef struct DropoutArgs {
  *   same bits for every tile, split and size of the batch.
  *   scale_a (m) and scale_b (n) fp32; NULL means 1.
  *   D  m x n row-major (N contiguous), leading dimension ldd >= n elements,
- *   any alignment of its own type; C (optional) like D with ldc, may be D.
+ *   any alignment of its own type; C (optional) like D with ldc, is D or does
+ *   not overlap it.
  *   bias (optional): n elements of bias_type.
  * m or n of 0: nothing is launched.  D must not overlap A, B, scales or bias.
  */

@@ -301,6 +301,30 @@ def test_every_tile_and_split_gives_the_same_bits(pkg, cuda, knobs):
             assert (out[0] == 77.0).all() and (out[m + 1] == 77.0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(300, 600, 6000), (700, 1040, 700)])
+def test_pairs_with_long_and_short_main_loops(pkg, cuda, dtype, m, n, k):
+    """One and two epilogue groups, several tiles per pair, the residual staged, unaligned and in place."""
+    a, b, sa, sb = int8s(pkg, m, k, 1), int8s(pkg, n, k, 2), scales(m, 3) * 0.01, scales(n, 4)
+    bias, residual = normal((n,), 5, dtype), normal((m, n), 6, dtype)
+    drop = pkg.Dropout(0.3, seed=3, row0=1, col0=2, row_elems=n + 2)
+    want = ref_product(a, sa, b, sb, bias, residual, drop)
+    shifted = torch.empty((m, n + 3), dtype=dtype, device="cuda")[:, 1:n + 1]
+    shifted.copy_(residual)
+    first = None
+    for kw in (dict(), dict(cta_group=2, tile_n=128), dict(cta_group=2, tile_n=256)):
+        for res in (residual, shifted):
+            d = pkg.gemm_int8(a, sa, b, sb, bias=bias, residual=res, dropout=drop, out_dtype=dtype, **kw)
+            first = d if first is None else first
+            assert torch.equal(d, first)
+        out = residual.clone()
+        pkg.gemm_int8(a, sa, b, sb, bias=bias, residual=out, dropout=drop, out=out, **kw)
+        assert torch.equal(out, first)
+        odd = drop._replace(col0=1)                       # pairs of a draw begin at odd channels
+        check_close(pkg.gemm_int8(a, sa, b, sb, dropout=odd, out_dtype=dtype, **kw), *ref_product(a, sa, b, sb, drop=odd))
+    check_close(first, *want)
+
+
 def test_refused_knobs(pkg, cuda):
     a, b, sa, sb = int8s(pkg, 4, 512, 1), int8s(pkg, 6, 512, 2), scales(4, 3), scales(6, 4)
     for knobs in (dict(tile_n=48), dict(cta_group=3), dict(cta_group=2, tile_n=64), dict(split_k=3),
@@ -530,6 +554,21 @@ def test_dropout(pkg, cuda, dtype, rows, cols, p):
     assert ((y == 0) | keep).all()
     check_close(y, want, want.abs())
     check_close(pkg.dropout(x, drop, residual=residual), want + residual.double(), want.abs() + residual.double().abs())
+
+
+@pytest.mark.parametrize("p,kept", [(1e-12, True), (1.0 - 1e-12, False)])
+def test_dropout_next_to_none_and_all(pkg, cuda, p, kept):
+    """Probabilities that round to 0 and to 1 in steps of 2^-32."""
+    x = normal((30, 50), 1)
+    x[0, 0] = float("nan")
+    y = pkg.dropout(x, pkg.Dropout(p))
+    q, s = pkg.quantize_int8(x[1:], dropout=pkg.Dropout(p))
+    d = pkg.gemm_int8(q, None, q, None, dropout=pkg.Dropout(p))
+    if kept:
+        assert torch.equal(y[1:], x[1:]) and torch.isnan(y[0, 0])
+        assert torch.equal(q, pkg.quantize_int8(x[1:])[0]) and torch.equal(d, pkg.gemm_int8(q, None, q, None))
+    else:
+        assert (y == 0).all() and (q == 0).all() and (d == 0).all()
 
 
 def test_dropout_rate(pkg, cuda):
