@@ -127,19 +127,18 @@ __global__ void __launch_bounds__(row_threads(NV)) quantize_rows_kernel(const __
 // whose phases overlap; the rows before the last such batch are read a second time,
 // from L2 (the strips at work at one time are smaller than it).
 constexpr int kStripBytes = 64;
-constexpr int kColThreads = 256;
 // Rows of a CTA in shared memory at a time: with fewer, more CTAs overlap their
 // phases, but more rows are read (and masked) twice.  8192 x 28672 bf16: 200 us
 // with 512, 218 with 1024; with dropout and sums 436 and 364.
 constexpr int rows_held(bool drop) { return drop ? 1024 : 512; }
-constexpr int kColWarps = kColThreads / 32;
 
 // Byte of row r in the held strip: a 64-byte gap after every 16 rows puts rows 16
 // apart, which the lanes of a warp read together, in different banks.
 __device__ __forceinline__ int held_at(int r) { return (r + (r >> 4)) * kStripBytes; }
 
-template <typename T, bool DROP>
-__global__ void __launch_bounds__(kColThreads) quantize_cols_kernel(const __grid_constant__ QuantParams p) {
+template <typename T, bool DROP, int kColWarps>
+__global__ void __launch_bounds__(32 * kColWarps) quantize_cols_kernel(const __grid_constant__ QuantParams p) {
+  constexpr int kColThreads = 32 * kColWarps;
   constexpr int V = Vec<T>::N;
   constexpr int COLS = kStripBytes / (int)sizeof(T);
   constexpr int LANES = kStripBytes / 16;      // threads that cover one row of the strip
@@ -356,20 +355,27 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
   return p.drop.on ? launch_rows<T, 4, true>(p, st) : launch_rows<T, 8, false>(p, st);
 }
 
+template <typename T, bool DROP, int kColWarps>
+cudaError_t launch_cols(QuantParams p, int peers, cudaStream_t st) {
+  constexpr int kCols = kStripBytes / (int)sizeof(T);
+  constexpr int kHeld = rows_held(DROP);
+  p.rows_held = p.row_chunk < kHeld ? p.row_chunk : kHeld;
+  const int64_t strips = (p.cols + kCols - 1) / kCols;
+  const auto fn = quantize_cols_kernel<T, DROP, kColWarps>;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeld / 16 * 17 * kStripBytes);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(fn, dim3((unsigned)(strips * peers)), dim3(32 * kColWarps),
+                           (size_t)(p.rows_held / 16 * 17 * kStripBytes), peers, st, p);
+}
+// Four warps per CTA start sooner and leave room for more CTAs; eight pay off for CTAs
+// with many rows (1024 x 8192 bf16 9.8 us and 11.4; with dropout and sums 16384 x 8192 272 us and 245).
 template <typename T>
 cudaError_t launch_cols(QuantParams p, cudaStream_t st) {
-  constexpr int kCols = kStripBytes / (int)sizeof(T);
   int peers = (int)((p.rows + 255) / 256);
   peers = peers < 1 ? 1 : (peers > 8 ? 8 : peers);
   p.row_chunk = (int32_t)(((p.rows + peers - 1) / peers + 15) / 16 * 16);
-  const int held = rows_held(p.drop.on);
-  p.rows_held = p.row_chunk < held ? p.row_chunk : held;
-  const int64_t strips = (p.cols + kCols - 1) / kCols;
-  auto fn = p.drop.on ? quantize_cols_kernel<T, true> : quantize_cols_kernel<T, false>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, held / 16 * 17 * kStripBytes);
-  if (e != cudaSuccess) return e;
-  return launch_overlapped(fn, dim3((unsigned)(strips * peers)), dim3(kColThreads),
-                           (size_t)(p.rows_held / 16 * 17 * kStripBytes), peers, st, p);
+  if (p.drop.on) return p.row_chunk <= 512 ? launch_cols<T, true, 4>(p, peers, st) : launch_cols<T, true, 8>(p, peers, st);
+  return p.row_chunk <= 1024 ? launch_cols<T, false, 4>(p, peers, st) : launch_cols<T, false, 8>(p, peers, st);
 }
 
 }  // namespace

@@ -322,7 +322,7 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
     if wk != k:
         raise ValueError(f"w must have {k} columns, as x has, got {wk}")
     sb = _vector(w_scale, "w_scale", n, index)
-    d = _output(out, m, n, x.dtype, x)
+    d = x.new_empty((m, n)) if out is None else _output(out, m, n, x.dtype, x)
     lda = _row_bytes(k)
     q = sa = 0
     if m > 8 or knobs or m * k > 16384:   # else no workspace is needed
