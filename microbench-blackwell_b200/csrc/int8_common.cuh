@@ -253,8 +253,9 @@ __device__ __forceinline__ void quantize_two(float x0, float x1, const RowScale2
     m.get(m0, m1);
     q0 = __float_as_uint(m0);
     q1 = __float_as_uint(m1);
-    q0 += d0 > 0.f || (d0 == 0.f && (q0 & 1u)) ? 1u : 0u;
-    q1 += d1 > 0.f || (d1 == 0.f && (q1 & 1u)) ? 1u : 0u;
+    // d > 0, or a tie (d = 0) above an odd f: d above the largest negative number or above zero.
+    q0 += d0 > __uint_as_float((q0 & 1u) * 0x80000001u) ? 1u : 0u;
+    q1 += d1 > __uint_as_float((q1 & 1u) * 0x80000001u) ? 1u : 0u;
   }
 }
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
