@@ -8,22 +8,26 @@ Torch tensors carry device memory and streams; all arithmetic runs in
 libgemm_sm100a.so kernels, enqueued on the current stream of the tensors'
 device.  Matrices are 2-D with unit stride along the last axis; int8 matrices
 have a row stride that is a multiple of 16 bytes (as ``quantize_int8`` makes
-them).  No call synchronises, and all of them can be captured into a CUDA graph
-after one call outside of it.  They build no autograd graph: the backward pass
-is ``linear_int8_backward``, and ``dropout`` itself for dropout.
+them).  No call synchronises, and all of them can be captured into a CUDA graph.
+They build no autograd graph: the backward pass is ``linear_int8_backward``, and
+``dropout`` itself for dropout.
+
+Checks, allocations and the C-ABI calls are in csrc/torch_host.cpp (built into
+lib/gemm_sm100a_torch.so): a small call is bound by the host.  A refused argument
+raises ValueError or GemmError before anything is launched.
 """
 from __future__ import annotations
 
 import ctypes as C
-import struct
+import importlib.machinery
+import importlib.util
 from typing import NamedTuple
 
 import torch
 
-from . import ERR_CANNOT_IMPLEMENT, GemmError, GemmInfo, OK, lib
+from . import GemmError, GemmInfo, PKG_DIR, lib
 
-TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
-_TYPES = {torch.bfloat16: TYPE_BF16, torch.float16: TYPE_FP16, torch.float32: TYPE_FP32}
+TORCH_LIB_PATH = PKG_DIR / "lib" / "gemm_sm100a_torch.so"
 MAX_INT8_K = 131071   # 2^14 * k stays below 2^31
 
 
@@ -88,17 +92,6 @@ class DropoutOpArgs(C.Structure):
     ]
 
 
-# The same layouts for struct.pack: one call fills an argument block several
-# times faster than field by field, which counts for single tokens.
-_DROP = "dQQPqqq"
-_GEMM_PACK = struct.Struct("@IiqqqPqPqPqPqPPPiiii" + _DROP + "PII")
-_QUANT_PACK = struct.Struct("@IiqqPqPqPPii" + _DROP)
-_BACKWARD_PACK = struct.Struct("@IiqqqPqPqPqPPqPqPiiPq" + _DROP + "P")
-_DROPOUT_PACK = struct.Struct("@IiqqPqPqPq" + _DROP)
-_NO_DROP = (0.0, 0, 0, 0, 0, 0, 0)
-_U64 = (1 << 64) - 1
-
-
 class Dropout(NamedTuple):
     """Dropout with probability ``p`` of elements of a matrix with ``row_elems`` columns in
     all, of which the call sees the part that begins at (``row0``, ``col0``): the mask is a
@@ -116,88 +109,44 @@ class Dropout(NamedTuple):
     row_elems: int | None = None
 
 
-def _drop_fields(drop: Dropout | None, cols: int, index: int):
-    if drop is None:
-        return _NO_DROP
-    p, seed, stream_id, row0, col0, row_elems = drop
-    if p == 0.0:
-        return _NO_DROP
-    word = 0
-    if isinstance(seed, torch.Tensor):
-        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.get_device() != index:
-            raise ValueError("a seed tensor holds one int64 on the operands' device")
-        seed, word = 0, seed.data_ptr()
-    return (p, seed & _U64, stream_id & _U64, word, row0, col0, col0 + cols if row_elems is None else row_elems)
+_host_module = None
 
 
-def _matrix(t: torch.Tensor, name: str, dtype=None, shape=None, index: int | None = None) -> int:
-    """Check one operand and return its row stride in elements.  `index`: the device it must be on."""
-    try:
-        (rows, cols), (ld, inner), dev = t.shape, t.stride(), t.get_device()
-    except (AttributeError, ValueError):
-        raise ValueError(f"{name} must be a 2-D tensor") from None
-    if dev < 0 or (index is not None and dev != index):
-        raise ValueError(f"{name} must be on the operands' CUDA device")
-    if dtype is not None and t.dtype is not dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and (rows, cols) != shape:
-        raise ValueError(f"{name} must have shape {shape}, got {(rows, cols)}")
-    if inner != 1 and cols > 1:
-        raise ValueError(f"{name} must have unit stride along its last axis")
-    if rows > 1:
-        if ld < cols:
-            raise ValueError(f"{name} has overlapping rows")
-        return ld
-    return cols or 1
+def _raise_gemm_error(code: int, what: str):
+    raise GemmError(code, what)
 
 
-def _floating(t: torch.Tensor, name: str) -> int:
-    code = _TYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
-    if code is None:
-        raise ValueError(f"{name} must be a bfloat16, float16 or float32 tensor")
-    return code
+def _host():
+    """The extension module (raises if it was not built: no fallback path exists)."""
+    global _host_module
+    if _host_module is None:
+        lib()
+        if not TORCH_LIB_PATH.exists():
+            raise RuntimeError(f"{TORCH_LIB_PATH} is missing: build it with `make -C {PKG_DIR}` "
+                               "(or __graft_entry__.build()); there is no CPU fallback")
+        loader = importlib.machinery.ExtensionFileLoader("gemm_sm100a_torch", str(TORCH_LIB_PATH))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("gemm_sm100a_torch", loader))
+        loader.exec_module(module)
+        module.set_raise(_raise_gemm_error)
+        _host_module = module
+    return _host_module
 
 
-def _int8(t: torch.Tensor, name: str, shape=None, index: int | None = None) -> int:
-    ld = _matrix(t, name, torch.int8, shape, index)
-    if ld & 15 and t.shape[0] <= 1:
-        ld = _pad16(ld)
-    if ld & 15:
-        raise ValueError(f"{name} must have a row stride that is a multiple of 16 bytes")
-    return ld
+_KNOBS = {"tile_n", "cta_group", "split_k", "timeout_ms", "flags"}
+_NO_KNOBS = (0, 0, 0, 0, 0)
 
 
-def _vector(t: torch.Tensor, name: str, n: int, index: int, dtype=torch.float32) -> int:
-    try:
-        (size,), (step,), dev = t.shape, t.stride(), t.get_device()
-    except (AttributeError, ValueError):
-        size = -1
-    if size != n or dev != index or (step != 1 and n > 1):
-        raise ValueError(f"{name} must be a contiguous vector of {n} elements on the operands' device")
-    if dtype is not None and t.dtype is not dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    return t.data_ptr()
-
-
-def _pad16(n: int) -> int:
-    return (n + 15) & ~15
-
-
-# The current stream's handle; the Stream object that torch.cuda.current_stream builds costs
-# 2 us, as much as a launch.
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _row_bytes(cols: int) -> int:
-    """Row stride of the int8 matrices made here: whole 128-byte lines, which a TMA row of an operand
-    then never straddles (777 x 5000 x 2056: 11.4 us with rows of 2176 bytes, 18.8 with 2064)."""
-    return (max(cols, 1) + 127) & ~127 if cols > 64 else _pad16(max(cols, 1))
+def _knob_values(knobs):
+    if not _KNOBS.issuperset(knobs):
+        raise TypeError(f"unknown knobs {sorted(set(knobs) - _KNOBS)}")
+    return tuple(knobs.get(k, 0) for k in ("tile_n", "cta_group", "split_k", "timeout_ms", "flags"))
 
 
 def empty_int8(rows: int, cols: int, device) -> torch.Tensor:
     """An int8 matrix whose row stride is a multiple of 16 bytes (of 128 for more than 64 columns)."""
-    return torch.empty_strided((rows, cols), (_row_bytes(cols), 1), dtype=torch.int8, device=device)
+    device = torch.device(device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return _host().empty(rows, cols, index)
 
 
 def quantize_int8(x: torch.Tensor, *, transpose: bool = False, dropout: Dropout | None = None,
@@ -209,62 +158,7 @@ def quantize_int8(x: torch.Tensor, *, transpose: bool = False, dropout: Dropout 
     max|x| / 127; a row with NaN or Inf gets that as its scale.  ``dropout`` masks ``x`` first and
     puts 1 / (1 - p) into the scales.  ``column_sums`` (with ``transpose``) adds the fp32 sums of
     the masked columns: (q, scale, sums)."""
-    code = _floating(x, "x")
-    ldx = _matrix(x, "x")
-    rows, cols = x.shape
-    if column_sums and not transpose:
-        raise ValueError("column_sums needs transpose=True")
-    q = empty_int8(cols, rows, x.device) if transpose else empty_int8(rows, cols, x.device)
-    scale = x.new_empty((cols if transpose else rows,), dtype=torch.float32)
-    sums = x.new_empty((cols,), dtype=torch.float32) if column_sums else None
-    if scale.shape[0]:
-        if not transpose and cols == 0:
-            raise ValueError("x has no columns")
-        args = _QUANT_PACK.pack(_QUANT_PACK.size, code, rows, cols, x.data_ptr(), ldx, q.data_ptr(), q.stride(0),
-                                scale.data_ptr(), 0 if sums is None else sums.data_ptr(), int(transpose), 0,
-                                *_drop_fields(dropout, cols, x.get_device()))
-        rc = lib().gemm_sm100a_quantize_int8(args, _raw_stream(x.get_device()))
-        if rc != OK:
-            raise GemmError(rc, "gemm_sm100a_quantize_int8")
-    return (q, scale) if sums is None else (q, scale, sums)
-
-
-def _output(out, m, n, dtype, like) -> torch.Tensor:
-    if out is None:
-        return like.new_empty((m, n), dtype=dtype)
-    _matrix(out, "out", dtype, (m, n), like.get_device())
-    return out
-
-
-_KNOBS = {"tile_n", "cta_group", "split_k", "timeout_ms", "flags"}
-
-
-def _tiles(knobs):
-    if not _KNOBS.issuperset(knobs):
-        raise TypeError(f"unknown knobs {sorted(set(knobs) - _KNOBS)}")
-    return knobs.get("tile_n", 0), knobs.get("cta_group", 0), knobs.get("split_k", 0)
-
-
-def _pack_gemm(index, code, m, n, k, a, lda, b, ldb, d, residual, a_scale, b_scale, bias, dropout, status, knobs):
-    ldd = d.stride(0) if m > 1 else max(n, 1)
-    c = ldc = 0
-    if residual is not None:
-        ldc = _matrix(residual, "residual", d.dtype, (m, n), index)
-        c = residual.data_ptr()
-    bias_ptr = bias_code = 0
-    if bias is not None:
-        bias_code = _floating(bias, "bias")
-        bias_ptr = _vector(bias, "bias", n, index, None)
-    return _GEMM_PACK.pack(_GEMM_PACK.size, code, m, n, k, a, lda, b, ldb, d.data_ptr(), ldd, c, ldc, a_scale, b_scale,
-                           bias_ptr, bias_code, *(_tiles(knobs) if knobs else (0, 0, 0)),
-                           *_drop_fields(dropout, n, index), 0 if status is None else status.data_ptr(),
-                           knobs.get("timeout_ms", 0), knobs.get("flags", 0))
-
-
-def _raise(rc, args, what):
-    info = GemmInfo()
-    lib().gemm_sm100a_int8_query(args, C.byref(info))
-    raise GemmError(rc, f"{what} ({info.reason.decode()})")
+    return _host().quantize(x, transpose, dropout, column_sums)
 
 
 def query_int8(args: Int8GemmArgs) -> tuple[int, GemmInfo]:
@@ -283,27 +177,8 @@ def gemm_int8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor, b_
     ``residual`` and ``out`` (which may be the residual) of ``out_dtype``.  The sum over k is
     exact, so the result does not depend on the batch or the tile.  ``status``: optional int32
     device word, as in ``gemm_into``.  Knobs: tile_n, cta_group, split_k, timeout_ms, flags."""
-    lda = _int8(a, "a")
-    index = a.get_device()
-    m, k = a.shape
-    ldb = _int8(b, "b", None, index)
-    n, bk = b.shape
-    if bk != k:
-        raise ValueError(f"b must have {k} columns, as a has, got {bk}")
-    if out is not None:
-        out_dtype = out.dtype
-    code = _TYPES.get(out_dtype)
-    if code is None:
-        raise ValueError("out_dtype must be bfloat16, float16 or float32")
-    d = _output(out, m, n, out_dtype, a)
-    sa = 0 if a_scale is None else _vector(a_scale, "a_scale", m, index)
-    sb = 0 if b_scale is None else _vector(b_scale, "b_scale", n, index)
-    args = _pack_gemm(index, code, m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, d, residual, sa, sb, bias, dropout,
-                      status, knobs)
-    rc = lib().gemm_sm100a_int8_launch(args, _raw_stream(index))
-    if rc != OK:
-        _raise(rc, args, "gemm_sm100a_int8_launch")
-    return d
+    return _host().gemm(a, a_scale, b, b_scale, bias, residual, dropout, out_dtype, out, status,
+                        *(_knob_values(knobs) if knobs else _NO_KNOBS))
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias: torch.Tensor | None = None,
@@ -313,27 +188,8 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
     x's type as output, bit for bit, in one or two launches.
 
     ``x`` (m, k); ``w`` (n, k) int8 and ``w_scale`` (n) as ``quantize_int8`` makes them."""
-    code = _floating(x, "x")
-    ldx = _matrix(x, "x")
-    index = x.get_device()
-    m, k = x.shape
-    ldw = _int8(w, "w", None, index)
-    n, wk = w.shape
-    if wk != k:
-        raise ValueError(f"w must have {k} columns, as x has, got {wk}")
-    sb = _vector(w_scale, "w_scale", n, index)
-    d = x.new_empty((m, n)) if out is None else _output(out, m, n, x.dtype, x)
-    lda = _row_bytes(k)
-    q = sa = 0
-    if m > 8 or knobs or m * k > 16384:   # else no workspace is needed
-        work = x.new_empty((m * (lda + 4) + 16,), dtype=torch.uint8)          # int8 tokens, then their scales
-        q = work.data_ptr()
-        sa = q + m * lda
-    args = _pack_gemm(index, code, m, n, k, q, lda, w.data_ptr(), ldw, d, residual, sa, sb, bias, dropout, status, knobs)
-    rc = lib().gemm_sm100a_int8_linear(args, x.data_ptr(), code, ldx, _raw_stream(index))
-    if rc != OK:
-        _raise(rc, args, "gemm_sm100a_int8_linear")
-    return d
+    return _host().linear(x, w, w_scale, bias, residual, dropout, out, status,
+                          *(_knob_values(knobs) if knobs else _NO_KNOBS))
 
 
 def linear_int8_backward(dy: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, wt_scale: torch.Tensor, *,
@@ -348,54 +204,11 @@ def linear_int8_backward(dy: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, wt
     ``quantize_int8(w, transpose=True)``: the products contract over n and m, so the scales lie
     along the other axis.  dx has x's type, dw ``dw_dtype``, dbias is fp32.  The residual's
     gradient is dy.  m = 0 gives zeros for dw and dbias."""
-    code = _floating(dy, "dy")
-    lddy = _matrix(dy, "dy")
-    index = dy.get_device()
-    m, n = dy.shape
-    _floating(x, "x")
-    ldx = _matrix(x, "x", dy.dtype, None, index)
-    xm, k = x.shape
-    if xm != m:
-        raise ValueError(f"x must have {m} rows, as dy has, got {xm}")
-    dw_code = _TYPES.get(dw_dtype)
-    if dw_code is None:
-        raise ValueError("dw_dtype must be bfloat16, float16 or float32")
-    ldwt = _int8(wt, "wt", (k, n), index)
-    scale = _vector(wt_scale, "wt_scale", k, index)
-    need = lib().gemm_sm100a_int8_backward_workspace(m, n, k)
-    if need < 0:
-        raise GemmError(ERR_CANNOT_IMPLEMENT, f"linear_int8_backward: sums over m and n are exact up to {MAX_INT8_K}")
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    dw = x.new_empty((n, k), dtype=dw_dtype)
-    dbias = x.new_empty((n,), dtype=torch.float32)
-    work = x.new_empty((need,), dtype=torch.uint8)
-    args = _BACKWARD_PACK.pack(_BACKWARD_PACK.size, code, m, n, k, dy.data_ptr(), lddy, x.data_ptr(), ldx, wt.data_ptr(),
-                               ldwt, scale, dx.data_ptr(), k, dw.data_ptr(), k, dbias.data_ptr(), dw_code, 0,
-                               work.data_ptr(), need, *_drop_fields(dropout, n, index),
-                               0 if status is None else status.data_ptr())
-    rc = lib().gemm_sm100a_int8_linear_backward(args, _raw_stream(index))
-    if rc != OK:
-        raise GemmError(rc, "gemm_sm100a_int8_linear_backward")
-    return dx, dw, dbias
+    return _host().backward(dy, x, wt, wt_scale, dropout, dw_dtype, status)
 
 
 def dropout(x: torch.Tensor, drop: Dropout, *, residual: torch.Tensor | None = None,
             out: torch.Tensor | None = None) -> torch.Tensor:
     """residual + dropout(x), computed in fp32 and rounded once.  The gradient with respect to x
     is the same call on dy without the residual.  ``out`` may be x or residual."""
-    code = _floating(x, "x")
-    ldx = _matrix(x, "x")
-    index = x.get_device()
-    rows, cols = x.shape
-    y = torch.empty_like(x, memory_format=torch.contiguous_format) if out is None else _output(out, rows, cols, x.dtype, x)
-    ldy = y.stride(0) if rows > 1 else max(cols, 1)
-    r = ldr = 0
-    if residual is not None:
-        ldr = _matrix(residual, "residual", x.dtype, (rows, cols), index)
-        r = residual.data_ptr()
-    args = _DROPOUT_PACK.pack(_DROPOUT_PACK.size, code, rows, cols, x.data_ptr(), ldx, r, ldr, y.data_ptr(), ldy,
-                              *_drop_fields(drop, cols, index))
-    rc = lib().gemm_sm100a_dropout(args, _raw_stream(index))
-    if rc != OK:
-        raise GemmError(rc, "gemm_sm100a_dropout")
-    return y
+    return _host().dropout(x, drop, residual, out)

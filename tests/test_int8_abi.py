@@ -20,18 +20,22 @@ def _gemm(pkg, **kw):
     return a
 
 
-def test_packed_layouts_match_the_structs(pkg):
-    import importlib
-    i8 = importlib.import_module("microbench_blackwell_b200.int8")
-    assert i8._GEMM_PACK.size == C.sizeof(pkg.Int8GemmArgs)
-    assert i8._QUANT_PACK.size == C.sizeof(pkg.Int8QuantArgs)
-    assert i8._DROPOUT_PACK.size == C.sizeof(pkg.DropoutOpArgs)
-    assert i8._BACKWARD_PACK.size == C.sizeof(pkg.Int8BackwardArgs)
-    packed = i8._GEMM_PACK.pack(208, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18, 19, 20,
-                                0.5, 21, 22, 23, 24, 25, 26, 27, 28, 29)
-    s = pkg.Int8GemmArgs.from_buffer_copy(packed)
-    assert (s.struct_size, s.d_type, s.m, s.lda, s.ldc, s.bias_type, s.split_k) == (208, 2, 3, 7, 13, 17, 20)
-    assert (s.drop.p, s.drop.seed, s.drop.row_elems, s.status, s.timeout_ms, s.flags) == (0.5, 21, 26, 27, 28, 29)
+def test_structs_have_the_sizes_of_the_header(pkg, tmp_path):
+    """The ctypes views against a C compiler's layout of the header."""
+    import subprocess
+    from pathlib import Path
+    names = ["DropoutArgs", "Int8GemmArgs", "Int8QuantArgs", "Int8BackwardArgs", "DropoutOpArgs"]
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "gemm_sm100a.h"\nint main(void) {'
+                   + "".join(f' printf("%zu ", sizeof({n}));' for n in names)
+                   + ' printf("%zu %zu %zu", offsetof(Int8GemmArgs, drop), offsetof(Int8QuantArgs, drop),'
+                     ' offsetof(Int8BackwardArgs, drop)); return 0; }\n')
+    root = Path(__file__).resolve().parent.parent
+    exe = tmp_path / "sizes"
+    subprocess.run(["gcc", f"-I{root / 'include'}", str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got[:5] == [C.sizeof(getattr(pkg, n)) for n in names]
+    assert got[5:] == [pkg.Int8GemmArgs.drop.offset, pkg.Int8QuantArgs.drop.offset, pkg.Int8BackwardArgs.drop.offset]
 
 
 def test_a_plain_problem_is_accepted(pkg):
