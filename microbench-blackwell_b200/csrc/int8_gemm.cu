@@ -69,6 +69,9 @@ constexpr uint32_t kTokAtom = 8 * kAtom;  // fused form: bytes of one K atom of 
 constexpr int kChannels = 128;          // channels per CTA
 constexpr int kMaxSplit = 8;            // CTAs that may share a tile's K (portable cluster size)
 
+template <int V>
+struct IntC { static constexpr int value = V; };
+
 struct Int8Params {
   void* d; int64_t ldd;
   const void* c; int64_t ldc;
@@ -432,6 +435,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
     // Rows of an even length that begin at an even index: even channels are the first of a draw's pair.
     const bool drop_pairs = p.drop.on && !p.drop.all && !((p.drop.row_elems | p.drop.col0) & 1);
+    const bool drop_odd_rows = p.drop.on && !p.drop.all && (p.drop.row_elems & 1);
     const uint64_t drop_step = (uint64_t)p.drop.row_elems * counter_rng::kGolden;   // two tokens on
     const uint32_t drop_thr = p.drop.threshold;
     const float drop_grow = p.drop.grow;
@@ -543,6 +547,28 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
               v[j] = (odd ? other : lo) >= drop_thr ? v[j] * drop_grow : 0.f;
               v[j + 1] = (odd ? hi : other) >= drop_thr ? v[j + 1] * drop_grow : 0.f;
             }
+          } else if (drop_odd_rows) {
+            // Rows of an odd length: of each two tokens, one (E) has its pairs at lanes 2 i, 2 i + 1 and
+            // the other (O) at lanes 2 i + 1, 2 i + 2.  The lower lane of a pair draws for both, and
+            // the upper one's word comes from one lane below; for lane 0, whose lower half would be in
+            // the warp before, lane l draws the word of token pair l beforehand.
+            const bool odd = lane & 1u;
+            const int swap = (int)((p.drop.row0 + tc + p.drop.col0) & 1);      // 1: token j is O, j + 1 is E
+            const uint64_t before = counter_rng::draw(key, (uint64_t)drop_index(p.drop, tc + 2 * ((int)lane % (CW / 2)) + 1 - swap,
+                                                                                ch - (int)lane) >> 1) >> 32;
+            const uint64_t first = (uint64_t)drop_index(p.drop, tc + (odd ? 1 - swap : swap), ch) >> 1;
+            uint64_t z = key + (first + 1) * counter_rng::kGolden;
+#pragma unroll
+            for (int j = 0; j < CW; j += 2, z += drop_step) {
+              const uint64_t h = counter_rng::mix64(z);
+              const uint32_t own = (uint32_t)h;
+              uint32_t below = __shfl_up_sync(0xFFFFFFFFu, (uint32_t)(h >> 32), 1);
+              const uint32_t first_lane = __shfl_sync(0xFFFFFFFFu, (uint32_t)before, j / 2);
+              if (lane == 0) below = first_lane;
+              const bool e = odd == (swap != 0);                               // token j's word is the own one
+              v[j] = (e ? own : below) >= drop_thr ? v[j] * drop_grow : 0.f;
+              v[j + 1] = (e ? below : own) >= drop_thr ? v[j + 1] * drop_grow : 0.f;
+            }
           } else {
 #pragma unroll
             for (int j = 0; j < CW; ++j)
@@ -616,8 +642,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     cluster_arrive();
     cluster_wait();
     if (warp >= 2 && warp < 6) {
-      // CTA `rank` finishes its share of the tokens: a warp takes a token, a lane
-      // four channels, with every peer's 16 bytes in flight at once.
+      // CTA `rank` finishes its share of the tokens: a warp takes a token, a lane four channels.
       int cb, tb;
       tile_coords(slot0, p, cb, tb);
       const int ch0 = cb * kChannels + 4 * (int)lane, t0 = tb * BN;
@@ -630,27 +655,44 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         bias[e] = in && p.bias ? load_as_f32(p.bias, p.bias_type, ch0 + e) : 0.f;
       }
       const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
-      for (int j = (int)rank * per + (int)warp - 2; j < (int)(rank + 1) * per; j += 4) {
-        const int t = t0 + j;
-        if (t >= p.m) break;
-        const uint32_t at = base + (uint32_t)((j * kChannels + 4 * (int)lane) * 4);
-        uint4 part[kMaxSplit];
+      // S peers and U tokens: 16 loads in flight per lane.
+      auto finish_tokens = [&](auto s_c) {
+        constexpr int S = decltype(s_c)::value, U = 16 / S;
+        const int j_end = min((int)(rank + 1) * per, p.m - t0);
+        for (int j0 = (int)rank * per + (int)warp - 2; j0 < j_end; j0 += 4 * U) {
+          uint4 part[U][S];
 #pragma unroll
-        for (int s = 0; s < kMaxSplit; ++s) part[s] = s < p.split ? ld_shared_cluster_v4(mapa_shared(at, (uint32_t)s)) : make_uint4(0, 0, 0, 0);
-        uint32_t sum[4] = {0, 0, 0, 0};
+          for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int s = 0; s < kMaxSplit; ++s) { sum[0] += part[s].x; sum[1] += part[s].y; sum[2] += part[s].z; sum[3] += part[s].w; }
-        const float sa = FUSE ? tok_rows[FUSE ? t : 0].scale : (p.sa ? p.sa[t] : 1.f);
-        T* const d = static_cast<T*>(p.d) + (int64_t)t * p.ldd + ch0;
+            for (int s = 0; s < S; ++s) {
+              const int j = min(j0 + 4 * u, j_end - 1);
+              part[u][s] = ld_shared_cluster_v4(mapa_shared(base + (uint32_t)((j * kChannels + 4 * (int)lane) * 4), (uint32_t)s));
+            }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (ch0 + e >= p.n) break;
-          float v = finish((int32_t)sum[e], sa, sb[e], bias[e]);
-          if (p.drop.on) v = drop_keeps(p.drop, key, drop_index(p.drop, t, ch0 + e)) ? v * p.drop.grow : 0.f;
-          if (p.c) v += to_f32(static_cast<const T*>(p.c)[(int64_t)t * p.ldc + ch0 + e]);
-          d[e] = from_f32<T>(v);
+          for (int u = 0; u < U; ++u) {
+            const int t = t0 + j0 + 4 * u;
+            if (j0 + 4 * u >= j_end) continue;
+            uint32_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+              sum[0] += part[u][s].x; sum[1] += part[u][s].y; sum[2] += part[u][s].z; sum[3] += part[u][s].w;
+            }
+            const float sa = FUSE ? tok_rows[FUSE ? t : 0].scale : (p.sa ? p.sa[t] : 1.f);
+            T* const d = static_cast<T*>(p.d) + (int64_t)t * p.ldd + ch0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (ch0 + e >= p.n) continue;
+              float v = finish((int32_t)sum[e], sa, sb[e], bias[e]);
+              if (p.drop.on) v = drop_keeps(p.drop, key, drop_index(p.drop, t, ch0 + e)) ? v * p.drop.grow : 0.f;
+              if (p.c) v += to_f32(static_cast<const T*>(p.c)[(int64_t)t * p.ldc + ch0 + e]);
+              d[e] = from_f32<T>(v);
+            }
+          }
         }
-      }
+      };
+      if (p.split == 2) finish_tokens(IntC<2>{});
+      else if (p.split == 4) finish_tokens(IntC<4>{});
+      else finish_tokens(IntC<8>{});
       __syncwarp();
     }
     cluster_arrive();
@@ -721,28 +763,27 @@ int sm_count() {
   return sms;
 }
 
-// CTAs that share a tile of 128 channels, for few tiles (at most `most_ctas` in all, at least
-// `least_kb` K atoms each).  One SM pulls some 75 of
-// HBM's 6500 bytes per ns, so 64 to 128 CTAs stream at full rate; more than one
-// wave of them, or clusters of 8 (of which the GPU holds 16 at a time or fewer),
-// cost more than they give.  16 tokens, 8192 x 8192: 14.3 us whole, 14.3 split in 2,
-// 18.0 in 4, 29.7 in 8; 2048 x 16384: 17.0 whole, 10.5 split in 4, 13.7 in 8.
-int split_for(int64_t tiles, int64_t kb, int64_t most_ctas, int64_t least_kb) {
+// Fused form: CTAs that share a tile of 128 channels.  One SM pulls some 75 of HBM's
+// 6500 bytes per ns, so 64 to 128 CTAs stream at full rate; more than one wave of them costs more than it gives.
+int fused_split(int64_t tiles, int64_t kb) {
   int s = 1;
-  while (s < 4 && tiles * s * 2 <= most_ctas && kb >= 2 * s * least_kb) s *= 2;
+  while (s < 4 && tiles * s * 2 <= 128 && kb >= 2 * s * 16) s *= 2;
   return s;
 }
 
 // Tile and split with the least estimated time, in SM cycles.  A K atom costs a CTA
 // what its tensor core needs (2 BN cycles at 8192 int8 multiply-adds a cycle; a pair
 // halves the tokens' rows but not this) or the bytes that it has to pull
-// from L2 at some 64 a cycle, whichever is more; the last tile's epilogue follows, 11
-// cycles a token; a split adds the exchange of the partial tiles.  The order of the
+// from L2 at some 64 a cycle, whichever is more; all of them cannot beat HBM (3400 bytes a cycle); the last
+// tile's epilogue follows, 11 cycles a token.  A split of K over up to 8 CTAs (one wave; the GPU
+// holds few clusters of 8 at a time) adds the exchange of the partial tiles (496 x 965 x 21956: 128-token
+// tiles whole 35.1 us, in 4 parts 18.4; 64 x 4096 x 4096: 32-token tiles whole 7.3, in 2 parts 8.6).  The order of the
 // candidates' measured times agreed in 18 of 18 problems of 48 to 4096 tokens (512 x 8192
 // x 8192: pairs of 256 tokens 28.3 us, of 128 31.6, single CTAs of 128 37.7, of 64 50.9).
 void choose(const Int8GemmArgs* a, int num_sms, int& cg, int& bn, int& split) {
   static const int kTiles[6][2] = {{1, 16}, {1, 32}, {1, 64}, {1, 128}, {2, 128}, {2, 256}};
   const int64_t kb = (a->k + kAtom - 1) / kAtom;
+  const int64_t hbm = (a->n + a->m) * a->k / 3400;
   int64_t best = INT64_MAX;
   int best_cg = cg ? cg : 1, best_bn = bn ? bn : 128, best_split = split ? split : 1;
   for (const auto& tile : kTiles) {
@@ -750,11 +791,13 @@ void choose(const Int8GemmArgs* a, int num_sms, int& cg, int& bn, int& split) {
     if ((cg && g != cg) || (bn && w != bn)) continue;
     const int64_t tiles = ((a->n + kChannels * g - 1) / (kChannels * g)) * ((a->m + w - 1) / w);
     const int64_t tensor = 2 * w, load = (kChannels * kAtom + (int64_t)w / g * kAtom) / 64;
-    const int64_t atom = tensor > load ? tensor : load;
-    const int s = split ? split : (g == 1 ? split_for(tiles, kb, 64, 16) : 1);
-    const int64_t slots = num_sms / g, waves = s > 1 ? 1 : (tiles + slots - 1) / slots;
-    const int64_t time = waves * ((kb + s - 1) / s) * atom + 11 * w + (s > 1 ? 3000 : 0);
-    if (time < best) { best = time; best_cg = g; best_bn = w; best_split = s; }
+    const int64_t atom = tensor > load ? tensor : load, slots = num_sms / g;
+    for (int s = 1; s <= (g == 1 ? kMaxSplit : 1); s *= 2) {
+      if (split ? s != split : s > 1 && (tiles * s > (s == 8 ? 64 : 128) || kb < 8 * s)) continue;
+      const int64_t waves = s > 1 ? 1 : (tiles + slots - 1) / slots, main = waves * ((kb + s - 1) / s) * atom;
+      const int64_t time = (main > hbm ? main : hbm) + 11 * w + (s > 1 ? 5000 : 0);
+      if (time < best) { best = time; best_cg = g; best_bn = w; best_split = s; }
+    }
   }
   cg = best_cg;
   bn = best_bn;
@@ -768,7 +811,7 @@ int resolve(const Int8GemmArgs* a, bool fused, Resolved& r) {
   if (rc != GEMM_OK) return rc;
   r.num_sms = sm_count();
   r.cg = a->cta_group; r.bn = a->tile_n; r.split = a->split_k;
-  if (fused) { r.cg = 1; r.bn = kFusedBN; r.split = split_for((a->n + kChannels - 1) / kChannels, (a->k + kAtom - 1) / kAtom, 128, 16); }
+  if (fused) { r.cg = 1; r.bn = kFusedBN; r.split = fused_split((a->n + kChannels - 1) / kChannels, (a->k + kAtom - 1) / kAtom); }
   choose(a, r.num_sms, r.cg, r.bn, r.split);
   if (r.cg != 1 && r.cg != 2) FAIL("cta_group must be 1 or 2");
   if (!supported(r.cg, r.bn)) FAIL("tile_n %d unsupported for cta_group %d", r.bn, r.cg);

@@ -264,6 +264,21 @@ def test_product_epilogue(pkg, cuda, dtype, m, n, k, bias_dtype, p):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(9, 131, 200), (70, 131, 200), (300, 515, 200), (700, 1031, 200), (40, 131, 4096)])
+@pytest.mark.parametrize("row0,col0", [(0, 0), (1, 0), (0, 1), (1, 1)])
+def test_product_dropout_with_rows_of_an_odd_length(pkg, cuda, dtype, m, n, k, row0, col0):
+    """Draws' pairs begin at even channels in one token and at odd ones in the next."""
+    a, b = int8s(pkg, m, k, m), int8s(pkg, n, k, n)
+    sa, sb = scales(m, 1) * 0.01, scales(n, 2)
+    drop = pkg.Dropout(0.4, seed=9, stream_id=1, row0=row0, col0=col0, row_elems=n + 2)
+    got = pkg.gemm_int8(a, sa, b, sb, dropout=drop, out_dtype=dtype)
+    keep = ref_keep(m, n, drop).to(got.device)
+    assert (got[~keep] == 0).all()
+    want, size = ref_product(a, sa, b, sb, None, None, drop)
+    check_close(got, want, size)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n", [(3, 131), (50, 131), (300, 515), (600, 777)])
 def test_product_writes_only_its_output(pkg, cuda, dtype, m, n):
     """D inside a larger buffer, at an odd column (element alignment) and at an aligned one."""
