@@ -655,9 +655,9 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         bias[e] = in && p.bias ? load_as_f32(p.bias, p.bias_type, ch0 + e) : 0.f;
       }
       const uint64_t key = p.drop.on ? drop_key(p.drop) : 0;
-      // S peers and U tokens: 16 loads in flight per lane.
+      // S peers and U tokens: 16 loads in flight per lane (a fused call has at most 2 tokens for a warp).
       auto finish_tokens = [&](auto s_c) {
-        constexpr int S = decltype(s_c)::value, U = 16 / S;
+        constexpr int S = decltype(s_c)::value, U = FUSE ? 2 : 16 / S;
         const int j_end = min((int)(rank + 1) * per, p.m - t0);
         for (int j0 = (int)rank * per + (int)warp - 2; j0 < j_end; j0 += 4 * U) {
           uint4 part[U][S];
