@@ -14,9 +14,9 @@
 // warps 2..5 run the epilogue (one TMEM lane quadrant each; in a pair with a short
 // main loop warps 6..9 take every other chunk).
 //
-// Measured on B200 (1000 W cap): 8192 x 8192 x 8192 in 326 us under ncu, tensor pipe
-// 96.5 % active, 3.37 PFLOP/s; 8192 x 28672 x 8192 back to back 1.39 ms, 2.77 PFLOP/s at the
-// clock that the power cap leaves.  One token x 8192 x 8192 in 14.5 us, 4.6 of
+// Measured on B200 (1000 W cap): 8192 x 8192 x 8192 in 335 us under ncu, tensor pipe
+// 96 % active, 3.28 PFLOP/s; 8192 x 28672 x 8192 back to back 1.39 ms, 2.77 PFLOP/s at the
+// clock that the power cap leaves.  One token x 8192 x 8192 in 14.8 us (from a graph), 4.5 of
 // the 6.55 TB/s that a copy reaches; about 4 us of it are launch, first loads and last stores
 // (a 1024 x 1024 layer takes 4.7 us in all).
 //   whole-K form   persistent CTAs (CTA pairs for large problems), two

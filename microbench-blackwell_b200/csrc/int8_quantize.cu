@@ -128,8 +128,8 @@ __global__ void __launch_bounds__(row_threads(NV)) quantize_rows_kernel(const __
 // from L2 (the strips at work at one time are smaller than it).
 constexpr int kStripBytes = 64;
 // Rows of a CTA in shared memory at a time: with fewer, more CTAs overlap their
-// phases, but more rows are read (and masked) twice.  8192 x 28672 bf16: 200 us
-// with 512, 218 with 1024; with dropout and sums 436 and 364.
+// phases, but more rows are read (and masked) twice.  8192 x 28672 bf16: 170 us
+// with 512, 206 with 1024; with dropout and sums 397 and 330.
 constexpr int rows_held(bool drop) { return drop ? 1024 : 512; }
 
 // Byte of row r in the held strip: a 64-byte gap after every 16 rows puts rows 16
