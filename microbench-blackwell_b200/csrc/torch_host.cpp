@@ -132,6 +132,18 @@ int64_t integer(PyObject* o) {
   return v;
 }
 
+int32_t knob(PyObject* o, const char* name) {
+  const int64_t v = integer(o);
+  if (v < 0 || v > INT32_MAX) refuse("%s must be between 0 and 2^31 - 1", name);
+  return (int32_t)v;
+}
+
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Refused();
+  return v == 1;
+}
+
 // A Dropout tuple (p, seed, stream_id, row0, col0, row_elems) or None.
 DropoutArgs dropout_args(PyObject* o, int64_t cols, int index) {
   DropoutArgs d;
@@ -234,6 +246,13 @@ PyObject* guarded(F&& body) {
     return body();
   } catch (const Refused&) {
     return nullptr;
+  } catch (const c10::OutOfMemoryError& e) {
+    PyObject* const torch = PyImport_ImportModule("torch");
+    PyObject* const type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    if (type) PyErr_SetString(type, e.what_without_backtrace());
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
+    return nullptr;
   } catch (const std::exception& e) {
     if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
@@ -263,11 +282,11 @@ void common(Int8GemmArgs& g, PyObject* bias, PyObject* residual, PyObject* drop,
   if (bias != Py_None) g.bias = vector(bias, "bias", g.n, index, &g.bias_type);
   g.drop = dropout_args(drop, g.n, index);
   g.status = status_word(status, index);
-  g.tile_n = (int32_t)integer(knobs[0]);
-  g.cta_group = (int32_t)integer(knobs[1]);
-  g.split_k = (int32_t)integer(knobs[2]);
-  g.timeout_ms = (uint32_t)integer(knobs[3]);
-  g.flags = (uint32_t)integer(knobs[4]);
+  g.tile_n = knob(knobs[0], "tile_n");
+  g.cta_group = knob(knobs[1], "cta_group");
+  g.split_k = knob(knobs[2], "split_k");
+  g.timeout_ms = (uint32_t)knob(knobs[3], "timeout_ms");
+  g.flags = (uint32_t)knob(knobs[4], "flags");
 }
 
 [[noreturn]] void failed_product(int rc, const Int8GemmArgs& g, const char* what) {
@@ -380,7 +399,7 @@ PyObject* py_quantize(PyObject*, PyObject* const* v, Py_ssize_t n) {
     count(n, 4);
     const Matrix x = matrix(v[0], "x", -1);
     const int code = floating(x, "x");
-    const bool transpose = PyObject_IsTrue(v[1]) == 1, sums = PyObject_IsTrue(v[3]) == 1;
+    const bool transpose = truth(v[1]), sums = truth(v[3]);
     if (sums && !transpose) refuse("column_sums needs transpose=True");
     if (!transpose && x.cols == 0 && x.rows > 0) refuse("x has no columns");
     Int8QuantArgs g;

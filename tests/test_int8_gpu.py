@@ -860,3 +860,16 @@ def test_host_memory_is_refused(pkg, cuda):
     assert L.gemm_sm100a_dropout(bytes(a), torch.cuda.current_stream().cuda_stream) == pkg.ERR_LAUNCH
     torch.cuda.synchronize()
     assert torch.equal(pkg.dropout(x, pkg.Dropout(0.0)), x)
+
+
+def test_out_of_memory_is_the_frameworks_own_error(pkg, cuda):
+    with pytest.raises(torch.OutOfMemoryError):
+        pkg.empty_int8(1 << 20, 1 << 22, cuda)
+
+
+def test_knobs_beyond_32_bits_are_refused(pkg, cuda):
+    a, b = int8s(pkg, 4, 64, 0), int8s(pkg, 5, 64, 1)
+    for knob in ("tile_n", "cta_group", "split_k", "timeout_ms", "flags"):
+        for value in (2 ** 32, -1):
+            with pytest.raises(ValueError, match=knob):
+                pkg.gemm_int8(a, None, b, None, **{knob: value})
