@@ -345,7 +345,8 @@ int gemm_sm100a_int8_launch(const Int8GemmArgs* args, void* stream);
  * or two launches.  args->a and args->scale_a are workspace of the caller
  * (m * lda bytes and m floats; their content afterwards is unspecified).  They
  * may be NULL where one launch quantises and multiplies: x_type equal to d_type,
- * m <= 8, m * k <= 16384 and no knob or flag set.
+ * m <= 8, m * k <= 16384, no knob or flag set and D apart from X.
+ * D may lie over X, with X as C too (the layer's result replaces its tokens).
  */
 int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream);
 

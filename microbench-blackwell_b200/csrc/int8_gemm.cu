@@ -958,13 +958,26 @@ int launch_product(const Int8GemmArgs& a, const Tokens* tokens, cudaStream_t st,
   return GEMM_OK;
 }
 
+// Whether a row of D shares a byte with one of the tokens (few of them, both of one element size).
+bool output_meets_tokens(const Int8GemmArgs& a, const void* x, int64_t ldx) {
+  const int64_t e = type_bytes(a.d_type);
+  const intptr_t x0 = reinterpret_cast<intptr_t>(x), d0 = reinterpret_cast<intptr_t>(a.d);
+  for (int64_t i = 0; i < a.m; ++i)
+    for (int64_t j = 0; j < a.m; ++j) {
+      const intptr_t xi = x0 + i * ldx * e, dj = d0 + j * a.ldd * e;
+      if (xi < dj + a.n * e && dj < xi + a.k * e) return true;
+    }
+  return false;
+}
+
 // Few tokens, no knob set and X of D's type: one launch.  Every CTA then quantises
 // the tokens for itself, which costs more than the launch it saves beyond some
 // 16384 of their elements: 8192 x 8192, 1 token 14.5 us against 16.9 in two
-// launches, 4 tokens 18.0 against 16.1.
-bool use_fused(const Int8GemmArgs& a, int32_t x_type) {
+// launches, 4 tokens 18.0 against 16.1.  A D that lies over the tokens (the layer's result
+// replaces them) needs two launches, the tokens being quantised before the first store.
+bool use_fused(const Int8GemmArgs& a, const void* x, int32_t x_type, int64_t ldx) {
   return a.m <= kFusedTokens && a.m * a.k <= kFusedElems && x_type == a.d_type && !a.tile_n && !a.cta_group && !a.split_k &&
-         !a.flags;
+         !a.flags && !output_meets_tokens(a, x, ldx);
 }
 
 }  // namespace
@@ -1000,7 +1013,7 @@ extern "C" int gemm_sm100a_int8_launch(const Int8GemmArgs* args, void* stream) {
 extern "C" int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream) {
   Resolved r;
   memset(&r, 0, sizeof(r));
-  const bool few = args && args->struct_size == sizeof(Int8GemmArgs) && use_fused(*args, x_type);
+  const bool few = args && args->struct_size == sizeof(Int8GemmArgs) && use_fused(*args, x, x_type, ldx);
   const int rc = check(args, !few, r);
   if (rc != GEMM_OK) return rc;
   if (args->m == 0 || args->n == 0) return GEMM_OK;

@@ -339,7 +339,11 @@ PyObject* py_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
     Output d = output(v[6], g.m, g.n, x.dtype, x.index);
     g.lda = row_bytes(g.k);
     at::Tensor work;
-    if (g.m > 8 || g.m * g.k > 16384 || g.tile_n || g.cta_group || g.split_k || g.flags) {   // else no workspace is needed
+    const uint8_t* const x0 = static_cast<const uint8_t*>(x.ptr);
+    const uint8_t* const d0 = static_cast<const uint8_t*>(d.ptr);
+    const int64_t e = (int64_t)x.t->element_size();
+    const bool over = d.given && g.m > 0 && x0 < d0 + ((g.m - 1) * d.ld + g.n) * e && d0 < x0 + ((g.m - 1) * x.ld + g.k) * e;
+    if (g.m > 8 || g.m * g.k > 16384 || g.tile_n || g.cta_group || g.split_k || g.flags || over) {   // else no workspace is needed
       work = empty({g.m * (g.lda + 4) + 16}, at::kByte, x.index);                            // int8 tokens, then their scales
       uint8_t* const q = static_cast<uint8_t*>(work.data_ptr());
       g.a = q;

@@ -185,7 +185,8 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
                 residual: torch.Tensor | None = None, dropout: Dropout | None = None,
                 out: torch.Tensor | None = None, status: torch.Tensor | None = None, **knobs) -> torch.Tensor:
     """x . w^T of floating tokens and int8 weights: ``quantize_int8(x)`` and ``gemm_int8`` with
-    x's type as output, bit for bit, in one or two launches.
+    x's type as output, bit for bit, in one or two launches.  ``out`` (and ``residual`` with it) may
+    be ``x``.
 
     ``x`` (m, k); ``w`` (n, k) int8 and ``w_scale`` (n) as ``quantize_int8`` makes them."""
     return _host().linear(x, w, w_scale, bias, residual, dropout, out, status,

@@ -101,6 +101,30 @@ def test_linear_refuses_bad_tokens(pkg, x, x_type, ldx):
         pkg.ERR_BAD_ARGS, pkg.ERR_CANNOT_IMPLEMENT)
 
 
+def _linear(pkg, x, ldx, **kw):
+    """A linear layer of few tokens without a workspace.  No device memory is behind the addresses, so a call
+    that is accepted ends at the search for D's device."""
+    args = _gemm(pkg, a=None, scale_a=None, **kw)
+    return pkg.lib().gemm_sm100a_int8_linear(bytes(args), C.c_void_p(x), 0, ldx, None)
+
+
+def test_linear_over_its_tokens_needs_a_workspace(pkg):
+    """In one launch a CTA would store D where another one still reads its tokens."""
+    kw = dict(m=3, n=256, k=256, d=0x100000, ldd=256)
+    assert _linear(pkg, 0x200000, 256, **kw) == pkg.ERR_LAUNCH                # apart
+    assert _linear(pkg, 0x100000 + 3 * 512, 256, **kw) == pkg.ERR_LAUNCH      # right behind D
+    assert _linear(pkg, 0x100000, 256, **kw) == pkg.ERR_BAD_ARGS              # in place
+    assert _linear(pkg, 0x100000 + 3 * 512 - 2, 256, **kw) == pkg.ERR_BAD_ARGS
+    assert _linear(pkg, 0x100000 - 3 * 512 + 2, 256, **kw) == pkg.ERR_BAD_ARGS
+    assert _linear(pkg, 0x100000 - 3 * 512, 256, **kw) == pkg.ERR_LAUNCH
+    # columns of one buffer: side by side, and one element too near
+    kw["ldd"] = 600
+    assert _linear(pkg, 0x100000 + 512, 600, **kw) == pkg.ERR_LAUNCH
+    assert _linear(pkg, 0x100000 + 510, 600, **kw) == pkg.ERR_BAD_ARGS
+    assert _linear(pkg, 0x100000 + 688, 600, **kw) == pkg.ERR_LAUNCH
+    assert _linear(pkg, 0x100000 + 690, 600, **kw) == pkg.ERR_BAD_ARGS        # its rows end in D's next ones
+
+
 def _quant(pkg, **kw):
     a = pkg.Int8QuantArgs()
     a.struct_size = C.sizeof(pkg.Int8QuantArgs)

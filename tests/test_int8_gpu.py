@@ -468,6 +468,34 @@ def test_a_token_does_not_depend_on_its_batch(pkg, cuda):
         assert torch.equal(pkg.linear_int8(x[:m], w, ws), full[:m]), m
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [1, 3, 8, 9, 40])
+def test_linear_in_place(pkg, cuda, dtype, m):
+    """The result replaces the tokens, alone and added to them, while other streams keep SMs busy; and
+    out beside the tokens in one buffer, or a row further down in it."""
+    k = 1024
+    first = normal((m, k), 1, dtype)
+    w, ws = pkg.quantize_int8(normal((k, k), 2, scale=0.05))
+    plain, added = pkg.linear_int8(first, w, ws), pkg.linear_int8(first, w, ws, residual=first)
+    big, side = normal((4096, 4096), 3), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        x, y = first.clone(), first.clone()
+        with torch.cuda.stream(side):
+            pkg.dropout(big, pkg.Dropout(0.5), out=big)
+        assert pkg.linear_int8(x, w, ws, out=x) is x
+        pkg.linear_int8(y, w, ws, residual=y, out=y)
+        assert torch.equal(x, plain) and torch.equal(y, added)
+    both = torch.zeros((m, 2 * k), dtype=dtype, device="cuda")
+    both[:, :k] = first
+    pkg.linear_int8(both[:, :k], w, ws, out=both[:, k:])
+    assert torch.equal(both[:, k:], plain) and torch.equal(both[:, :k], first)
+    rows = torch.zeros((m + 1, k), dtype=dtype, device="cuda")
+    rows[:m] = first
+    pkg.linear_int8(rows[:m], w, ws, out=rows[1:])
+    assert torch.equal(rows[1:], plain) and torch.equal(rows[0], first[0])
+
+
 # ------------------------------------------------------------------ backward
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 64, 100), (5, 33, 7), (77, 300, 130), (333, 1000, 250), (600, 129, 1000)])
