@@ -388,8 +388,9 @@ int gemm_sm100a_quantize_int8(const Int8QuantArgs* args, void* stream);
  * with transpose = 1; dW n x k of dw_type.  dx, dw and dbias may each be NULL (not
  * wanted; wt is read for dx only, x for dw only).  m, n <= 131071 (sums over them).
  * workspace: gemm_sm100a_int8_backward_workspace(m, n, k) bytes, 16-byte aligned,
- * of this call alone until it has run.  m = 0 sets dW and dbias to 0.  Refusals come before the first
- * launch.  Asynchronous, capturable.
+ * of this call alone until it has run.  dX and dW may lie over X or dY (not over each
+ * other); dbias and the workspace overlap nothing.  m = 0 sets dW and dbias to 0.
+ * Refusals come before the first launch.  Asynchronous, capturable.
  */
 typedef struct Int8BackwardArgs {
   uint32_t struct_size;    /* sizeof(Int8BackwardArgs) */

@@ -107,19 +107,13 @@ extern "C" int gemm_sm100a_int8_linear_backward(const Int8BackwardArgs* a, void*
   const float* const zts = reinterpret_cast<const float*>(ws + w.zt_scale);
   const float* const xts = reinterpret_cast<const float*>(ws + w.xt_scale);
   int rc = GEMM_OK;
-  if (a->dx) {
-    rc = quantize(a->dy, n, a->lddy, false, &a->drop, w.z, w.z_scale, nullptr);
-    if (rc == GEMM_OK) rc = product(m, k, n, ws + w.z, row_bytes(n), zs, a->wt, a->ldwt, a->wt_scale, a->dx, a->lddx, a->type);
-    if (rc != GEMM_OK) return rc;
-  }
-  if (a->dw || a->dbias) {
-    rc = quantize(a->dy, n, a->lddy, true, &a->drop, w.zt, w.zt_scale, a->dbias);
-    if (rc != GEMM_OK) return rc;
-  }
-  if (a->dw) {
-    rc = quantize(a->x, k, a->ldx, true, nullptr, w.xt, w.xt_scale, nullptr);
-    if (rc == GEMM_OK)
-      rc = product(n, k, m, ws + w.zt, row_bytes(m), zts, ws + w.xt, row_bytes(m), xts, a->dw, a->lddw, a->dw_type);
-  }
+  // All quantisations before the first product: dX and dW may replace X or dY.
+  if (a->dx) rc = quantize(a->dy, n, a->lddy, false, &a->drop, w.z, w.z_scale, nullptr);
+  if (rc == GEMM_OK && (a->dw || a->dbias)) rc = quantize(a->dy, n, a->lddy, true, &a->drop, w.zt, w.zt_scale, a->dbias);
+  if (rc == GEMM_OK && a->dw) rc = quantize(a->x, k, a->ldx, true, nullptr, w.xt, w.xt_scale, nullptr);
+  if (rc == GEMM_OK && a->dx)
+    rc = product(m, k, n, ws + w.z, row_bytes(n), zs, a->wt, a->ldwt, a->wt_scale, a->dx, a->lddx, a->type);
+  if (rc == GEMM_OK && a->dw)
+    rc = product(n, k, m, ws + w.zt, row_bytes(m), zts, ws + w.xt, row_bytes(m), xts, a->dw, a->lddw, a->dw_type);
   return rc;
 }

@@ -577,6 +577,34 @@ def test_backward_of_some_gradients(pkg, cuda, wanted):
     assert (work[need:] == 77).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("over", ["x", "dy", "dw"])
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_backward_over_its_inputs(pkg, cuda, dtype, over, p):
+    """dX in the place of X or of dY, and dX in the place of dY with dW in the place of X."""
+    import ctypes
+    m = n = k = 96
+    dy, x = normal((m, n), 1, dtype), normal((m, k), 2, dtype)
+    wt, wts = pkg.quantize_int8(normal((n, k), 3, scale=0.02), transpose=True)
+    drop = pkg.Dropout(p, seed=8) if p else None
+    want = pkg.linear_int8_backward(dy, x, wt, wts, dropout=drop, dw_dtype=dtype)
+    dx = x if over == "x" else dy
+    dw = x if over == "dw" else torch.empty((n, k), dtype=dtype, device="cuda")
+    db = torch.empty((n,), device="cuda")
+    need = pkg.lib().gemm_sm100a_int8_backward_workspace(m, n, k)
+    work = torch.empty((need,), dtype=torch.uint8, device="cuda")
+    code = TYPES.index(dtype)
+    a = pkg.Int8BackwardArgs(struct_size=0, type=code, m=m, n=n, k=k, dy=dy.data_ptr(), lddy=n, x=x.data_ptr(), ldx=k,
+                             wt=wt.data_ptr(), ldwt=wt.stride(0), wt_scale=wts.data_ptr(), dx=dx.data_ptr(), lddx=k,
+                             dw=dw.data_ptr(), lddw=k, dbias=db.data_ptr(), dw_type=code, workspace=work.data_ptr(),
+                             workspace_bytes=need)
+    a.struct_size = ctypes.sizeof(a)
+    a.drop.p, a.drop.seed, a.drop.row_elems = p, 8, n
+    assert pkg.lib().gemm_sm100a_int8_linear_backward(bytes(a), torch.cuda.current_stream().cuda_stream) == pkg.OK
+    for got, t in zip((dx, dw, db), want):
+        assert torch.equal(got, t)
+
+
 def test_backward_of_no_tokens(pkg, cuda):
     wt, wts = pkg.quantize_int8(normal((20, 30), 3), transpose=True)
     dx, dw, db = pkg.linear_int8_backward(torch.empty((0, 20), device="cuda"), torch.empty((0, 30), device="cuda"), wt, wts)
