@@ -917,23 +917,30 @@ struct Tokens {        // floating tokens of the fused form
   int64_t ldx;
 };
 
-// One product; the device of D is current.
-int launch_product(const Int8GemmArgs& a, const Tokens* tokens, cudaStream_t st, int dev) {
+// A product that is ready to be launched: nothing can refuse it any more.
+struct Prepared {
   Resolved r;
+  CUtensorMap tw, tt, td, tc;
+  KernelFn fn;
+  int threads;
+};
+
+// The device of D is current.
+int prepare_product(const Int8GemmArgs& a, const Tokens* tokens, int dev, Prepared& q) {
+  Resolved& r = q.r;
   const int rc = resolve(&a, tokens != nullptr, r);
   if (rc != GEMM_OK) return rc;
   if (!get_encode()) return GEMM_ERR_LAUNCH;
-  CUtensorMap tw, tt, td, tc;
-  memset(&tt, 0, sizeof(tt));
-  memset(&td, 0, sizeof(td));
-  memset(&tc, 0, sizeof(tc));
-  if (!encode_2d(&tw, a.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.ldb, kAtom, kChannels, 128))
+  memset(&q.tt, 0, sizeof(q.tt));
+  memset(&q.td, 0, sizeof(q.td));
+  memset(&q.tc, 0, sizeof(q.tc));
+  if (!encode_2d(&q.tw, a.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.n, (uint64_t)a.ldb, kAtom, kChannels, 128))
     return GEMM_ERR_CANNOT_IMPLEMENT;
   if (tokens) {
     r.p.x = tokens->x;
     r.p.ldx = tokens->ldx;
     r.p.x_wide = rows_16b(tokens->x, tokens->ldx, type_bytes(a.d_type)) ? 1 : 0;
-  } else if (!encode_2d(&tt, a.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.m, (uint64_t)a.lda, kAtom,
+  } else if (!encode_2d(&q.tt, a.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)a.k, (uint64_t)a.m, (uint64_t)a.lda, kAtom,
                         (uint32_t)(r.bn / r.cg), 128)) {
     return GEMM_ERR_CANNOT_IMPLEMENT;
   }
@@ -941,17 +948,22 @@ int launch_product(const Int8GemmArgs& a, const Tokens* tokens, cudaStream_t st,
     const CUtensorMapDataType t = a.d_type == GEMM_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                 : a.d_type == GEMM_TYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
     const uint32_t tokens_box = (uint32_t)(r.bn < 32 ? r.bn : 32);
-    if (!encode_2d(&td, a.d, t, (uint64_t)a.n, (uint64_t)a.m, (uint64_t)(a.ldd * type_bytes(a.d_type)), kChannels, tokens_box, 0))
+    if (!encode_2d(&q.td, a.d, t, (uint64_t)a.n, (uint64_t)a.m, (uint64_t)(a.ldd * type_bytes(a.d_type)), kChannels, tokens_box, 0))
       return GEMM_ERR_CANNOT_IMPLEMENT;
     if (r.p.c_staged &&
-        !encode_2d(&tc, a.c, t, (uint64_t)a.n, (uint64_t)a.m, (uint64_t)(a.ldc * type_bytes(a.d_type)), kChannels, tokens_box, 0))
+        !encode_2d(&q.tc, a.c, t, (uint64_t)a.n, (uint64_t)a.m, (uint64_t)(a.ldc * type_bytes(a.d_type)), kChannels, tokens_box, 0))
       return GEMM_ERR_CANNOT_IMPLEMENT;
   }
-  KernelFn fn = a.d_type == GEMM_TYPE_BF16 ? pick<__nv_bfloat16>(r.cg, r.bn, tokens != nullptr)
-              : a.d_type == GEMM_TYPE_FP16 ? pick<__half>(r.cg, r.bn, tokens != nullptr) : pick<float>(r.cg, r.bn, tokens != nullptr);
-  if (!ensure_smem_attr(fn, dev, tokens ? kSmemLimit - kStaticSmem : kSmemLimit)) return GEMM_ERR_LAUNCH;
-  if (launch_overlapped(fn, dim3((unsigned)r.grid), dim3(tokens ? threads_for(1, true) : 64 + 128 * r.p.groups), (size_t)r.smem_bytes,
-                        r.split > 1 ? r.split : r.cg, st, tw, tt, td, tc, r.p) != cudaSuccess) {
+  q.fn = a.d_type == GEMM_TYPE_BF16 ? pick<__nv_bfloat16>(r.cg, r.bn, tokens != nullptr)
+       : a.d_type == GEMM_TYPE_FP16 ? pick<__half>(r.cg, r.bn, tokens != nullptr) : pick<float>(r.cg, r.bn, tokens != nullptr);
+  q.threads = tokens ? threads_for(1, true) : 64 + 128 * r.p.groups;
+  return ensure_smem_attr(q.fn, dev, tokens ? kSmemLimit - kStaticSmem : kSmemLimit) ? GEMM_OK : GEMM_ERR_LAUNCH;
+}
+
+int launch_prepared(const Prepared& q, cudaStream_t st) {
+  const Resolved& r = q.r;
+  if (launch_overlapped(q.fn, dim3((unsigned)r.grid), dim3((unsigned)q.threads), (size_t)r.smem_bytes,
+                        r.split > 1 ? r.split : r.cg, st, q.tw, q.tt, q.td, q.tc, r.p) != cudaSuccess) {
     cudaGetLastError();
     return GEMM_ERR_LAUNCH;
   }
@@ -1007,7 +1019,9 @@ extern "C" int gemm_sm100a_int8_launch(const Int8GemmArgs* args, void* stream) {
   if (args->m == 0 || args->n == 0) return GEMM_OK;
   PointerDeviceGuard guard(args->d);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
-  return launch_product(*args, nullptr, reinterpret_cast<cudaStream_t>(stream), guard.dev);
+  Prepared q;
+  const int rp = prepare_product(*args, nullptr, guard.dev, q);
+  return rp != GEMM_OK ? rp : launch_prepared(q, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream) {
@@ -1023,15 +1037,19 @@ extern "C" int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, 
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   PointerDeviceGuard guard(args->d);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
-  if (few) {
-    const Tokens tokens = {x, ldx};
-    return launch_product(*args, &tokens, st, guard.dev);
+  // The product is prepared before the tokens are quantised: a refused call launches nothing.
+  const Tokens tokens = {x, ldx};
+  Prepared p;
+  const int rp = prepare_product(*args, few ? &tokens : nullptr, guard.dev, p);
+  if (rp != GEMM_OK) return rp;
+  if (!few) {
+    Int8QuantArgs q;
+    memset(&q, 0, sizeof(q));
+    q.struct_size = sizeof(q);
+    q.x_type = x_type; q.rows = args->m; q.cols = args->k; q.x = x; q.ldx = ldx;
+    q.q = const_cast<void*>(args->a); q.ldq = args->lda; q.scale = const_cast<float*>(args->scale_a);
+    const int rq = gemm_sm100a_quantize_int8(&q, stream);
+    if (rq != GEMM_OK) return rq;
   }
-  Int8QuantArgs q;
-  memset(&q, 0, sizeof(q));
-  q.struct_size = sizeof(q);
-  q.x_type = x_type; q.rows = args->m; q.cols = args->k; q.x = x; q.ldx = ldx;
-  q.q = const_cast<void*>(args->a); q.ldq = args->lda; q.scale = const_cast<float*>(args->scale_a);
-  const int rq = gemm_sm100a_quantize_int8(&q, stream);
-  return rq != GEMM_OK ? rq : launch_product(*args, nullptr, st, guard.dev);
+  return launch_prepared(p, st);
 }

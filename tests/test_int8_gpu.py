@@ -439,6 +439,26 @@ def test_linear_is_quantise_then_product(pkg, cuda, dtype, m, n, k):
         check_close(y, *want, scale_err=U32)
 
 
+def test_linear_refuses_knobs_before_it_quantises(pkg, cuda):
+    """A refused call launches nothing: the workspace and the output stay as they were."""
+    import ctypes
+    m, n, k = 20, 64, 512
+    x = normal((m, k), 1, torch.bfloat16)
+    w, ws = pkg.quantize_int8(normal((n, k), 2))
+    work, scale = torch.full((m, k), 77, dtype=torch.int8, device="cuda"), torch.full((m,), 77.0, device="cuda")
+    out = torch.full((m, n), 77.0, dtype=torch.bfloat16, device="cuda")
+    for knobs in (dict(tile_n=48), dict(cta_group=3), dict(cta_group=2, tile_n=64), dict(split_k=3), dict(split_k=8),
+                  dict(cta_group=2, tile_n=256, split_k=2)):
+        a = pkg.Int8GemmArgs(struct_size=0, d_type=0, m=m, n=n, k=k, a=work.data_ptr(), lda=k, b=w.data_ptr(),
+                             ldb=w.stride(0), d=out.data_ptr(), ldd=n, scale_a=scale.data_ptr(), scale_b=ws.data_ptr(), **knobs)
+        a.struct_size = ctypes.sizeof(a)
+        rc = pkg.lib().gemm_sm100a_int8_linear(bytes(a), x.data_ptr(), 0, k, torch.cuda.current_stream().cuda_stream)
+        assert rc == pkg.ERR_CANNOT_IMPLEMENT
+        assert (work == 77).all() and (scale == 77).all() and (out == 77).all()
+        with pytest.raises(pkg.GemmError):
+            pkg.linear_int8(x, w, ws, **knobs)
+
+
 def test_linear_strided_tokens(pkg, cuda):
     big = normal((70, 700), 1, torch.bfloat16)
     w, ws = pkg.quantize_int8(normal((300, 513), 5, scale=0.02))
