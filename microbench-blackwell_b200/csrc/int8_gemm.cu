@@ -155,6 +155,7 @@ __device__ __forceinline__ void stage_tokens(const Int8Params& p, uint32_t tok, 
     }
   };
   if (tid < kFusedTokens) top[tid] = 0u;
+  __syncwarp();
   named_bar_sync(2, N);
   walk(0, nvec, [&](int t, int e, const Vec<X>& v) {
     // One shared atomic per warp where its vectors are of one token.
@@ -167,11 +168,13 @@ __device__ __forceinline__ void stage_tokens(const Int8Params& p, uint32_t tok, 
       atomicMax(&top[t], m);
     }
   });
+  __syncwarp();
   named_bar_sync(2, N);
   if (tid < p.m) {
     rows[tid] = row_scale(top[tid]);
     st_shared_u32(sa_s + 4u * tid, __float_as_uint(rows[tid].scale));
   }
+  __syncwarp();
   named_bar_sync(2, N);
   const int e0 = kb_begin * (kAtom / V), e1 = min(nvec, kb_end * (kAtom / V));
   walk(e0, e1 - e0, [&](int t, int e, const Vec<X>& v) {
@@ -278,6 +281,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
     for (int g = 0; g < kMaxGroups; ++g) st_shared_u32(lost_flag0 + 4u * g, 0u);
     fence_mbar_init();
   }
+  __syncwarp();   // here and below: barriers and tensor memory instructions need a warp's lanes together
   if constexpr (CG == 2) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
   // Until here nothing of this launch depended on the kernels before it, and it holds
   // no tensor memory while it waits for them (one of them might still need some).
@@ -489,6 +493,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         // whichever gave up (here or on a chunk of C) says so before the first barrier, and
         // none can say so again before all have looked.
         if (!ok && lane == 0) st_shared_u32(lost_flag, 1u);
+        __syncwarp();
         named_bar_sync(bar_id, 128);
         const bool lost = ld_shared_volatile_u32(lost_flag) != 0u;
         named_bar_sync(bar_id, 128);
@@ -511,6 +516,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       }
 #pragma unroll 1
       for (int i = (int)grp; i < NCH; i += groups) {
+        __syncwarp();
         uint32_t r[CW];
         if constexpr (CW == 32) tmem_ld32(t_row + (uint32_t)(i * CW), r); else tmem_ld16(t_row + (uint32_t)(i * CW), r);
         tmem_ld_wait();
@@ -600,6 +606,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
             for (int j = 0; j < CW; ++j) v[j] += staged<T>(at + (uint32_t)(j * kChannels * (int)sizeof(T)));
           } else {
             if (issuer) bulk_wait_group_read<1>();
+            __syncwarp();
             named_bar_sync(bar_id, 128);
           }
 #pragma unroll

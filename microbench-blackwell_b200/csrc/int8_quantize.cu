@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(32 * kColWarps) quantize_cols_kernel(const __g
     cta_max[threadIdx.x] = m;
     cta_sum[threadIdx.x] = s;
   }
+  __syncwarp();
   cluster.sync();
   // One thread per column combines the peers' results.
   if (threadIdx.x < COLS) {
@@ -329,6 +330,7 @@ __global__ void __launch_bounds__(32 * kColWarps) quantize_cols_kernel(const __g
       store(c0 + 1, qa + p.ldq, w1);
     }
   }
+  __syncwarp();                      // sets of a warp end at different rows; the wait needs all its lanes together
   sm100::cluster_wait();             // until the peers have read this CTA's
 }
 

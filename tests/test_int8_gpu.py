@@ -127,6 +127,18 @@ def test_quantize_transposed_long_columns(pkg, cuda, dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [255, 272, 500, 700, 1000, 1025, 1290, 1300, 1537, 1792, 1793, 2040])
+def test_quantize_transposed_every_cluster_size(pkg, cuda, dtype, rows):
+    """One to eight CTAs per strip, rows that fill the last 16-row sets of a warp unevenly, strips that
+    end inside 64 bytes."""
+    x = normal((rows, 83), rows + 1, dtype)
+    q, scale, sums = pkg.quantize_int8(x, transpose=True, column_sums=True)
+    check_quantized(q, scale, x.t())
+    # A thread adds at most ceil(256 / 32) rows of a CTA, then 3 + 4 + 8 partial sums of lanes, warps and CTAs.
+    assert ((sums.double() - x.double().sum(0)).abs() <= 24 * U32 * x.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_quantize_ties_go_to_even(pkg, cuda, dtype):
     """amax = 254 makes every odd value a tie: 127 x / 254 = x / 2."""
     x = torch.arange(-254, 255, device="cuda", dtype=torch.float32)
