@@ -59,6 +59,10 @@ __host__ __device__ constexpr int threads_for(int cg, bool fuse) {
   return 64 + (fuse ? 32 * kStageWarps : 128 * (cg == 2 ? kMaxGroups : 1));
 }
 constexpr int kSmemLimit = 232448;      // 227 KiB of opt-in dynamic shared memory per CTA
+// More than half of an SM's 228 KiB: at most one CTA of these kernels, or of the floating product's,
+// per SM.  A CTA waits for tensor memory without a limit, and those of a pair or a split for one another:
+// two kernels of different streams that share two SMs could each hold what the other one's CTA waits for.
+constexpr int kMinSmemPerCta = 120 * 1024;
 constexpr int kBarrierBytes = 1024;
 constexpr int kStaticSmem = 512;        // bound of the static shared memory of the fused form
 constexpr int kMaxStages = 32;
@@ -876,6 +880,7 @@ int resolve(const Int8GemmArgs* a, bool fused, Resolved& r) {
   p.k = (int32_t)a->k;
   p.sa_offset = p.stg_offset + (uint32_t)(p.groups * p.stg_bufs) * p.stg_bytes;
   r.smem_bytes = 1024 + (int64_t)p.sa_offset + p.groups * 4 * r.bn * 4;
+  if (r.smem_bytes < kMinSmemPerCta) r.smem_bytes = kMinSmemPerCta;
   p.status = a->status;
   p.timeout_ns = (uint64_t)(a->timeout_ms ? a->timeout_ms : 4000u) * 1000000ull;
   p.flags = a->flags;

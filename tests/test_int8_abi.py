@@ -80,6 +80,18 @@ def test_refused_products(pkg, kw, rc, frag):
     assert L.gemm_sm100a_int8_linear(bytes(_gemm(pkg, **kw)), C.c_void_p(0x70000), 0, 256, None) == got
 
 
+@pytest.mark.parametrize("d_type", [0, 1, 2])
+@pytest.mark.parametrize("knobs", [dict()] + [dict(cta_group=1, tile_n=bn, split_k=s) for bn in (16, 32, 64, 128)
+                                              for s in (1, 2, 4, 8)] + [dict(cta_group=2, tile_n=bn) for bn in (128, 256)])
+def test_one_cta_per_sm(pkg, d_type, knobs):
+    """CTAs of a split or a pair wait for one another and, without a limit, for tensor memory: two kernels must
+    not share SMs, or each could hold what the other one waits for.  An SM has 228 KiB of shared memory."""
+    for k in (1024, 1152, 4096, 20000):
+        for c in (None, 0x60000):
+            rc, info = pkg.query_int8(_gemm(pkg, k=k, lda=20480, ldb=20480, d_type=d_type, c=c, ldc=128, **knobs))
+            assert rc == pkg.OK and 2 * info.smem_bytes > 228 * 1024 and info.smem_bytes <= 227 * 1024
+
+
 def test_null_argument_blocks(pkg):
     L = pkg.lib()
     assert L.gemm_sm100a_int8_launch(None, None) == pkg.ERR_BAD_ARGS
