@@ -36,6 +36,15 @@ __device__ __forceinline__ float load_as_f32(const void* p, int t, int64_t i) {
 __device__ __forceinline__ float finish(int32_t acc, float sa, float sb, float bias) {
   return fmaf(__int2float_rn(acc) * sa, sb, bias);
 }
+// The sum times a larger scale than this might leave the range of fp32 (2^31 * 2^96 does not)
+// where the output does not.  The channel's scale then comes first: only if it is as
+// large too can that product overflow, and so does the output.
+constexpr float kLargeScale = 0x1p96f;
+__device__ __forceinline__ bool is_large(float sa) { return fabsf(sa) > kLargeScale; }
+__device__ __forceinline__ float finish_large(int32_t acc, float sa, float sb, float bias) {
+  const bool large = is_large(sa);
+  return finish(acc, large ? sb : sa, large ? sa : sb, bias);
+}
 
 // Two 16-bit values, rounded, the first in the low half.
 template <typename T>

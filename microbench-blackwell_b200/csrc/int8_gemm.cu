@@ -480,15 +480,21 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
       const bool ch_ok = ch < p.n;
       const float sb = ch_ok ? (p.sb ? p.sb[ch] : 1.f) : 0.f;
       const float bias = ch_ok && p.bias ? load_as_f32(p.bias, p.bias_type, ch) : 0.f;
+      bool large = false;    // one of the tile's tokens has a large scale
       if constexpr (!FUSE) {
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < (BN + 31) / 32; ++i) {
           const int t = i * 32 + (int)lane;
-          if (t < BN) st_shared_u32(sa_s + 4u * t, __float_as_uint(t0 + t < p.m ? (p.sa ? p.sa[t0 + t] : 1.f) : 0.f));
+          const float sa = t < BN && t0 + t < p.m ? (p.sa ? p.sa[t0 + t] : 1.f) : 0.f;
+          large |= is_large(sa);
+          if (t < BN) st_shared_u32(sa_s + 4u * t, __float_as_uint(sa));
         }
         __syncwarp();
+      } else {
+        large = (int)lane < p.m && is_large(tok_rows[lane & (kFusedTokens - 1)].scale);
       }
+      large = __any_sync(0xFFFFFFFFu, large);
       const bool ok = __all_sync(0xffffffffu, wait_bar<false>(tfull_bar + 8u * acc, acc_phase, ctl, ROLE_EPILOGUE, acc));
       if (!p.tma_store) {
         if (!ok) break;
@@ -533,13 +539,19 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
         }
         const int tc = t0 + i * CW;
         float v[CW];
+        if (!large) {
 #pragma unroll
-        for (int j = 0; j < CW; j += 4) {
-          const uint4 sa = ld_shared_v4(sa_s + 4u * (uint32_t)(i * CW + j));
-          v[j] = finish((int32_t)r[j], __uint_as_float(sa.x), sb, bias);
-          v[j + 1] = finish((int32_t)r[j + 1], __uint_as_float(sa.y), sb, bias);
-          v[j + 2] = finish((int32_t)r[j + 2], __uint_as_float(sa.z), sb, bias);
-          v[j + 3] = finish((int32_t)r[j + 3], __uint_as_float(sa.w), sb, bias);
+          for (int j = 0; j < CW; j += 4) {
+            const uint4 sa = ld_shared_v4(sa_s + 4u * (uint32_t)(i * CW + j));
+            v[j] = finish((int32_t)r[j], __uint_as_float(sa.x), sb, bias);
+            v[j + 1] = finish((int32_t)r[j + 1], __uint_as_float(sa.y), sb, bias);
+            v[j + 2] = finish((int32_t)r[j + 2], __uint_as_float(sa.z), sb, bias);
+            v[j + 3] = finish((int32_t)r[j + 3], __uint_as_float(sa.w), sb, bias);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < CW; ++j)
+            v[j] = finish_large((int32_t)r[j], __uint_as_float(ld_shared_u32(sa_s + 4u * (uint32_t)(i * CW + j))), sb, bias);
         }
         if (p.drop.on) {
           const int64_t index = drop_index(p.drop, tc, ch);
@@ -693,7 +705,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: chann
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               if (ch0 + e >= p.n) continue;
-              float v = finish((int32_t)sum[e], sa, sb[e], bias[e]);
+              float v = finish_large((int32_t)sum[e], sa, sb[e], bias[e]);
               if (p.drop.on) v = drop_keeps(p.drop, key, drop_index(p.drop, t, ch0 + e)) ? v * p.drop.grow : 0.f;
               if (p.c) v += to_f32(static_cast<const T*>(p.c)[(int64_t)t * p.ldc + ch0 + e]);
               d[e] = from_f32<T>(v);

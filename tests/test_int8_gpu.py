@@ -387,6 +387,42 @@ def test_product_extreme_sums(pkg, cuda):
         check_close(d, want, want.abs())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("knobs", [dict()] + [dict(cta_group=1, tile_n=64, split_k=s) for s in (1, 4)]
+                         + [dict(cta_group=2, tile_n=bn) for bn in (128, 256)], ids=str)
+def test_product_scales_far_from_one(pkg, cuda, dtype, knobs):
+    """Outputs of ordinary size from scales whose product with the sum alone would leave fp32, some tokens'
+    large, some channels', zero channels among them."""
+    m, n, k = 301, 520, 1024
+    a, b, bias, residual = int8s(pkg, m, k, 1), int8s(pkg, n, k, 2), normal((n,), 3), normal((m, n), 4, dtype)
+    for rows, lift in ((m, 2.0 ** 120), (m, 2.0 ** -110), (5, 2.0 ** 120), (1, 2.0 ** 96)):
+        sa, sb = scales(m, 3) * 0.01 * lift, scales(n, 4) / lift
+        sb[::7] = 0.0
+        if rows == m:
+            sa[::3] /= min(lift, 2.0 ** 100)           # ordinary tokens in the same tile
+        for kw in (dict(), dict(bias=bias, residual=residual[:rows], dropout=pkg.Dropout(0.25, seed=2))):
+            d = pkg.gemm_int8(a[:rows], sa[:rows].contiguous(), b, sb, out_dtype=dtype, **kw, **knobs)
+            want, size = ref_product(a[:rows], sa[:rows], b, sb, kw.get("bias"), kw.get("residual"), kw.get("dropout"))
+            # Ordinary tokens with large channels: what lies half a step beyond the type's largest value rounds to Inf
+            # (fp16 from 65520; the step above a value v <= 65504 is at least eps v / 2).
+            top = torch.finfo(dtype).max
+            over = want.abs() > top * (1 + torch.finfo(dtype).eps)
+            assert torch.equal(d[over].double(), want[over].sign() * math.inf)
+            check_close(torch.where(over, 0.0, d).to(dtype), torch.where(over, 0.0, want), size.clamp(max=top))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 512), (1, 16000), (8, 2048), (8, 130), (60, 512), (400, 640)])
+def test_linear_of_tokens_far_from_one(pkg, cuda, dtype, m, k):
+    """Tokens next to the end of fp32's range, and small weights: whole-K, split and one-launch forms."""
+    x, n = (normal((m, k), 1).double().clamp(-3, 3) * 1e37).to(dtype), 300
+    w, ws = pkg.quantize_int8((normal((n, k), 2).double() * 1e-34).float())
+    y = pkg.linear_int8(x, w, ws)
+    check_close(y, *ref_product(*ref_quantize(x), w, ws), scale_err=U32)
+    q, s = pkg.quantize_int8(x)
+    assert torch.equal(y, pkg.gemm_int8(q, s, w, ws, out_dtype=dtype))
+
+
 def test_product_nan_rows_touch_only_themselves(pkg, cuda):
     m, n, k = 40, 200, 256
     a, b, sa, sb = int8s(pkg, m, k, 1), int8s(pkg, n, k, 2), scales(m, 3), scales(n, 4)
