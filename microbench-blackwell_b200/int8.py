@@ -145,6 +145,8 @@ def _knob_values(knobs):
 def empty_int8(rows: int, cols: int, device) -> torch.Tensor:
     """An int8 matrix whose row stride is a multiple of 16 bytes (of 128 for more than 64 columns)."""
     device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"an int8 matrix for these operators is on a CUDA device, not on {device}")
     index = torch.cuda.current_device() if device.index is None else device.index
     return _host().empty(rows, cols, index)
 

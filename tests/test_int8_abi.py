@@ -240,3 +240,10 @@ def test_python_helpers_refuse_host_tensors(pkg):
         pkg.quantize_int8(x.to(torch.float64))
     with pytest.raises(ValueError):
         pkg.quantize_int8(x[0])
+
+
+@pytest.mark.parametrize("device", ["cpu", "meta", torch.device("cpu")])
+def test_int8_matrices_are_on_cuda_devices(pkg, device):
+    """A device of another kind is refused, not replaced by the current CUDA device."""
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.empty_int8(4, 32, device)
