@@ -351,7 +351,10 @@ PyObject* py_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     g.b = w.ptr; g.ldb = w.ld; g.d = d.ptr; g.ldd = d.ld;
     const int rc = gemm_sm100a_int8_linear(&g, x.ptr, code, x.ld, stream_of(x.index));
-    if (rc != GEMM_OK) failed_product(rc, g, "gemm_sm100a_int8_linear");
+    if (rc != GEMM_OK) {
+      if (!g.a) g.a = g.b;   // for the reason only: without a workspace the query would name its absence
+      failed_product(rc, g, "gemm_sm100a_int8_linear");
+    }
     return d.wrap();
   });
 }

@@ -507,6 +507,19 @@ def test_linear_refuses_knobs_before_it_quantises(pkg, cuda):
             pkg.linear_int8(x, w, ws, **knobs)
 
 
+@pytest.mark.parametrize("m", [1, 8, 40])
+def test_linear_names_the_reason_of_a_refusal(pkg, cuda, m):
+    """The same one with and without a workspace for the tokens."""
+    w, ws = pkg.quantize_int8(normal((50, 64), 2))
+    x = normal((m, 64), 1)
+    for reason, call in (("16-byte aligned", lambda: pkg.linear_int8(x[:, 1:17], w[:, 1:17], ws)),
+                         ("empty problem", lambda: pkg.linear_int8(x[:, :0], w[:, :0], ws)),
+                         ("dropout p", lambda: pkg.linear_int8(x, w, ws, dropout=pkg.Dropout(1.5))),
+                         ("row_elems", lambda: pkg.linear_int8(x, w, ws, dropout=pkg.Dropout(0.5, row_elems=49)))):
+        with pytest.raises(pkg.GemmError, match=reason):
+            call()
+
+
 def test_linear_strided_tokens(pkg, cuda):
     big = normal((70, 700), 1, torch.bfloat16)
     w, ws = pkg.quantize_int8(normal((300, 513), 5, scale=0.02))
