@@ -53,65 +53,62 @@ __global__ void __launch_bounds__(row_threads(NV)) quantize_rows_kernel(const __
   sm100::grid_dependency_wait();
   sm100::grid_launch_dependents();
   const uint64_t key = DROP ? drop_key(p.drop) : 0;
-  for (int64_t row0 = (int64_t)blockIdx.x * blockDim.y; row0 < p.rows; row0 += (int64_t)gridDim.x * blockDim.y) {
-    const int64_t row = row0 + threadIdx.y;
-    const bool live = row < p.rows;
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    Vec<T> v[NV];
-    auto load = [&](int chunk) {
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const bool live = row < p.rows;
+  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+  Vec<T> v[NV];
+  auto load = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = (chunk * per_chunk + i * TX + tx) * V;
+      v[i] = load_vec<T>(x + e, live ? (int)min((int64_t)V, p.cols - e) : 0, p.wide);
+    }
+    if constexpr (DROP) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int e = (chunk * per_chunk + i * TX + tx) * V;
-        v[i] = load_vec<T>(x + e, live ? (int)min((int64_t)V, p.cols - e) : 0, p.wide);
+        const int64_t e = (int64_t)(chunk * per_chunk + i * TX + tx) * V;
+        drop_vec<T>(p.drop, key, drop_index(p.drop, row, e), v[i]);
       }
-      if constexpr (DROP) {
+    }
+  };
+  uint32_t top = 0;   // largest |x| so far: packed halves (16-bit T) or fp32 bits
+  for (int c = 0; c < chunks; ++c) {
+    load(c);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int64_t e = (int64_t)(chunk * per_chunk + i * TX + tx) * V;
-          drop_vec<T>(p.drop, key, drop_index(p.drop, row, e), v[i]);
-        }
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) top = max(top, v[i].w[j] & 0x7FFFFFFFu);
+        else top = __vmaxu2(top, v[i].w[j] & 0x7FFF7FFFu);
       }
-    };
-    uint32_t top = 0;   // largest |x| so far: packed halves (16-bit T) or fp32 bits
-    for (int c = 0; c < chunks; ++c) {
-      load(c);
+  }
+  if constexpr (sizeof(T) == 2) top = abs_bits_to_f32<T>(max(top & 0xFFFFu, top >> 16));
+  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  if (TX > 32) {
+    const int warp = threadIdx.y * (TX >> 5) + (tx >> 5);
+    if ((tx & 31) == 0) warp_max[warp] = top;
+    __syncthreads();
+    const int w = tx & 31;
+    top = __reduce_max_sync(0xFFFFFFFFu, w < (TX >> 5) ? warp_max[threadIdx.y * (TX >> 5) + w] : 0u);
+  }
+  const RowScale s = row_scale(top);
+  if (live && tx == 0) p.scale[row] = DROP ? s.scale * p.drop.grow : s.scale;
+  for (int c = 0; c < chunks; ++c) {
+    if (chunks > 1) load(c);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      const int e = (c * per_chunk + i * TX + tx) * V;
+      if (!live || e >= p.cols) continue;
+      uint32_t w[V / 4];
+      quantize_vec<T>(v[i], s, w);
+      uint8_t* q = p.q + row * p.ldq + e;
+      if (p.cols - e >= V) {
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(q) = w[0];
+      } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (sizeof(T) == 4) top = max(top, v[i].w[j] & 0x7FFFFFFFu);
-          else top = __vmaxu2(top, v[i].w[j] & 0x7FFF7FFFu);
-        }
-    }
-    if constexpr (sizeof(T) == 2) top = abs_bits_to_f32<T>(max(top & 0xFFFFu, top >> 16));
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if (TX > 32) {
-      const int warp = threadIdx.y * (TX >> 5) + (tx >> 5);
-      if ((tx & 31) == 0) warp_max[warp] = top;
-      __syncthreads();
-      const int w = tx & 31;
-      top = __reduce_max_sync(0xFFFFFFFFu, w < (TX >> 5) ? warp_max[threadIdx.y * (TX >> 5) + w] : 0u);
-      __syncthreads();
-    }
-    const RowScale s = row_scale(top);
-    if (live && tx == 0) p.scale[row] = DROP ? s.scale * p.drop.grow : s.scale;
-    for (int c = 0; c < chunks; ++c) {
-      if (chunks > 1) load(c);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int e = (c * per_chunk + i * TX + tx) * V;
-        if (!live || e >= p.cols) continue;
-        uint32_t w[V / 4];
-        quantize_vec<T>(v[i], s, w);
-        uint8_t* q = p.q + row * p.ldq + e;
-        if (p.cols - e >= V) {
-          if constexpr (V == 8) *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
-          else *reinterpret_cast<uint32_t*>(q) = w[0];
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (e + j < p.cols) q[j] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
-        }
+        for (int j = 0; j < V; ++j)
+          if (e + j < p.cols) q[j] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
       }
     }
   }
@@ -342,8 +339,7 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
   tx = (tx + 31) / 32 * 32;
   if (tx > row_threads(NV)) tx = row_threads(NV);
   const int ry = tx >= 128 ? 1 : (int)(128 / tx);
-  int64_t blocks = (p.rows + ry - 1) / ry;
-  if (blocks > 0x7FFFFFFF) blocks = 0x7FFFFFFF;
+  const int64_t blocks = (p.rows + ry - 1) / ry;   // at most 2^30
   return launch_overlapped(quantize_rows_kernel<T, NV, DROP>, dim3((unsigned)blocks), dim3((unsigned)tx, (unsigned)ry), 0, 1, st, p);
 }
 // Many loads in flight per thread for large X; two where one wave of threads covers

@@ -999,6 +999,26 @@ def test_host_memory_is_refused(pkg, cuda):
     assert torch.equal(pkg.dropout(x, pkg.Dropout(0.0)), x)
 
 
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int8, torch.int32, torch.bool, torch.complex64, torch.float8_e4m3fn])
+def test_other_types_are_refused(pkg, cuda, dtype):
+    """Tensors on the device, of types that no kernel reads."""
+    bad, good = torch.zeros((4, 64), device="cuda").to(dtype), torch.zeros((4, 64), device="cuda")
+    w, ws = pkg.quantize_int8(torch.ones((64, 64), device="cuda"))
+    for call in (lambda: pkg.quantize_int8(bad), lambda: pkg.quantize_int8(bad, transpose=True),
+                 lambda: pkg.linear_int8(bad, w, ws), lambda: pkg.linear_int8(good, w, ws, bias=bad[0]),
+                 lambda: pkg.linear_int8(good, w, ws, residual=bad), lambda: pkg.linear_int8(good, w, ws, out=bad),
+                 lambda: pkg.linear_int8(good, w, bad[0]), lambda: pkg.dropout(bad, pkg.Dropout(0.5)),
+                 lambda: pkg.dropout(good, pkg.Dropout(0.5), residual=bad), lambda: pkg.dropout(good, pkg.Dropout(0.5), out=bad),
+                 lambda: pkg.linear_int8_backward(bad, good, w, ws), lambda: pkg.linear_int8_backward(good, bad, w, ws),
+                 lambda: pkg.linear_int8_backward(good, good, w, ws, dw_dtype=dtype),
+                 lambda: pkg.gemm_int8(w, ws, w, ws, out_dtype=dtype)):
+        with pytest.raises(ValueError):
+            call()
+    if dtype != torch.int8:
+        with pytest.raises(ValueError):
+            pkg.linear_int8(good, torch.zeros((64, 64), device="cuda").to(dtype), ws)
+
+
 def test_out_of_memory_is_the_frameworks_own_error(pkg, cuda):
     with pytest.raises(torch.OutOfMemoryError):
         pkg.empty_int8(1 << 20, 1 << 22, cuda)
