@@ -302,12 +302,13 @@ typedef struct DropoutArgs {
  *   A  m x k int8 (tokens), B  n x k int8 (channels), K contiguous, rows of
  *   lda / ldb bytes (multiples of 16, bases 16-byte aligned); bytes between k
  *   and the row stride are not used.  The sum is exact in int32 (k <= 131071),
- *   everything after it fp32, rounded once to d_type.  The result has the
+ *   everything after it fp32, rounded once to d_type (scales of any size: no
+ *   intermediate result leaves the range of fp32 where D does not).  The result has the
  *   same bits for every tile, split and size of the batch.
  *   scale_a (m) and scale_b (n) fp32; NULL means 1.
  *   D  m x n row-major (N contiguous), leading dimension ldd >= n elements,
- *   any alignment of its own type; C (optional) like D with ldc, is D or does
- *   not overlap it.
+ *   any alignment of its own type; C (optional) like D with ldc, is D (same
+ *   stride) or does not overlap it (else refused).
  *   bias (optional): n elements of bias_type.
  * m or n of 0: nothing is launched.  D must not overlap A, B, scales or bias.
  */
@@ -419,7 +420,8 @@ int gemm_sm100a_int8_linear_backward(const Int8BackwardArgs* args, void* stream)
  * Y = residual + dropout(X), rows x cols row-major with their own row strides
  * (elements), all of one type, any alignment of that type; computed in fp32 and
  * rounded once.  Its gradient is the same call on dY without the residual.
- * Y may be X or residual (same stride).
+ * Y may be X or residual (same stride); Y that overlaps one of them in another way
+ * is refused.
  */
 typedef struct DropoutOpArgs {
   uint32_t struct_size;    /* sizeof(DropoutOpArgs) */

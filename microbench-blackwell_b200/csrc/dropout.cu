@@ -104,6 +104,10 @@ extern "C" int gemm_sm100a_dropout(const DropoutOpArgs* a, void* stream) {
   if (a->ldx < a->cols || a->ldy < a->cols || (a->residual && a->ldr < a->cols)) return GEMM_ERR_CANNOT_IMPLEMENT;
   if ((reinterpret_cast<uintptr_t>(a->x) | reinterpret_cast<uintptr_t>(a->y) | reinterpret_cast<uintptr_t>(a->residual)) % e)
     return GEMM_ERR_CANNOT_IMPLEMENT;
+  // A shifted overlap would read elements that other threads have stored already.
+  if (!in_place_or_apart(a->x, a->ldx, a->y, a->ldy, a->rows, a->cols, e) ||
+      (a->residual && !in_place_or_apart(a->residual, a->ldr, a->y, a->ldy, a->rows, a->cols, e)))
+    return GEMM_ERR_CANNOT_IMPLEMENT;
   p.x = a->x; p.ldx = a->ldx; p.res = a->residual; p.ldr = a->ldr; p.y = a->y; p.ldy = a->ldy;
   p.rows = a->rows; p.cols = a->cols;
   p.wide = rows_16b(a->x, a->ldx, e) && rows_16b(a->y, a->ldy, e) && (!a->residual || rows_16b(a->residual, a->ldr, e));

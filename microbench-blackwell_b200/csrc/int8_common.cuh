@@ -358,6 +358,32 @@ inline int drop_resolve(const DropoutArgs& a, int64_t rows, int64_t cols, Drop& 
   return GEMM_OK;
 }
 
+// Whether two matrices of `rows` rows each (at least one, strides no shorter than a row; all in bytes)
+// share a byte.  Matrices side by side in one buffer do not, though their extents cross.
+inline bool rows_meet(const void* p, int64_t p_step, int64_t p_len, const void* q, int64_t q_step, int64_t q_len, int64_t rows) {
+  const int64_t p0 = (int64_t)reinterpret_cast<uintptr_t>(p), q0 = (int64_t)reinterpret_cast<uintptr_t>(q);
+  const int64_t last = rows - 1;
+  if (q0 + last * q_step + q_len <= p0 || p0 + last * p_step + p_len <= q0) return false;
+  if (rows == 1 || p_step < p_len || q_step < q_len) return true;
+  if (p_step == q_step) {
+    // Row j of q begins `in` bytes into the stretch of row j + by of p.
+    const int64_t d = q0 - p0, by = d >= 0 ? d / p_step : -((p_step - 1 - d) / p_step), in = d - by * p_step;
+    auto both = [&](int64_t shift) { return shift < rows && -shift < rows; };
+    return (in < p_len && both(by)) || (in + q_len > p_step && both(by + 1));
+  }
+  for (int64_t i = 0; i < rows; ++i) {          // the last row of q that begins before the end of p's row i
+    const int64_t a = p0 + i * p_step, b = a + p_len;
+    if (b <= q0) continue;
+    const int64_t j = (b - 1 - q0) / q_step;
+    if (q0 + (j < last ? j : last) * q_step + q_len > a) return true;
+  }
+  return false;
+}
+// An operand that an output may replace, element by element: it is the output, or apart from it.
+inline bool in_place_or_apart(const void* p, int64_t ldp, const void* out, int64_t ldo, int64_t rows, int64_t cols, int64_t e) {
+  return (p == out && (ldp == ldo || rows == 1)) || !rows_meet(p, ldp * e, cols * e, out, ldo * e, cols * e, rows);
+}
+
 // Whether every row of a (base, stride in elements) matrix starts on a 16-byte boundary.
 inline bool rows_16b(const void* p, int64_t ld, int elem_bytes) {
   return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * elem_bytes)) & 15) == 0;

@@ -767,6 +767,7 @@ int check(const Int8GemmArgs* a, bool tokens, Resolved& r) {
     if ((reinterpret_cast<uintptr_t>(a->d) | reinterpret_cast<uintptr_t>(a->c)) % e) FAIL("D/C must be aligned to their element");
     if (a->ldd < a->n) FAIL("ldd must be >= n");
     if (a->c && a->ldc < a->n) FAIL("ldc must be >= n");
+    if (a->c && !in_place_or_apart(a->c, a->ldc, a->d, a->ldd, a->m, a->n, (int64_t)e)) FAIL("C must be D or lie apart from it");
     if ((reinterpret_cast<uintptr_t>(a->scale_a) | reinterpret_cast<uintptr_t>(a->scale_b)) & 3) FAIL("scales must be 4-byte aligned");
     if (a->bias && reinterpret_cast<uintptr_t>(a->bias) % type_bytes(a->bias_type)) FAIL("bias must be aligned to its element");
   }
@@ -994,18 +995,6 @@ int launch_prepared(const Prepared& q, cudaStream_t st) {
   return GEMM_OK;
 }
 
-// Whether a row of D shares a byte with one of the tokens (few of them, both of one element size).
-bool output_meets_tokens(const Int8GemmArgs& a, const void* x, int64_t ldx) {
-  const int64_t e = type_bytes(a.d_type);
-  const intptr_t x0 = reinterpret_cast<intptr_t>(x), d0 = reinterpret_cast<intptr_t>(a.d);
-  for (int64_t i = 0; i < a.m; ++i)
-    for (int64_t j = 0; j < a.m; ++j) {
-      const intptr_t xi = x0 + i * ldx * e, dj = d0 + j * a.ldd * e;
-      if (xi < dj + a.n * e && dj < xi + a.k * e) return true;
-    }
-  return false;
-}
-
 // Few tokens, no knob set and X of D's type: one launch.  Every CTA then quantises
 // the tokens for itself, which costs more than the launch it saves beyond some
 // 16384 of their elements: 8192 x 8192, 1 token 14.5 us against 16.9 in two
@@ -1013,7 +1002,8 @@ bool output_meets_tokens(const Int8GemmArgs& a, const void* x, int64_t ldx) {
 // replaces them) needs two launches, the tokens being quantised before the first store.
 bool use_fused(const Int8GemmArgs& a, const void* x, int32_t x_type, int64_t ldx) {
   return a.m <= kFusedTokens && a.m * a.k <= kFusedElems && x_type == a.d_type && !a.tile_n && !a.cta_group && !a.split_k &&
-         !a.flags && !output_meets_tokens(a, x, ldx);
+         !a.flags && (a.m < 1 || !rows_meet(x, ldx * type_bytes(x_type), a.k * type_bytes(x_type), a.d,
+                                            a.ldd * type_bytes(x_type), a.n * type_bytes(x_type), a.m));
 }
 
 }  // namespace

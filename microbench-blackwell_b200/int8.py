@@ -176,8 +176,8 @@ def gemm_int8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor, b_
     """residual + dropout(a_scale[i] * b_scale[j] * (a . b^T) + bias[j]), (m, n), rounded once.
 
     ``a`` (m, k) and ``b`` (n, k) int8, ``a_scale`` (m) and ``b_scale`` (n) fp32 (None = 1);
-    ``residual`` and ``out`` (which may be the residual) of ``out_dtype``.  The sum over k is
-    exact, so the result does not depend on the batch or the tile.  ``status``: optional int32
+    ``residual`` and ``out`` of ``out_dtype``; ``out`` is the residual or apart from it, and apart
+    from the other operands.  The sum over k is exact, so the result does not depend on the batch or the tile.  ``status``: optional int32
     device word, as in ``gemm_into``.  Knobs: tile_n, cta_group, split_k, timeout_ms, flags."""
     return _host().gemm(a, a_scale, b, b_scale, bias, residual, dropout, out_dtype, out, status,
                         *(_knob_values(knobs) if knobs else _NO_KNOBS))
@@ -213,5 +213,6 @@ def linear_int8_backward(dy: torch.Tensor, x: torch.Tensor, wt: torch.Tensor, wt
 def dropout(x: torch.Tensor, drop: Dropout, *, residual: torch.Tensor | None = None,
             out: torch.Tensor | None = None) -> torch.Tensor:
     """residual + dropout(x), computed in fp32 and rounded once.  The gradient with respect to x
-    is the same call on dy without the residual.  ``out`` may be x or residual."""
+    is the same call on dy without the residual.  ``out`` may be x or residual; another overlap is
+    refused."""
     return _host().dropout(x, drop, residual, out)

@@ -92,6 +92,56 @@ def test_one_cta_per_sm(pkg, d_type, knobs):
             assert rc == pkg.OK and 2 * info.smem_bytes > 228 * 1024 and info.smem_bytes <= 227 * 1024
 
 
+# (offset of the output behind the operand in elements, its stride, whether they share an element), for 4 rows of
+# 32 elements with a stride of 80: in place, shifted by less than a row, side by side, one element too near, one or
+# more rows further down, right behind, and with a stride of its own.
+OVERLAPS = [(0, 80, False), (1, 80, True), (-1, 80, True), (31, 80, True), (32, 80, False), (48, 80, False), (49, 80, True),
+            (80, 80, True), (-80, 80, True), (240, 80, True), (241, 80, True), (272, 80, False), (320, 80, False),
+            (-240, 80, True), (-272, 80, False), (-271, 80, True), (0, 88, True), (32, 88, False), (32, 160, False),
+            (32, 112, True), (272, 88, False)]
+
+
+def _rows(start, ld):
+    return {start + i * ld + j for i in range(4) for j in range(32)}
+
+
+@pytest.mark.parametrize("offset,ld,meet", OVERLAPS)
+def test_outputs_over_other_operands(pkg, offset, ld, meet):
+    """In place or apart; anything between is refused.  (No device memory is behind the addresses: what is
+    accepted ends at the search for the output's device.)"""
+    assert meet == (offset != 0 and not _rows(0, 80).isdisjoint(_rows(offset, ld)) or (offset == 0 and ld != 80))
+    L, at, out = pkg.lib(), 0x100000, 0x100000 + 2 * offset
+    want = pkg.ERR_CANNOT_IMPLEMENT if meet else pkg.ERR_LAUNCH
+    far = dict(residual=0x400000, ldr=32)
+    assert L.gemm_sm100a_dropout(bytes(_drop(pkg, rows=4, x=at, ldx=80, y=out, ldy=ld)), None) == want
+    assert L.gemm_sm100a_dropout(bytes(_drop(pkg, rows=4, x=at, ldx=80, y=out, ldy=ld, **far)), None) == want
+    assert L.gemm_sm100a_dropout(bytes(_drop(pkg, rows=4, x=0x400000, ldx=32, residual=at, ldr=80, y=out, ldy=ld)), None) == want
+    args = _gemm(pkg, m=4, n=32, c=at, ldc=80, d=out, ldd=ld)
+    rc, info = pkg.query_int8(args)
+    assert (rc, b"apart" in info.reason) == ((pkg.ERR_CANNOT_IMPLEMENT, True) if meet else (pkg.OK, False))
+    assert L.gemm_sm100a_int8_launch(bytes(args), None) == want
+
+
+def test_overlap_against_sets_of_elements(pkg):
+    """The refusal of C over D for random small matrices in one buffer, equal strides and others."""
+    import random
+    rng = random.Random(5)
+    seen = [0, 0]
+    for _ in range(4000):
+        m, n = rng.randint(1, 6), rng.randint(1, 9)
+        ldc = n + rng.choice([0, 1, 3, n, 2 * n])
+        ldd = ldc if rng.random() < 0.5 else n + rng.choice([0, 1, 2, n, 3 * n])
+        shift = rng.randint(-m * ldd - 2, m * ldc + 2)
+        c = {i * ldc + j for i in range(m) for j in range(n)}
+        d = {shift + i * ldd + j for i in range(m) for j in range(n)}
+        same = shift == 0 and (ldc == ldd or m == 1)
+        rc, _ = pkg.query_int8(_gemm(pkg, m=m, n=n, c=0x100000, ldc=ldc, d=0x100000 + 2 * shift, ldd=ldd))
+        fine = same or c.isdisjoint(d)
+        assert rc == (pkg.OK if fine else pkg.ERR_CANNOT_IMPLEMENT), (m, n, ldc, ldd, shift)
+        seen[fine] += 1
+    assert min(seen) > 500
+
+
 def test_null_argument_blocks(pkg):
     L = pkg.lib()
     assert L.gemm_sm100a_int8_launch(None, None) == pkg.ERR_BAD_ARGS

@@ -775,6 +775,32 @@ def test_dropout_in_place_strided_and_empty(pkg, cuda):
     assert torch.equal(pkg.dropout(before, pkg.Dropout(0.0)), before)
 
 
+def test_outputs_beside_and_over_other_operands(pkg, cuda):
+    """Columns of one buffer and rows behind one another are apart; a shifted overlap is refused and
+    leaves everything as it was."""
+    drop = pkg.Dropout(0.3, seed=4)
+    m, n, k = 20, 64, 128
+    buf = normal((m, 3 * n), 1, torch.bfloat16)
+    first = buf.clone()
+    x, y, z = buf[:, :n], buf[:, n:2 * n], buf[:, 2 * n:]
+    want = pkg.dropout(x.contiguous(), drop, residual=z.contiguous())
+    assert torch.equal(pkg.dropout(x, drop, residual=z, out=y), want)
+    a, b, sa, sb = int8s(pkg, m, k, 1), int8s(pkg, n, k, 2), scales(m, 3), scales(n, 4)
+    want = pkg.gemm_int8(a, sa, b, sb, residual=z.contiguous())
+    assert torch.equal(pkg.gemm_int8(a, sa, b, sb, residual=z, out=y), want)
+    assert torch.equal(buf[:, :n], first[:, :n]) and torch.equal(buf[:, 2 * n:], first[:, 2 * n:])
+    rows = first.clone()
+    w, ws = pkg.quantize_int8(normal((n, n), 5))
+    for call in (lambda: pkg.dropout(rows[:, :n], drop, out=rows[:, 1:n + 1]),
+                 lambda: pkg.dropout(rows[:-1], drop, out=rows[1:]),
+                 lambda: pkg.dropout(rows[:, n:2 * n], drop, residual=rows[:, :n], out=rows[:, 8:n + 8]),
+                 lambda: pkg.gemm_int8(a, sa, b, sb, residual=rows[:, :n], out=rows[:, 8:n + 8]),
+                 lambda: pkg.linear_int8(rows[:8, :n], w, ws, residual=rows[:8, :n], out=rows[1:9, :n])):
+        with pytest.raises(pkg.GemmError):
+            call()
+    assert torch.equal(rows, first)
+
+
 def test_dropout_seed_from_the_device(pkg, cuda):
     x = normal((50, 100), 1)
     word = torch.tensor([41], dtype=torch.int64, device="cuda")
