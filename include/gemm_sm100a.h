@@ -333,8 +333,9 @@ typedef struct Int8GemmArgs {
   uint32_t flags;          /* 0 or GEMM_FLAG_INJECT_STALL */
 } Int8GemmArgs;
 
-/* Validate and resolve without launching (GemmInfo.tile_m is the channels of a
- * tile, tile_n its tokens). */
+/* Validate and resolve gemm_sm100a_int8_launch without launching (GemmInfo.tile_m is the
+ * channels of a tile, tile_n its tokens).  The one-launch form of the linear layer below has
+ * its own tiles and is not described. */
 int gemm_sm100a_int8_query(const Int8GemmArgs* args, GemmInfo* info);
 
 /* Enqueue one product; asynchronous, allocates nothing, capturable. */
@@ -362,6 +363,7 @@ int gemm_sm100a_int8_linear(const Int8GemmArgs* args, const void* x, int32_t x_t
  * optionally the sum of each column (fp32) in col_sums.
  * With drop.p > 0, x is first masked; the factor 1 / (1 - p) enters scale and
  * col_sums (indices count elements of X as stored, transposed or not).
+ * q, scale and col_sums overlap neither X nor one another.
  * ldq is a multiple of 16 bytes, q 16-byte aligned; bytes of q beyond the last
  * element of a row are left as they were.  rows or cols of 0: with transpose
  * and rows = 0 the scales are 2^-126 and the sums 0, else nothing is written.

@@ -32,7 +32,7 @@ struct DropoutParams {
 template <typename T, bool RES, bool ON>
 __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
   constexpr int V = Vec<T>::N;
-  constexpr int UN = sizeof(T) == 4 ? 2 : 1;   // rows at a time (16384 x 8192 bf16 with residual 133 us, 140 with two)
+  constexpr int UN = sizeof(T) == 4 ? 2 : 1;   // rows at a time (16384 x 8192 bf16 with residual 127 us, 133 with two)
   const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * V;
   sm100::grid_dependency_wait();
   sm100::grid_launch_dependents();

@@ -14,11 +14,11 @@
 // warps 2..5 run the epilogue (one TMEM lane quadrant each; in a pair with a short
 // main loop warps 6..9 take every other chunk).
 //
-// Measured on B200 (1000 W cap): 8192 x 8192 x 8192 in 335 us under ncu, tensor pipe
-// 96 % active, 3.28 PFLOP/s; 8192 x 28672 x 8192 back to back 1.39 ms, 2.77 PFLOP/s at the
-// clock that the power cap leaves.  One token x 8192 x 8192 in 14.8 us (from a graph), 4.5 of
-// the 6.55 TB/s that a copy reaches; about 4 us of it are launch, first loads and last stores
-// (a 1024 x 1024 layer takes 4.7 us in all).
+// Measured on B200 (1000 W cap): 8192 x 8192 x 8192 in 344 us under ncu, tensor pipe
+// 96 % active, 3.19 PFLOP/s, and in 361 us back to back; 8192 x 28672 x 8192 back to back
+// 1.39 ms, 2.77 PFLOP/s at the clock that the power cap leaves.  One token x 8192 x 8192 in
+// 14.5 us (from a graph), 4.6 of the 6.55 TB/s that a copy reaches; about 4 us of it are
+// launch, first loads and last stores (a 1024 x 1024 layer takes 4.8 us in all).
 //   whole-K form   persistent CTAs (CTA pairs for large problems), two
 //                  accumulators, so a tile's epilogue overlaps the next mainloop.
 //   split-K form   for few tiles: the CTAs of a cluster share one tile's K and
@@ -800,10 +800,11 @@ int fused_split(int64_t tiles, int64_t kb) {
 // halves the tokens' rows but not this) or the bytes that it has to pull
 // from L2 at some 64 a cycle, whichever is more; all of them cannot beat HBM (3400 bytes a cycle); the last
 // tile's epilogue follows, 11 cycles a token.  A split of K over up to 8 CTAs (one wave; the GPU
-// holds few clusters of 8 at a time) adds the exchange of the partial tiles (496 x 965 x 21956: 128-token
-// tiles whole 35.1 us, in 4 parts 18.4; 64 x 4096 x 4096: 32-token tiles whole 7.3, in 2 parts 8.6).  The order of the
-// candidates' measured times agreed in 18 of 18 problems of 48 to 4096 tokens (512 x 8192
-// x 8192: pairs of 256 tokens 28.3 us, of 128 31.6, single CTAs of 128 37.7, of 64 50.9).
+// holds few clusters of 8 at a time) adds the exchange of the partial tiles.  Measured over all
+// candidates of 30 problems of 14 to 4096 tokens, the choice is within 3 % of the best in 25
+// (512 x 8192 x 8192: pairs of 256 tokens 28.6 us, of 128 32.2, single CTAs of 128 38.4, of 64 51.3;
+// 496 x 965 x 21956: 128-token tiles in 4 parts 18.5, in 2 parts 23.7).  Farthest off is
+// 64 x 4096 x 4096: 8.8 us in 2 parts, 32-token tiles whole 7.3.
 void choose(const Int8GemmArgs* a, int num_sms, int& cg, int& bn, int& split) {
   static const int kTiles[6][2] = {{1, 16}, {1, 32}, {1, 64}, {1, 128}, {2, 128}, {2, 256}};
   const int64_t kb = (a->k + kAtom - 1) / kAtom;
@@ -997,8 +998,8 @@ int launch_prepared(const Prepared& q, cudaStream_t st) {
 
 // Few tokens, no knob set and X of D's type: one launch.  Every CTA then quantises
 // the tokens for itself, which costs more than the launch it saves beyond some
-// 16384 of their elements: 8192 x 8192, 1 token 14.5 us against 16.9 in two
-// launches, 4 tokens 18.0 against 16.1.  A D that lies over the tokens (the layer's result
+// 16384 of their elements: 8192 x 8192, 1 token 14.5 us against 17.2 in two
+// launches, 4 tokens 18.0 against 17.2.  A D that lies over the tokens (the layer's result
 // replaces them) needs two launches, the tokens being quantised before the first store.
 bool use_fused(const Int8GemmArgs& a, const void* x, int32_t x_type, int64_t ldx) {
   return a.m <= kFusedTokens && a.m * a.k <= kFusedElems && x_type == a.d_type && !a.tile_n && !a.cta_group && !a.split_k &&

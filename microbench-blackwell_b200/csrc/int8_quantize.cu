@@ -3,8 +3,9 @@
 //
 //   amax = max |x| over the row (column),  q = rint(127 x / amax),  scale = amax / 127
 //
-// Both kernels read X once from HBM and write one byte per element; they are
-// bound by those bytes.
+// Both kernels read X once from HBM and write one byte per element.  Rows longer than a
+// block's registers, and columns longer than the shared memory of a cluster, are read
+// a second time, from L2.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(row_threads(NV)) quantize_rows_kernel(const __
 constexpr int kStripBytes = 64;
 // Rows of a CTA in shared memory at a time: with fewer, more CTAs overlap their
 // phases, but more rows are read (and masked) twice.  8192 x 28672 bf16: 170 us
-// with 512, 206 with 1024; with dropout and sums 397 and 330.
+// with 512, 206 with 1024; with dropout and sums 397 and 330 (kernel times, from a graph).
 constexpr int rows_held(bool drop) { return drop ? 1024 : 512; }
 
 // Byte of row r in the held strip: a 64-byte gap after every 16 rows puts rows 16
@@ -343,7 +344,7 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
   return launch_overlapped(quantize_rows_kernel<T, NV, DROP>, dim3((unsigned)blocks), dim3((unsigned)tx, (unsigned)ry), 0, 1, st, p);
 }
 // Many loads in flight per thread for large X; two where one wave of threads covers
-// it (333 x 1000 fp32 2.1 us, 3.7 with eight; 16384 x 8192 bf16 99 us, 71 with eight).  The
+// it (333 x 1000 fp32 1.9 us, 3.7 with eight; 16384 x 8192 bf16 99 us, 70 with eight).  The
 // mask's words need registers: four with dropout.
 template <typename T>
 cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
@@ -366,7 +367,7 @@ cudaError_t launch_cols(QuantParams p, int peers, cudaStream_t st) {
                            (size_t)(p.rows_held / 16 * 17 * kStripBytes), peers, st, p);
 }
 // Four warps per CTA start sooner and leave room for more CTAs; eight pay off for CTAs
-// with many rows (1024 x 8192 bf16 9.8 us and 11.4; with dropout and sums 16384 x 8192 272 us and 245).
+// with many rows (1024 x 8192 bf16 9.8 us and 11.4; with dropout and sums 16384 x 8192 272 us and 247).
 template <typename T>
 cudaError_t launch_cols(QuantParams p, cudaStream_t st) {
   int peers = (int)((p.rows + 255) / 256);
