@@ -302,8 +302,8 @@ typedef struct DropoutArgs {
  *   A  m x k int8 (tokens), B  n x k int8 (channels), K contiguous, rows of
  *   lda / ldb bytes (multiples of 16, bases 16-byte aligned); bytes between k
  *   and the row stride are not used.  The sum is exact in int32 (k <= 131071),
- *   everything after it fp32, rounded once to d_type (scales of any size: no
- *   intermediate result leaves the range of fp32 where D does not).  The result has the
+ *   everything after it fp32, rounded once to d_type (scale_b first where
+ *   |scale_a| > 2^96, which alone could take the sum out of range).  The result has the
  *   same bits for every tile, split and size of the batch.
  *   scale_a (m) and scale_b (n) fp32; NULL means 1.
  *   D  m x n row-major (N contiguous), leading dimension ldd >= n elements,
@@ -391,8 +391,8 @@ int gemm_sm100a_quantize_int8(const Int8QuantArgs* args, void* stream);
  * with transpose = 1; dW n x k of dw_type.  dx, dw and dbias may each be NULL (not
  * wanted; wt is read for dx only, x for dw only).  m, n <= 131071 (sums over them).
  * workspace: gemm_sm100a_int8_backward_workspace(m, n, k) bytes, 16-byte aligned,
- * of this call alone until it has run.  dX and dW may lie over X or dY (not over each
- * other); dbias and the workspace overlap nothing.  m = 0 sets dW and dbias to 0.
+ * of this call alone until it has run.  dX and dW may lie over X or dY, not over each
+ * other, wt or wt_scale; dbias and the workspace overlap nothing.  m = 0 sets dW and dbias to 0.
  * Refusals come before the first launch.  Asynchronous, capturable.
  */
 typedef struct Int8BackwardArgs {

@@ -358,11 +358,12 @@ inline int drop_resolve(const DropoutArgs& a, int64_t rows, int64_t cols, Drop& 
   return GEMM_OK;
 }
 
-// Whether two matrices of `rows` rows each (at least one, strides no shorter than a row; all in bytes)
-// share a byte.  Matrices side by side in one buffer do not, though their extents cross.
+// Whether two matrices of `rows` rows each (at least one; lengths and strides in bytes) share a byte; also
+// where a stride is shorter than its rows and the extents cross.  Matrices side by side in one buffer do not, though their extents cross.
 inline bool rows_meet(const void* p, int64_t p_step, int64_t p_len, const void* q, int64_t q_step, int64_t q_len, int64_t rows) {
   const int64_t p0 = (int64_t)reinterpret_cast<uintptr_t>(p), q0 = (int64_t)reinterpret_cast<uintptr_t>(q);
   const int64_t last = rows - 1;
+  if (p_len <= 0 || q_len <= 0) return false;
   if (q0 + last * q_step + q_len <= p0 || p0 + last * p_step + p_len <= q0) return false;
   if (rows == 1 || p_step < p_len || q_step < q_len) return true;
   if (p_step == q_step) {

@@ -177,8 +177,9 @@ def gemm_int8(a: torch.Tensor, a_scale: torch.Tensor | None, b: torch.Tensor, b_
 
     ``a`` (m, k) and ``b`` (n, k) int8, ``a_scale`` (m) and ``b_scale`` (n) fp32 (None = 1);
     ``residual`` and ``out`` of ``out_dtype``; ``out`` is the residual or apart from it, and apart
-    from the other operands.  The sum over k is exact, so the result does not depend on the batch or the tile.  ``status``: optional int32
-    device word, as in ``gemm_into``.  Knobs: tile_n, cta_group, split_k, timeout_ms, flags."""
+    from the other operands.  The sum over k is exact, so the result does not depend on the batch or
+    the tile.  ``status``: optional int32 device word, as in ``gemm_into``.  Knobs: tile_n, cta_group,
+    split_k, timeout_ms, flags."""
     return _host().gemm(a, a_scale, b, b_scale, bias, residual, dropout, out_dtype, out, status,
                         *(_knob_values(knobs) if knobs else _NO_KNOBS))
 

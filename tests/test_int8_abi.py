@@ -180,6 +180,7 @@ def test_linear_over_its_tokens_needs_a_workspace(pkg):
     assert _linear(pkg, 0x100000 - 3 * 512 + 2, 256, **kw) == pkg.ERR_BAD_ARGS
     assert _linear(pkg, 0x100000 - 3 * 512, 256, **kw) == pkg.ERR_LAUNCH
     # columns of one buffer: side by side, and one element too near
+    assert _linear(pkg, 0x100000 - 8, 256, **dict(kw, n=0, ldd=0)) == pkg.OK   # no D at all
     kw["ldd"] = 600
     assert _linear(pkg, 0x100000 + 512, 600, **kw) == pkg.ERR_LAUNCH
     assert _linear(pkg, 0x100000 + 510, 600, **kw) == pkg.ERR_BAD_ARGS
