@@ -437,6 +437,123 @@ typedef struct DropoutOpArgs {
 
 int gemm_sm100a_dropout(const DropoutOpArgs* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * 4-bit floating linear layers: e2m1 values with a scale for each block of 16
+ * or 32 elements along K and one for each row, their quantiser and product.
+ * ------------------------------------------------------------------------ */
+
+/*
+ * A 4-bit matrix of rows x cols:
+ *   values     two to a byte, the even column in the low four bits; row stride in bytes.  With an odd
+ *              number of columns the last byte's high bits are 0.
+ *   scales     block 16: unsigned e4m3, block 32: e8m0 (2^(byte - 127)).  In tiles of 128 rows x 4
+ *              scales: row r, block column c at byte
+ *                ((r / 128) * tiles + c / 4) * 512 + (r % 32) * 16 + ((r % 128) / 32) * 4 + c % 4
+ *              with tiles = ceil(cols / 256) * (block == 16 ? 4 : 2), 16-byte aligned.  The scales of the
+ *              block columns beyond cols are stored too and must not be NaN (the quantiser writes
+ *              0, or 1 for e8m0); those of rows beyond the last are not used.
+ *              (For columns in multiples of 256 this is the layout of GemmArgs.sfa.)
+ *   row_scale  fp32, one for each row.
+ * An element stands for value * scale * row_scale.
+ */
+
+/* Bytes of the scales of a rows x cols matrix, -1 for sizes that are refused. */
+int64_t gemm_sm100a_fp4_scale_bytes(int64_t rows, int64_t cols, int32_t block);
+
+/*
+ * Quantise the rows of X:
+ *   row_scale g = 2^(floor(log2 max|x|) - 10), at least 2^-126;  y = x / g in fp32 (exact from 2^-126 on)
+ *   scale     s = the least e4m3 number (block 16) or power of two from 2^-126 on (block 32) with
+ *                 6 s >= max|y| over the block
+ *   value     q = y / s rounded to e2m1, ties to the even code, decided exactly
+ * A row with a NaN or an infinity gets that as its row scale and zeros as values: what is computed from
+ * it is NaN, and no other row is touched.  The three outputs overlap neither X nor one another.
+ * values is 16-byte aligned, ldv a multiple of 16; bytes behind a row's last element are left as they were.
+ */
+typedef struct Fp4QuantArgs {
+  uint32_t struct_size;    /* sizeof(Fp4QuantArgs) */
+  int32_t  x_type;         /* GEMM_TYPE_* */
+  int64_t  rows, cols;
+  const void* x;       int64_t ldx;
+  void*    values;     int64_t ldv;   /* bytes */
+  void*    scales;
+  float*   row_scale;
+  int32_t  block;          /* 16 or 32 */
+  int32_t  reserved;       /* 0 */
+} Fp4QuantArgs;
+
+int gemm_sm100a_quantize_fp4(const Fp4QuantArgs* args, void* stream);
+
+/* Y = value * scale * row_scale (row_scale NULL: 1), computed in fp32, where powers of two as row scales keep it
+ * exact unless it leaves fp32's range, and rounded to y_type. */
+typedef struct Fp4DequantArgs {
+  uint32_t struct_size;    /* sizeof(Fp4DequantArgs) */
+  int32_t  y_type;         /* GEMM_TYPE_* */
+  int64_t  rows, cols;
+  const void* values;  int64_t ldv;   /* bytes */
+  const void* scales;
+  const float* row_scale;
+  void*    y;          int64_t ldy;
+  int32_t  block;
+  int32_t  reserved;       /* 0 */
+} Fp4DequantArgs;
+
+int gemm_sm100a_dequantize_fp4(const Fp4DequantArgs* args, void* stream);
+
+/*
+ *   D = C + a_row_scale[i] * b_row_scale[j] * sum_k A[i][k] B[j][k] + bias[j]
+ *
+ * A  m x k (tokens) and B  n x k (channels), 4-bit, with one block size; values 16-byte aligned,
+ * lda / ldb in bytes and multiples of 16 (bytes behind the last element's are not used).  Products and
+ * block scales are exact; the sum is the tensor cores' fp32, whose order depends on the tile and the
+ * split; the row scales, bias and residual fp32, rounded once to d_type (bf16 or fp16: fp32's last
+ * bits are not in the sum).  Row scales NULL: 1.
+ * D and C as in Int8GemmArgs: m x n row-major, any alignment of their type, C is D or lies apart from it.
+ * m or n of 0: nothing is launched.  D must not overlap any other operand.
+ */
+typedef struct Fp4GemmArgs {
+  uint32_t struct_size;    /* sizeof(Fp4GemmArgs) */
+  int32_t  d_type;         /* GEMM_TYPE_BF16 or GEMM_TYPE_FP16: D and C */
+  int64_t  m, n, k;
+  const void* a;  int64_t lda;
+  const void* a_scales;
+  const float* a_row_scale;
+  const void* b;  int64_t ldb;
+  const void* b_scales;
+  const float* b_row_scale;
+  void*       d;  int64_t ldd;
+  const void* c;  int64_t ldc;
+  const void* bias;
+  int32_t  bias_type;      /* GEMM_TYPE_* */
+  int32_t  block;          /* 16 or 32 */
+  int32_t  tile_n;         /* tokens per tile; 0 = chosen from the sizes */
+  int32_t  cta_group;      /* 1 or 2 (CTA pair); 0 = chosen */
+  int32_t  split_k;        /* CTAs that share one tile's K; 0 = chosen */
+  int32_t  reserved;       /* 0 */
+  int32_t* status;         /* optional device int32, as in GemmArgs */
+  uint32_t timeout_ms;     /* device wait budget; 0 = 4000 ms */
+  uint32_t flags;          /* 0 or GEMM_FLAG_INJECT_STALL */
+} Fp4GemmArgs;
+
+/* Validate and resolve gemm_sm100a_fp4_launch without launching (GemmInfo.tile_m is the channels of a
+ * tile, tile_n its tokens). */
+int gemm_sm100a_fp4_query(const Fp4GemmArgs* args, GemmInfo* info);
+
+/* Enqueue one product; asynchronous, allocates nothing, capturable. */
+int gemm_sm100a_fp4_launch(const Fp4GemmArgs* args, void* stream);
+
+/*
+ * Quantise the rows of X (m x k of x_type, row stride ldx elements) and multiply, in one or two launches.
+ * args->a, a_scales and a_row_scale are workspace of the caller (m * lda bytes,
+ * gemm_sm100a_fp4_scale_bytes(m, k, block) bytes, m floats; their content afterwards is unspecified).
+ * They may be NULL where one launch quantises and multiplies: gemm_sm100a_fp4_linear_workspace == 0.
+ * D may lie over X, with X as C too.
+ */
+int gemm_sm100a_fp4_linear(const Fp4GemmArgs* args, const void* x, int32_t x_type, int64_t ldx, void* stream);
+
+/* Whether gemm_sm100a_fp4_linear reads args->a, a_scales and a_row_scale (1) or needs no workspace (0). */
+int gemm_sm100a_fp4_linear_workspace(const Fp4GemmArgs* args, const void* x, int32_t x_type, int64_t ldx);
+
 #ifdef __cplusplus
 }
 #endif

@@ -73,6 +73,8 @@ EXPORTED = (
     "gemm_sm100a_int8_query", "gemm_sm100a_int8_launch", "gemm_sm100a_int8_linear",
     "gemm_sm100a_int8_backward_workspace", "gemm_sm100a_int8_linear_backward",
     "gemm_sm100a_quantize_int8", "gemm_sm100a_dropout",
+    "gemm_sm100a_fp4_scale_bytes", "gemm_sm100a_quantize_fp4", "gemm_sm100a_dequantize_fp4",
+    "gemm_sm100a_fp4_query", "gemm_sm100a_fp4_launch", "gemm_sm100a_fp4_linear", "gemm_sm100a_fp4_linear_workspace",
 )
 
 
@@ -114,7 +116,7 @@ def lib():
         L.gemm_sm100a_umma_peak.argtypes = [i32, i32, i32, i32, i32, vp, vp]
         L.gemm_sm100a_tma_read_probe.restype = C.c_int
         L.gemm_sm100a_tma_read_probe.argtypes = [vp, i64, i32, i32, i32, i32, vp, vp]
-        # Argument blocks of the int8 operators are passed as packed bytes (int8.py).
+        # Argument blocks of the int8 and 4-bit operators are passed as packed bytes (int8.py, fp4.py).
         L.gemm_sm100a_int8_query.restype = C.c_int
         L.gemm_sm100a_int8_query.argtypes = [C.c_char_p, C.POINTER(GemmInfo)]
         L.gemm_sm100a_int8_launch.restype = C.c_int
@@ -129,6 +131,17 @@ def lib():
         L.gemm_sm100a_quantize_int8.argtypes = [C.c_char_p, vp]
         L.gemm_sm100a_dropout.restype = C.c_int
         L.gemm_sm100a_dropout.argtypes = [C.c_char_p, vp]
+        L.gemm_sm100a_fp4_scale_bytes.restype = i64
+        L.gemm_sm100a_fp4_scale_bytes.argtypes = [i64, i64, i32]
+        for name in ("quantize_fp4", "dequantize_fp4", "fp4_launch"):
+            fn = getattr(L, "gemm_sm100a_" + name)
+            fn.restype, fn.argtypes = C.c_int, [C.c_char_p, vp]
+        L.gemm_sm100a_fp4_query.restype = C.c_int
+        L.gemm_sm100a_fp4_query.argtypes = [C.c_char_p, C.POINTER(GemmInfo)]
+        L.gemm_sm100a_fp4_linear.restype = C.c_int
+        L.gemm_sm100a_fp4_linear.argtypes = [C.c_char_p, vp, i32, i64, vp]
+        L.gemm_sm100a_fp4_linear_workspace.restype = C.c_int
+        L.gemm_sm100a_fp4_linear_workspace.argtypes = [C.c_char_p, vp, i32, i64]
         _lib = L
     return _lib
 
@@ -308,3 +321,5 @@ def sf_bytes(rows: int, cols: int) -> int:
 from .torch_api import Operands, make_operands, gemm, gemm_into, flops  # noqa: E402,F401
 from .int8 import (Dropout, DropoutArgs, DropoutOpArgs, Int8BackwardArgs, Int8GemmArgs, Int8QuantArgs, MAX_INT8_K,  # noqa: E402,F401
                    dropout, empty_int8, gemm_int8, linear_int8, linear_int8_backward, quantize_int8, query_int8)
+from .fp4 import (Fp4, Fp4DequantArgs, Fp4GemmArgs, Fp4QuantArgs, dequantize_fp4, fp4_scale_bytes, gemm_fp4,  # noqa: E402,F401
+                  linear_fp4, quantize_fp4, query_fp4)

@@ -1,0 +1,233 @@
+// fp4_quantize.cu -- rows of a floating matrix to 4-bit operands (fp4_common.cuh) and back.  Both are bound by
+// the bytes of the floating side: 2 or 4 an element against 0.56.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+
+#include "device_guard.cuh"
+#include "fp4_common.cuh"
+#include "gemm_sm100a.h"
+#include "row_vec.cuh"
+#include "sm100_ptx.cuh"
+
+using namespace int8op;
+using rowvec::kUnit;
+
+namespace {
+
+struct QuantParams {
+  const void* x;
+  int64_t ldx, rows, cols;
+  uint8_t* values;
+  int64_t ldv;
+  uint8_t* scales;
+  int64_t tiles;
+  float* row_scale;
+};
+
+// A row belongs to blockDim.x threads (a block holds blockDim.y rows); each keeps NU units in
+// registers between the row's maximum and the rounding, so X is read once.  Longer rows are read
+// again (from L2) chunk by chunk.
+template <typename T, int BLOCK, int NU>
+__global__ void __launch_bounds__(512) quantize_fp4_kernel(const __grid_constant__ QuantParams p) {
+  __shared__ uint32_t warp_max[16];
+  const int tx = threadIdx.x, TX = blockDim.x;
+  const int units = (int)(p.tiles * 4 * (BLOCK / 16));        // those of whole atoms of K: their scales are stored too
+  const int per_chunk = NU * TX;
+  const int chunks = (units + per_chunk - 1) / per_chunk;
+  sm100::grid_dependency_wait();
+  sm100::grid_launch_dependents();
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const bool live = row < p.rows;
+  const T* const x = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
+  const int cols = live ? (int)p.cols : 0;
+  rowvec::Unit<T> v[NU];
+  auto load = [&](int chunk) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int e = (chunk * per_chunk + i * TX + tx) * kUnit;
+      v[i] = rowvec::load_unit<T>(x + e, cols - e);
+    }
+  };
+  uint32_t top = 0;   // largest |x| so far: packed halves (16-bit T) or fp32 bits
+  for (int c = 0; c < chunks; ++c) {
+    load(c);
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+      for (int j = 0; j < rowvec::Unit<T>::W; ++j) {
+        if constexpr (sizeof(T) == 4) top = max(top, v[i].w[j] & 0x7FFFFFFFu);
+        else top = __vmaxu2(top, v[i].w[j] & 0x7FFF7FFFu);
+      }
+  }
+  if constexpr (sizeof(T) == 2) top = abs_bits_to_f32<T>(max(top & 0xFFFFu, top >> 16));
+  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  if (TX > 32) {
+    const int warp = threadIdx.y * (TX >> 5) + (tx >> 5);
+    if ((tx & 31) == 0) warp_max[warp] = top;
+    __syncthreads();
+    const int w = tx & 31;
+    top = __reduce_max_sync(0xFFFFFFFFu, w < (TX >> 5) ? warp_max[threadIdx.y * (TX >> 5) + w] : 0u);
+  }
+  const fp4op::RowScale s = fp4op::row_scale(top);
+  if (live && tx == 0) p.row_scale[row] = s.scale;
+  for (int c = 0; c < chunks; ++c) {
+    if (chunks > 1) load(c);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int unit = c * per_chunk + i * TX + tx;
+      if ((unit & ~31) >= units) break;      // whole warps
+      float y[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) y[j] = s.up == 0.f ? 0.f : v[i].get(j) * s.up;
+      uint32_t q[2];
+      const uint32_t code = fp4op::quantize_unit<BLOCK>(y, q);
+      fp4op::store_scale_codes<BLOCK>(p.scales, row, p.tiles, unit, code, live && unit < units);
+      const int n = cols - unit * kUnit;
+      if (n > 0) fp4op::store_codes(p.values + row * p.ldv + unit * 8, q, n);
+    }
+  }
+}
+
+template <typename T, int BLOCK, int NU>
+cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
+  const int64_t units = p.tiles * 4 * (BLOCK / 16);
+  int64_t tx = ((units + NU - 1) / NU + 31) / 32 * 32;
+  if (tx > 512) tx = 512;
+  const int ry = tx >= 128 ? 1 : (int)(128 / tx);
+  const int64_t blocks = (p.rows + ry - 1) / ry;   // at most 2^30
+  return launch_overlapped(quantize_fp4_kernel<T, BLOCK, NU>, dim3((unsigned)blocks), dim3((unsigned)tx, (unsigned)ry), 0, 1, st, p);
+}
+template <typename T>
+cudaError_t launch_rows(const QuantParams& p, int block, cudaStream_t st) {
+  constexpr int NU = sizeof(T) == 4 ? 2 : 4;
+  const bool small = p.rows * ((p.cols + 15) / 16) <= 148 * 1024;
+  if (block == 16) return small ? launch_rows<T, 16, 1>(p, st) : launch_rows<T, 16, NU>(p, st);
+  return small ? launch_rows<T, 32, 1>(p, st) : launch_rows<T, 32, NU>(p, st);
+}
+
+// ----------------------------------------------------------------- back
+struct DequantParams {
+  const uint8_t* values;
+  int64_t ldv, rows, cols;
+  const uint8_t* scales;
+  int64_t tiles;
+  const float* row_scale;
+  void* y;
+  int64_t ldy;
+};
+
+// value * scale has at most seven bits; a row scale that is a power of two keeps it exact within fp32's range.
+template <typename T, int BLOCK>
+__global__ void __launch_bounds__(256) dequantize_fp4_kernel(const __grid_constant__ DequantParams p) {
+  const int unit = (int)blockIdx.x * (int)blockDim.x + (int)threadIdx.x;
+  const int e = unit * kUnit;
+  sm100::grid_dependency_wait();
+  sm100::grid_launch_dependents();
+  const int n = (int)min((int64_t)kUnit, p.cols - e);
+  for (int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row < p.rows; row += (int64_t)gridDim.y * blockDim.y) {
+    uint32_t q[2] = {0u, 0u};
+    float s = 0.f, g = 1.f;
+    if (n > 0) {
+      const uint8_t* const at = p.values + row * p.ldv + unit * 8;
+      if (n == kUnit && (reinterpret_cast<uintptr_t>(at) & 7) == 0) {
+        const uint2 u = *reinterpret_cast<const uint2*>(at);
+        q[0] = u.x;
+        q[1] = u.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (2 * j < n) q[j / 4] |= (uint32_t)at[j] << (8 * (j & 3));
+      }
+      const uint32_t code = p.scales[fp4op::scale_at(row, unit / (BLOCK / 16), p.tiles)];
+      s = BLOCK == 16 ? fp4op::decode_e4m3(code) : fp4op::decode_e8m0(code);
+      if (p.row_scale) g = p.row_scale[row];
+    }
+    rowvec::Unit<T> o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t h;
+      asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
+          : "=r"(h) : "r"(q[j / 4] >> (8 * (j & 3))));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      o.set2(2 * j, f.x * s * g, f.y * s * g);
+    }
+    rowvec::store_unit<T>(static_cast<T*>(p.y) + row * p.ldy + e, o, n);
+  }
+}
+
+template <typename T>
+cudaError_t launch_back(const DequantParams& p, int block, cudaStream_t st) {
+  const int64_t units = (p.cols + kUnit - 1) / kUnit;
+  int tx = 32;
+  while (tx < 256 && tx < units) tx *= 2;
+  const int ty = 256 / tx;
+  const int64_t gx = (units + tx - 1) / tx;
+  int64_t gy = (p.rows + ty - 1) / ty;
+  const int64_t most = (148 * 32 + gx - 1) / gx;
+  if (gy > most) gy = most;
+  if (gy > 65535) gy = 65535;
+  return launch_overlapped(block == 16 ? dequantize_fp4_kernel<T, 16> : dequantize_fp4_kernel<T, 32>, dim3((unsigned)gx, (unsigned)gy),
+                           dim3((unsigned)tx, (unsigned)ty), 0, 1, st, p);
+}
+
+bool sizes_ok(int type, int64_t rows, int64_t cols, int block) {
+  return type_ok(type) && fp4op::block_ok(block) && rows >= 0 && cols >= 0 && rows <= INT32_MAX / 2 && cols <= INT32_MAX / 2;
+}
+int status_of(cudaError_t err) {
+  if (err == cudaSuccess) return GEMM_OK;
+  cudaGetLastError();
+  return GEMM_ERR_LAUNCH;
+}
+
+}  // namespace
+
+extern "C" int64_t gemm_sm100a_fp4_scale_bytes(int64_t rows, int64_t cols, int32_t block) {
+  if (!sizes_ok(GEMM_TYPE_BF16, rows, cols, block)) return -1;
+  return (rows + 127) / 128 * fp4op::scale_tiles(cols, block) * 512;
+}
+
+extern "C" int gemm_sm100a_quantize_fp4(const Fp4QuantArgs* a, void* stream) {
+  if (!a || a->struct_size != sizeof(Fp4QuantArgs)) return GEMM_ERR_BAD_ARGS;
+  if (!sizes_ok(a->x_type, a->rows, a->cols, a->block)) return GEMM_ERR_CANNOT_IMPLEMENT;
+  if (a->rows == 0 || a->cols == 0) return GEMM_OK;
+  if (!a->x || !a->values || !a->scales || !a->row_scale) return GEMM_ERR_BAD_ARGS;
+  const int e = type_bytes(a->x_type);
+  if (a->ldx < a->cols || reinterpret_cast<uintptr_t>(a->x) % e != 0 || a->ldv < (a->cols + 1) / 2 || a->ldv % 16 != 0 ||
+      ((reinterpret_cast<uintptr_t>(a->values) | reinterpret_cast<uintptr_t>(a->scales)) & 15) != 0 ||
+      (reinterpret_cast<uintptr_t>(a->row_scale) & 3) != 0)
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  QuantParams p;
+  memset(&p, 0, sizeof(p));
+  p.x = a->x; p.ldx = a->ldx; p.rows = a->rows; p.cols = a->cols;
+  p.values = static_cast<uint8_t*>(a->values); p.ldv = a->ldv;
+  p.scales = static_cast<uint8_t*>(a->scales); p.tiles = fp4op::scale_tiles(a->cols, a->block);
+  p.row_scale = a->row_scale;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  PointerDeviceGuard guard(a->values);
+  if (!guard.ok) return GEMM_ERR_LAUNCH;
+  return status_of(a->x_type == GEMM_TYPE_BF16 ? launch_rows<__nv_bfloat16>(p, a->block, st)
+                 : a->x_type == GEMM_TYPE_FP16 ? launch_rows<__half>(p, a->block, st) : launch_rows<float>(p, a->block, st));
+}
+
+extern "C" int gemm_sm100a_dequantize_fp4(const Fp4DequantArgs* a, void* stream) {
+  if (!a || a->struct_size != sizeof(Fp4DequantArgs)) return GEMM_ERR_BAD_ARGS;
+  if (!sizes_ok(a->y_type, a->rows, a->cols, a->block)) return GEMM_ERR_CANNOT_IMPLEMENT;
+  if (a->rows == 0 || a->cols == 0) return GEMM_OK;
+  if (!a->y || !a->values || !a->scales) return GEMM_ERR_BAD_ARGS;
+  const int e = type_bytes(a->y_type);
+  if (a->ldy < a->cols || reinterpret_cast<uintptr_t>(a->y) % e != 0 || a->ldv < (a->cols + 1) / 2 ||
+      (reinterpret_cast<uintptr_t>(a->row_scale) & 3) != 0)
+    return GEMM_ERR_CANNOT_IMPLEMENT;
+  DequantParams p;
+  memset(&p, 0, sizeof(p));
+  p.values = static_cast<const uint8_t*>(a->values); p.ldv = a->ldv; p.rows = a->rows; p.cols = a->cols;
+  p.scales = static_cast<const uint8_t*>(a->scales); p.tiles = fp4op::scale_tiles(a->cols, a->block);
+  p.row_scale = a->row_scale; p.y = a->y; p.ldy = a->ldy;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  PointerDeviceGuard guard(a->y);
+  if (!guard.ok) return GEMM_ERR_LAUNCH;
+  return status_of(a->y_type == GEMM_TYPE_BF16 ? launch_back<__nv_bfloat16>(p, a->block, st)
+                 : a->y_type == GEMM_TYPE_FP16 ? launch_back<__half>(p, a->block, st) : launch_back<float>(p, a->block, st));
+}

@@ -1,0 +1,165 @@
+// row_vec.cuh -- rows of a matrix in units of 16 consecutive elements per thread, at any alignment of
+// the rows.
+//
+// Contiguous tensors whose rows have an odd length start most rows off 16-byte boundaries.  Element by element
+// such a row takes 16 loads per unit; here it takes the 16-byte blocks that the unit touches and a
+// shift by the row's misalignment, the same for all of its units.  A block is read whole where
+// any byte of it belongs to the row: it lies in the same 16 bytes of memory as that one, so the read
+// stays in range of the allocation, and what is not the row's is dropped.
+#pragma once
+#include <cstdint>
+
+#include "int8_common.cuh"
+
+namespace rowvec {
+
+using namespace int8op;
+
+constexpr int kUnit = 16;      // elements of a unit
+
+// Words [0, N) of `w` become those `bytes` (0..14, even) further on; w has N + 4 words.
+template <int N>
+__device__ __forceinline__ void shift_words(uint32_t (&w)[N + 4], uint32_t bytes) {
+  if (bytes & 8u) {
+#pragma unroll
+    for (int j = 0; j < N + 2; ++j) w[j] = w[j + 2];
+  }
+  if (bytes & 4u) {
+#pragma unroll
+    for (int j = 0; j < N + 1; ++j) w[j] = w[j + 1];
+  }
+  if (bytes & 2u) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
+  }
+}
+
+// A unit of T as packed words.
+template <typename T>
+struct Unit {
+  static constexpr int W = kUnit * (int)sizeof(T) / 4;
+  uint32_t w[W];
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint16_t h = (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu);
+      T v;
+      __builtin_memcpy(&v, &h, 2);
+      return to_f32(v);
+    }
+  }
+  // Elements i and i + 1 (i even), rounded.
+  __device__ __forceinline__ void set2(int i, float f0, float f1) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = __float_as_uint(f0);
+      w[i + 1] = __float_as_uint(f1);
+    } else {
+      w[i / 2] = pack2<T>(f0, f1);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j] = 0u;
+  }
+};
+
+enum Cache { kStream, kKeep };   // read once, or again by other rows
+
+template <Cache C>
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+  uint4 v;
+  if constexpr (C == kStream)
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  else
+    v = *reinterpret_cast<const uint4*>(p);
+  return v;
+}
+
+// Elements [0, n) of a unit at p (n <= 0: none; the rest reads as 0).  p is aligned to T.
+template <typename T, Cache C = kStream>
+__device__ __forceinline__ Unit<T> load_unit(const T* ptr, int n) {
+  constexpr int W = Unit<T>::W, B = W / 4;
+  const uint8_t* const p = reinterpret_cast<const uint8_t*>(ptr);
+  const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+  const int bytes = min(n, kUnit) * (int)sizeof(T);
+  Unit<T> u;
+  if (off == 0) {
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (16 * j < bytes) v = load16<C>(p + 16 * j);
+      u.w[4 * j] = v.x; u.w[4 * j + 1] = v.y; u.w[4 * j + 2] = v.z; u.w[4 * j + 3] = v.w;
+    }
+  } else {
+    uint32_t w[W + 4];
+#pragma unroll
+    for (int j = 0; j <= B; ++j) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (bytes > 0 && 16 * j - (int)off < bytes) v = load16<C>(p - off + 16 * j);
+      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+    }
+    shift_words<W>(w, off);
+#pragma unroll
+    for (int j = 0; j < W; ++j) u.w[j] = w[j];
+  }
+  if (bytes < 4 * W) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const int left = bytes - 4 * j;
+      if (left < 4) u.w[j] = left == 2 ? u.w[j] & 0xFFFFu : 0u;
+    }
+  }
+  return u;
+}
+
+// Elements [a, b) of a unit, one by one.
+template <typename T>
+__device__ __forceinline__ void store_elements(T* p, const Unit<T>& u, int a, int b) {
+#pragma unroll
+  for (int i = 0; i < kUnit; ++i)
+    if (i >= a && i < b) {
+      if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(p)[i] = u.w[i];
+      else reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(i & 1 ? u.w[i / 2] >> 16 : u.w[i / 2] & 0xFFFFu);
+    }
+}
+
+// Elements [0, n) of the units of a warp, called by all of its lanes; lane l + 1's unit follows lane l's in the
+// row (in other lanes' rows nothing is assumed).  Off 16-byte boundaries a lane also writes the end of the
+// unit before it, so that whole blocks are written; only at both ends of the warp's stretch elements are.
+template <typename T>
+__device__ __forceinline__ void store_unit(T* ptr, const Unit<T>& u, int n) {
+  constexpr int W = Unit<T>::W, B = W / 4, E = (int)sizeof(T);
+  uint8_t* const p = reinterpret_cast<uint8_t*>(ptr);
+  const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+  if (off == 0) {      // uniform over the warp
+    if (n >= kUnit) {
+#pragma unroll
+      for (int j = 0; j < B; ++j) *reinterpret_cast<uint4*>(p + 16 * j) = make_uint4(u.w[4 * j], u.w[4 * j + 1], u.w[4 * j + 2], u.w[4 * j + 3]);
+    } else if (n > 0) {
+      store_elements<T>(ptr, u, 0, n);
+    }
+    return;
+  }
+  uint32_t w[W + 4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = __shfl_up_sync(0xFFFFFFFFu, u.w[W - 4 + j], 1);
+#pragma unroll
+  for (int j = 0; j < W; ++j) w[4 + j] = u.w[j];
+  const int head = (16 - (int)off) / E;      // own elements in the block that begins in the unit before
+  const int lane = (int)(threadIdx.x & 31u);
+  shift_words<W>(w, 16u - off);              // words of the blocks from p - off
+  const bool first_whole = lane > 0 && n >= head;                 // the unit before a valid one is full
+  if (n > 0 && !first_whole) store_elements<T>(ptr, u, 0, min(n, head));
+#pragma unroll
+  for (int j = 0; j < B; ++j) {
+    const bool whole = j == 0 ? first_whole : n >= head + 16 / E * j;
+    if (whole) *reinterpret_cast<uint4*>(p - off + 16 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  }
+  // What of this unit lies beyond its last whole block: the next lane writes it, if that has enough to fill the block.
+  const int whole_end = n < head ? n : min(kUnit - (16 / E - head), head + (n - head) / (16 / E) * (16 / E));
+  const bool next_writes = lane < 31 && n >= kUnit && n - kUnit >= head;
+  if (n > whole_end && !next_writes) store_elements<T>(ptr, u, whole_end, min(n, kUnit));
+}
+
+}  // namespace rowvec

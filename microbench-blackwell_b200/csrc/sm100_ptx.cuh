@@ -401,6 +401,20 @@ __device__ __forceinline__ void mma_nvf4(uint32_t d_tmem, uint64_t a_desc, uint6
          "r"(pred)
       : "memory");
 }
+// Block-scaled MXFP4: e2m1 x e2m1 with ue8m0 scales per 32 K elements: two of the four scale bytes of a
+// 32-bit TMEM word, which ones by the scale ids in `idesc`.
+template <int CG>
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate,
+                                         uint32_t pred = 1u) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %8, 0;\n\t"
+      "@q tcgen05.mma.cta_group::%7.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate), "n"(CG),
+         "r"(pred)
+      : "memory");
+}
 
 // Arrive on `bar` (this CTA) once every prior tcgen05 op of this thread completes.
 __device__ __forceinline__ void mma_commit(uint32_t bar, uint32_t pred = 1u) {

@@ -1,8 +1,8 @@
-// torch_host.cpp -- the host side of the int8 operators for PyTorch callers:
+// torch_host.cpp -- the host side of the int8 and 4-bit operators for PyTorch callers:
 // argument checks, output and workspace allocation, and the C-ABI call, as one
 // CPython extension.  A small call is bound by the host, and in Python its
 // checks, allocations and argument packing took twice as long as the launch.
-// The functions take positional arguments only; int8.py gives them their
+// The functions take positional arguments only; int8.py and fp4.py give them their
 // signatures and documentation.
 #include <Python.h>
 
@@ -467,6 +467,211 @@ PyObject* py_dropout(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// ------------------------------------------------------------------ 4-bit operands
+// An Fp4 tuple (values, scales, row_scale, cols, block).
+struct Fp4Operand {
+  void* values;
+  int64_t rows, cols, ld;
+  void* scales;
+  const float* row_scale;
+  int32_t block;
+  int index;
+};
+
+const at::Tensor& bytes(PyObject* o, const char* name, const char* part, int dims, int index) {
+  if (THPVariable_Check(o)) {
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.dim() == dims && t.layout() == c10::kStrided && t.scalar_type() == at::kByte && t.is_cuda() && (index < 0 || t.get_device() == index))
+      return t;
+  }
+  refuse("%s.%s must be a %d-D uint8 tensor on the operands' CUDA device", name, part, dims);
+}
+
+int32_t block_arg(PyObject* o) {
+  const int64_t b = integer(o);
+  if (b != 16 && b != 32) refuse("block must be 16 or 32");
+  return (int32_t)b;
+}
+
+Fp4Operand fp4_operand(PyObject* o, const char* name, int index) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5) refuse("%s must be an Fp4", name);
+  Fp4Operand f;
+  const at::Tensor& v = bytes(PyTuple_GET_ITEM(o, 0), name, "values", 2, index);
+  f.index = v.get_device();
+  const at::Tensor& s = bytes(PyTuple_GET_ITEM(o, 1), name, "scales", 1, f.index);
+  f.cols = integer(PyTuple_GET_ITEM(o, 3));
+  f.block = block_arg(PyTuple_GET_ITEM(o, 4));
+  f.rows = v.size(0);
+  if (f.cols < 0 || v.size(1) != (f.cols + 1) / 2)
+    refuse("%s.values must have %lld columns for %lld elements", name, (long long)((f.cols + 1) / 2), (long long)f.cols);
+  f.ld = v.stride(0);
+  if (v.stride(1) != 1 && v.size(1) > 1) refuse("%s.values must have unit stride along its last axis", name);
+  if (f.rows <= 1) f.ld = pad16(v.size(1));
+  if ((f.ld & 15) || f.ld < v.size(1)) refuse("%s.values must have a row stride that is a multiple of 16 bytes", name);
+  const int64_t need = gemm_sm100a_fp4_scale_bytes(f.rows, f.cols, f.block);
+  if (need < 0) refuse("%s is too large", name);
+  if (s.size(0) < need || (s.stride(0) != 1 && need > 1)) refuse("%s.scales must hold %lld contiguous bytes", name, (long long)need);
+  f.values = v.data_ptr();
+  f.scales = s.data_ptr();
+  PyObject* const r = PyTuple_GET_ITEM(o, 2);
+  f.row_scale = r == Py_None ? nullptr : static_cast<const float*>(vector(r, "row_scale", f.rows, f.index, nullptr));
+  return f;
+}
+
+// (x, block) -> (values, scales, row_scale)
+PyObject* py_quantize_fp4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count(n, 2);
+    const Matrix x = matrix(v[0], "x", -1);
+    Fp4QuantArgs g;
+    memset(&g, 0, sizeof(g));
+    g.struct_size = sizeof(g);
+    g.x_type = floating(x, "x");
+    g.block = block_arg(v[1]);
+    g.rows = x.rows; g.cols = x.cols;
+    g.x = x.ptr; g.ldx = x.ld;
+    if (x.cols == 0 && x.rows > 0) refuse("x has no columns");
+    const int64_t scale_bytes = gemm_sm100a_fp4_scale_bytes(x.rows, x.cols, g.block);
+    if (scale_bytes < 0) failed(GEMM_ERR_CANNOT_IMPLEMENT, "gemm_sm100a_quantize_fp4", "dimension too large");
+    const int64_t width = (x.cols + 1) / 2;
+    at::Tensor q = at::Tensor(at::detail::empty_strided_cuda({x.rows, width}, {row_bytes(width), 1}, at::kByte,
+                                                             at::Device(at::kCUDA, (c10::DeviceIndex)x.index)));
+    at::Tensor scales = empty({scale_bytes}, at::kByte, x.index), rows = empty({x.rows}, at::kFloat, x.index);
+    g.values = q.data_ptr(); g.ldv = q.stride(0);
+    g.scales = scales.data_ptr();
+    g.row_scale = static_cast<float*>(rows.data_ptr());
+    const int rc = gemm_sm100a_quantize_fp4(&g, stream_of(x.index));
+    if (rc != GEMM_OK) failed(rc, "gemm_sm100a_quantize_fp4", "");
+    PyObject* const r = PyTuple_New(3);
+    if (!r) throw Refused();
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(q)));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(scales)));
+    PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(rows)));
+    return r;
+  });
+}
+
+// (q, dtype, out)
+PyObject* py_dequantize_fp4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count(n, 3);
+    const Fp4Operand q = fp4_operand(v[0], "q", -1);
+    at::ScalarType t;
+    if (v[2] != Py_None) {
+      const Matrix d = matrix(v[2], "out", q.index);
+      floating(d, "out");
+      t = d.dtype;
+    } else {
+      t = dtype_arg(v[1], "dtype");
+    }
+    Output y = output(v[2], q.rows, q.cols, t, q.index);
+    Fp4DequantArgs g;
+    memset(&g, 0, sizeof(g));
+    g.struct_size = sizeof(g);
+    g.y_type = type_code(t);
+    g.block = q.block;
+    g.rows = q.rows; g.cols = q.cols;
+    g.values = q.values; g.ldv = q.ld; g.scales = q.scales; g.row_scale = q.row_scale;
+    g.y = y.ptr; g.ldy = y.ld;
+    const int rc = gemm_sm100a_dequantize_fp4(&g, stream_of(q.index));
+    if (rc != GEMM_OK) failed(rc, "gemm_sm100a_dequantize_fp4", "");
+    return y.wrap();
+  });
+}
+
+// The part of Fp4GemmArgs that products and linear layers share.
+void common_fp4(Fp4GemmArgs& g, PyObject* bias, PyObject* residual, PyObject* status, PyObject* const* knobs, at::ScalarType t, int index) {
+  g.struct_size = sizeof(g);
+  g.d_type = type_code(t);
+  if (residual != Py_None) {
+    const Matrix c = matrix(residual, "residual", index);
+    same_type(c, "residual", t);
+    shape(c, "residual", g.m, g.n);
+    g.c = c.ptr;
+    g.ldc = c.ld;
+  }
+  if (bias != Py_None) g.bias = vector(bias, "bias", g.n, index, &g.bias_type);
+  g.status = status_word(status, index);
+  g.tile_n = knob(knobs[0], "tile_n");
+  g.cta_group = knob(knobs[1], "cta_group");
+  g.split_k = knob(knobs[2], "split_k");
+  g.timeout_ms = (uint32_t)knob(knobs[3], "timeout_ms");
+  g.flags = (uint32_t)knob(knobs[4], "flags");
+}
+
+at::ScalarType result_type(PyObject* out, PyObject* dtype, const char* name, int index) {
+  if (out == Py_None) return dtype_arg(dtype, name);
+  const Matrix d = matrix(out, "out", index);
+  floating(d, "out");
+  return d.dtype;
+}
+
+[[noreturn]] void failed_fp4(int rc, const Fp4GemmArgs& g, const char* what) {
+  GemmInfo info;
+  gemm_sm100a_fp4_query(&g, &info);
+  failed(rc, what, info.reason);
+}
+
+// (a, b, bias, residual, out_dtype, out, status, tile_n, cta_group, split_k, timeout_ms, flags)
+PyObject* py_gemm_fp4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count(n, 12);
+    const Fp4Operand a = fp4_operand(v[0], "a", -1), b = fp4_operand(v[1], "b", a.index);
+    if (b.cols != a.cols) refuse("b must have %lld columns, as a has, got %lld", (long long)a.cols, (long long)b.cols);
+    if (b.block != a.block) refuse("b must have blocks of %d, as a has, got %d", (int)a.block, (int)b.block);
+    Fp4GemmArgs g;
+    memset(&g, 0, sizeof(g));
+    g.m = a.rows; g.n = b.rows; g.k = a.cols;
+    g.block = a.block;
+    const at::ScalarType t = result_type(v[5], v[4], "out_dtype", a.index);
+    common_fp4(g, v[2], v[3], v[6], v + 7, t, a.index);
+    Output d = output(v[5], g.m, g.n, t, a.index);
+    g.a = a.values; g.lda = a.ld; g.a_scales = a.scales; g.a_row_scale = a.row_scale;
+    g.b = b.values; g.ldb = b.ld; g.b_scales = b.scales; g.b_row_scale = b.row_scale;
+    g.d = d.ptr; g.ldd = d.ld;
+    const int rc = gemm_sm100a_fp4_launch(&g, stream_of(a.index));
+    if (rc != GEMM_OK) failed_fp4(rc, g, "gemm_sm100a_fp4_launch");
+    return d.wrap();
+  });
+}
+
+// (x, w, bias, residual, out_dtype, out, status, tile_n, cta_group, split_k, timeout_ms, flags)
+PyObject* py_linear_fp4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count(n, 12);
+    const Matrix x = matrix(v[0], "x", -1);
+    const int code = floating(x, "x");
+    const Fp4Operand w = fp4_operand(v[1], "w", x.index);
+    if (w.cols != x.cols) refuse("w must have %lld columns, as x has, got %lld", (long long)x.cols, (long long)w.cols);
+    Fp4GemmArgs g;
+    memset(&g, 0, sizeof(g));
+    g.m = x.rows; g.n = w.rows; g.k = x.cols;
+    g.block = w.block;
+    const at::ScalarType t = v[5] == Py_None && v[4] == Py_None ? x.dtype : result_type(v[5], v[4], "out_dtype", x.index);
+    common_fp4(g, v[2], v[3], v[6], v + 7, t, x.index);
+    Output d = output(v[5], g.m, g.n, t, x.index);
+    g.b = w.values; g.ldb = w.ld; g.b_scales = w.scales; g.b_row_scale = w.row_scale;
+    g.d = d.ptr; g.ldd = d.ld;
+    g.lda = row_bytes((g.k + 1) / 2);
+    at::Tensor work;
+    if (gemm_sm100a_fp4_linear_workspace(&g, x.ptr, code, x.ld)) {
+      const int64_t values = g.m * g.lda, scales = gemm_sm100a_fp4_scale_bytes(g.m, g.k, g.block);
+      if (scales < 0) failed(GEMM_ERR_CANNOT_IMPLEMENT, "gemm_sm100a_fp4_linear", "dimension too large");
+      work = empty({values + scales + 4 * g.m + 16}, at::kByte, x.index);     // 4-bit tokens, their scales, their row scales
+      uint8_t* const q = static_cast<uint8_t*>(work.data_ptr());
+      g.a = q;
+      g.a_scales = q + values;
+      g.a_row_scale = reinterpret_cast<const float*>(q + values + scales);
+    }
+    const int rc = gemm_sm100a_fp4_linear(&g, x.ptr, code, x.ld, stream_of(x.index));
+    if (rc != GEMM_OK) {
+      if (!g.a) { g.a = g.b; g.a_scales = g.b_scales; }   // for the reason only
+      failed_fp4(rc, g, "gemm_sm100a_fp4_linear");
+    }
+    return d.wrap();
+  });
+}
+
 // (rows, cols, device index)
 PyObject* py_empty(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&] {
@@ -485,7 +690,9 @@ PyObject* py_set_raise(PyObject*, PyObject* f) {
 #define FAST(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {
     FAST("gemm", py_gemm), FAST("linear", py_linear), FAST("backward", py_backward), FAST("quantize", py_quantize),
-    FAST("dropout", py_dropout), FAST("empty", py_empty), {"set_raise", py_set_raise, METH_O, nullptr},
+    FAST("dropout", py_dropout), FAST("empty", py_empty),
+    FAST("quantize_fp4", py_quantize_fp4), FAST("dequantize_fp4", py_dequantize_fp4), FAST("gemm_fp4", py_gemm_fp4),
+    FAST("linear_fp4", py_linear_fp4), {"set_raise", py_set_raise, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "gemm_sm100a_torch", nullptr, -1, g_methods};
 
