@@ -554,6 +554,83 @@ int gemm_sm100a_fp4_linear(const Fp4GemmArgs* args, const void* x, int32_t x_typ
 /* Whether gemm_sm100a_fp4_linear reads args->a, a_scales and a_row_scale (1) or needs no workspace (0). */
 int gemm_sm100a_fp4_linear_workspace(const Fp4GemmArgs* args, const void* x, int32_t x_type, int64_t ldx);
 
+/* ------------------------------------------------------------------------
+ * The residual stream around a block: the norm after it, its gate and scale, the
+ * stream's update and the norm before the next block.
+ * ------------------------------------------------------------------------ */
+
+/*
+ *   z     = post_weight ? y * r(y) * post_weight : y
+ *   x_out = x + (gate * scale) * z                          rounded to `type`
+ *   h     = x_out * r(x_out) * weight                       of the rounded x_out
+ *   r(v)  = 1 / sqrt(mean(v^2) + eps) of a row, the mean and its root in 64 bits, r rounded to fp32
+ * Everything else is one fp32 operation after the other, from left to right, each rounded.
+ * x, y, x_out, h and a gate matrix are of `type`, rows x cols with their own strides (elements), any alignment of
+ * that type; weight, post_weight and a gate vector (ldg = 0) have cols elements of param_type: `type` or fp32.
+ * weight NULL: 1.  gate NULL: 1.  y NULL: x_out is x, which is not written again (x_out NULL too).
+ * block 16 or 32: h, before any rounding, becomes a 4-bit matrix (values, scales, row_scale as in Fp4QuantArgs; h is NULL).
+ * cols <= 16384.  x_out may be x or y (same stride); otherwise outputs overlap nothing.
+ */
+typedef struct ResidualNormArgs {
+  uint32_t struct_size;    /* sizeof(ResidualNormArgs) */
+  int32_t  type;           /* GEMM_TYPE_* */
+  int64_t  rows, cols;
+  const void* x;       int64_t ldx;
+  const void* y;       int64_t ldy;
+  void*    x_out;      int64_t ldo;
+  void*    h;          int64_t ldh;
+  const void* weight;
+  const void* post_weight;
+  const void* gate;    int64_t ldg;   /* 0: a vector */
+  int32_t  param_type;
+  int32_t  block;          /* 0: h is floating */
+  double   eps;            /* >= 0 */
+  float    scale;
+  int32_t  reserved;       /* 0 */
+  void*    values;     int64_t ldv;
+  void*    scales;
+  float*   row_scale;
+} ResidualNormArgs;
+
+int gemm_sm100a_residual_norm(const ResidualNormArgs* args, void* stream);
+
+/*
+ * Its gradients, for dh and dx_out (NULL: 0) and the x_out, y, weights, gate, scale and eps of the call:
+ *   g    = dx_out + the gradient of h towards x_out        dx = g
+ *   dy   = the gradient of (gate * scale) * z towards y for g
+ * of `type`, and the fp32 sums over rows dweight, dpost_weight and, for a gate vector, dgate; a gate
+ * matrix has dgate of `type` (lddg).  y NULL: no dy, dpost_weight, dgate.  dweight, dpost_weight and dgate may be NULL
+ * (not wanted).  Sums are taken in an order that depends on the sizes alone.  rows = 0 sets the fp32 sums to 0.
+ * workspace: gemm_sm100a_residual_norm_workspace(rows, cols) bytes, 16-byte aligned, of this call alone until it has
+ * run.  Outputs overlap nothing.
+ */
+typedef struct ResidualNormBackwardArgs {
+  uint32_t struct_size;    /* sizeof(ResidualNormBackwardArgs) */
+  int32_t  type;
+  int64_t  rows, cols;
+  const void* dh;      int64_t lddh;
+  const void* dx_out;  int64_t lddo;
+  const void* x_out;   int64_t ldo;
+  const void* y;       int64_t ldy;
+  const void* weight;
+  const void* post_weight;
+  const void* gate;    int64_t ldg;   /* 0: a vector */
+  int32_t  param_type;
+  float    scale;
+  double   eps;
+  void*    dx;         int64_t lddx;
+  void*    dy;         int64_t lddy;
+  float*   dweight;
+  float*   dpost_weight;
+  void*    dgate;      int64_t lddg;
+  void*    workspace;  int64_t workspace_bytes;
+} ResidualNormBackwardArgs;
+
+/* Bytes of workspace, -1 for sizes that are refused. */
+int64_t gemm_sm100a_residual_norm_workspace(int64_t rows, int64_t cols);
+
+int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,7 @@ EXPORTED = (
     "gemm_sm100a_quantize_int8", "gemm_sm100a_dropout",
     "gemm_sm100a_fp4_scale_bytes", "gemm_sm100a_quantize_fp4", "gemm_sm100a_dequantize_fp4",
     "gemm_sm100a_fp4_query", "gemm_sm100a_fp4_launch", "gemm_sm100a_fp4_linear", "gemm_sm100a_fp4_linear_workspace",
+    "gemm_sm100a_residual_norm", "gemm_sm100a_residual_norm_workspace", "gemm_sm100a_residual_norm_backward",
 )
 
 
@@ -116,7 +117,7 @@ def lib():
         L.gemm_sm100a_umma_peak.argtypes = [i32, i32, i32, i32, i32, vp, vp]
         L.gemm_sm100a_tma_read_probe.restype = C.c_int
         L.gemm_sm100a_tma_read_probe.argtypes = [vp, i64, i32, i32, i32, i32, vp, vp]
-        # Argument blocks of the int8 and 4-bit operators are passed as packed bytes (int8.py, fp4.py).
+        # Argument blocks of the operators below are passed as packed bytes (int8.py, fp4.py, norm.py).
         L.gemm_sm100a_int8_query.restype = C.c_int
         L.gemm_sm100a_int8_query.argtypes = [C.c_char_p, C.POINTER(GemmInfo)]
         L.gemm_sm100a_int8_launch.restype = C.c_int
@@ -133,7 +134,7 @@ def lib():
         L.gemm_sm100a_dropout.argtypes = [C.c_char_p, vp]
         L.gemm_sm100a_fp4_scale_bytes.restype = i64
         L.gemm_sm100a_fp4_scale_bytes.argtypes = [i64, i64, i32]
-        for name in ("quantize_fp4", "dequantize_fp4", "fp4_launch"):
+        for name in ("quantize_fp4", "dequantize_fp4", "fp4_launch", "residual_norm", "residual_norm_backward"):
             fn = getattr(L, "gemm_sm100a_" + name)
             fn.restype, fn.argtypes = C.c_int, [C.c_char_p, vp]
         L.gemm_sm100a_fp4_query.restype = C.c_int
@@ -142,6 +143,8 @@ def lib():
         L.gemm_sm100a_fp4_linear.argtypes = [C.c_char_p, vp, i32, i64, vp]
         L.gemm_sm100a_fp4_linear_workspace.restype = C.c_int
         L.gemm_sm100a_fp4_linear_workspace.argtypes = [C.c_char_p, vp, i32, i64]
+        L.gemm_sm100a_residual_norm_workspace.restype = i64
+        L.gemm_sm100a_residual_norm_workspace.argtypes = [i64, i64]
         _lib = L
     return _lib
 
@@ -323,3 +326,5 @@ from .int8 import (Dropout, DropoutArgs, DropoutOpArgs, Int8BackwardArgs, Int8Ge
                    dropout, empty_int8, gemm_int8, linear_int8, linear_int8_backward, quantize_int8, query_int8)
 from .fp4 import (Fp4, Fp4DequantArgs, Fp4GemmArgs, Fp4QuantArgs, dequantize_fp4, fp4_scale_bytes, gemm_fp4,  # noqa: E402,F401
                   linear_fp4, quantize_fp4, query_fp4)
+from .norm import (NormGrads, ResidualNormArgs, ResidualNormBackwardArgs, residual_norm,  # noqa: E402,F401
+                   residual_norm_backward)

@@ -1,9 +1,9 @@
-// torch_host.cpp -- the host side of the int8 and 4-bit operators for PyTorch callers:
+// torch_host.cpp -- the host side of the int8 and 4-bit operators and the norms for PyTorch callers:
 // argument checks, output and workspace allocation, and the C-ABI call, as one
 // CPython extension.  A small call is bound by the host, and in Python its
 // checks, allocations and argument packing took twice as long as the launch.
-// The functions take positional arguments only; int8.py and fp4.py give them their
-// signatures and documentation.
+// The functions take positional arguments only; int8.py, fp4.py and norm.py give them
+// their signatures and documentation.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
@@ -672,6 +672,182 @@ PyObject* py_linear_fp4(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// ------------------------------------------------------------------ norms around a block
+double real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Refused();
+  return v;
+}
+
+// weight, post_weight and a vector gate: one type, x's or fp32.
+struct Params {
+  int32_t type;      // -1 before the first
+  int32_t x_type;
+  int64_t n;
+  int index;
+  const void* get(PyObject* o, const char* name) {
+    if (o == Py_None) return nullptr;
+    int32_t code;
+    const void* p = vector(o, name, n, index, &code);
+    if (code != x_type && code != GEMM_TYPE_FP32) refuse("%s must have x's type or be float32", name);
+    if (type >= 0 && code != type) refuse("weight, post_weight and a gate vector must have one type");
+    type = code;
+    return p;
+  }
+};
+
+// The gate: a vector of n elements (ld 0), or a matrix like x.
+const void* gate_arg(PyObject* o, Params& params, const Matrix& x, int64_t& ld) {
+  ld = 0;
+  if (o == Py_None) return nullptr;
+  if (THPVariable_Check(o) && THPVariable_Unpack(o).dim() == 2) {
+    const Matrix g = matrix(o, "gate", x.index);
+    same_type(g, "gate", x.dtype);
+    shape(g, "gate", x.rows, x.cols);
+    ld = g.ld;
+    return g.ptr;
+  }
+  return params.get(o, "gate");
+}
+
+Matrix like(PyObject* o, const char* name, const Matrix& x) {
+  const Matrix m = matrix(o, name, x.index);
+  same_type(m, name, x.dtype);
+  shape(m, name, x.rows, x.cols);
+  return m;
+}
+
+// (x, y, weight, post_weight, gate, scale, eps, fp4, out) -> (x_out, h) or (x_out, values, scales, row_scale)
+PyObject* py_residual_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count(n, 9);
+    const Matrix x = matrix(v[0], "x", -1);
+    ResidualNormArgs g;
+    memset(&g, 0, sizeof(g));
+    g.struct_size = sizeof(g);
+    g.type = floating(x, "x");
+    g.rows = x.rows; g.cols = x.cols;
+    g.x = x.ptr; g.ldx = x.ld;
+    Params params = {-1, g.type, x.cols, x.index};
+    g.weight = params.get(v[2], "weight");
+    const bool block = v[1] != Py_None;
+    Output xo;
+    if (block) {
+      const Matrix y = like(v[1], "y", x);
+      g.y = y.ptr; g.ldy = y.ld;
+      g.post_weight = params.get(v[3], "post_weight");
+      g.gate = gate_arg(v[4], params, x, g.ldg);
+      xo = output(v[8], x.rows, x.cols, x.dtype, x.index);
+      g.x_out = xo.ptr; g.ldo = xo.ld;
+    } else {
+      if (v[3] != Py_None || v[4] != Py_None || v[8] != Py_None) refuse("post_weight, gate and out need y");
+      xo.given = v[0];
+    }
+    g.param_type = params.type < 0 ? g.type : params.type;
+    g.scale = (float)real(v[5]);
+    g.eps = real(v[6]);
+    const int64_t four = integer(v[7]);
+    if (four != 0 && four != 16 && four != 32) refuse("fp4 must be 0, 16 or 32");
+    g.block = (int32_t)four;
+    at::Tensor h, scales, rows;
+    if (four) {
+      const int64_t scale_bytes = gemm_sm100a_fp4_scale_bytes(x.rows, x.cols, g.block), width = (x.cols + 1) / 2;
+      if (scale_bytes < 0) failed(GEMM_ERR_CANNOT_IMPLEMENT, "gemm_sm100a_residual_norm", "dimension too large");
+      h = at::Tensor(at::detail::empty_strided_cuda({x.rows, width}, {row_bytes(width), 1}, at::kByte,
+                                                    at::Device(at::kCUDA, (c10::DeviceIndex)x.index)));
+      scales = empty({scale_bytes}, at::kByte, x.index);
+      rows = empty({x.rows}, at::kFloat, x.index);
+      g.values = h.data_ptr(); g.ldv = h.stride(0);
+      g.scales = scales.data_ptr();
+      g.row_scale = static_cast<float*>(rows.data_ptr());
+    } else {
+      h = empty({x.rows, x.cols}, x.dtype, x.index);
+      g.h = h.data_ptr(); g.ldh = x.cols;
+    }
+    const int rc = gemm_sm100a_residual_norm(&g, stream_of(x.index));
+    if (rc != GEMM_OK) failed(rc, "gemm_sm100a_residual_norm", x.cols > 16384 || x.cols < 1 ? "1 to 16384 columns" : "");
+    PyObject* const r = PyTuple_New(four ? 4 : 2);
+    if (!r) throw Refused();
+    PyTuple_SET_ITEM(r, 0, xo.wrap());
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(h)));
+    if (four) {
+      PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(scales)));
+      PyTuple_SET_ITEM(r, 3, THPVariable_Wrap(std::move(rows)));
+    }
+    return r;
+  });
+}
+
+// (dh, dx_out, x_out, y, weight, post_weight, gate, scale, eps) -> (dx, dy, dweight, dpost_weight, dgate)
+PyObject* py_residual_norm_backward(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded([&] {
+    count(n, 9);
+    const Matrix x = matrix(v[2], "x_out", -1);
+    ResidualNormBackwardArgs g;
+    memset(&g, 0, sizeof(g));
+    g.struct_size = sizeof(g);
+    g.type = floating(x, "x_out");
+    g.rows = x.rows; g.cols = x.cols;
+    g.x_out = x.ptr; g.ldo = x.ld;
+    const Matrix dh = like(v[0], "dh", x);
+    g.dh = dh.ptr; g.lddh = dh.ld;
+    if (v[1] != Py_None) {
+      const Matrix d = like(v[1], "dx_out", x);
+      g.dx_out = d.ptr; g.lddo = d.ld;
+    }
+    Params params = {-1, g.type, x.cols, x.index};
+    g.weight = params.get(v[4], "weight");
+    const bool block = v[3] != Py_None;
+    if (block) {
+      const Matrix y = like(v[3], "y", x);
+      g.y = y.ptr; g.ldy = y.ld;
+      g.post_weight = params.get(v[5], "post_weight");
+      g.gate = gate_arg(v[6], params, x, g.ldg);
+    } else if (v[5] != Py_None || v[6] != Py_None) {
+      refuse("post_weight and gate need y");
+    }
+    g.param_type = params.type < 0 ? g.type : params.type;
+    g.scale = (float)real(v[7]);
+    g.eps = real(v[8]);
+    g.workspace_bytes = gemm_sm100a_residual_norm_workspace(x.rows, x.cols);
+    if (g.workspace_bytes < 0) failed(GEMM_ERR_CANNOT_IMPLEMENT, "gemm_sm100a_residual_norm_backward", "1 to 16384 columns");
+    const at::Tensor dx = empty({x.rows, x.cols}, x.dtype, x.index), work = empty({g.workspace_bytes}, at::kByte, x.index);
+    at::Tensor dy, dw, dp, dg;
+    g.dx = dx.data_ptr(); g.lddx = x.cols;
+    g.workspace = work.data_ptr();
+    if (block) {
+      dy = empty({x.rows, x.cols}, x.dtype, x.index);
+      g.dy = dy.data_ptr(); g.lddy = x.cols;
+    }
+    if (g.weight) {
+      dw = empty({x.cols}, at::kFloat, x.index);
+      g.dweight = static_cast<float*>(dw.data_ptr());
+    }
+    if (g.post_weight) {
+      dp = empty({x.cols}, at::kFloat, x.index);
+      g.dpost_weight = static_cast<float*>(dp.data_ptr());
+    }
+    if (g.gate) {
+      dg = g.ldg ? empty({x.rows, x.cols}, x.dtype, x.index) : empty({x.cols}, at::kFloat, x.index);
+      g.dgate = dg.data_ptr(); g.lddg = x.cols;
+    }
+    const int rc = gemm_sm100a_residual_norm_backward(&g, stream_of(x.index));
+    if (rc != GEMM_OK) failed(rc, "gemm_sm100a_residual_norm_backward", "");
+    PyObject* const r = PyTuple_New(5);
+    if (!r) throw Refused();
+    const at::Tensor* const all[5] = {&dx, &dy, &dw, &dp, &dg};
+    for (int i = 0; i < 5; ++i) {
+      if (all[i]->defined()) {
+        PyTuple_SET_ITEM(r, i, THPVariable_Wrap(*all[i]));
+      } else {
+        Py_INCREF(Py_None);
+        PyTuple_SET_ITEM(r, i, Py_None);
+      }
+    }
+    return r;
+  });
+}
+
 // (rows, cols, device index)
 PyObject* py_empty(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded([&] {
@@ -692,7 +868,8 @@ PyMethodDef g_methods[] = {
     FAST("gemm", py_gemm), FAST("linear", py_linear), FAST("backward", py_backward), FAST("quantize", py_quantize),
     FAST("dropout", py_dropout), FAST("empty", py_empty),
     FAST("quantize_fp4", py_quantize_fp4), FAST("dequantize_fp4", py_dequantize_fp4), FAST("gemm_fp4", py_gemm_fp4),
-    FAST("linear_fp4", py_linear_fp4), {"set_raise", py_set_raise, METH_O, nullptr},
+    FAST("linear_fp4", py_linear_fp4), FAST("residual_norm", py_residual_norm),
+    FAST("residual_norm_backward", py_residual_norm_backward), {"set_raise", py_set_raise, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "gemm_sm100a_torch", nullptr, -1, g_methods};
 
