@@ -15,6 +15,8 @@
 
 #include <cstdint>
 #include <cstring>
+#include <initializer_list>
+#include <utility>
 
 #include "device_guard.cuh"
 #include "fp4_common.cuh"
@@ -30,22 +32,123 @@ namespace {
 
 constexpr int kMaxCols = 16384;
 constexpr int kMaxThreads = 512;
+constexpr int kMaxStages = 4;
+constexpr int kSmemLimit = 224 * 1024;     // dynamic shared memory of a block, and of an SM's blocks together
 
-// Squares of a unit.  Those of 16-bit elements are exact in fp32 and added there, 16 at a time; where that leaves
-// fp32's range (or comes near its end) the row is summed again in 64 bits.
-template <typename T>
-__device__ __forceinline__ double squares(const Unit<T>& u, bool wide) {
-  if (sizeof(T) == 4 || wide) {
-    double s = 0.0;
+// ----------------------------------------------------------------- rows in flight
+// A group of blockDim.x threads (whole warps) takes rows of its own, blockDim.y groups to a block.  Each thread copies
+// its units of the coming rows into its own slots of shared memory (cp.async, so that no barrier is needed and no
+// registers are held), several rows ahead: the bytes on their way are what keeps HBM busy while the group goes through
+// a row's sums.  The 16-byte chunks of a unit lie blockDim.x * blockDim.y slots apart (no bank conflicts).  A unit off
+// 16-byte boundaries (never with WIDE) takes one chunk more, and is shifted when it is read.
+// n: elements of the unit in the row (beyond 16: all).
+template <typename T, bool WIDE>
+__device__ __forceinline__ void issue_unit(uint32_t slot, uint32_t stride, const uint8_t* p, int n) {
+  constexpr int B = Unit<T>::W / 4;
+  const int off = WIDE ? 0 : (int)(reinterpret_cast<uintptr_t>(p) & 15u);
+  if (n >= kUnit) {
 #pragma unroll
-    for (int j = 0; j < kUnit; ++j) s = fma((double)u.get(j), (double)u.get(j), s);
-    return s;
+    for (int j = 0; j < B; ++j) sm100::cp_async_16(slot + (uint32_t)j * stride, p - off + 16 * j, 16u);
+    if (!WIDE && off) sm100::cp_async_16(slot + (uint32_t)B * stride, p - off + 16 * B, 16u);
+  } else if (n > 0) {
+    const int bytes = n * (int)sizeof(T);
+#pragma unroll
+    for (int j = 0; j <= (WIDE ? B - 1 : B); ++j) {
+      const bool any = 16 * j - off < bytes;       // (a copy of no bytes zeroes its chunk; its address is in range all the same)
+      sm100::cp_async_16(slot + (uint32_t)j * stride, any ? p - off + 16 * j : p - off, any ? 16u : 0u);
+    }
   }
-  float s = 0.f;
-#pragma unroll
-  for (int j = 0; j < kUnit; ++j) s = fmaf(u.get(j), u.get(j), s);
-  return (double)s;
 }
+template <typename T, bool WIDE>
+__device__ __forceinline__ Unit<T> take_unit(uint32_t slot, uint32_t stride, uint32_t off, int n) {
+  constexpr int W = Unit<T>::W, B = W / 4;
+  Unit<T> u;
+  if (n <= 0) {
+    u.clear();
+    return u;
+  }
+  auto chunk = [&](int j, uint32_t* w) {
+    const uint4 v = sm100::ld_shared_v4(slot + (uint32_t)j * stride);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  };
+  if (WIDE || off == 0) {
+#pragma unroll
+    for (int j = 0; j < B; ++j) chunk(j, u.w + 4 * j);
+  } else {
+    uint32_t w[W + 4];
+#pragma unroll
+    for (int j = 0; j <= B; ++j) chunk(j, w + 4 * j);
+    rowvec::shift_words<W>(w, off);
+#pragma unroll
+    for (int j = 0; j < W; ++j) u.w[j] = w[j];
+  }
+  if (n < kUnit) rowvec::clip(u, n * (int)sizeof(T));
+  return u;
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ void put_unit(uint8_t* p, const Unit<T>& u, int n) {
+  if constexpr (WIDE) {
+    if (n >= kUnit) {
+#pragma unroll
+      for (int j = 0; j < Unit<T>::W / 4; ++j) *reinterpret_cast<uint4*>(p + 16 * j) = make_uint4(u.w[4 * j], u.w[4 * j + 1], u.w[4 * j + 2], u.w[4 * j + 3]);
+    } else if (n > 0) {
+      rowvec::store_elements<T>(reinterpret_cast<T*>(p), u, 0, n);
+    }
+  } else {
+    rowvec::store_unit<T>(reinterpret_cast<T*>(p), u, n);
+  }
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until all but the newest n groups of this thread's copies have landed.
+__device__ __forceinline__ void wait_copies(int n) {
+  switch (n) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+  }
+}
+
+__device__ __forceinline__ void group_sync() {
+  if (blockDim.x == 32) __syncwarp();
+  else sm100::named_bar_sync(1 + threadIdx.y, blockDim.x);
+}
+
+// ----------------------------------------------------------------- statistics
+template <typename T>
+__device__ __forceinline__ F2 pair(const Unit<T>& u, int j) { return F2(u.get(2 * j), u.get(2 * j + 1)); }
+__device__ __forceinline__ float both(F2 v) {
+  float a, b;
+  v.get(a, b);
+  return a + b;
+}
+__device__ __forceinline__ F2 f2(float v) { return F2(v, v); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ float squares(const Unit<T>& u) {
+  F2 s = f2(0.f);
+#pragma unroll
+  for (int j = 0; j < kUnit / 2; ++j) s = fma2(pair(u, j), pair(u, j), s);
+  return both(s);
+}
+template <typename T>
+__device__ __forceinline__ double squares_wide(const Unit<T>& u) {
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < kUnit; ++j) s = fma((double)u.get(j), (double)u.get(j), s);
+  return s;
+}
+// Where the fp32 part of a sum of squares may have left its range (or come near its end), 64 bits do it again.
 __device__ __forceinline__ bool out_of_range(double s) { return !(s > 1e-30 && s < 1e38); }
 
 // 1 / sqrt(v), rounded to fp32 from an error of 2^-43 or less.
@@ -55,500 +158,648 @@ __device__ __forceinline__ float inverse_root(double v) {
   return (float)fma(0.5 * r, fma(-v * r, r, 1.0), r);
 }
 
-// Row sums of blockDim.x threads (whole warps); blockDim.y rows at a time, all threads of the block call.
-// `slot` alternates between calls.
-struct RowSums {
-  double part[2][kMaxThreads / 32];
-};
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
-}
-__device__ __forceinline__ double row_sum(double v, RowSums& sums, int slot) {
-  v = warp_sum(v);
+// The sum over the group's warps of a value that the lanes of each warp hold; all threads of the group call, with `part`
+// alternating between calls.
+__device__ __forceinline__ double across_warps(double v, double* part) {
   const int warps = (int)blockDim.x >> 5;
   if (warps == 1) return v;
-  const int first = (int)threadIdx.y * warps;
-  if ((threadIdx.x & 31u) == 0) sums.part[slot][first + (threadIdx.x >> 5)] = v;
-  __syncthreads();
-  double s = 0.0;
-  for (int i = 0; i < warps; ++i) s += sums.part[slot][first + i];
-  return s;
+  double* const mine = part + threadIdx.y * warps;
+  if ((threadIdx.x & 31u) == 0) mine[threadIdx.x >> 5] = v;
+  group_sync();
+  double s[2] = {0.0, 0.0};
+#pragma unroll 4
+  for (int i = 0; i < warps; ++i) s[i & 1] += mine[i];
+  return s[0] + s[1];
 }
 
 struct NormParams {
-  const void* x; int64_t ldx;
-  const void* y; int64_t ldy;
-  void* xo; int64_t ldo;
-  void* h; int64_t ldh;
+  const uint8_t* x; int64_t ldx;       // strides in bytes
+  const uint8_t* y; int64_t ldy;
+  uint8_t* xo; int64_t ldo;
+  uint8_t* h; int64_t ldh;
   const void* w;
   const void* wp;
-  const void* gate; int64_t ldg;
+  const uint8_t* gate; int64_t ldg;
   int64_t rows;
   int32_t cols;
   float scale;
-  double eps;
+  double eps, inv_n;
   uint8_t* values; int64_t ldv;
   uint8_t* scales;
   float* row_scale;
   int64_t tiles;
+  int32_t stages, chunks;      // rows ahead; chunks of a unit (one more where a matrix has rows off 16-byte boundaries)
+  int32_t gate_ahead;          // a gate matrix is copied ahead too
+  int32_t param32;             // the vectors are fp32 (else of T)
 };
 
-// Element j of (gate scale), in the order of the definition.
-template <typename P>
-__device__ __forceinline__ Unit<float> gate_scale(const Unit<P>& g, float scale) {
-  Unit<float> k;
+// A vector's elements at a thread's unit as fp32 pairs; ones where there is no vector.
+template <typename T>
+__device__ __forceinline__ void load_params(const void* v, int param32, int e, int n, F2 (&o)[kUnit / 2]) {
+  if (!v) {
 #pragma unroll
-  for (int j = 0; j < kUnit; ++j) k.w[j] = __float_as_uint(__fmul_rn(g.get(j), scale));
-  return k;
+    for (int j = 0; j < kUnit / 2; ++j) o[j] = f2(1.f);
+  } else if (sizeof(T) == 4 || param32) {
+    const Unit<float> u = rowvec::load_unit<float, rowvec::kKeep>(static_cast<const float*>(v) + e, n);
+#pragma unroll
+    for (int j = 0; j < kUnit / 2; ++j) o[j] = pair(u, j);
+  } else {
+    const Unit<T> u = rowvec::load_unit<T, rowvec::kKeep>(static_cast<const T*>(v) + e, n);
+#pragma unroll
+    for (int j = 0; j < kUnit / 2; ++j) o[j] = pair(u, j);
+  }
 }
 
-template <typename T, typename P, int BLOCK, int NU>
-__global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const __grid_constant__ NormParams p) {
-  __shared__ RowSums sums;
+// NU units to a thread, blockDim.x units apart.  Where they fit, the vectors stay in registers for all of the group's
+// rows (as w and wp gate scale); two units of fp32 elements leave no room, and they are read again for each row.
+// Two units to a thread halve what the statistics cost per element: 16384 x 8192 bf16 in @2@ us, @1@ with one; a call of few
+// rows is done sooner with one (1 x 8192: @a@ and @b@).
+template <typename T, int BLOCK, int NU, bool WIDE>
+__global__ void __launch_bounds__(NU == 2 && sizeof(T) == 2 ? 512 : kMaxThreads) residual_norm_kernel(const __grid_constant__ NormParams p) {
+  extern __shared__ __align__(16) uint8_t slots[];
+  __shared__ double part[2][kMaxThreads / 32];
   __shared__ uint32_t warp_max[kMaxThreads / 32];
+  constexpr int E = (int)sizeof(T);
+  constexpr bool KEEP = NU == 1 || E == 2;
   const int tx = threadIdx.x, TX = blockDim.x;
-  sm100::grid_dependency_wait();
-  sm100::grid_launch_dependents();
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  const bool live = row < p.rows;
-  const int cols = live ? p.cols : 0;
-  const int64_t r0 = live ? row : 0;
-  Unit<T> x[NU], y[NU];
+  const uint32_t stride = (uint32_t)(TX * (int)blockDim.y) * 16u;
+  const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * TX + tx) * 16u;
+  const uint32_t per_unit = (uint32_t)p.chunks * stride;
+  const bool matrix = p.ldg != 0;
+  const uint32_t per_stage = (uint32_t)((1 + (p.y ? 1 : 0) + p.gate_ahead) * NU) * per_unit;
+  const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
+  int e[NU], n[NU];
 #pragma unroll
   for (int i = 0; i < NU; ++i) {
-    const int e = (i * TX + tx) * kUnit;
-    x[i] = rowvec::load_unit<T>(static_cast<const T*>(p.x) + r0 * p.ldx + e, cols - e);
-    if (p.y) y[i] = rowvec::load_unit<T>(static_cast<const T*>(p.y) + r0 * p.ldy + e, cols - e);
+    e[i] = (i * TX + tx) * kUnit;
+    n[i] = p.cols - e[i];
   }
-  auto inverse_rms = [&](const Unit<T> (&v)[NU], int slot) {
-    double s = 0.0;
+  sm100::grid_dependency_wait();
+  sm100::grid_launch_dependents();
+  auto issue = [&](int64_t row, uint32_t slot) {
+    if (row < p.rows) {
 #pragma unroll
-    for (int i = 0; i < NU; ++i) s += squares<T>(v[i], false);
-    s = row_sum(s, sums, slot);
-    if constexpr (sizeof(T) == 2) {
-      // All rows of the block go this way, or none.
-      if (blockDim.y == 1 ? out_of_range(s) : __syncthreads_or(out_of_range(s))) {
-        __syncthreads();
+      for (int i = 0; i < NU; ++i) {
+        issue_unit<T, WIDE>(slot, stride, p.x + row * p.ldx + e[i] * E, n[i]);
+        slot += per_unit;
+        if (p.y) {
+          issue_unit<T, WIDE>(slot, stride, p.y + row * p.ldy + e[i] * E, n[i]);
+          slot += per_unit;
+        }
+        if (p.gate_ahead) {
+          issue_unit<T, WIDE>(slot, stride, p.gate + row * p.ldg + e[i] * E, n[i]);
+          slot += per_unit;
+        }
+      }
+    }
+    commit_copies();
+  };
+  for (int s = 0; s < p.stages; ++s) issue(first + s * step, mine + (uint32_t)s * per_stage);
+
+  F2 vw[KEEP ? NU : 1][kUnit / 2], vk[KEEP ? NU : 1][kUnit / 2];
+  auto load_w = [&](int i) { load_params<T>(p.w, p.param32, e[i], n[i], vw[KEEP ? i : 0]); };
+  auto load_k = [&](int i) {
+    F2 g[kUnit / 2];
+    load_params<T>(p.wp, p.param32, e[i], n[i], vk[KEEP ? i : 0]);
+    load_params<T>(matrix ? nullptr : p.gate, p.param32, e[i], n[i], g);
+#pragma unroll
+    for (int j = 0; j < kUnit / 2; ++j) vk[KEEP ? i : 0][j] = mul2(vk[KEEP ? i : 0][j], mul2(g[j], f2(p.scale)));
+  };
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      load_w(i);
+      if (p.y) load_k(i);
+    }
+  }
+
+  int flip = 0;       // a call's buffer is written again by the second call after it, with a barrier between
+  auto inverse_rms = [&](const Unit<T> (&v)[NU]) {
+    double* const at = part[flip ^= 1];
+    double s = 0.0;
+    if constexpr (E == 4) {
+#pragma unroll
+      for (int i = 0; i < NU; ++i) s += squares_wide<T>(v[i]);
+      s = across_warps(warp_sum(s), at);
+    } else {
+      // Sums of squares of a warp's elements in fp32, beyond in 64 bits.
+      float f = 0.f;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) f += squares<T>(v[i]);
+      s = across_warps((double)warp_sum(f), at);
+      if (out_of_range(s)) {
+        group_sync();
         s = 0.0;
 #pragma unroll
-        for (int i = 0; i < NU; ++i) s += squares<T>(v[i], true);
-        s = row_sum(s, sums, slot);
+        for (int i = 0; i < NU; ++i) s += squares_wide<T>(v[i]);
+        s = across_warps(warp_sum(s), at);
       }
     }
-    return inverse_root(s / p.cols + p.eps);
+    return inverse_root(fma(s, p.inv_n, p.eps));
   };
-  if (p.y) {
-    const float q = p.wp ? inverse_rms(y, 0) : 1.f;
+
+  int stage = 0;
+  for (int64_t row = first; row < p.rows; row += step) {
+    const uint32_t at = mine + (uint32_t)stage * per_stage;
+    const uint8_t* const rx = p.x + row * p.ldx;
+    const uint8_t* const ry = p.y + row * p.ldy;
+    const uint8_t* const rg = p.gate + row * p.ldg;
+    auto low = [](const uint8_t* q) { return (uint32_t)reinterpret_cast<uintptr_t>(q) & 15u; };      // (units are multiples of 16 bytes)
+    wait_copies(p.stages - 1);
+    Unit<T> x[NU], y[NU], gate[NU];
+    {
+      uint32_t slot = at;
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int e = (i * TX + tx) * kUnit;
-      float z[kUnit];
-#pragma unroll
-      for (int j = 0; j < kUnit; ++j) z[j] = y[i].get(j);
-      if (p.wp) {
-        const Unit<P> wp = rowvec::load_unit<P, rowvec::kKeep>(static_cast<const P*>(p.wp) + e, cols - e);
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) z[j] = __fmul_rn(__fmul_rn(z[j], q), wp.get(j));
+      for (int i = 0; i < NU; ++i) {
+        x[i] = take_unit<T, WIDE>(slot, stride, low(rx), n[i]);
+        slot += per_unit;
+        if (p.y) {
+          y[i] = take_unit<T, WIDE>(slot, stride, low(ry), n[i]);
+          slot += per_unit;
+        }
+        if (p.gate_ahead) {
+          gate[i] = take_unit<T, WIDE>(slot, stride, low(rg), n[i]);
+          slot += per_unit;
+        } else if (matrix) {
+          gate[i] = rowvec::load_unit<T>(reinterpret_cast<const T*>(rg) + e[i], n[i]);
+        }
       }
-      if (!p.gate) {
+    }
+    issue(row + p.stages * step, at);
+    if (++stage == p.stages) stage = 0;
+    if (p.y) {
+      const F2 q = f2(p.wp ? inverse_rms(y) : 1.f);
+      uint8_t* const out = p.xo + row * p.ldo;
 #pragma unroll
-        for (int j = 0; j < kUnit; ++j) z[j] = __fmul_rn(z[j], p.scale);
-      } else {
-        const Unit<float> k = p.ldg ? gate_scale(rowvec::load_unit<T>(static_cast<const T*>(p.gate) + r0 * p.ldg + e, cols - e), p.scale)
-                                    : gate_scale(rowvec::load_unit<P, rowvec::kKeep>(static_cast<const P*>(p.gate) + e, cols - e), p.scale);
+      for (int i = 0; i < NU; ++i) {
+        if constexpr (!KEEP) load_k(i);
 #pragma unroll
-        for (int j = 0; j < kUnit; ++j) z[j] = __fmul_rn(z[j], k.get(j));
+        for (int j = 0; j < kUnit / 2; ++j) {
+          F2 z = mul2(pair(y[i], j), q), k = vk[KEEP ? i : 0][j];
+          if (matrix) k = mul2(k, pair(gate[i], j));
+          float a, b;
+          fma2(z, k, pair(x[i], j)).get(a, b);
+          x[i].set2(2 * j, a, b);
+        }
+        put_unit<T, WIDE>(out + e[i] * E, x[i], n[i]);
       }
-#pragma unroll
-      for (int j = 0; j < kUnit; j += 2) x[i].set2(j, __fadd_rn(x[i].get(j), z[j]), __fadd_rn(x[i].get(j + 1), z[j + 1]));
-      rowvec::store_unit<T>(static_cast<T*>(p.xo) + r0 * p.ldo + e, x[i], cols - e);
     }
-  }
-  const float r = inverse_rms(x, 1);
-  // h of a unit, in fp32.
-  auto norm = [&](int i, float (&h)[kUnit]) {
-    const int e = (i * TX + tx) * kUnit;
+    const F2 r = f2(inverse_rms(x));
+    // h of a unit, in fp32.
+    auto norm = [&](int i, float (&h)[kUnit]) {
+      if constexpr (!KEEP) load_w(i);
 #pragma unroll
-    for (int j = 0; j < kUnit; ++j) h[j] = __fmul_rn(x[i].get(j), r);
-    if (p.w) {
-      const Unit<P> w = rowvec::load_unit<P, rowvec::kKeep>(static_cast<const P*>(p.w) + e, cols - e);
+      for (int j = 0; j < kUnit / 2; ++j) mul2(mul2(pair(x[i], j), r), vw[KEEP ? i : 0][j]).get(h[2 * j], h[2 * j + 1]);
+    };
+    if constexpr (BLOCK == 0) {
+      uint8_t* const out = p.h + row * p.ldh;
 #pragma unroll
-      for (int j = 0; j < kUnit; ++j) h[j] = __fmul_rn(h[j], w.get(j));
-    }
-  };
-  if constexpr (BLOCK == 0) {
+      for (int i = 0; i < NU; ++i) {
+        float h[kUnit];
+        norm(i, h);
+        Unit<T> o;
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int e = (i * TX + tx) * kUnit;
-      float h[kUnit];
-      norm(i, h);
-      Unit<T> o;
+        for (int j = 0; j < kUnit; j += 2) o.set2(j, h[j], h[j + 1]);
+        put_unit<T, WIDE>(out + e[i] * E, o, n[i]);
+      }
+    } else {
+      float h[NU][kUnit];
+      uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < kUnit; j += 2) o.set2(j, h[j], h[j + 1]);
-      rowvec::store_unit<T>(static_cast<T*>(p.h) + r0 * p.ldh + e, o, cols - e);
-    }
-  } else {
-    uint32_t top = 0;
+      for (int i = 0; i < NU; ++i) {
+        norm(i, h[i]);
+        if (n[i] < kUnit) {
+          // Zeros beyond the row (an infinite r has made NaN of them).
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      float h[kUnit];
-      norm(i, h);
+          for (int j = 0; j < kUnit; ++j)
+            if (j >= n[i]) h[i][j] = 0.f;
+        }
 #pragma unroll
-      for (int j = 0; j < kUnit; ++j)
-        if ((i * TX + tx) * kUnit + j < cols) top = max(top, __float_as_uint(h[j]) & 0x7FFFFFFFu);
-    }
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    if (TX > 32) {
-      const int first = (int)threadIdx.y * (TX >> 5);
-      if ((tx & 31) == 0) warp_max[first + (tx >> 5)] = top;
-      __syncthreads();
-      top = __reduce_max_sync(0xFFFFFFFFu, (tx & 31) < (TX >> 5) ? warp_max[first + (tx & 31)] : 0u);
-    }
-    const fp4op::RowScale s = fp4op::row_scale(top);
-    if (live && tx == 0) p.row_scale[row] = s.scale;
-    const int units = (int)p.tiles * 4 * (BLOCK / 16);
+        for (int j = 0; j < kUnit; ++j) top = max(top, __float_as_uint(h[i][j]) & 0x7FFFFFFFu);
+      }
+      top = __reduce_max_sync(0xFFFFFFFFu, top);
+      if (TX > 32) {
+        // (The barrier of the next row's statistics lies between this row's reads and that row's writes.)
+        uint32_t* const group = warp_max + (int)threadIdx.y * (TX >> 5);
+        if ((tx & 31) == 0) group[tx >> 5] = top;
+        group_sync();
+        top = __reduce_max_sync(0xFFFFFFFFu, (tx & 31) < (TX >> 5) ? group[tx & 31] : 0u);
+      }
+      const fp4op::RowScale s = fp4op::row_scale(top);
+      if (tx == 0) p.row_scale[row] = s.scale;
+      const int units = (int)p.tiles * 4 * (BLOCK / 16);
 #pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      const int unit = i * TX + tx;
-      if ((unit & ~31) >= units) break;      // whole warps
-      float h[kUnit];
-      norm(i, h);
+      for (int i = 0; i < NU; ++i) {
+        const int unit = i * TX + tx;
+        if ((unit & ~31) >= units) break;      // whole warps
 #pragma unroll
-      for (int j = 0; j < kUnit; ++j) h[j] = s.up == 0.f || unit * kUnit + j >= cols ? 0.f : h[j] * s.up;
-      uint32_t q[2];
-      const uint32_t code = fp4op::quantize_unit<BLOCK>(h, q);
-      fp4op::store_scale_codes<BLOCK>(p.scales, row, p.tiles, unit, code, live && unit < units);
-      const int n = cols - unit * kUnit;
-      if (n > 0) fp4op::store_codes(p.values + row * p.ldv + unit * 8, q, n);
+        for (int j = 0; j < kUnit; ++j) h[i][j] = s.up == 0.f ? 0.f : h[i][j] * s.up;
+        uint32_t q[2];
+        const uint32_t code = fp4op::quantize_unit<BLOCK>(h[i], q);
+        fp4op::store_scale_codes<BLOCK>(p.scales, row, p.tiles, unit, code, unit < units);
+        if (n[i] > 0) fp4op::store_codes(p.values + row * p.ldv + unit * 8, q, n[i]);
+      }
     }
   }
 }
 
-template <typename T, typename P, int BLOCK, int NU>
-cudaError_t launch_forward(const NormParams& p, cudaStream_t st) {
+// Threads of a row, rows of a block and blocks, all resident at once; `bytes`: shared memory of a thread and row.
+struct Shape {
+  int tx, ty, blocks, stages;
+  size_t smem;
+};
+Shape shape_of(int64_t rows, int units, int per_thread, int bytes) {
+  Shape s;
+  s.tx = ((units + per_thread - 1) / per_thread + 31) / 32 * 32;
+  int64_t ty = kMaxThreads / s.tx;
+  const int64_t spread = (rows + 147) / 148;       // rows over all SMs before more of them in a block
+  if (ty > spread) ty = spread;
+  if (ty > 8) ty = 8;
+  s.ty = (int)(ty < 1 ? 1 : ty);
+  const int threads = s.tx * s.ty, resident = kMaxThreads / threads;
+  const int64_t blocks = (rows + s.ty - 1) / s.ty, most = 148 * resident;
+  s.blocks = (int)(blocks < most ? blocks : most);
+  s.stages = kSmemLimit / resident / (bytes * threads);
+  if (s.stages > kMaxStages) s.stages = kMaxStages;
+  const int64_t each = (rows + (int64_t)s.blocks * s.ty - 1) / ((int64_t)s.blocks * s.ty);
+  if (s.stages > each) s.stages = (int)each;
+  s.smem = (size_t)s.stages * bytes * threads;
+  return s;
+}
+
+// Whether the rows of all matrices start on 16-byte boundaries (strides in bytes; an absent one does not count).
+bool all_wide(std::initializer_list<std::pair<const void*, int64_t>> matrices) {
+  uintptr_t bits = 0;
+  for (const auto& m : matrices)
+    if (m.first) bits |= reinterpret_cast<uintptr_t>(m.first) | (uintptr_t)m.second;
+  return (bits & 15) == 0;
+}
+
+template <typename T, int BLOCK, int NU, bool WIDE>
+cudaError_t launch_forward(const NormParams& p0, cudaStream_t st) {
+  NormParams p = p0;
   const int units = BLOCK ? (int)p.tiles * 4 * (BLOCK / 16) : (p.cols + kUnit - 1) / kUnit;
-  int tx = ((units + NU - 1) / NU + 31) / 32 * 32;
-  const int ty = tx >= 128 ? 1 : 128 / tx;
-  return launch_overlapped(residual_norm_kernel<T, P, BLOCK, NU>, dim3((unsigned)((p.rows + ty - 1) / ty)), dim3((unsigned)tx, (unsigned)ty), 0, 1, st, p);
+  const bool matrix = p.ldg != 0;
+  p.chunks = kUnit * (int)sizeof(T) / 16 + (WIDE ? 0 : 1);
+  const int two = (1 + (p.y ? 1 : 0)) * NU * p.chunks * 16;
+  Shape s = shape_of(p.rows, units, NU, two + (matrix ? NU * p.chunks * 16 : 0));
+  p.gate_ahead = matrix;
+  if (s.stages == 0) {        // three fp32 rows of more than 14000 elements
+    s = shape_of(p.rows, units, NU, two);
+    p.gate_ahead = 0;
+  }
+  p.stages = s.stages;
+  const auto fn = residual_norm_kernel<T, BLOCK, NU, WIDE>;
+  // (Always the same limit: calls of other sizes may be between this line and the launch.)
+  const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+  if (err != cudaSuccess) return err;
+  return launch_overlapped(fn, dim3((unsigned)s.blocks), dim3((unsigned)s.tx, (unsigned)s.ty), s.smem, 1, st, p);
 }
-template <typename T, typename P, int BLOCK>
+template <typename T, int BLOCK, bool WIDE>
 cudaError_t launch_forward(const NormParams& p, cudaStream_t st) {
-  return p.cols <= kMaxThreads * kUnit / 2 ? launch_forward<T, P, BLOCK, 1>(p, st) : launch_forward<T, P, BLOCK, 2>(p, st);
+  const bool one = p.cols <= kMaxThreads * kUnit && (sizeof(T) == 4 || p.rows <= 148);
+  return one ? launch_forward<T, BLOCK, 1, WIDE>(p, st) : launch_forward<T, BLOCK, 2, WIDE>(p, st);
 }
-template <typename T, typename P>
+template <typename T>
 cudaError_t launch_forward(const NormParams& p, int block, cudaStream_t st) {
-  return block == 0 ? launch_forward<T, P, 0>(p, st) : block == 16 ? launch_forward<T, P, 16>(p, st) : launch_forward<T, P, 32>(p, st);
+  const bool wide = all_wide({{p.x, p.ldx}, {p.y, p.ldy}, {p.ldg ? p.gate : nullptr, p.ldg}, {p.xo, p.ldo}, {p.h, p.ldh}});
+  if (wide) return block == 0 ? launch_forward<T, 0, true>(p, st) : block == 16 ? launch_forward<T, 16, true>(p, st) : launch_forward<T, 32, true>(p, st);
+  return block == 0 ? launch_forward<T, 0, false>(p, st) : block == 16 ? launch_forward<T, 16, false>(p, st) : launch_forward<T, 32, false>(p, st);
 }
 
 // ----------------------------------------------------------------- backward
 struct BackParams {
-  const void* dh; int64_t lddh;
-  const void* dxo; int64_t lddo;
-  const void* xo; int64_t ldo;
-  const void* y; int64_t ldy;
+  const uint8_t* in[5]; int64_t ld[5];   // x_out, dh, dx_out, y, gate (strides in bytes; NULL where absent, the gate where it is no matrix)
   const void* w;
   const void* wp;
-  const void* gate; int64_t ldg;
-  void* dx; int64_t lddx;
-  void* dy; int64_t lddy;
-  void* dgate; int64_t lddg;     // matrix; NULL where it is a vector
-  float* parts;                  // [CTA][3][cols]: dw, dwp, dgate
+  const void* gate;                      // as a vector
+  uint8_t* dx; int64_t lddx;
+  uint8_t* dy; int64_t lddy;
+  uint8_t* dgate; int64_t lddg;          // matrix; NULL where it is a vector
+  float* parts;                          // [block][2][cols]
   int64_t rows;
   int32_t cols;
   float scale;
-  double eps;
+  double eps, inv_n;
+  int32_t stages, chunks;
+  int32_t param32;
 };
 
+// Row sums: 0 x^2, 1 y^2, 2 dn x, 3 P dx', 4 P dn, 5 P x.
 struct BackSums {
-  double squares[2][2][kMaxThreads / 32];
-  float4 dots[2][kMaxThreads / 32];
+  float part[kMaxThreads / 32][8];
+  double wide[2][kMaxThreads / 32];
+  float4 row[8];                 // r, q and the two coefficients, one row to a group
 };
 
-// A thread's units lie blockDim.x units apart (one; two for rows of more than 8192 elements, whose column sums then are in
-// shared memory: HELD).  The row is read twice, the second time from the caches.
-template <typename T, typename P, bool HELD>
+// Sums over the warp of eight values per lane: lane l ends with the one of index l / 4.
+__device__ __forceinline__ float warp_sums(float (&v)[8]) {
+  const int lane = (int)(threadIdx.x & 31u);
+#pragma unroll
+  for (int half = 4; half > 0; half /= 2) {
+    const bool upper = lane & (4 * half);
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float send = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, 4 * half);
+    }
+  }
+  float s = v[0] + __shfl_xor_sync(0xFFFFFFFFu, v[0], 2);
+  return s + __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+}
+
+// One unit to a thread and the rows in flight in shared memory, or (HELD, rows of more than 8192 elements) two units, rows read
+// twice from global memory (the second time from the caches) and the column sums in shared memory.
+//  The column sums are two: of dh x r, and of g k y q, in which a vector's k is left out: dpost and a
+// vector's dgate are that sum times what their columns share.
+template <typename T, bool HELD, bool WIDE>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(const __grid_constant__ BackParams p) {
-  extern __shared__ float held[];          // [3][cols rounded up to units]: column sums (HELD, and to add those of blockDim.y rows)
+  extern __shared__ __align__(16) uint8_t slots[];
   __shared__ BackSums sums;
+  float* const held = reinterpret_cast<float*>(slots);       // [2][cols rounded up to units]
+  constexpr int NU = HELD ? 2 : 1, E = (int)sizeof(T);
   const int tx = threadIdx.x, TX = blockDim.x;
   const int width = (p.cols + kUnit - 1) / kUnit * kUnit;
-  constexpr int NU = HELD ? 2 : 1;
-  float cw[kUnit], cp[kUnit], cg[kUnit];
+  const uint32_t stride = (uint32_t)(TX * (int)blockDim.y) * 16u;
+  const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * TX + tx) * 16u;
+  const uint32_t per_unit = (uint32_t)p.chunks * stride;
+  enum { X, DH, DX, Y, G };
+  const bool matrix = p.in[G] != nullptr, block = p.in[Y] != nullptr;
+  uint32_t slot_of[5], present = 0;
 #pragma unroll
-  for (int j = 0; j < kUnit; ++j) cw[j] = cp[j] = cg[j] = 0.f;
+  for (int m = 0; m < 5; ++m) slot_of[m] = per_unit * (p.in[m] ? present++ : 0u);
+  const uint32_t per_stage = present * per_unit;
+  auto unit_at = [&](int i) { return (i * TX + tx) * kUnit; };
   if constexpr (HELD) {
-    for (int i = tx; i < 3 * width; i += TX) held[i] = 0.f;
+    for (int i = tx; i < 2 * width; i += TX) held[i] = 0.f;
     __syncthreads();
   }
   sm100::grid_dependency_wait();
   sm100::grid_launch_dependents();
-  const float inv_n = 1.f / (float)p.cols;
-  int slot = 0;
-  const int64_t step = (int64_t)gridDim.x * blockDim.y;
-  for (int64_t base = (int64_t)blockIdx.x * blockDim.y; base < p.rows; base += step, slot ^= 1) {
-    const int64_t row = base + threadIdx.y;
-    const bool live = row < p.rows;
-    const int cols = live ? p.cols : 0;
-    const int64_t r0 = live ? row : 0;
-    auto load = [&](const void* m, int64_t ld, int e) { return rowvec::load_unit<T, rowvec::kKeep>(static_cast<const T*>(m) + r0 * ld + e, cols - e); };
-    auto param = [&](const void* v, int e) { return rowvec::load_unit<P, rowvec::kKeep>(static_cast<const P*>(v) + e, p.cols - e); };
-    // k of a unit: gate scale, or scale alone.
-    auto factor = [&](int e) {
-      Unit<float> k;
-      if (p.gate) return p.ldg ? gate_scale(load(p.gate, p.ldg, e), p.scale) : gate_scale(param(p.gate, e), p.scale);
+  const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
+  auto issue = [&](int64_t row, uint32_t slot) {
+    if (row < p.rows) {
+      const int e = unit_at(0);
 #pragma unroll
-      for (int j = 0; j < kUnit; ++j) k.w[j] = __float_as_uint(p.scale);
-      return k;
+      for (int m = 0; m < 5; ++m)
+        if (p.in[m]) issue_unit<T, WIDE>(slot + slot_of[m], stride, p.in[m] + row * p.ld[m] + e * E, p.cols - e);
+    }
+    commit_copies();
+  };
+  if constexpr (!HELD)
+    for (int s = 0; s < p.stages; ++s) issue(first + s * step, mine + (uint32_t)s * per_stage);
+
+  F2 vw[kUnit / 2], vk[kUnit / 2];       // w, and k wp (wp scale with a gate matrix)
+  auto load_vectors = [&](int e) {
+    F2 k[kUnit / 2];
+    load_params<T>(p.w, p.param32, e, p.cols - e, vw);
+    load_params<T>(p.wp, p.param32, e, p.cols - e, vk);
+    load_params<T>(p.gate, p.param32, e, p.cols - e, k);
+#pragma unroll
+    for (int j = 0; j < kUnit / 2; ++j) vk[j] = mul2(vk[j], mul2(k[j], f2(p.scale)));
+  };
+  F2 cw[kUnit / 2], cs[kUnit / 2];
+#pragma unroll
+  for (int j = 0; j < kUnit / 2; ++j) cw[j] = cs[j] = f2(0.f);
+  if constexpr (!HELD) load_vectors(unit_at(0));
+  const float inv_n = (float)p.inv_n;
+  const int warps = TX >> 5, first_warp = (int)threadIdx.y * warps, lane = tx & 31;
+
+  int stage = 0;
+  for (int64_t row = first; row < p.rows; row += step) {
+    const uint32_t at = mine + (uint32_t)stage * per_stage;
+    if constexpr (!HELD) wait_copies(p.stages - 1);
+    auto get = [&](int m, int i) {
+      const int e = unit_at(i), n = p.cols - e;
+      Unit<T> u;
+      if (!p.in[m]) u.clear();
+      else if constexpr (HELD) u = rowvec::load_unit<T, rowvec::kKeep>(reinterpret_cast<const T*>(p.in[m] + row * p.ld[m]) + e, n);
+      else u = take_unit<T, WIDE>(at + slot_of[m], stride, WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(p.in[m] + row * p.ld[m]) & 15u, n);
+      return u;
     };
-    // ---- row sums
-    double sx = 0.0, sy = 0.0;
-    float a = 0.f, b1 = 0.f, b2 = 0.f, b3 = 0.f;
-    auto add = [&](int i, bool wide) {
-      const int e = (i * TX + tx) * kUnit;
-      const Unit<T> x = load(p.xo, p.ldo, e);
-      sx += squares<T>(x, wide);
-      Unit<T> y;
+  // ---- row sums
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      if constexpr (HELD) load_vectors(unit_at(i));
+      const Unit<T> x = get(X, i), dh = get(DH, i);
+      F2 s0 = f2(0.f), s2 = f2(0.f);
+#pragma unroll
+      for (int j = 0; j < kUnit / 2; ++j) {
+        const F2 xv = pair(x, j);
+        s0 = fma2(xv, xv, s0);
+        s2 = fma2(mul2(pair(dh, j), vw[j]), xv, s2);
+      }
+      v[0] += both(s0);
+      v[2] += both(s2);
       if (p.wp) {
-        y = load(p.y, p.ldy, e);
-        sy += squares<T>(y, wide);
-      }
-      if (wide) return;
-      const Unit<T> dh = load(p.dh, p.lddh, e);
-      float dn[kUnit];
+        const Unit<T> y = get(Y, i), d = get(DX, i), g = get(G, i);
+        F2 s1 = f2(0.f), s3 = f2(0.f), s4 = f2(0.f), s5 = f2(0.f);
 #pragma unroll
-      for (int j = 0; j < kUnit; ++j) dn[j] = dh.get(j);
-      if (p.w) {
-        const Unit<P> w = param(p.w, e);
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) dn[j] *= w.get(j);
-      }
-#pragma unroll
-      for (int j = 0; j < kUnit; ++j) a = fmaf(dn[j], x.get(j), a);
-      if (p.wp) {
-        const Unit<float> k = factor(e);
-        const Unit<P> wp = param(p.wp, e);
-        Unit<T> d;
-        if (p.dxo) d = load(p.dxo, p.lddo, e); else d.clear();
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-          const float f = k.get(j) * wp.get(j) * y.get(j);
-          b1 = fmaf(f, d.get(j), b1);
-          b2 = fmaf(f, dn[j], b2);
-          b3 = fmaf(f, x.get(j), b3);
+        for (int j = 0; j < kUnit / 2; ++j) {
+          const F2 yv = pair(y, j);
+          s1 = fma2(yv, yv, s1);
+          F2 f = mul2(vk[j], yv);
+          if (matrix) f = mul2(f, pair(g, j));
+          s3 = fma2(f, pair(d, j), s3);
+          s4 = fma2(f, mul2(pair(dh, j), vw[j]), s4);
+          s5 = fma2(f, pair(x, j), s5);
         }
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < NU; ++i) add(i, false);
-    auto exchange = [&](int s, bool dots) {
-      const int warps = TX >> 5, first = (int)threadIdx.y * warps, at = first + (tx >> 5);
-      sx = warp_sum(sx);
-      if (p.wp) sy = warp_sum(sy);
-      if (dots) {
-        a = warp_sum(a);
-        if (p.wp) { b1 = warp_sum(b1); b2 = warp_sum(b2); b3 = warp_sum(b3); }
-      }
-      if (warps == 1) return;
-      if ((tx & 31) == 0) {
-        sums.squares[s][0][at] = sx;
-        sums.squares[s][1][at] = sy;
-        if (dots) sums.dots[s][at] = make_float4(a, b1, b2, b3);
-      }
-      __syncthreads();
-      sx = sy = 0.0;
-      if (dots) a = b1 = b2 = b3 = 0.f;
-      for (int i = first; i < first + warps; ++i) {
-        sx += sums.squares[s][0][i];
-        sy += sums.squares[s][1][i];
-        if (dots) {
-          const float4 d = sums.dots[s][i];
-          a += d.x; b1 += d.y; b2 += d.z; b3 += d.w;
-        }
-      }
-    };
-    exchange(slot, true);
-    if constexpr (sizeof(T) == 2) {
-      const bool again = out_of_range(sx) || (p.wp && out_of_range(sy));
-      if (blockDim.y == 1 ? again : __syncthreads_or(again)) {
-        __syncthreads();
-        sx = sy = 0.0;
-#pragma unroll
-        for (int i = 0; i < NU; ++i) add(i, true);
-        exchange(slot, false);
-        __syncthreads();
+        v[1] += both(s1);
+        v[3] += both(s3);
+        v[4] += both(s4);
+        v[5] += both(s5);
       }
     }
-    const float r = inverse_root(sx / p.cols + p.eps);
-    const float q = p.wp ? inverse_root(sy / p.cols + p.eps) : 1.f;
-    const float back = r * r * r * (a * inv_n);
-    const float back2 = q * q * q * ((b1 + r * b2 - back * b3) * inv_n);
+    const float s = warp_sums(v);
+    if ((lane & 3) == 0) sums.part[first_warp + (tx >> 5)][lane >> 2] = s;
+    group_sync();
+    // The group's first warp adds the warps' sums: lane l the values 4 (l & 1) .. + 3 of warp l / 2.
+    if (tx < 32) {
+      float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+      if ((lane >> 1) < warps) t = *reinterpret_cast<const float4*>(&sums.part[first_warp + (lane >> 1)][4 * (lane & 1)]);
+#pragma unroll
+      for (int o = 2; o < 32; o *= 2) {
+        t.x += __shfl_xor_sync(0xFFFFFFFFu, t.x, o);
+        t.y += __shfl_xor_sync(0xFFFFFFFFu, t.y, o);
+        t.z += __shfl_xor_sync(0xFFFFFFFFu, t.z, o);
+        t.w += __shfl_xor_sync(0xFFFFFFFFu, t.w, o);
+      }
+      const float b2 = __shfl_sync(0xFFFFFFFFu, t.x, 1), b3 = __shfl_sync(0xFFFFFFFFu, t.y, 1);
+      if (lane == 0) {
+        // r, q and the coefficients; or -1 for statistics that have to be taken in 64 bits, and what the coefficients need.
+        const bool again = out_of_range(t.x) || (p.wp && out_of_range(t.y));
+        const float r = again ? -1.f : inverse_root(fma((double)t.x, p.inv_n, p.eps)), q = p.wp && !again ? inverse_root(fma((double)t.y, p.inv_n, p.eps)) : 1.f;
+        const float back = r * r * r * (t.z * inv_n);
+        sums.row[threadIdx.y] = again ? make_float4(-1.f, t.z, t.w, 0.f) : make_float4(r, q, back, q * q * q * ((t.w + r * b2 - back * b3) * inv_n));
+        if (again) { sums.part[first_warp][0] = b2; sums.part[first_warp][1] = b3; }
+      }
+    }
+    group_sync();
+    float4 c = sums.row[threadIdx.y];
+    if (c.x < 0.f) {       // of the whole group
+      const float b2 = sums.part[first_warp][0], b3 = sums.part[first_warp][1];
+      double sx = 0.0, sy = 0.0;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        sx += squares_wide<T>(get(X, i));
+        if (p.wp) sy += squares_wide<T>(get(Y, i));
+      }
+      group_sync();
+      sx = across_warps(warp_sum(sx), sums.wide[0]);
+      sy = across_warps(warp_sum(sy), sums.wide[1]);
+      const float r = inverse_root(fma(sx, p.inv_n, p.eps)), q = p.wp ? inverse_root(fma(sy, p.inv_n, p.eps)) : 1.f;
+      const float back = r * r * r * (c.y * inv_n);
+      c = make_float4(r, q, back, q * q * q * ((c.z + r * b2 - back * b3) * inv_n));
+    }
     // ---- gradients
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int e = (i * TX + tx) * kUnit;
-      const Unit<T> x = load(p.xo, p.ldo, e), dh = load(p.dh, p.lddh, e);
+      const int e = unit_at(i);
+      if constexpr (HELD) load_vectors(e);
+      const Unit<T> x = get(X, i), dh = get(DH, i), d = get(DX, i);
       Unit<T> o;
-      float g[kUnit];
-      if (p.dxo) {
-        const Unit<T> d = load(p.dxo, p.lddo, e);
+      F2 g[kUnit / 2];
+      const F2 r = f2(c.x), q = f2(c.y), back = f2(-c.z), back2 = f2(-c.w);
 #pragma unroll
-        for (int j = 0; j < kUnit; ++j) g[j] = d.get(j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) g[j] = 0.f;
-      }
-      float nw[kUnit], np[kUnit], ng[kUnit];         // this row's parts of the column sums
-      if (p.w) {
-        const Unit<P> w = param(p.w, e);
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-          g[j] += r * (dh.get(j) * w.get(j)) - back * x.get(j);
-          nw[j] = dh.get(j) * (x.get(j) * r);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-          g[j] += r * dh.get(j) - back * x.get(j);
-          nw[j] = 0.f;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kUnit; j += 2) o.set2(j, g[j], g[j + 1]);
-      if (p.dx) rowvec::store_unit<T>(static_cast<T*>(p.dx) + r0 * p.lddx + e, o, cols - e);
-#pragma unroll
-      for (int j = 0; j < kUnit; ++j) np[j] = ng[j] = 0.f;
-      if (p.y) {
-        const Unit<T> y = load(p.y, p.ldy, e);
-        const Unit<float> k = factor(e);
-        if (p.wp) {
-          const Unit<P> wp = param(p.wp, e);
-#pragma unroll
-          for (int j = 0; j < kUnit; j += 2) {
-            float d[2];
-#pragma unroll
-            for (int l = 0; l < 2; ++l) {
-              const float yn = y.get(j + l) * q, dz = g[j + l] * k.get(j + l);
-              np[j + l] = dz * yn;
-              ng[j + l] = g[j + l] * (yn * wp.get(j + l)) * p.scale;
-              d[l] = q * (dz * wp.get(j + l)) - back2 * y.get(j + l);
-            }
-            o.set2(j, d[0], d[1]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kUnit; j += 2) {
-            ng[j] = g[j] * y.get(j) * p.scale;
-            ng[j + 1] = g[j + 1] * y.get(j + 1) * p.scale;
-            o.set2(j, g[j] * k.get(j), g[j + 1] * k.get(j + 1));
-          }
-        }
-        if (p.dy) rowvec::store_unit<T>(static_cast<T*>(p.dy) + r0 * p.lddy + e, o, cols - e);
-        if (p.dgate) {
-#pragma unroll
-          for (int j = 0; j < kUnit; j += 2) o.set2(j, ng[j], ng[j + 1]);
-          rowvec::store_unit<T>(static_cast<T*>(p.dgate) + r0 * p.lddg + e, o, cols - e);
-        }
-      }
-      // (Elements beyond the row are zeros; a row that is not there has no part, whatever its statistics.)
-      if (live && e < p.cols) {
+      for (int j = 0; j < kUnit / 2; ++j) {
+        const F2 xv = pair(x, j), dv = pair(dh, j);
+        g[j] = fma2(r, mul2(dv, vw[j]), fma2(back, xv, pair(d, j)));
+        const F2 part = mul2(dv, mul2(xv, r));
         if constexpr (HELD) {
-#pragma unroll
-          for (int j = 0; j < kUnit; ++j) {
-            held[e + j] += nw[j];
-            held[width + e + j] += np[j];
-            held[2 * width + e + j] += ng[j];
-          }
+          float a, b;
+          part.get(a, b);
+          if (e + 2 * j < width) { held[e + 2 * j] += a; held[e + 2 * j + 1] += b; }
         } else {
-#pragma unroll
-          for (int j = 0; j < kUnit; ++j) { cw[j] += nw[j]; cp[j] += np[j]; cg[j] += ng[j]; }
+          cw[j] = add2(cw[j], part);
         }
+        float a, b;
+        g[j].get(a, b);
+        o.set2(2 * j, a, b);
       }
+      put_unit<T, WIDE>(p.dx + row * p.lddx + e * E, o, p.cols - e);
+      if (!block) continue;
+      const Unit<T> y = get(Y, i), gate = get(G, i);
+      Unit<T> og;
+#pragma unroll
+      for (int j = 0; j < kUnit / 2; ++j) {
+        const F2 yv = pair(y, j), yn = mul2(yv, q), gv = matrix ? pair(gate, j) : f2(1.f);
+        F2 part = mul2(g[j], yn);
+        F2 t = mul2(mul2(g[j], vk[j]), gv);        // g k wp
+        float a, b;
+        if (matrix) {
+          mul2(part, vk[j]).get(a, b);             // (vk holds wp scale)
+          og.set2(2 * j, a, b);
+          part = mul2(part, mul2(gv, f2(p.scale)));
+        }
+        if constexpr (HELD) {
+          part.get(a, b);
+          if (e + 2 * j < width) { held[width + e + 2 * j] += a; held[width + e + 2 * j + 1] += b; }
+        } else {
+          cs[j] = add2(cs[j], part);
+        }
+        t = p.wp ? fma2(q, t, mul2(back2, yv)) : t;
+        t.get(a, b);
+        o.set2(2 * j, a, b);
+      }
+      put_unit<T, WIDE>(p.dy + row * p.lddy + e * E, o, p.cols - e);
+      if (p.dgate) put_unit<T, WIDE>(p.dgate + row * p.lddg + e * E, og, p.cols - e);
     }
+    if constexpr (!HELD) issue(row + p.stages * step, at);
+    if (++stage == p.stages) stage = 0;
   }
-  // ---- this CTA's column sums
-  float* const out = p.parts + (int64_t)blockIdx.x * 3 * p.cols;
+  // ---- this block's column sums
+  wait_copies(0);
+  __syncthreads();
   if constexpr (!HELD) {
-    const int e = tx * kUnit;
+    const int e = unit_at(0);
     for (int t = 0; t < (int)blockDim.y; ++t) {
       if ((int)threadIdx.y == t && e < p.cols) {
 #pragma unroll
-        for (int j = 0; j < kUnit; ++j) {
-          held[e + j] = t ? held[e + j] + cw[j] : cw[j];
-          held[width + e + j] = t ? held[width + e + j] + cp[j] : cp[j];
-          held[2 * width + e + j] = t ? held[2 * width + e + j] + cg[j] : cg[j];
+        for (int j = 0; j < kUnit / 2; ++j) {
+          float a, b;
+          cw[j].get(a, b);
+          held[e + 2 * j] = t ? held[e + 2 * j] + a : a;
+          held[e + 2 * j + 1] = t ? held[e + 2 * j + 1] + b : b;
+          cs[j].get(a, b);
+          held[width + e + 2 * j] = t ? held[width + e + 2 * j] + a : a;
+          held[width + e + 2 * j + 1] = t ? held[width + e + 2 * j + 1] + b : b;
         }
       }
       __syncthreads();
     }
-  } else {
-    __syncthreads();
   }
+  float* const out = p.parts + (int64_t)blockIdx.x * 2 * p.cols;
   const int all = TX * (int)blockDim.y, me = (int)threadIdx.y * TX + tx;
-#pragma unroll
-  for (int v = 0; v < 3; ++v)
-    for (int i = me; i < p.cols; i += all) out[v * p.cols + i] = held[v * width + i];
+  for (int i = me; i < p.cols; i += all) {
+    out[i] = held[i];
+    out[p.cols + i] = held[width + i];
+  }
 }
 
 struct ColumnParams {
   const float* parts;
-  float* out[3];
-  int32_t ctas, cols;
+  float* dw;
+  float* dp;
+  float* dg;
+  const void* wp;
+  const void* gate;
+  int32_t param_type, blocks, cols;
+  int32_t matrix;
+  float scale;
 };
-// Sums of the CTAs' parts: 32 columns of one output per block, 8 slices of the parts.
+// Sums of the blocks' parts: 32 columns per block, 8 slices of the parts; then what the columns of dpost and dgate share.
 __global__ void __launch_bounds__(256) residual_norm_columns_kernel(const __grid_constant__ ColumnParams p) {
   __shared__ float slice[8][33];
   sm100::grid_dependency_wait();
   sm100::grid_launch_dependents();
-  float* const out = p.out[blockIdx.y];
-  if (!out) return;
+  const bool second = blockIdx.y == 1;
+  if (second ? !p.dp && !p.dg : !p.dw) return;
   const int c = (int)blockIdx.x * 32 + (int)threadIdx.x;
   float s = 0.f;
   if (c < p.cols) {
     const float* const at = p.parts + (int64_t)blockIdx.y * p.cols + c;
 #pragma unroll 8
-    for (int i = (int)threadIdx.y; i < p.ctas; i += 8) s += at[(int64_t)i * 3 * p.cols];
+    for (int i = (int)threadIdx.y; i < p.blocks; i += 8) s += at[(int64_t)i * 2 * p.cols];
   }
   slice[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && c < p.cols) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) s += slice[i][threadIdx.x];
-    out[c] = s;
+    if (!second) {
+      p.dw[c] = s;
+    } else {
+      if (p.dp) p.dp[c] = p.matrix ? s : s * (p.gate ? load_as_f32(p.gate, p.param_type, c) * p.scale : p.scale);
+      if (p.dg) p.dg[c] = s * ((p.wp ? load_as_f32(p.wp, p.param_type, c) : 1.f) * p.scale);
+    }
   }
 }
 
-// Threads of a row, rows of a CTA and CTAs of the backward pass.
-struct BackShape {
-  int tx, ty, ctas, held_bytes;
-  bool held;
-};
-BackShape back_shape(int64_t rows, int64_t cols) {
-  BackShape s;
+// `chunks`: those of a thread's units in all matrices.
+Shape back_shape(int64_t rows, int64_t cols, int chunks) {
   const int units = (int)((cols + kUnit - 1) / kUnit);
-  s.held = units > kMaxThreads;
-  s.tx = s.held ? kMaxThreads : (units + 31) / 32 * 32;
-  s.ty = s.tx >= 256 ? 1 : 256 / s.tx;
-  if (s.ty > rows) s.ty = rows < 1 ? 1 : (int)rows;
-  const int64_t groups = (rows + s.ty - 1) / s.ty, most = 148 * (s.tx > 256 || s.held ? 1 : 2);
-  s.ctas = (int)(groups < most ? groups : most);
-  s.held_bytes = 3 * units * kUnit * 4;
+  if (units > kMaxThreads) {
+    Shape s;
+    s.tx = kMaxThreads; s.ty = 1; s.stages = 0;
+    s.blocks = (int)(rows < 148 ? rows : 148);
+    s.smem = (size_t)units * kUnit * 8;
+    return s;
+  }
+  Shape s = shape_of(rows, units, 1, chunks * 16);
+  const size_t sums = (size_t)units * kUnit * 8;
+  if (s.smem < sums) s.smem = sums;
   return s;
 }
 
-template <typename T, typename P>
-cudaError_t launch_backward(const BackParams& p, const BackShape& s, cudaStream_t st) {
-  const auto fn = s.held ? residual_norm_backward_kernel<T, P, true> : residual_norm_backward_kernel<T, P, false>;
-  // (Always the same limit: calls of other sizes may be between this line and the launch.)
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * kMaxCols * 4);
+template <typename T>
+cudaError_t launch_backward(BackParams p, const Shape& s, bool wide, cudaStream_t st) {
+  const auto fn = p.cols > kMaxThreads * kUnit ? residual_norm_backward_kernel<T, true, false>
+                : wide ? residual_norm_backward_kernel<T, false, true> : residual_norm_backward_kernel<T, false, false>;
+  p.stages = s.stages;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(fn, dim3((unsigned)s.ctas), dim3((unsigned)s.tx, (unsigned)s.ty), (size_t)s.held_bytes, 1, st, p);
+  return launch_overlapped(fn, dim3((unsigned)s.blocks), dim3((unsigned)s.tx, (unsigned)s.ty), s.smem, 1, st, p);
 }
 
 int status_of(cudaError_t err) {
@@ -595,24 +846,23 @@ extern "C" int gemm_sm100a_residual_norm(const ResidualNormArgs* a, void* stream
     return GEMM_ERR_CANNOT_IMPLEMENT;
   NormParams p;
   memset(&p, 0, sizeof(p));
-  p.x = a->x; p.ldx = a->ldx; p.y = a->y; p.ldy = a->ldy; p.xo = a->x_out; p.ldo = a->ldo; p.h = a->h; p.ldh = a->ldh;
-  p.w = a->weight; p.wp = a->post_weight; p.gate = a->gate; p.ldg = a->gate ? a->ldg : 0;
-  p.rows = a->rows; p.cols = (int32_t)a->cols; p.scale = a->scale; p.eps = a->eps;
+  p.x = static_cast<const uint8_t*>(a->x); p.ldx = a->ldx * e; p.y = static_cast<const uint8_t*>(a->y); p.ldy = a->ldy * e;
+  p.xo = static_cast<uint8_t*>(a->x_out); p.ldo = a->ldo * e; p.h = static_cast<uint8_t*>(a->h); p.ldh = a->ldh * e;
+  p.w = a->weight; p.wp = a->post_weight; p.gate = static_cast<const uint8_t*>(a->gate); p.ldg = matrix ? a->ldg * e : 0;
+  p.rows = a->rows; p.cols = (int32_t)a->cols; p.scale = a->scale; p.eps = a->eps; p.inv_n = 1.0 / (double)a->cols;
+  p.param32 = a->param_type == GEMM_TYPE_FP32;
   p.values = static_cast<uint8_t*>(a->values); p.ldv = a->ldv; p.scales = static_cast<uint8_t*>(a->scales); p.row_scale = a->row_scale;
   p.tiles = a->block ? fp4op::scale_tiles(a->cols, a->block) : 0;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   PointerDeviceGuard guard(a->block ? a->values : a->h);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
-  const bool p32 = a->param_type == GEMM_TYPE_FP32;
-  if (a->type == GEMM_TYPE_BF16)
-    return status_of(p32 ? launch_forward<__nv_bfloat16, float>(p, a->block, st) : launch_forward<__nv_bfloat16, __nv_bfloat16>(p, a->block, st));
-  if (a->type == GEMM_TYPE_FP16) return status_of(p32 ? launch_forward<__half, float>(p, a->block, st) : launch_forward<__half, __half>(p, a->block, st));
-  return status_of(launch_forward<float, float>(p, a->block, st));
+  return status_of(a->type == GEMM_TYPE_BF16 ? launch_forward<__nv_bfloat16>(p, a->block, st)
+                 : a->type == GEMM_TYPE_FP16 ? launch_forward<__half>(p, a->block, st) : launch_forward<float>(p, a->block, st));
 }
 
 extern "C" int64_t gemm_sm100a_residual_norm_workspace(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 1 || cols > kMaxCols || rows > INT32_MAX / 2) return -1;
-  return rows == 0 ? 0 : (int64_t)back_shape(rows, cols).ctas * 3 * cols * 4;
+  return rows == 0 ? 0 : (int64_t)back_shape(rows, cols, 1).blocks * 2 * cols * 4;
 }
 
 extern "C" int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs* a, void* stream) {
@@ -640,7 +890,7 @@ extern "C" int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs
     return GEMM_OK;
   }
   if (!a->dh || !a->x_out || !a->dx || (a->y && !a->dy) || !a->workspace) return GEMM_ERR_BAD_ARGS;
-  const Mat ins[5] = {{a->dh, a->lddh}, {a->dx_out, a->lddo}, {a->x_out, a->ldo}, {a->y, a->ldy}, {matrix ? a->gate : nullptr, a->ldg}};
+  const Mat ins[5] = {{a->x_out, a->ldo}, {a->dh, a->lddh}, {a->dx_out, a->lddo}, {a->y, a->ldy}, {matrix ? a->gate : nullptr, a->ldg}};
   const Mat outs[3] = {{a->dx, a->lddx}, {a->dy, a->lddy}, {matrix ? a->dgate : nullptr, a->lddg}};
   for (const Mat& m : ins)
     if (m.p && (m.ld < a->cols || !aligned(m.p, e))) return GEMM_ERR_CANNOT_IMPLEMENT;
@@ -656,29 +906,43 @@ extern "C" int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs
       if (outs[i].p && outs[j].p && rows_meet(outs[j].p, outs[j].ld * e, a->cols * e, outs[i].p, outs[i].ld * e, a->cols * e, a->rows))
         return GEMM_ERR_CANNOT_IMPLEMENT;
   }
-  const BackShape s = back_shape(a->rows, a->cols);
-  if (a->workspace_bytes < (int64_t)s.ctas * 3 * a->cols * 4) return GEMM_ERR_BAD_ARGS;
+  bool in_wide = true, wide = true;
+  int matrices = 0;
+  for (const Mat& m : ins) {
+    in_wide &= !m.p || rows_16b(m.p, m.ld, e);
+    matrices += m.p ? 1 : 0;
+  }
+  for (const Mat& m : outs) wide &= !m.p || rows_16b(m.p, m.ld, e);
+  wide &= in_wide;
+  const int chunks = kUnit * e / 16 + (wide ? 0 : 1);
+  const Shape s = back_shape(a->rows, a->cols, matrices * chunks);
+  if (a->workspace_bytes < (int64_t)s.blocks * 2 * a->cols * 4) return GEMM_ERR_BAD_ARGS;
   BackParams p;
   memset(&p, 0, sizeof(p));
-  p.dh = a->dh; p.lddh = a->lddh; p.dxo = a->dx_out; p.lddo = a->lddo; p.xo = a->x_out; p.ldo = a->ldo; p.y = a->y; p.ldy = a->ldy;
-  p.w = a->weight; p.wp = a->post_weight; p.gate = a->gate; p.ldg = a->gate ? a->ldg : 0;
-  p.dx = a->dx; p.lddx = a->lddx; p.dy = a->dy; p.lddy = a->lddy; p.dgate = matrix ? a->dgate : nullptr; p.lddg = a->lddg;
+  for (int i = 0; i < 5; ++i) {
+    p.in[i] = static_cast<const uint8_t*>(ins[i].p);
+    p.ld[i] = ins[i].ld * e;
+  }
+  p.w = a->weight; p.wp = a->post_weight; p.gate = matrix ? nullptr : a->gate;
+  p.dx = static_cast<uint8_t*>(a->dx); p.lddx = a->lddx * e; p.dy = static_cast<uint8_t*>(a->dy); p.lddy = a->lddy * e;
+  p.dgate = matrix ? static_cast<uint8_t*>(a->dgate) : nullptr; p.lddg = a->lddg * e;
   p.parts = static_cast<float*>(a->workspace);
-  p.rows = a->rows; p.cols = (int32_t)a->cols; p.scale = a->scale; p.eps = a->eps;
+  p.rows = a->rows; p.cols = (int32_t)a->cols; p.scale = a->scale; p.eps = a->eps; p.inv_n = 1.0 / (double)a->cols;
+  p.param32 = a->param_type == GEMM_TYPE_FP32;
+  p.chunks = chunks;
   PointerDeviceGuard guard(a->dx);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
-  const bool p32 = a->param_type == GEMM_TYPE_FP32;
-  cudaError_t err;
-  if (a->type == GEMM_TYPE_BF16) err = p32 ? launch_backward<__nv_bfloat16, float>(p, s, st) : launch_backward<__nv_bfloat16, __nv_bfloat16>(p, s, st);
-  else if (a->type == GEMM_TYPE_FP16) err = p32 ? launch_backward<__half, float>(p, s, st) : launch_backward<__half, __half>(p, s, st);
-  else err = launch_backward<float, float>(p, s, st);
+  cudaError_t err = a->type == GEMM_TYPE_BF16 ? launch_backward<__nv_bfloat16>(p, s, wide, st)
+                  : a->type == GEMM_TYPE_FP16 ? launch_backward<__half>(p, s, wide, st) : launch_backward<float>(p, s, wide, st);
   if (err == cudaSuccess && any) {
     ColumnParams c;
+    memset(&c, 0, sizeof(c));
     c.parts = p.parts;
-    for (int i = 0; i < 3; ++i) c.out[i] = sums[i];
-    c.ctas = s.ctas;
-    c.cols = p.cols;
-    err = launch_overlapped(residual_norm_columns_kernel, dim3((unsigned)((p.cols + 31) / 32), 3), dim3(32, 8), 0, 1, st, c);
+    c.dw = sums[0]; c.dp = sums[1]; c.dg = sums[2];
+    c.wp = a->post_weight; c.gate = matrix ? nullptr : a->gate;
+    c.param_type = a->param_type; c.blocks = s.blocks; c.cols = p.cols;
+    c.matrix = matrix; c.scale = a->scale;
+    err = launch_overlapped(residual_norm_columns_kernel, dim3((unsigned)((p.cols + 31) / 32), 2), dim3(32, 8), 0, 1, st, c);
   }
   return status_of(err);
 }

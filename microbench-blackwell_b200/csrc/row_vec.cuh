@@ -64,6 +64,18 @@ struct Unit {
   }
 };
 
+// Zeros beyond the first `bytes` of a unit.
+template <typename T>
+__device__ __forceinline__ void clip(Unit<T>& u, int bytes) {
+  if (bytes < 4 * Unit<T>::W) {
+#pragma unroll
+    for (int j = 0; j < Unit<T>::W; ++j) {
+      const int left = bytes - 4 * j;
+      if (left < 4) u.w[j] = left == 2 ? u.w[j] & 0xFFFFu : 0u;
+    }
+  }
+}
+
 enum Cache { kStream, kKeep };   // read once, or again by other rows
 
 template <Cache C>
@@ -103,13 +115,7 @@ __device__ __forceinline__ Unit<T> load_unit(const T* ptr, int n) {
 #pragma unroll
     for (int j = 0; j < W; ++j) u.w[j] = w[j];
   }
-  if (bytes < 4 * W) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const int left = bytes - 4 * j;
-      if (left < 4) u.w[j] = left == 2 ? u.w[j] & 0xFFFFu : 0u;
-    }
-  }
+  clip(u, bytes);
   return u;
 }
 
