@@ -31,7 +31,10 @@ using rowvec::Unit;
 namespace {
 
 constexpr int kMaxCols = 16384;
-constexpr int kMaxThreads = 512;
+constexpr int kMaxThreads = 512;           // of a group, and of a backward or few-row block
+constexpr int kManyThreads = 768;          // of a forward block of many rows
+template <typename T>
+constexpr int many_threads() { return sizeof(T) == 2 ? kManyThreads : kMaxThreads; }
 constexpr int kMaxStages = 4;
 constexpr int kSmemLimit = 224 * 1024;     // dynamic shared memory of a block, and of an SM's blocks together
 
@@ -53,7 +56,8 @@ __device__ __forceinline__ void issue_unit(uint32_t slot, uint32_t stride, const
   } else if (n > 0) {
     const int bytes = n * (int)sizeof(T);
 #pragma unroll
-    for (int j = 0; j <= (WIDE ? B - 1 : B); ++j) {
+    for (int j = 0; j <= B; ++j) {
+      if (j == B && off == 0) break;               // (there may be no slot for it)
       const bool any = 16 * j - off < bytes;       // (a copy of no bytes zeroes its chunk; its address is in range all the same)
       sm100::cp_async_16(slot + (uint32_t)j * stride, any ? p - off + 16 * j : p - off, any ? 16u : 0u);
     }
@@ -117,6 +121,27 @@ __device__ __forceinline__ void group_sync() {
 // ----------------------------------------------------------------- statistics
 template <typename T>
 __device__ __forceinline__ F2 pair(const Unit<T>& u, int j) { return F2(u.get(2 * j), u.get(2 * j + 1)); }
+// Row `row` of a matrix.  (Opaque: the compiler would otherwise carry a running pointer for every chunk of every unit.)
+template <typename P>
+__device__ __forceinline__ P* row_of(P* base, int64_t row, int64_t ld) {
+  P* r = base + row * ld;
+  asm volatile("" : "+l"(r));
+  return r;
+}
+// A condition that is the same for all rows, hidden: the compiler would otherwise make a copy of the loop for each case.
+__device__ __forceinline__ bool each_row(bool c) {
+  int v = c;
+  asm volatile("" : "+r"(v));
+  return v != 0;
+}
+// Makes the compiler unpack a unit again instead of holding its elements in registers over a barrier.
+template <typename T>
+__device__ __forceinline__ void forget(Unit<T>& u) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < Unit<T>::W; ++j) asm volatile("" : "+r"(u.w[j]));
+  }
+}
 __device__ __forceinline__ float both(F2 v) {
   float a, b;
   v.get(a, b);
@@ -191,6 +216,8 @@ struct NormParams {
   int32_t stages, chunks;      // rows ahead; chunks of a unit (one more where a matrix has rows off 16-byte boundaries)
   int32_t gate_ahead;          // a gate matrix is copied ahead too
   int32_t param32;             // the vectors are fp32 (else of T)
+  int32_t vectors_at;          // many rows: byte of the vectors in shared memory
+  int32_t block;               // of the 4-bit form
 };
 
 // A vector's elements at a thread's unit as fp32 pairs; ones where there is no vector.
@@ -210,23 +237,25 @@ __device__ __forceinline__ void load_params(const void* v, int param32, int e, i
   }
 }
 
-// NU units to a thread, blockDim.x units apart.  Where they fit, the vectors stay in registers for all of the group's
-// rows (as w and wp gate scale); two units of fp32 elements leave no room, and they are read again for each row.
-// Two units to a thread halve what the statistics cost per element: 16384 x 8192 bf16 in @2@ us, @1@ with one; a call of few
-// rows is done sooner with one (1 x 8192: @a@ and @b@).
-template <typename T, int BLOCK, int NU, bool WIDE>
-__global__ void __launch_bounds__(NU == 2 && sizeof(T) == 2 ? 512 : kMaxThreads) residual_norm_kernel(const __grid_constant__ NormParams p) {
+// NU units to a thread, blockDim.x units apart.
+//  Few rows (NU 1): the vectors stay in registers.
+//  Many rows (NU 2, which halves what the statistics cost per element): the vectors lie in shared memory as w and wp gate scale,
+//    in fp32, where all groups of the block read them, and up to four groups of 8192-element rows hide one another's
+//    barriers.  Rows that leave no room for them read them from the caches each time.
+// KIND 0: no y; 1: y; 2: y and a gate matrix.  (What can be absent from call to call is decided here where
+// the compiler would otherwise make a copy of the loop for each case, with the registers of all.)
+template <typename T, bool FOUR, int NU, bool WIDE, int KIND>
+__global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
-  __shared__ double part[2][kMaxThreads / 32];
-  __shared__ uint32_t warp_max[kMaxThreads / 32];
+  __shared__ double part[2][kManyThreads / 32];
+  __shared__ uint32_t warp_max[kManyThreads / 32];
   constexpr int E = (int)sizeof(T);
-  constexpr bool KEEP = NU == 1 || E == 2;
+  constexpr bool KEEP = NU == 1, SHARED = NU == 2 && E == 2, BLOCK = KIND > 0, MATRIX = KIND == 2;
   const int tx = threadIdx.x, TX = blockDim.x;
   const uint32_t stride = (uint32_t)(TX * (int)blockDim.y) * 16u;
   const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * TX + tx) * 16u;
   const uint32_t per_unit = (uint32_t)p.chunks * stride;
-  const bool matrix = p.ldg != 0;
-  const uint32_t per_stage = (uint32_t)((1 + (p.y ? 1 : 0) + p.gate_ahead) * NU) * per_unit;
+  const uint32_t per_stage = (uint32_t)(((BLOCK ? 2 : 1) + (MATRIX ? p.gate_ahead : 0)) * NU) * per_unit;
   const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
   int e[NU], n[NU];
 #pragma unroll
@@ -238,16 +267,18 @@ __global__ void __launch_bounds__(NU == 2 && sizeof(T) == 2 ? 512 : kMaxThreads)
   sm100::grid_launch_dependents();
   auto issue = [&](int64_t row, uint32_t slot) {
     if (row < p.rows) {
+      const uint8_t* const rx = row_of(p.x, row, p.ldx);
+      const uint8_t* const ry = row_of(p.y, row, p.ldy);
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        issue_unit<T, WIDE>(slot, stride, p.x + row * p.ldx + e[i] * E, n[i]);
+        issue_unit<T, WIDE>(slot, stride, rx + e[i] * E, n[i]);
         slot += per_unit;
-        if (p.y) {
-          issue_unit<T, WIDE>(slot, stride, p.y + row * p.ldy + e[i] * E, n[i]);
+        if (BLOCK) {
+          issue_unit<T, WIDE>(slot, stride, ry + e[i] * E, n[i]);
           slot += per_unit;
         }
-        if (p.gate_ahead) {
-          issue_unit<T, WIDE>(slot, stride, p.gate + row * p.ldg + e[i] * E, n[i]);
+        if (MATRIX && p.gate_ahead) {
+          issue_unit<T, WIDE>(slot, stride, row_of(p.gate, row, p.ldg) + e[i] * E, n[i]);
           slot += per_unit;
         }
       }
@@ -256,21 +287,49 @@ __global__ void __launch_bounds__(NU == 2 && sizeof(T) == 2 ? 512 : kMaxThreads)
   };
   for (int s = 0; s < p.stages; ++s) issue(first + s * step, mine + (uint32_t)s * per_stage);
 
-  F2 vw[KEEP ? NU : 1][kUnit / 2], vk[KEEP ? NU : 1][kUnit / 2];
-  auto load_w = [&](int i) { load_params<T>(p.w, p.param32, e[i], n[i], vw[KEEP ? i : 0]); };
+  F2 vw[kUnit / 2], vk[kUnit / 2];
+  auto load_w = [&](int i) { load_params<T>(p.w, p.param32, e[i], n[i], vw); };
   auto load_k = [&](int i) {
     F2 g[kUnit / 2];
-    load_params<T>(p.wp, p.param32, e[i], n[i], vk[KEEP ? i : 0]);
-    load_params<T>(matrix ? nullptr : p.gate, p.param32, e[i], n[i], g);
+    load_params<T>(p.wp, p.param32, e[i], n[i], vk);
+    load_params<T>(MATRIX ? nullptr : p.gate, p.param32, e[i], n[i], g);
 #pragma unroll
-    for (int j = 0; j < kUnit / 2; ++j) vk[KEEP ? i : 0][j] = mul2(vk[KEEP ? i : 0][j], mul2(g[j], f2(p.scale)));
+    for (int j = 0; j < kUnit / 2; ++j) vk[j] = mul2(vk[j], mul2(g[j], f2(p.scale)));
+  };
+  // Shared vectors: four elements of a unit to a slot, slots of one kind side by side (no bank conflicts).
+  const uint32_t vectors = sm100::smem_u32(slots) + (uint32_t)p.vectors_at, per_chunk = (uint32_t)(NU * TX) * 16u;
+  auto slot_at = [&](int which, int i) { return vectors + (uint32_t)(which * 4) * per_chunk + (uint32_t)(i * TX + tx) * 16u; };
+  auto keep = [&](int which, int i, const F2 (&v)[kUnit / 2]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float f[4];
+      v[2 * c].get(f[0], f[1]);
+      v[2 * c + 1].get(f[2], f[3]);
+      sm100::st_shared_v4(slot_at(which, i) + (uint32_t)c * per_chunk, __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+  };
+  // Pairs 2 c and 2 c + 1 of a unit's vector.
+  auto kept = [&](int which, int i, int c, F2& a, F2& b) {
+    const uint4 u = sm100::ld_shared_v4(slot_at(which, i) + (uint32_t)c * per_chunk);
+    a = F2(__uint_as_float(u.x), __uint_as_float(u.y));
+    b = F2(__uint_as_float(u.z), __uint_as_float(u.w));
   };
   if constexpr (KEEP) {
+    load_w(0);
+    if (BLOCK) load_k(0);
+  } else if (SHARED) {
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      load_w(i);
-      if (p.y) load_k(i);
+      if (((int)threadIdx.y - i) % (int)blockDim.y == 0 || blockDim.y == 1) {
+        load_w(i);
+        keep(0, i, vw);
+        if (BLOCK) {
+          load_k(i);
+          keep(1, i, vk);
+        }
+      }
     }
+    __syncthreads();
   }
 
   int flip = 0;       // a call's buffer is written again by the second call after it, with a barrier between
@@ -313,46 +372,63 @@ __global__ void __launch_bounds__(NU == 2 && sizeof(T) == 2 ? 512 : kMaxThreads)
       for (int i = 0; i < NU; ++i) {
         x[i] = take_unit<T, WIDE>(slot, stride, low(rx), n[i]);
         slot += per_unit;
-        if (p.y) {
+        if (BLOCK) {
           y[i] = take_unit<T, WIDE>(slot, stride, low(ry), n[i]);
           slot += per_unit;
         }
-        if (p.gate_ahead) {
+        if (MATRIX && p.gate_ahead) {
           gate[i] = take_unit<T, WIDE>(slot, stride, low(rg), n[i]);
           slot += per_unit;
-        } else if (matrix) {
+        } else if (MATRIX) {
           gate[i] = rowvec::load_unit<T>(reinterpret_cast<const T*>(rg) + e[i], n[i]);
         }
       }
     }
     issue(row + p.stages * step, at);
     if (++stage == p.stages) stage = 0;
-    if (p.y) {
+    if constexpr (BLOCK) {
       const F2 q = f2(p.wp ? inverse_rms(y) : 1.f);
-      uint8_t* const out = p.xo + row * p.ldo;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) forget(y[i]);
+      uint8_t* const out = row_of(p.xo, row, p.ldo);
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        if constexpr (!KEEP) load_k(i);
+        if (!KEEP && !SHARED) load_k(i);
 #pragma unroll
-        for (int j = 0; j < kUnit / 2; ++j) {
-          F2 z = mul2(pair(y[i], j), q), k = vk[KEEP ? i : 0][j];
-          if (matrix) k = mul2(k, pair(gate[i], j));
-          float a, b;
-          fma2(z, k, pair(x[i], j)).get(a, b);
-          x[i].set2(2 * j, a, b);
+        for (int c = 0; c < 4; ++c) {
+          F2 k[2] = {vk[2 * c], vk[2 * c + 1]};
+          if (SHARED) kept(1, i, c, k[0], k[1]);
+#pragma unroll
+          for (int l = 0; l < 2; ++l) {
+            const int j = 2 * c + l;
+            if (MATRIX) k[l] = mul2(k[l], pair(gate[i], j));
+            float a, b;
+            fma2(mul2(pair(y[i], j), q), k[l], pair(x[i], j)).get(a, b);
+            x[i].set2(2 * j, a, b);
+          }
         }
         put_unit<T, WIDE>(out + e[i] * E, x[i], n[i]);
       }
     }
     const F2 r = f2(inverse_rms(x));
+#pragma unroll
+    for (int i = 0; i < NU; ++i) forget(x[i]);
     // h of a unit, in fp32.
     auto norm = [&](int i, float (&h)[kUnit]) {
-      if constexpr (!KEEP) load_w(i);
+      if (!KEEP && !SHARED) load_w(i);
 #pragma unroll
-      for (int j = 0; j < kUnit / 2; ++j) mul2(mul2(pair(x[i], j), r), vw[KEEP ? i : 0][j]).get(h[2 * j], h[2 * j + 1]);
+      for (int c = 0; c < 4; ++c) {
+        F2 w[2] = {vw[2 * c], vw[2 * c + 1]};
+        if (SHARED) kept(0, i, c, w[0], w[1]);
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+          const int j = 2 * c + l;
+          mul2(mul2(pair(x[i], j), r), w[l]).get(h[2 * j], h[2 * j + 1]);
+        }
+      }
     };
-    if constexpr (BLOCK == 0) {
-      uint8_t* const out = p.h + row * p.ldh;
+    if constexpr (!FOUR) {
+      uint8_t* const out = row_of(p.h, row, p.ldh);
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         float h[kUnit];
@@ -387,7 +463,7 @@ __global__ void __launch_bounds__(NU == 2 && sizeof(T) == 2 ? 512 : kMaxThreads)
       }
       const fp4op::RowScale s = fp4op::row_scale(top);
       if (tx == 0) p.row_scale[row] = s.scale;
-      const int units = (int)p.tiles * 4 * (BLOCK / 16);
+      const int units = (int)p.tiles * 4 * (p.block / 16);
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         const int unit = i * TX + tx;
@@ -395,8 +471,8 @@ __global__ void __launch_bounds__(NU == 2 && sizeof(T) == 2 ? 512 : kMaxThreads)
 #pragma unroll
         for (int j = 0; j < kUnit; ++j) h[i][j] = s.up == 0.f ? 0.f : h[i][j] * s.up;
         uint32_t q[2];
-        const uint32_t code = fp4op::quantize_unit<BLOCK>(h[i], q);
-        fp4op::store_scale_codes<BLOCK>(p.scales, row, p.tiles, unit, code, unit < units);
+        if (p.block == 16) fp4op::store_scale_codes<16>(p.scales, row, p.tiles, unit, fp4op::quantize_unit<16>(h[i], q), unit < units);
+        else fp4op::store_scale_codes<32>(p.scales, row, p.tiles, unit, fp4op::quantize_unit<32>(h[i], q), unit < units);
         if (n[i] > 0) fp4op::store_codes(p.values + row * p.ldv + unit * 8, q, n[i]);
       }
     }
@@ -408,18 +484,24 @@ struct Shape {
   int tx, ty, blocks, stages;
   size_t smem;
 };
-Shape shape_of(int64_t rows, int units, int per_thread, int bytes) {
+// `most_threads` of a block; `fixed`: shared memory of a block beside the rows'.
+Shape shape_of(int64_t rows, int units, int per_thread, int bytes, int most_threads = kMaxThreads, int fixed = 0) {
   Shape s;
   s.tx = ((units + per_thread - 1) / per_thread + 31) / 32 * 32;
-  int64_t ty = kMaxThreads / s.tx;
+  const int room = kSmemLimit - fixed;
+  int64_t ty = most_threads / s.tx;
   const int64_t spread = (rows + 147) / 148;       // rows over all SMs before more of them in a block
   if (ty > spread) ty = spread;
-  if (ty > 8) ty = 8;
+  if (ty > room / (bytes * s.tx)) ty = room / (bytes * s.tx);
+  if (ty > (s.tx == 32 ? 32 : 15)) ty = s.tx == 32 ? 32 : 15;       // named barriers
   s.ty = (int)(ty < 1 ? 1 : ty);
-  const int threads = s.tx * s.ty, resident = kMaxThreads / threads;
+  const int threads = s.tx * s.ty;
+  int resident = fixed ? 1 : most_threads / threads;
+  if (resident > room / (bytes * threads)) resident = room / (bytes * threads);      // at least one row ahead
+  if (resident < 1) resident = 1;
   const int64_t blocks = (rows + s.ty - 1) / s.ty, most = 148 * resident;
   s.blocks = (int)(blocks < most ? blocks : most);
-  s.stages = kSmemLimit / resident / (bytes * threads);
+  s.stages = room / resident / (bytes * threads);
   if (s.stages > kMaxStages) s.stages = kMaxStages;
   const int64_t each = (rows + (int64_t)s.blocks * s.ty - 1) / ((int64_t)s.blocks * s.ty);
   if (s.stages > each) s.stages = (int)each;
@@ -434,37 +516,39 @@ bool all_wide(std::initializer_list<std::pair<const void*, int64_t>> matrices) {
     if (m.first) bits |= reinterpret_cast<uintptr_t>(m.first) | (uintptr_t)m.second;
   return (bits & 15) == 0;
 }
+bool rows_wide(const NormParams& p) { return all_wide({{p.x, p.ldx}, {p.y, p.ldy}, {p.ldg ? p.gate : nullptr, p.ldg}}); }
 
-template <typename T, int BLOCK, int NU, bool WIDE>
+template <typename T, bool FOUR, int NU, bool WIDE, int KIND>
 cudaError_t launch_forward(const NormParams& p0, cudaStream_t st) {
   NormParams p = p0;
-  const int units = BLOCK ? (int)p.tiles * 4 * (BLOCK / 16) : (p.cols + kUnit - 1) / kUnit;
-  const bool matrix = p.ldg != 0;
-  p.chunks = kUnit * (int)sizeof(T) / 16 + (WIDE ? 0 : 1);
-  const int two = (1 + (p.y ? 1 : 0)) * NU * p.chunks * 16;
-  Shape s = shape_of(p.rows, units, NU, two + (matrix ? NU * p.chunks * 16 : 0));
-  p.gate_ahead = matrix;
-  if (s.stages == 0) {        // three fp32 rows of more than 14000 elements
-    s = shape_of(p.rows, units, NU, two);
-    p.gate_ahead = 0;
-  }
+  constexpr bool SHARED = NU == 2 && sizeof(T) == 2;
+  const int units = FOUR ? (int)p.tiles * 4 * (p.block / 16) : (p.cols + kUnit - 1) / kUnit;
+  p.chunks = kUnit * (int)sizeof(T) / 16 + (WIDE || rows_wide(p) ? 0 : 1);
+  const int two = (KIND ? 2 : 1) * NU * p.chunks * 16, three = two + (KIND == 2 ? NU * p.chunks * 16 : 0);
+  const int tx = ((units + NU - 1) / NU + 31) / 32 * 32, vectors = SHARED ? tx * NU * kUnit * 4 * (KIND ? 2 : 1) : 0;
+  // A gate matrix is not copied ahead where there is no room for it (rows of more than some 14000 elements).
+  p.gate_ahead = KIND == 2 && vectors + three * tx <= kSmemLimit;
+  const Shape s = shape_of(p.rows, units, NU, p.gate_ahead ? three : two, NU == 2 ? many_threads<T>() : kMaxThreads, vectors);
+  if (s.stages < 1) return cudaErrorInvalidValue;
   p.stages = s.stages;
-  const auto fn = residual_norm_kernel<T, BLOCK, NU, WIDE>;
+  p.vectors_at = (int32_t)s.smem;
+  const auto fn = residual_norm_kernel<T, FOUR, NU, WIDE, KIND>;
   // (Always the same limit: calls of other sizes may be between this line and the launch.)
   const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (err != cudaSuccess) return err;
-  return launch_overlapped(fn, dim3((unsigned)s.blocks), dim3((unsigned)s.tx, (unsigned)s.ty), s.smem, 1, st, p);
+  return launch_overlapped(fn, dim3((unsigned)s.blocks), dim3((unsigned)s.tx, (unsigned)s.ty), s.smem + vectors, 1, st, p);
 }
-template <typename T, int BLOCK, bool WIDE>
+template <typename T, bool FOUR, int KIND>
 cudaError_t launch_forward(const NormParams& p, cudaStream_t st) {
-  const bool one = p.cols <= kMaxThreads * kUnit && (sizeof(T) == 4 || p.rows <= 148);
-  return one ? launch_forward<T, BLOCK, 1, WIDE>(p, st) : launch_forward<T, BLOCK, 2, WIDE>(p, st);
+  if (p.cols <= kMaxThreads * kUnit && p.rows <= 148) return launch_forward<T, FOUR, 1, false, KIND>(p, st);
+  const bool wide = rows_wide(p) && all_wide({{p.xo, p.ldo}, {p.h, p.ldh}});
+  return wide ? launch_forward<T, FOUR, 2, true, KIND>(p, st) : launch_forward<T, FOUR, 2, false, KIND>(p, st);
 }
 template <typename T>
-cudaError_t launch_forward(const NormParams& p, int block, cudaStream_t st) {
-  const bool wide = all_wide({{p.x, p.ldx}, {p.y, p.ldy}, {p.ldg ? p.gate : nullptr, p.ldg}, {p.xo, p.ldo}, {p.h, p.ldh}});
-  if (wide) return block == 0 ? launch_forward<T, 0, true>(p, st) : block == 16 ? launch_forward<T, 16, true>(p, st) : launch_forward<T, 32, true>(p, st);
-  return block == 0 ? launch_forward<T, 0, false>(p, st) : block == 16 ? launch_forward<T, 16, false>(p, st) : launch_forward<T, 32, false>(p, st);
+cudaError_t launch_forward(const NormParams& p, cudaStream_t st) {
+  const int kind = !p.y ? 0 : p.ldg ? 2 : 1;
+  if (p.block) return kind == 0 ? launch_forward<T, true, 0>(p, st) : kind == 1 ? launch_forward<T, true, 1>(p, st) : launch_forward<T, true, 2>(p, st);
+  return kind == 0 ? launch_forward<T, false, 0>(p, st) : kind == 1 ? launch_forward<T, false, 1>(p, st) : launch_forward<T, false, 2>(p, st);
 }
 
 // ----------------------------------------------------------------- backward
@@ -524,7 +608,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
   const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * TX + tx) * 16u;
   const uint32_t per_unit = (uint32_t)p.chunks * stride;
   enum { X, DH, DX, Y, G };
-  const bool matrix = p.in[G] != nullptr, block = p.in[Y] != nullptr;
+  const bool with_matrix = p.in[G] != nullptr, with_block = p.in[Y] != nullptr, with_post = p.wp != nullptr;
   uint32_t slot_of[5], present = 0;
 #pragma unroll
   for (int m = 0; m < 5; ++m) slot_of[m] = per_unit * (p.in[m] ? present++ : 0u);
@@ -542,7 +626,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
       const int e = unit_at(0);
 #pragma unroll
       for (int m = 0; m < 5; ++m)
-        if (p.in[m]) issue_unit<T, WIDE>(slot + slot_of[m], stride, p.in[m] + row * p.ld[m] + e * E, p.cols - e);
+        if (each_row(p.in[m])) issue_unit<T, WIDE>(slot + slot_of[m], stride, row_of(p.in[m], row, p.ld[m]) + e * E, p.cols - e);
     }
     commit_copies();
   };
@@ -569,11 +653,12 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
   for (int64_t row = first; row < p.rows; row += step) {
     const uint32_t at = mine + (uint32_t)stage * per_stage;
     if constexpr (!HELD) wait_copies(p.stages - 1);
+    const bool matrix = each_row(with_matrix), block = each_row(with_block), post = each_row(with_post);
     auto get = [&](int m, int i) {
       const int e = unit_at(i), n = p.cols - e;
       Unit<T> u;
-      if (!p.in[m]) u.clear();
-      else if constexpr (HELD) u = rowvec::load_unit<T, rowvec::kKeep>(reinterpret_cast<const T*>(p.in[m] + row * p.ld[m]) + e, n);
+      if (each_row(!p.in[m])) u.clear();
+      else if constexpr (HELD) u = rowvec::load_unit<T, rowvec::kKeep>(reinterpret_cast<const T*>(row_of(p.in[m], row, p.ld[m])) + e, n);
       else u = take_unit<T, WIDE>(at + slot_of[m], stride, WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(p.in[m] + row * p.ld[m]) & 15u, n);
       return u;
     };
@@ -592,7 +677,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
       }
       v[0] += both(s0);
       v[2] += both(s2);
-      if (p.wp) {
+      if (post) {
         const Unit<T> y = get(Y, i), d = get(DX, i), g = get(G, i);
         F2 s1 = f2(0.f), s3 = f2(0.f), s4 = f2(0.f), s5 = f2(0.f);
 #pragma unroll
@@ -643,7 +728,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         sx += squares_wide<T>(get(X, i));
-        if (p.wp) sy += squares_wide<T>(get(Y, i));
+        if (post) sy += squares_wide<T>(get(Y, i));
       }
       group_sync();
       sx = across_warps(warp_sum(sx), sums.wide[0]);
@@ -677,7 +762,7 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         g[j].get(a, b);
         o.set2(2 * j, a, b);
       }
-      put_unit<T, WIDE>(p.dx + row * p.lddx + e * E, o, p.cols - e);
+      put_unit<T, WIDE>(row_of(p.dx, row, p.lddx) + e * E, o, p.cols - e);
       if (!block) continue;
       const Unit<T> y = get(Y, i), gate = get(G, i);
       Unit<T> og;
@@ -698,12 +783,12 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
         } else {
           cs[j] = add2(cs[j], part);
         }
-        t = p.wp ? fma2(q, t, mul2(back2, yv)) : t;
+        t = post ? fma2(q, t, mul2(back2, yv)) : t;
         t.get(a, b);
         o.set2(2 * j, a, b);
       }
-      put_unit<T, WIDE>(p.dy + row * p.lddy + e * E, o, p.cols - e);
-      if (p.dgate) put_unit<T, WIDE>(p.dgate + row * p.lddg + e * E, og, p.cols - e);
+      put_unit<T, WIDE>(row_of(p.dy, row, p.lddy) + e * E, o, p.cols - e);
+      if (each_row(p.dgate)) put_unit<T, WIDE>(row_of(p.dgate, row, p.lddg) + e * E, og, p.cols - e);
     }
     if constexpr (!HELD) issue(row + p.stages * step, at);
     if (++stage == p.stages) stage = 0;
@@ -796,6 +881,7 @@ template <typename T>
 cudaError_t launch_backward(BackParams p, const Shape& s, bool wide, cudaStream_t st) {
   const auto fn = p.cols > kMaxThreads * kUnit ? residual_norm_backward_kernel<T, true, false>
                 : wide ? residual_norm_backward_kernel<T, false, true> : residual_norm_backward_kernel<T, false, false>;
+  if (s.stages < 1 && p.cols <= kMaxThreads * kUnit) return cudaErrorInvalidValue;
   p.stages = s.stages;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (e != cudaSuccess) return e;
@@ -856,8 +942,9 @@ extern "C" int gemm_sm100a_residual_norm(const ResidualNormArgs* a, void* stream
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   PointerDeviceGuard guard(a->block ? a->values : a->h);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
-  return status_of(a->type == GEMM_TYPE_BF16 ? launch_forward<__nv_bfloat16>(p, a->block, st)
-                 : a->type == GEMM_TYPE_FP16 ? launch_forward<__half>(p, a->block, st) : launch_forward<float>(p, a->block, st));
+  p.block = a->block;
+  return status_of(a->type == GEMM_TYPE_BF16 ? launch_forward<__nv_bfloat16>(p, st)
+                 : a->type == GEMM_TYPE_FP16 ? launch_forward<__half>(p, st) : launch_forward<float>(p, st));
 }
 
 extern "C" int64_t gemm_sm100a_residual_norm_workspace(int64_t rows, int64_t cols) {
