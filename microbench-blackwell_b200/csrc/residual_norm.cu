@@ -39,68 +39,66 @@ constexpr int kMaxStages = 4;
 constexpr int kSmemLimit = 224 * 1024;     // dynamic shared memory of a block, and of an SM's blocks together
 
 // ----------------------------------------------------------------- rows in flight
-// A group of blockDim.x threads (whole warps) takes rows of its own, blockDim.y groups to a block.  Each thread copies
-// its units of the coming rows into its own slots of shared memory (cp.async, so that no barrier is needed and no
-// registers are held), several rows ahead: the bytes on their way are what keeps HBM busy while the group goes through
-// a row's sums.  The 16-byte chunks of a unit lie blockDim.x * blockDim.y slots apart (no bank conflicts).  A unit off
-// 16-byte boundaries (never with WIDE) takes one chunk more, and is shifted when it is read.
-// n: elements of the unit in the row (beyond 16: all).
+// A group of blockDim.x threads (whole warps) takes rows of its own, blockDim.y groups to a block.  A warp copies the
+// stretches of the coming rows that its lanes' units make up, 32 units each, into a place of its own in shared memory
+// (cp.async: no barrier of the block is needed and no registers are held), one or more rows ahead: the bytes on their way
+// are what keeps HBM busy while the group goes through a row's sums.  Lanes copy neighbouring 16-byte chunks (whole
+// sectors) and read those of their own unit, so a warp's lanes wait for one another before they read, and before the
+// place is copied to again.  Chunk c lies at c ^ (c / 8 mod E): lanes that read E chunks each then meet all banks.
+// A stretch off 16-byte boundaries (never with WIDE) takes one chunk more, and is shifted when it is read.  Every chunk holds
+// a byte of the row, so that no copy leaves the 16 bytes around one.
+// n: elements of the row from the stretch's first on.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void issue_unit(uint32_t slot, uint32_t stride, const uint8_t* p, int n) {
-  constexpr int B = Unit<T>::W / 4;
+__device__ __forceinline__ void issue_stretch(uint32_t place, const uint8_t* p, int n) {
+  constexpr int E = (int)sizeof(T);
+  const int lane = (int)(threadIdx.x & 31u);
   const int off = WIDE ? 0 : (int)(reinterpret_cast<uintptr_t>(p) & 15u);
-  if (n >= kUnit) {
+  const uint32_t dst = place + 16u * (uint32_t)(lane ^ ((lane >> 3) & (E - 1)));
+  const uint8_t* const src = p - off + 16 * lane;
+  if (n >= 32 * kUnit) {
 #pragma unroll
-    for (int j = 0; j < B; ++j) sm100::cp_async_16(slot + (uint32_t)j * stride, p - off + 16 * j, 16u);
-    if (!WIDE && off) sm100::cp_async_16(slot + (uint32_t)B * stride, p - off + 16 * B, 16u);
+    for (int j = 0; j < E; ++j) sm100::cp_async_16(dst + 512u * j, src + 512 * j, 16u);
+    if (!WIDE && off && lane == 0) sm100::cp_async_16(dst + 512u * E, src + 512 * E, 16u);
   } else if (n > 0) {
-    const int bytes = n * (int)sizeof(T);
+    const int chunks = (off + n * E + 15) / 16;
 #pragma unroll
-    for (int j = 0; j <= B; ++j) {
-      if (j == B && off == 0) break;               // (there may be no slot for it)
-      const bool any = 16 * j - off < bytes;       // (a copy of no bytes zeroes its chunk; its address is in range all the same)
-      sm100::cp_async_16(slot + (uint32_t)j * stride, any ? p - off + 16 * j : p - off, any ? 16u : 0u);
-    }
+    for (int j = 0; j <= E; ++j)
+      if (32 * j + lane < chunks) sm100::cp_async_16(dst + 512u * j, src + 512 * j, 16u);
   }
 }
+// A lane's unit; off: the stretch's offset from a 16-byte boundary, n: elements of the row from the unit's first on.
 template <typename T, bool WIDE>
-__device__ __forceinline__ Unit<T> take_unit(uint32_t slot, uint32_t stride, uint32_t off, int n) {
-  constexpr int W = Unit<T>::W, B = W / 4;
+__device__ __forceinline__ Unit<T> take_unit(uint32_t place, uint32_t off, int n) {
+  constexpr int W = Unit<T>::W, E = (int)sizeof(T);
   Unit<T> u;
   if (n <= 0) {
     u.clear();
     return u;
   }
+  const int first = E * (int)(threadIdx.x & 31u);
   auto chunk = [&](int j, uint32_t* w) {
-    const uint4 v = sm100::ld_shared_v4(slot + (uint32_t)j * stride);
+    const int c = first + j;
+    const uint4 v = sm100::ld_shared_v4(place + 16u * (uint32_t)(c ^ ((c >> 3) & (E - 1))));
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   };
   if (WIDE || off == 0) {
 #pragma unroll
-    for (int j = 0; j < B; ++j) chunk(j, u.w + 4 * j);
+    for (int j = 0; j < E; ++j) chunk(j, u.w + 4 * j);
   } else {
     uint32_t w[W + 4];
 #pragma unroll
-    for (int j = 0; j <= B; ++j) chunk(j, w + 4 * j);
+    for (int j = 0; j <= E; ++j) chunk(j, w + 4 * j);
     rowvec::shift_words<W>(w, off);
 #pragma unroll
     for (int j = 0; j < W; ++j) u.w[j] = w[j];
   }
-  if (n < kUnit) rowvec::clip(u, n * (int)sizeof(T));
+  if (n < kUnit) rowvec::clip(u, n * E);
   return u;
 }
 template <typename T, bool WIDE>
 __device__ __forceinline__ void put_unit(uint8_t* p, const Unit<T>& u, int n) {
-  if constexpr (WIDE) {
-    if (n >= kUnit) {
-#pragma unroll
-      for (int j = 0; j < Unit<T>::W / 4; ++j) *reinterpret_cast<uint4*>(p + 16 * j) = make_uint4(u.w[4 * j], u.w[4 * j + 1], u.w[4 * j + 2], u.w[4 * j + 3]);
-    } else if (n > 0) {
-      rowvec::store_elements<T>(reinterpret_cast<T*>(p), u, 0, n);
-    }
-  } else {
-    rowvec::store_unit<T>(reinterpret_cast<T*>(p), u, n);
-  }
+  if constexpr (WIDE) rowvec::store_aligned<T>(p, u, n);
+  else rowvec::store_unit<T>(reinterpret_cast<T*>(p), u, n);
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // Until all but the newest n groups of this thread's copies have landed.
@@ -213,7 +211,8 @@ struct NormParams {
   uint8_t* scales;
   float* row_scale;
   int64_t tiles;
-  int32_t stages, chunks;      // rows ahead; chunks of a unit (one more where a matrix has rows off 16-byte boundaries)
+  int32_t stages;              // rows ahead
+  uint32_t place;              // bytes of a stretch in shared memory
   int32_t gate_ahead;          // a gate matrix is copied ahead too
   int32_t param32;             // the vectors are fp32 (else of T)
   int32_t vectors_at;          // many rows: byte of the vectors in shared memory
@@ -252,10 +251,10 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
   constexpr int E = (int)sizeof(T);
   constexpr bool KEEP = NU == 1, SHARED = NU == 2 && E == 2, BLOCK = KIND > 0, MATRIX = KIND == 2;
   const int tx = threadIdx.x, TX = blockDim.x;
-  const uint32_t stride = (uint32_t)(TX * (int)blockDim.y) * 16u;
-  const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * TX + tx) * 16u;
-  const uint32_t per_unit = (uint32_t)p.chunks * stride;
-  const uint32_t per_stage = (uint32_t)(((BLOCK ? 2 : 1) + (MATRIX ? p.gate_ahead : 0)) * NU) * per_unit;
+  // Places of this warp: stage by stage, then unit by unit, then matrix by matrix.
+  const uint32_t per_unit = p.place, per_stage = (uint32_t)(((BLOCK ? 2 : 1) + (MATRIX ? p.gate_ahead : 0)) * NU) * per_unit;
+  const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * (TX >> 5) + (tx >> 5)) * (uint32_t)p.stages * per_stage;
+  const int lane_e = (tx & 31) * kUnit;       // elements from a warp's first unit to this lane's
   const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
   int e[NU], n[NU];
 #pragma unroll
@@ -271,14 +270,14 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
       const uint8_t* const ry = row_of(p.y, row, p.ldy);
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        issue_unit<T, WIDE>(slot, stride, rx + e[i] * E, n[i]);
+        issue_stretch<T, WIDE>(slot, rx + (e[i] - lane_e) * E, n[i] + lane_e);
         slot += per_unit;
         if (BLOCK) {
-          issue_unit<T, WIDE>(slot, stride, ry + e[i] * E, n[i]);
+          issue_stretch<T, WIDE>(slot, ry + (e[i] - lane_e) * E, n[i] + lane_e);
           slot += per_unit;
         }
         if (MATRIX && p.gate_ahead) {
-          issue_unit<T, WIDE>(slot, stride, row_of(p.gate, row, p.ldg) + e[i] * E, n[i]);
+          issue_stretch<T, WIDE>(slot, row_of(p.gate, row, p.ldg) + (e[i] - lane_e) * E, n[i] + lane_e);
           slot += per_unit;
         }
       }
@@ -365,25 +364,27 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
     const uint8_t* const rg = p.gate + row * p.ldg;
     auto low = [](const uint8_t* q) { return (uint32_t)reinterpret_cast<uintptr_t>(q) & 15u; };      // (units are multiples of 16 bytes)
     wait_copies(p.stages - 1);
+    __syncwarp();
     Unit<T> x[NU], y[NU], gate[NU];
     {
       uint32_t slot = at;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        x[i] = take_unit<T, WIDE>(slot, stride, low(rx), n[i]);
+        x[i] = take_unit<T, WIDE>(slot, low(rx), n[i]);
         slot += per_unit;
         if (BLOCK) {
-          y[i] = take_unit<T, WIDE>(slot, stride, low(ry), n[i]);
+          y[i] = take_unit<T, WIDE>(slot, low(ry), n[i]);
           slot += per_unit;
         }
         if (MATRIX && p.gate_ahead) {
-          gate[i] = take_unit<T, WIDE>(slot, stride, low(rg), n[i]);
+          gate[i] = take_unit<T, WIDE>(slot, low(rg), n[i]);
           slot += per_unit;
         } else if (MATRIX) {
           gate[i] = rowvec::load_unit<T>(reinterpret_cast<const T*>(rg) + e[i], n[i]);
         }
       }
     }
+    __syncwarp();
     issue(row + p.stages * step, at);
     if (++stage == p.stages) stage = 0;
     if constexpr (BLOCK) {
@@ -479,36 +480,39 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
   }
 }
 
-// Threads of a row, rows of a block and blocks, all resident at once; `bytes`: shared memory of a thread and row.
+// Threads of a row, rows of a block and blocks, all resident at once.
 struct Shape {
   int tx, ty, blocks, stages;
   size_t smem;
 };
-// `most_threads` of a block; `fixed`: shared memory of a block beside the rows'.
+// `bytes`: shared memory of a warp and row; `most_threads` of a block; `fixed`: shared memory of a block beside the rows'.
 Shape shape_of(int64_t rows, int units, int per_thread, int bytes, int most_threads = kMaxThreads, int fixed = 0) {
   Shape s;
   s.tx = ((units + per_thread - 1) / per_thread + 31) / 32 * 32;
+  const int warps = s.tx / 32;
   const int room = kSmemLimit - fixed;
   int64_t ty = most_threads / s.tx;
   const int64_t spread = (rows + 147) / 148;       // rows over all SMs before more of them in a block
   if (ty > spread) ty = spread;
-  if (ty > room / (bytes * s.tx)) ty = room / (bytes * s.tx);
+  if (ty > room / (bytes * warps)) ty = room / (bytes * warps);
   if (ty > (s.tx == 32 ? 32 : 15)) ty = s.tx == 32 ? 32 : 15;       // named barriers
   s.ty = (int)(ty < 1 ? 1 : ty);
-  const int threads = s.tx * s.ty;
+  const int threads = s.tx * s.ty, row_bytes = bytes * warps * s.ty;
   int resident = fixed ? 1 : most_threads / threads;
-  if (resident > room / (bytes * threads)) resident = room / (bytes * threads);      // at least one row ahead
+  if (resident > room / row_bytes) resident = room / row_bytes;      // at least one row ahead
   if (resident < 1) resident = 1;
   const int64_t blocks = (rows + s.ty - 1) / s.ty, most = 148 * resident;
   s.blocks = (int)(blocks < most ? blocks : most);
-  s.stages = room / resident / (bytes * threads);
+  s.stages = room / resident / row_bytes;
   if (s.stages > kMaxStages) s.stages = kMaxStages;
   const int64_t each = (rows + (int64_t)s.blocks * s.ty - 1) / ((int64_t)s.blocks * s.ty);
   if (s.stages > each) s.stages = (int)each;
-  s.smem = (size_t)s.stages * bytes * threads;
+  s.smem = (size_t)s.stages * row_bytes;
   return s;
 }
 
+// A stretch in shared memory.
+uint32_t place_bytes(int e, bool wide) { return (uint32_t)(32 * e + (wide ? 0 : 1)) * 16u; }
 // Whether the rows of all matrices start on 16-byte boundaries (strides in bytes; an absent one does not count).
 bool all_wide(std::initializer_list<std::pair<const void*, int64_t>> matrices) {
   uintptr_t bits = 0;
@@ -523,11 +527,11 @@ cudaError_t launch_forward(const NormParams& p0, cudaStream_t st) {
   NormParams p = p0;
   constexpr bool SHARED = NU == 2 && sizeof(T) == 2;
   const int units = FOUR ? (int)p.tiles * 4 * (p.block / 16) : (p.cols + kUnit - 1) / kUnit;
-  p.chunks = kUnit * (int)sizeof(T) / 16 + (WIDE || rows_wide(p) ? 0 : 1);
-  const int two = (KIND ? 2 : 1) * NU * p.chunks * 16, three = two + (KIND == 2 ? NU * p.chunks * 16 : 0);
+  p.place = place_bytes((int)sizeof(T), WIDE || rows_wide(p));
+  const int two = (KIND ? 2 : 1) * NU * (int)p.place, three = two + (KIND == 2 ? NU * (int)p.place : 0);
   const int tx = ((units + NU - 1) / NU + 31) / 32 * 32, vectors = SHARED ? tx * NU * kUnit * 4 * (KIND ? 2 : 1) : 0;
   // A gate matrix is not copied ahead where there is no room for it (rows of more than some 14000 elements).
-  p.gate_ahead = KIND == 2 && vectors + three * tx <= kSmemLimit;
+  p.gate_ahead = KIND == 2 && vectors + three * (tx / 32) <= kSmemLimit;
   const Shape s = shape_of(p.rows, units, NU, p.gate_ahead ? three : two, NU == 2 ? many_threads<T>() : kMaxThreads, vectors);
   if (s.stages < 1) return cudaErrorInvalidValue;
   p.stages = s.stages;
@@ -565,7 +569,8 @@ struct BackParams {
   int32_t cols;
   float scale;
   double eps, inv_n;
-  int32_t stages, chunks;
+  int32_t stages;
+  uint32_t place;
   int32_t param32;
 };
 
@@ -604,15 +609,14 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
   constexpr int NU = HELD ? 2 : 1, E = (int)sizeof(T);
   const int tx = threadIdx.x, TX = blockDim.x;
   const int width = (p.cols + kUnit - 1) / kUnit * kUnit;
-  const uint32_t stride = (uint32_t)(TX * (int)blockDim.y) * 16u;
-  const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * TX + tx) * 16u;
-  const uint32_t per_unit = (uint32_t)p.chunks * stride;
+  const uint32_t per_unit = p.place;
   enum { X, DH, DX, Y, G };
   const bool with_matrix = p.in[G] != nullptr, with_block = p.in[Y] != nullptr, with_post = p.wp != nullptr;
   uint32_t slot_of[5], present = 0;
 #pragma unroll
   for (int m = 0; m < 5; ++m) slot_of[m] = per_unit * (p.in[m] ? present++ : 0u);
   const uint32_t per_stage = present * per_unit;
+  const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * (TX >> 5) + (tx >> 5)) * (uint32_t)p.stages * per_stage;
   auto unit_at = [&](int i) { return (i * TX + tx) * kUnit; };
   if constexpr (HELD) {
     for (int i = tx; i < 2 * width; i += TX) held[i] = 0.f;
@@ -623,10 +627,10 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
   const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
   auto issue = [&](int64_t row, uint32_t slot) {
     if (row < p.rows) {
-      const int e = unit_at(0);
+      const int e = unit_at(0) - (tx & 31) * kUnit;
 #pragma unroll
       for (int m = 0; m < 5; ++m)
-        if (each_row(p.in[m])) issue_unit<T, WIDE>(slot + slot_of[m], stride, row_of(p.in[m], row, p.ld[m]) + e * E, p.cols - e);
+        if (each_row(p.in[m])) issue_stretch<T, WIDE>(slot + slot_of[m], row_of(p.in[m], row, p.ld[m]) + e * E, p.cols - e);
     }
     commit_copies();
   };
@@ -652,14 +656,17 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
   int stage = 0;
   for (int64_t row = first; row < p.rows; row += step) {
     const uint32_t at = mine + (uint32_t)stage * per_stage;
-    if constexpr (!HELD) wait_copies(p.stages - 1);
+    if constexpr (!HELD) {
+      wait_copies(p.stages - 1);
+      __syncwarp();
+    }
     const bool matrix = each_row(with_matrix), block = each_row(with_block), post = each_row(with_post);
     auto get = [&](int m, int i) {
       const int e = unit_at(i), n = p.cols - e;
       Unit<T> u;
       if (each_row(!p.in[m])) u.clear();
       else if constexpr (HELD) u = rowvec::load_unit<T, rowvec::kKeep>(reinterpret_cast<const T*>(row_of(p.in[m], row, p.ld[m])) + e, n);
-      else u = take_unit<T, WIDE>(at + slot_of[m], stride, WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(p.in[m] + row * p.ld[m]) & 15u, n);
+      else u = take_unit<T, WIDE>(at + slot_of[m], WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(p.in[m] + row * p.ld[m]) & 15u, n);
       return u;
     };
   // ---- row sums
@@ -790,7 +797,10 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
       put_unit<T, WIDE>(row_of(p.dy, row, p.lddy) + e * E, o, p.cols - e);
       if (each_row(p.dgate)) put_unit<T, WIDE>(row_of(p.dgate, row, p.lddg) + e * E, og, p.cols - e);
     }
-    if constexpr (!HELD) issue(row + p.stages * step, at);
+    if constexpr (!HELD) {
+      __syncwarp();
+      issue(row + p.stages * step, at);
+    }
     if (++stage == p.stages) stage = 0;
   }
   // ---- this block's column sums
@@ -861,8 +871,8 @@ __global__ void __launch_bounds__(256) residual_norm_columns_kernel(const __grid
   }
 }
 
-// `chunks`: those of a thread's units in all matrices.
-Shape back_shape(int64_t rows, int64_t cols, int chunks) {
+// `bytes`: a warp's stretches of all matrices.
+Shape back_shape(int64_t rows, int64_t cols, int bytes) {
   const int units = (int)((cols + kUnit - 1) / kUnit);
   if (units > kMaxThreads) {
     Shape s;
@@ -871,7 +881,7 @@ Shape back_shape(int64_t rows, int64_t cols, int chunks) {
     s.smem = (size_t)units * kUnit * 8;
     return s;
   }
-  Shape s = shape_of(rows, units, 1, chunks * 16);
+  Shape s = shape_of(rows, units, 1, bytes);
   const size_t sums = (size_t)units * kUnit * 8;
   if (s.smem < sums) s.smem = sums;
   return s;
@@ -1001,8 +1011,8 @@ extern "C" int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs
   }
   for (const Mat& m : outs) wide &= !m.p || rows_16b(m.p, m.ld, e);
   wide &= in_wide;
-  const int chunks = kUnit * e / 16 + (wide ? 0 : 1);
-  const Shape s = back_shape(a->rows, a->cols, matrices * chunks);
+  const uint32_t place = place_bytes(e, wide);
+  const Shape s = back_shape(a->rows, a->cols, matrices * (int)place);
   if (a->workspace_bytes < (int64_t)s.blocks * 2 * a->cols * 4) return GEMM_ERR_BAD_ARGS;
   BackParams p;
   memset(&p, 0, sizeof(p));
@@ -1016,7 +1026,7 @@ extern "C" int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs
   p.parts = static_cast<float*>(a->workspace);
   p.rows = a->rows; p.cols = (int32_t)a->cols; p.scale = a->scale; p.eps = a->eps; p.inv_n = 1.0 / (double)a->cols;
   p.param32 = a->param_type == GEMM_TYPE_FP32;
-  p.chunks = chunks;
+  p.place = place;
   PointerDeviceGuard guard(a->dx);
   if (!guard.ok) return GEMM_ERR_LAUNCH;
   cudaError_t err = a->type == GEMM_TYPE_BF16 ? launch_backward<__nv_bfloat16>(p, s, wide, st)

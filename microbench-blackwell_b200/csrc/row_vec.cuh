@@ -76,6 +76,22 @@ __device__ __forceinline__ void clip(Unit<T>& u, int bytes) {
   }
 }
 
+// 32 bytes at once: a thread's 16-bit unit, or half of an fp32 one.  (Lanes 32 bytes apart that move 16 at a time ask
+// for every sector twice: 16384 x 8192 bf16 to 4 bits @q1@ us that way, @q2@ with this.)
+template <bool STREAM>
+__device__ __forceinline__ void load32(uint32_t* w, const uint8_t* p) {
+  if constexpr (STREAM)
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
+  else
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void store32(uint8_t* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
 enum Cache { kStream, kKeep };   // read once, or again by other rows
 
 template <Cache C>
@@ -96,6 +112,11 @@ __device__ __forceinline__ Unit<T> load_unit(const T* ptr, int n) {
   const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
   const int bytes = min(n, kUnit) * (int)sizeof(T);
   Unit<T> u;
+  if (n >= kUnit && ((uint32_t)reinterpret_cast<uintptr_t>(p) & 31u) == 0) {
+#pragma unroll
+    for (int j = 0; j < W / 8; ++j) load32<C == kStream>(u.w + 8 * j, p + 32 * j);
+    return u;
+  }
   if (off == 0) {
 #pragma unroll
     for (int j = 0; j < B; ++j) {
@@ -130,6 +151,23 @@ __device__ __forceinline__ void store_elements(T* p, const Unit<T>& u, int a, in
     }
 }
 
+// Elements [0, n) of a unit at a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void store_aligned(uint8_t* p, const Unit<T>& u, int n) {
+  constexpr int W = Unit<T>::W;
+  if (n >= kUnit) {
+    if (((uint32_t)reinterpret_cast<uintptr_t>(p) & 31u) == 0) {
+#pragma unroll
+      for (int j = 0; j < W / 8; ++j) store32(p + 32 * j, u.w + 8 * j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < W / 4; ++j) *reinterpret_cast<uint4*>(p + 16 * j) = make_uint4(u.w[4 * j], u.w[4 * j + 1], u.w[4 * j + 2], u.w[4 * j + 3]);
+    }
+  } else if (n > 0) {
+    store_elements<T>(reinterpret_cast<T*>(p), u, 0, n);
+  }
+}
+
 // Elements [0, n) of the units of a warp, called by all of its lanes; lane l + 1's unit follows lane l's in the
 // row (in other lanes' rows nothing is assumed).  Off 16-byte boundaries a lane also writes the end of the
 // unit before it, so that whole blocks are written; only at both ends of the warp's stretch elements are.
@@ -139,12 +177,7 @@ __device__ __forceinline__ void store_unit(T* ptr, const Unit<T>& u, int n) {
   uint8_t* const p = reinterpret_cast<uint8_t*>(ptr);
   const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
   if (off == 0) {      // uniform over the warp
-    if (n >= kUnit) {
-#pragma unroll
-      for (int j = 0; j < B; ++j) *reinterpret_cast<uint4*>(p + 16 * j) = make_uint4(u.w[4 * j], u.w[4 * j + 1], u.w[4 * j + 2], u.w[4 * j + 3]);
-    } else if (n > 0) {
-      store_elements<T>(ptr, u, 0, n);
-    }
+    store_aligned<T>(p, u, n);
     return;
   }
   uint32_t w[W + 4];
