@@ -600,7 +600,7 @@ int gemm_sm100a_residual_norm(const ResidualNormArgs* args, void* stream);
  *   dy   = the gradient of (gate * scale) * z towards y for g
  * of `type`, and the fp32 sums over rows dweight, dpost_weight and, for a gate vector, dgate; a gate
  * matrix has dgate of `type` (lddg).  y NULL: no dy, dpost_weight, dgate.  dweight, dpost_weight and dgate may be NULL
- * (not wanted).  Sums are taken in an order that depends on the sizes alone.  rows = 0 sets the fp32 sums to 0.
+ * (not wanted).  The same call takes its sums in the same order.  rows = 0 sets the fp32 sums to 0.
  * workspace: gemm_sm100a_residual_norm_workspace(rows, cols) bytes, 16-byte aligned, of this call alone until it has
  * run.  Outputs overlap nothing.
  */

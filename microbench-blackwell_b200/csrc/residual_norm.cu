@@ -236,6 +236,32 @@ __device__ __forceinline__ void load_params(const void* v, int param32, int e, i
   }
 }
 
+// Vectors that all groups of a block read, in shared memory: four elements of a unit to a slot, the slots of one kind side by
+// side for all units (no bank conflicts).
+struct SharedVectors {
+  uint32_t base, per_chunk;
+  __device__ __forceinline__ uint32_t at(int which, int unit) const { return base + (uint32_t)(which * 4) * per_chunk + (uint32_t)unit * 16u; }
+  __device__ __forceinline__ void put(int which, int unit, const F2 (&v)[kUnit / 2]) const {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float f[4];
+      v[2 * c].get(f[0], f[1]);
+      v[2 * c + 1].get(f[2], f[3]);
+      sm100::st_shared_v4(at(which, unit) + (uint32_t)c * per_chunk, __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+  }
+  // Pairs 2 c and 2 c + 1 of a unit.
+  __device__ __forceinline__ void get(int which, int unit, int c, F2& a, F2& b) const {
+    const uint4 u = sm100::ld_shared_v4(at(which, unit) + (uint32_t)c * per_chunk);
+    a = F2(__uint_as_float(u.x), __uint_as_float(u.y));
+    b = F2(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  __device__ __forceinline__ void get(int which, int unit, F2 (&v)[kUnit / 2]) const {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) get(which, unit, c, v[2 * c], v[2 * c + 1]);
+  }
+};
+
 // NU units to a thread, blockDim.x units apart.
 //  Few rows (NU 1): the vectors stay in registers.
 //  Many rows (NU 2, which halves what the statistics cost per element): the vectors lie in shared memory as w and wp gate scale,
@@ -295,24 +321,7 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
 #pragma unroll
     for (int j = 0; j < kUnit / 2; ++j) vk[j] = mul2(vk[j], mul2(g[j], f2(p.scale)));
   };
-  // Shared vectors: four elements of a unit to a slot, slots of one kind side by side (no bank conflicts).
-  const uint32_t vectors = sm100::smem_u32(slots) + (uint32_t)p.vectors_at, per_chunk = (uint32_t)(NU * TX) * 16u;
-  auto slot_at = [&](int which, int i) { return vectors + (uint32_t)(which * 4) * per_chunk + (uint32_t)(i * TX + tx) * 16u; };
-  auto keep = [&](int which, int i, const F2 (&v)[kUnit / 2]) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float f[4];
-      v[2 * c].get(f[0], f[1]);
-      v[2 * c + 1].get(f[2], f[3]);
-      sm100::st_shared_v4(slot_at(which, i) + (uint32_t)c * per_chunk, __float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-    }
-  };
-  // Pairs 2 c and 2 c + 1 of a unit's vector.
-  auto kept = [&](int which, int i, int c, F2& a, F2& b) {
-    const uint4 u = sm100::ld_shared_v4(slot_at(which, i) + (uint32_t)c * per_chunk);
-    a = F2(__uint_as_float(u.x), __uint_as_float(u.y));
-    b = F2(__uint_as_float(u.z), __uint_as_float(u.w));
-  };
+  const SharedVectors vectors = {sm100::smem_u32(slots) + (uint32_t)p.vectors_at, (uint32_t)(NU * TX) * 16u};
   if constexpr (KEEP) {
     load_w(0);
     if (BLOCK) load_k(0);
@@ -321,10 +330,10 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
     for (int i = 0; i < NU; ++i) {
       if (((int)threadIdx.y - i) % (int)blockDim.y == 0 || blockDim.y == 1) {
         load_w(i);
-        keep(0, i, vw);
+        vectors.put(0, i * TX + tx, vw);
         if (BLOCK) {
           load_k(i);
-          keep(1, i, vk);
+          vectors.put(1, i * TX + tx, vk);
         }
       }
     }
@@ -398,7 +407,7 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           F2 k[2] = {vk[2 * c], vk[2 * c + 1]};
-          if (SHARED) kept(1, i, c, k[0], k[1]);
+          if (SHARED) vectors.get(1, i * TX + tx, c, k[0], k[1]);
 #pragma unroll
           for (int l = 0; l < 2; ++l) {
             const int j = 2 * c + l;
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         F2 w[2] = {vw[2 * c], vw[2 * c + 1]};
-        if (SHARED) kept(0, i, c, w[0], w[1]);
+        if (SHARED) vectors.get(0, i * TX + tx, c, w[0], w[1]);
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
           const int j = 2 * c + l;
@@ -572,6 +581,7 @@ struct BackParams {
   int32_t stages;
   uint32_t place;
   int32_t param32;
+  int32_t vectors_at;
 };
 
 // Row sums: 0 x^2, 1 y^2, 2 dn x, 3 P dx', 4 P dn, 5 P x.
@@ -597,25 +607,24 @@ __device__ __forceinline__ float warp_sums(float (&v)[8]) {
   return s + __shfl_xor_sync(0xFFFFFFFFu, s, 1);
 }
 
-// One unit to a thread and the rows in flight in shared memory, or (HELD, rows of more than 8192 elements) two units, rows read
-// twice from global memory (the second time from the caches) and the column sums in shared memory.
-//  The column sums are two: of dh x r, and of g k y q, in which a vector's k is left out: dpost and a
-// vector's dgate are that sum times what their columns share.
-template <typename T, bool HELD, bool WIDE>
-__global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(const __grid_constant__ BackParams p) {
+// As in the forward kernel: NU units to a thread, the vectors in registers (NU 1) or shared memory (NU 2), the coming row on its
+// way while other groups are at work.  A row stays in shared memory for both of its passes.
+//  HELD (rows of more than 8192 elements): two units, rows read twice from global memory (the second time from the
+// caches) and the column sums in shared memory.
+//  The column sums are two: of dh x r, and of g y q (times a gate matrix' k): dpost and a vector's dgate are the second
+// times what their columns share.
+//  KIND 0: no y; 1: y; 2: y and its norm; 3, 4: 1, 2 with a gate matrix.
+template <typename T, int NU, bool HELD, bool WIDE, int KIND>
+__global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(const __grid_constant__ BackParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ BackSums sums;
   float* const held = reinterpret_cast<float*>(slots);       // [2][cols rounded up to units]
-  constexpr int NU = HELD ? 2 : 1, E = (int)sizeof(T);
+  constexpr int E = (int)sizeof(T);
+  constexpr bool BLOCK = KIND > 0, POST = KIND == 2 || KIND == 4, MATRIX = KIND > 2, SHARED = NU == 2 && !HELD;
+  enum { X, DH, DX, Y, G };
   const int tx = threadIdx.x, TX = blockDim.x;
   const int width = (p.cols + kUnit - 1) / kUnit * kUnit;
-  const uint32_t per_unit = p.place;
-  enum { X, DH, DX, Y, G };
-  const bool with_matrix = p.in[G] != nullptr, with_block = p.in[Y] != nullptr, with_post = p.wp != nullptr;
-  uint32_t slot_of[5], present = 0;
-#pragma unroll
-  for (int m = 0; m < 5; ++m) slot_of[m] = per_unit * (p.in[m] ? present++ : 0u);
-  const uint32_t per_stage = present * per_unit;
+  const uint32_t per_stage = (uint32_t)((BLOCK ? 4 : 3) + (MATRIX ? 1 : 0)) * NU * p.place;
   const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * (TX >> 5) + (tx >> 5)) * (uint32_t)p.stages * per_stage;
   auto unit_at = [&](int i) { return (i * TX + tx) * kUnit; };
   if constexpr (HELD) {
@@ -627,10 +636,17 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
   const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
   auto issue = [&](int64_t row, uint32_t slot) {
     if (row < p.rows) {
-      const int e = unit_at(0) - (tx & 31) * kUnit;
 #pragma unroll
-      for (int m = 0; m < 5; ++m)
-        if (each_row(p.in[m])) issue_stretch<T, WIDE>(slot + slot_of[m], row_of(p.in[m], row, p.ld[m]) + e * E, p.cols - e);
+      for (int m = 0; m < 5; ++m) {
+        if ((m == Y && !BLOCK) || (m == G && !MATRIX)) continue;
+        const uint8_t* const r = row_of(p.in[m], row, p.ld[m]);
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+          const int e = unit_at(i) - (tx & 31) * kUnit;
+          if (m != DX || each_row(p.in[DX])) issue_stretch<T, WIDE>(slot, r + e * E, p.cols - e);
+          slot += p.place;
+        }
+      }
     }
     commit_copies();
   };
@@ -638,7 +654,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
     for (int s = 0; s < p.stages; ++s) issue(first + s * step, mine + (uint32_t)s * per_stage);
 
   F2 vw[kUnit / 2], vk[kUnit / 2];       // w, and k wp (wp scale with a gate matrix)
-  auto load_vectors = [&](int e) {
+  auto load_vectors = [&](int i) {
+    const int e = unit_at(i);
     F2 k[kUnit / 2];
     load_params<T>(p.w, p.param32, e, p.cols - e, vw);
     load_params<T>(p.wp, p.param32, e, p.cols - e, vk);
@@ -646,10 +663,25 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
 #pragma unroll
     for (int j = 0; j < kUnit / 2; ++j) vk[j] = mul2(vk[j], mul2(k[j], f2(p.scale)));
   };
-  F2 cw[kUnit / 2], cs[kUnit / 2];
+  const SharedVectors vectors = {sm100::smem_u32(slots) + (uint32_t)p.vectors_at, (uint32_t)(NU * TX) * 16u};
+  if constexpr (SHARED) {
 #pragma unroll
-  for (int j = 0; j < kUnit / 2; ++j) cw[j] = cs[j] = f2(0.f);
-  if constexpr (!HELD) load_vectors(unit_at(0));
+    for (int i = 0; i < NU; ++i) {
+      if (((int)threadIdx.y - i) % (int)blockDim.y == 0 || blockDim.y == 1) {
+        load_vectors(i);
+        vectors.put(0, i * TX + tx, vw);
+        vectors.put(1, i * TX + tx, vk);
+      }
+    }
+    __syncthreads();
+  } else if constexpr (!HELD) {
+    load_vectors(0);
+  }
+  F2 cw[NU][kUnit / 2], cs[NU][kUnit / 2];
+#pragma unroll
+  for (int i = 0; i < NU; ++i)
+#pragma unroll
+    for (int j = 0; j < kUnit / 2; ++j) cw[i][j] = cs[i][j] = f2(0.f);
   const float inv_n = (float)p.inv_n;
   const int warps = TX >> 5, first_warp = (int)threadIdx.y * warps, lane = tx & 31;
 
@@ -660,48 +692,54 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
       wait_copies(p.stages - 1);
       __syncwarp();
     }
-    const bool matrix = each_row(with_matrix), block = each_row(with_block), post = each_row(with_post);
     auto get = [&](int m, int i) {
       const int e = unit_at(i), n = p.cols - e;
       Unit<T> u;
-      if (each_row(!p.in[m])) u.clear();
+      if (m == DX && each_row(!p.in[DX])) u.clear();
       else if constexpr (HELD) u = rowvec::load_unit<T, rowvec::kKeep>(reinterpret_cast<const T*>(row_of(p.in[m], row, p.ld[m])) + e, n);
-      else u = take_unit<T, WIDE>(at + slot_of[m], WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(p.in[m] + row * p.ld[m]) & 15u, n);
+      else u = take_unit<T, WIDE>(at + (uint32_t)(m * NU + i) * p.place, WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(p.in[m] + row * p.ld[m]) & 15u, n);
       return u;
     };
-  // ---- row sums
+    // ---- row sums
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      if constexpr (HELD) load_vectors(unit_at(i));
+      if constexpr (HELD) load_vectors(i);
+      if constexpr (SHARED) vectors.get(0, i * TX + tx, vw);
       const Unit<T> x = get(X, i), dh = get(DH, i);
       F2 s0 = f2(0.f), s2 = f2(0.f);
+      if constexpr (!POST) {
 #pragma unroll
-      for (int j = 0; j < kUnit / 2; ++j) {
-        const F2 xv = pair(x, j);
-        s0 = fma2(xv, xv, s0);
-        s2 = fma2(mul2(pair(dh, j), vw[j]), xv, s2);
-      }
-      v[0] += both(s0);
-      v[2] += both(s2);
-      if (post) {
-        const Unit<T> y = get(Y, i), d = get(DX, i), g = get(G, i);
+        for (int j = 0; j < kUnit / 2; ++j) {
+          const F2 xv = pair(x, j);
+          s0 = fma2(xv, xv, s0);
+          s2 = fma2(mul2(pair(dh, j), vw[j]), xv, s2);
+        }
+      } else {
+        const Unit<T> y = get(Y, i), d = get(DX, i);
+        Unit<T> g;
+        if constexpr (MATRIX) g = get(G, i);
+        if constexpr (SHARED) vectors.get(1, i * TX + tx, vk);
         F2 s1 = f2(0.f), s3 = f2(0.f), s4 = f2(0.f), s5 = f2(0.f);
 #pragma unroll
         for (int j = 0; j < kUnit / 2; ++j) {
-          const F2 yv = pair(y, j);
+          const F2 xv = pair(x, j), yv = pair(y, j), dn = mul2(pair(dh, j), vw[j]);
+          s0 = fma2(xv, xv, s0);
           s1 = fma2(yv, yv, s1);
+          s2 = fma2(dn, xv, s2);
           F2 f = mul2(vk[j], yv);
-          if (matrix) f = mul2(f, pair(g, j));
+          if constexpr (MATRIX) f = mul2(f, pair(g, j));
           s3 = fma2(f, pair(d, j), s3);
-          s4 = fma2(f, mul2(pair(dh, j), vw[j]), s4);
-          s5 = fma2(f, pair(x, j), s5);
+          s4 = fma2(f, dn, s4);
+          s5 = fma2(f, xv, s5);
         }
         v[1] += both(s1);
         v[3] += both(s3);
         v[4] += both(s4);
         v[5] += both(s5);
       }
+      v[0] += both(s0);
+      v[2] += both(s2);
     }
     const float s = warp_sums(v);
     if ((lane & 3) == 0) sums.part[first_warp + (tx >> 5)][lane >> 2] = s;
@@ -720,8 +758,8 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
       const float b2 = __shfl_sync(0xFFFFFFFFu, t.x, 1), b3 = __shfl_sync(0xFFFFFFFFu, t.y, 1);
       if (lane == 0) {
         // r, q and the coefficients; or -1 for statistics that have to be taken in 64 bits, and what the coefficients need.
-        const bool again = out_of_range(t.x) || (p.wp && out_of_range(t.y));
-        const float r = again ? -1.f : inverse_root(fma((double)t.x, p.inv_n, p.eps)), q = p.wp && !again ? inverse_root(fma((double)t.y, p.inv_n, p.eps)) : 1.f;
+        const bool again = out_of_range(t.x) || (POST && out_of_range(t.y));
+        const float r = again ? -1.f : inverse_root(fma((double)t.x, p.inv_n, p.eps)), q = POST && !again ? inverse_root(fma((double)t.y, p.inv_n, p.eps)) : 1.f;
         const float back = r * r * r * (t.z * inv_n);
         sums.row[threadIdx.y] = again ? make_float4(-1.f, t.z, t.w, 0.f) : make_float4(r, q, back, q * q * q * ((t.w + r * b2 - back * b3) * inv_n));
         if (again) { sums.part[first_warp][0] = b2; sums.part[first_warp][1] = b3; }
@@ -732,70 +770,79 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
     if (c.x < 0.f) {       // of the whole group
       const float b2 = sums.part[first_warp][0], b3 = sums.part[first_warp][1];
       double sx = 0.0, sy = 0.0;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < NU; ++i) {
         sx += squares_wide<T>(get(X, i));
-        if (post) sy += squares_wide<T>(get(Y, i));
+        if constexpr (POST) sy += squares_wide<T>(get(Y, i));
       }
       group_sync();
       sx = across_warps(warp_sum(sx), sums.wide[0]);
       sy = across_warps(warp_sum(sy), sums.wide[1]);
-      const float r = inverse_root(fma(sx, p.inv_n, p.eps)), q = p.wp ? inverse_root(fma(sy, p.inv_n, p.eps)) : 1.f;
+      const float r = inverse_root(fma(sx, p.inv_n, p.eps)), q = POST ? inverse_root(fma(sy, p.inv_n, p.eps)) : 1.f;
       const float back = r * r * r * (c.y * inv_n);
       c = make_float4(r, q, back, q * q * q * ((c.z + r * b2 - back * b3) * inv_n));
     }
     // ---- gradients
+    const F2 r = f2(c.x), q = f2(c.y), back = f2(-c.z), back2 = f2(-c.w);
+    uint8_t* const out_x = row_of(p.dx, row, p.lddx);
+    uint8_t* const out_y = BLOCK ? row_of(p.dy, row, p.lddy) : nullptr;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int e = unit_at(i);
-      if constexpr (HELD) load_vectors(e);
-      const Unit<T> x = get(X, i), dh = get(DH, i), d = get(DX, i);
+      if constexpr (HELD) load_vectors(i);
+      if constexpr (SHARED) vectors.get(0, i * TX + tx, vw);
       Unit<T> o;
       F2 g[kUnit / 2];
-      const F2 r = f2(c.x), q = f2(c.y), back = f2(-c.z), back2 = f2(-c.w);
+      {
+        const Unit<T> x = get(X, i), dh = get(DH, i), d = get(DX, i);
 #pragma unroll
-      for (int j = 0; j < kUnit / 2; ++j) {
-        const F2 xv = pair(x, j), dv = pair(dh, j);
-        g[j] = fma2(r, mul2(dv, vw[j]), fma2(back, xv, pair(d, j)));
-        const F2 part = mul2(dv, mul2(xv, r));
-        if constexpr (HELD) {
+        for (int j = 0; j < kUnit / 2; ++j) {
+          const F2 xv = pair(x, j), dv = pair(dh, j);
+          g[j] = fma2(r, mul2(dv, vw[j]), fma2(back, xv, pair(d, j)));
+          if constexpr (HELD) {
+            float a, b;
+            mul2(dv, mul2(xv, r)).get(a, b);
+            if (e + 2 * j < width) { held[e + 2 * j] += a; held[e + 2 * j + 1] += b; }
+          } else {
+            cw[i][j] = fma2(dv, mul2(xv, r), cw[i][j]);
+          }
           float a, b;
-          part.get(a, b);
-          if (e + 2 * j < width) { held[e + 2 * j] += a; held[e + 2 * j + 1] += b; }
-        } else {
-          cw[j] = add2(cw[j], part);
+          g[j].get(a, b);
+          o.set2(2 * j, a, b);
         }
-        float a, b;
-        g[j].get(a, b);
-        o.set2(2 * j, a, b);
       }
-      put_unit<T, WIDE>(row_of(p.dx, row, p.lddx) + e * E, o, p.cols - e);
-      if (!block) continue;
-      const Unit<T> y = get(Y, i), gate = get(G, i);
-      Unit<T> og;
+      put_unit<T, WIDE>(out_x + e * E, o, p.cols - e);
+      if constexpr (BLOCK) {
+        if constexpr (SHARED) vectors.get(1, i * TX + tx, vk);
+        const Unit<T> y = get(Y, i);
+        Unit<T> gate, og;
+        if constexpr (MATRIX) gate = get(G, i);
 #pragma unroll
-      for (int j = 0; j < kUnit / 2; ++j) {
-        const F2 yv = pair(y, j), yn = mul2(yv, q), gv = matrix ? pair(gate, j) : f2(1.f);
-        F2 part = mul2(g[j], yn);
-        F2 t = mul2(mul2(g[j], vk[j]), gv);        // g k wp
-        float a, b;
-        if (matrix) {
-          mul2(part, vk[j]).get(a, b);             // (vk holds wp scale)
-          og.set2(2 * j, a, b);
-          part = mul2(part, mul2(gv, f2(p.scale)));
+        for (int j = 0; j < kUnit / 2; ++j) {
+          const F2 yv = pair(y, j), yn = POST ? mul2(yv, q) : yv;
+          F2 gv = g[j], t = mul2(gv, vk[j]);                     // g k wp
+          float a, b;
+          if constexpr (MATRIX) {
+            mul2(t, yn).get(a, b);                               // (vk holds wp scale)
+            og.set2(2 * j, a, b);
+            const F2 k = pair(gate, j);
+            t = mul2(t, k);
+            gv = mul2(gv, mul2(k, f2(p.scale)));
+          }
+          if constexpr (HELD) {
+            mul2(gv, yn).get(a, b);
+            if (e + 2 * j < width) { held[width + e + 2 * j] += a; held[width + e + 2 * j + 1] += b; }
+          } else {
+            cs[i][j] = fma2(gv, yn, cs[i][j]);
+          }
+          if constexpr (POST) t = fma2(q, t, mul2(back2, yv));
+          t.get(a, b);
+          o.set2(2 * j, a, b);
         }
-        if constexpr (HELD) {
-          part.get(a, b);
-          if (e + 2 * j < width) { held[width + e + 2 * j] += a; held[width + e + 2 * j + 1] += b; }
-        } else {
-          cs[j] = add2(cs[j], part);
-        }
-        t = post ? fma2(q, t, mul2(back2, yv)) : t;
-        t.get(a, b);
-        o.set2(2 * j, a, b);
+        put_unit<T, WIDE>(out_y + e * E, o, p.cols - e);
+        if constexpr (MATRIX)
+          if (each_row(p.dgate)) put_unit<T, WIDE>(row_of(p.dgate, row, p.lddg) + e * E, og, p.cols - e);
       }
-      put_unit<T, WIDE>(row_of(p.dy, row, p.lddy) + e * E, o, p.cols - e);
-      if (each_row(p.dgate)) put_unit<T, WIDE>(row_of(p.dgate, row, p.lddg) + e * E, og, p.cols - e);
     }
     if constexpr (!HELD) {
       __syncwarp();
@@ -807,18 +854,23 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_backward_kernel(con
   wait_copies(0);
   __syncthreads();
   if constexpr (!HELD) {
-    const int e = unit_at(0);
     for (int t = 0; t < (int)blockDim.y; ++t) {
-      if ((int)threadIdx.y == t && e < p.cols) {
+      if ((int)threadIdx.y == t) {
 #pragma unroll
-        for (int j = 0; j < kUnit / 2; ++j) {
-          float a, b;
-          cw[j].get(a, b);
-          held[e + 2 * j] = t ? held[e + 2 * j] + a : a;
-          held[e + 2 * j + 1] = t ? held[e + 2 * j + 1] + b : b;
-          cs[j].get(a, b);
-          held[width + e + 2 * j] = t ? held[width + e + 2 * j] + a : a;
-          held[width + e + 2 * j + 1] = t ? held[width + e + 2 * j + 1] + b : b;
+        for (int i = 0; i < NU; ++i) {
+          const int e = unit_at(i);
+          if (e < p.cols) {
+#pragma unroll
+            for (int j = 0; j < kUnit / 2; ++j) {
+              float a, b;
+              cw[i][j].get(a, b);
+              held[e + 2 * j] = t ? held[e + 2 * j] + a : a;
+              held[e + 2 * j + 1] = t ? held[e + 2 * j + 1] + b : b;
+              cs[i][j].get(a, b);
+              held[width + e + 2 * j] = t ? held[width + e + 2 * j] + a : a;
+              held[width + e + 2 * j + 1] = t ? held[width + e + 2 * j + 1] + b : b;
+            }
+          }
         }
       }
       __syncthreads();
@@ -871,8 +923,10 @@ __global__ void __launch_bounds__(256) residual_norm_columns_kernel(const __grid
   }
 }
 
-// `bytes`: a warp's stretches of all matrices.
-Shape back_shape(int64_t rows, int64_t cols, int bytes) {
+// Units to a thread: two for 16-bit elements and more rows than SMs.
+int back_units(int type, int64_t rows) { return type != GEMM_TYPE_FP32 && rows > 148 ? 2 : 1; }
+// `bytes`: a unit's stretches of a warp in all matrices.
+Shape back_shape(int type, int64_t rows, int64_t cols, int bytes) {
   const int units = (int)((cols + kUnit - 1) / kUnit);
   if (units > kMaxThreads) {
     Shape s;
@@ -881,21 +935,43 @@ Shape back_shape(int64_t rows, int64_t cols, int bytes) {
     s.smem = (size_t)units * kUnit * 8;
     return s;
   }
-  Shape s = shape_of(rows, units, 1, bytes);
-  const size_t sums = (size_t)units * kUnit * 8;
-  if (s.smem < sums) s.smem = sums;
-  return s;
+  const int nu = back_units(type, rows), vectors = nu == 2 ? ((units + 1) / 2 + 31) / 32 * 32 * 2 * kUnit * 8 : 0;
+  return shape_of(rows, units, nu, nu * bytes, kMaxThreads, vectors);
+}
+// No call has more blocks: with two units there is one to an SM, with one (where rows ahead never limit them) they go by the sizes.
+int64_t most_blocks(int64_t rows, int64_t cols) {
+  const int64_t two = rows < 148 ? rows : 148, a = back_shape(GEMM_TYPE_FP32, rows, cols, 1).blocks;
+  return a > two ? a : two;
 }
 
-template <typename T>
+template <typename T, int KIND>
 cudaError_t launch_backward(BackParams p, const Shape& s, bool wide, cudaStream_t st) {
-  const auto fn = p.cols > kMaxThreads * kUnit ? residual_norm_backward_kernel<T, true, false>
-                : wide ? residual_norm_backward_kernel<T, false, true> : residual_norm_backward_kernel<T, false, false>;
-  if (s.stages < 1 && p.cols <= kMaxThreads * kUnit) return cudaErrorInvalidValue;
+  constexpr bool FP32 = sizeof(T) == 4;
+  const int nu = back_units(FP32 ? GEMM_TYPE_FP32 : GEMM_TYPE_BF16, p.rows);
+  void (*fn)(BackParams);
+  if (p.cols > kMaxThreads * kUnit) {
+    fn = residual_norm_backward_kernel<T, 2, true, false, KIND>;
+  } else if (nu == 2) {
+    fn = wide ? residual_norm_backward_kernel<T, FP32 ? 1 : 2, false, true, KIND> : residual_norm_backward_kernel<T, FP32 ? 1 : 2, false, false, KIND>;
+  } else {
+    fn = FP32 && wide ? residual_norm_backward_kernel<T, 1, false, FP32, KIND> : residual_norm_backward_kernel<T, 1, false, false, KIND>;
+  }
   p.stages = s.stages;
+  if (s.stages < 1 && p.cols <= kMaxThreads * kUnit) return cudaErrorInvalidValue;
+  const int units = (p.cols + kUnit - 1) / kUnit, vectors = nu == 2 && units <= kMaxThreads ? s.tx * 2 * kUnit * 8 : 0;
+  p.vectors_at = (int32_t)s.smem;
+  size_t smem = s.smem + vectors;
+  const size_t sums = (size_t)units * kUnit * 8;        // the column sums lie over it all in the end
+  if (smem < sums) smem = sums;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(fn, dim3((unsigned)s.blocks), dim3((unsigned)s.tx, (unsigned)s.ty), s.smem, 1, st, p);
+  return launch_overlapped(fn, dim3((unsigned)s.blocks), dim3((unsigned)s.tx, (unsigned)s.ty), smem, 1, st, p);
+}
+template <typename T>
+cudaError_t launch_backward(const BackParams& p, const Shape& s, bool wide, cudaStream_t st) {
+  if (!p.in[3]) return launch_backward<T, 0>(p, s, wide, st);
+  if (!p.in[4]) return p.wp ? launch_backward<T, 2>(p, s, wide, st) : launch_backward<T, 1>(p, s, wide, st);
+  return p.wp ? launch_backward<T, 4>(p, s, wide, st) : launch_backward<T, 3>(p, s, wide, st);
 }
 
 int status_of(cudaError_t err) {
@@ -959,7 +1035,8 @@ extern "C" int gemm_sm100a_residual_norm(const ResidualNormArgs* a, void* stream
 
 extern "C" int64_t gemm_sm100a_residual_norm_workspace(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 1 || cols > kMaxCols || rows > INT32_MAX / 2) return -1;
-  return rows == 0 ? 0 : (int64_t)back_shape(rows, cols, 1).blocks * 2 * cols * 4;
+  if (rows == 0) return 0;
+  return most_blocks(rows, cols) * 2 * cols * 4;
 }
 
 extern "C" int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs* a, void* stream) {
@@ -1003,16 +1080,11 @@ extern "C" int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs
       if (outs[i].p && outs[j].p && rows_meet(outs[j].p, outs[j].ld * e, a->cols * e, outs[i].p, outs[i].ld * e, a->cols * e, a->rows))
         return GEMM_ERR_CANNOT_IMPLEMENT;
   }
-  bool in_wide = true, wide = true;
-  int matrices = 0;
-  for (const Mat& m : ins) {
-    in_wide &= !m.p || rows_16b(m.p, m.ld, e);
-    matrices += m.p ? 1 : 0;
-  }
+  bool wide = true;
+  for (const Mat& m : ins) wide &= !m.p || rows_16b(m.p, m.ld, e);
   for (const Mat& m : outs) wide &= !m.p || rows_16b(m.p, m.ld, e);
-  wide &= in_wide;
   const uint32_t place = place_bytes(e, wide);
-  const Shape s = back_shape(a->rows, a->cols, matrices * (int)place);
+  const Shape s = back_shape(a->type, a->rows, a->cols, ((a->y ? 4 : 3) + (matrix ? 1 : 0)) * (int)place);
   if (a->workspace_bytes < (int64_t)s.blocks * 2 * a->cols * 4) return GEMM_ERR_BAD_ARGS;
   BackParams p;
   memset(&p, 0, sizeof(p));
