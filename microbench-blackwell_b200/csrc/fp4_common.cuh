@@ -30,14 +30,18 @@ __host__ __device__ constexpr int64_t scale_at(int64_t row, int64_t col, int64_t
 }
 
 struct RowScale {
-  float up;      // 1 / g, 0 for a row with NaN or Inf
-  float scale;   // g, or the NaN or Inf
+  float up;      // 1 / g
+  float scale;   // g, or the NaN or Inf of the row, whose elements then count as zeros
+  __device__ __forceinline__ bool lost() const { return (__float_as_uint(scale) & 0x7F800000u) == 0x7F800000u; }
+  // g is so far from 1 that it has to be applied to the elements (which is exact) before anything else: the
+  // scales of their blocks in x's own unit might leave fp32's range.
+  __device__ __forceinline__ bool far() const { return !(scale > 0x1p-100f && scale < 0x1p100f); }
 };
 // `bits`: the largest |x| of the row as fp32 bits (integer maximum, so NaN > Inf > finite).
 __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
   RowScale s;
   if (bits >= 0x7F800000u) {
-    s.up = 0.f;
+    s.up = 1.f;
     s.scale = __uint_as_float(bits);
     return s;
   }
@@ -61,19 +65,28 @@ struct BlockScale {
   float s, r;      // the scale and 1 / s rounded to nearest (0 for s = 0)
 };
 // From the largest |y| of a block, finite and below 2048.
-//  e4m3: the nearest to top / 6 or, where 6 times that is below top, the next one.  (fp32's 1/6 times 6 s
-//    rounds back to s, so a top that is exactly 6 s stays at s.)
+//  e4m3: top / 6 rounded up to four significant bits (from 2^-6 on; in steps of 2^-9 below), and one step more where 6 times that
+//    is still below top.  (fp32's 1/6 times 6 s rounds back to s, so a top that is exactly 6 s stays at s.)  1 / s: one Newton
+//    step from the approximation is 2^-46 off, and no 8 / (8 + m) is that near to the middle of two fp32 numbers.
 //  e8m0: 6 * 2^k >= 2^e m with k = e - 2 for m <= 3/2, else e - 1.
 template <int BLOCK>
 __device__ __forceinline__ BlockScale block_scale(float top) {
   BlockScale b;
   if constexpr (BLOCK == 16) {
-    uint16_t c;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(c) : "f"(0.f), "f"(top * kSixth));
-    b.code = c;
-    b.s = decode_e4m3(b.code);
-    if (6.f * b.s < top) b.s = decode_e4m3(++b.code);
-    b.r = b.s > 0.f ? __frcp_rn(b.s) : 0.f;
+    const float t = top * kSixth;
+    if (t >= 0x1p-6f) {
+      uint32_t u = (__float_as_uint(t) + 0xFFFFFu) & 0xFFF00000u;
+      if (6.f * __uint_as_float(u) < top) u += 0x100000u;
+      b.code = (u >> 20) - 8u * (127u - 7u);
+      b.s = __uint_as_float(u);
+    } else {
+      b.code = __float2uint_ru(t * 512.f);
+      if ((float)b.code * (6.f / 512.f) < top) ++b.code;
+      b.s = (float)b.code * 0x1p-9f;
+    }
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(b.s));
+    b.r = b.s > 0.f ? fmaf(fmaf(-b.s, r, 1.f), r, r) : 0.f;
   } else {
     const uint32_t u = __float_as_uint(top);
     const int k = (int)(u >> 23) - 2 + ((u & 0x7FFFFFu) > 0x400000u ? 1 : 0);
@@ -95,41 +108,46 @@ __device__ __forceinline__ uint32_t pack8(const float (&z)[8]) {
   return w;
 }
 
-// Codes of 8 elements y of a block.  The quotient y / s has to be decided exactly at the seven borders
-// between codes, where bf16 blocks lie often: one correction of y r gives it rounded to nearest (r being 1 / s
-// rounded to nearest), and a quotient that is not a border, with s of four bits and y of 24, does not round to
-// one.  Division by a power of two is exact as it is.
+// Codes of 8 elements x = g y of a block.  The quotient y / s has to be decided exactly at the seven borders
+// between codes, where bf16 blocks lie often: one correction of x (r / g) gives it rounded to nearest (r being 1 / s
+// rounded to nearest, and g a power of two), and a quotient that is not a border, with s of four bits and y of 24, does
+// not round to one.  Division by powers of two is exact as it is (in two steps: together they might leave fp32's range).
 template <int BLOCK>
-__device__ __forceinline__ uint32_t round8(const float (&y)[8], const BlockScale& b) {
+__device__ __forceinline__ uint32_t round8(const float* x, const BlockScale& b, float up, float g) {
   using int8op::F2;
   float z[8];
-  const F2 r(b.r, b.r), ns(-b.s, -b.s);
+  const F2 r(b.r * up, b.r * up), ns(-b.s * g, -b.s * g), r1(b.r, b.r), u(up, up);
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
-    const F2 v(y[j], y[j + 1]);
-    F2 t = int8op::mul2(v, r);
-    if constexpr (BLOCK == 16) t = int8op::fma2(int8op::fma2(ns, t, v), r, t);
+    const F2 v(x[j], x[j + 1]);
+    F2 t;
+    if constexpr (BLOCK == 16) {
+      t = int8op::mul2(v, r);
+      t = int8op::fma2(int8op::fma2(ns, t, v), r, t);
+    } else {
+      t = int8op::mul2(int8op::mul2(v, u), r1);
+    }
     t.get(z[j], z[j + 1]);
   }
   return pack8(z);
 }
 
-// The 16 elements of a thread's unit (a warp's lanes hold consecutive units of a row; all of them call): codes in
-// two words, and this block's scale code.  Blocks of 32 are two lanes'.
+// Elements of a row that is far from 1, and the largest of them, times 1 / g; zeros for a row that is lost.
+__device__ __forceinline__ void bring_near(float (&x)[16], float& top, const RowScale& s) {
+  const bool lost = s.lost();
+  top = lost ? 0.f : top * s.up;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) x[j] = lost ? 0.f : x[j] * s.up;
+}
+
+// The 16 elements of a thread's unit (a warp's lanes hold consecutive units of a row; all of them call) and the largest
+// magnitude among them: codes in two words, and this block's scale code.  Blocks of 32 are two lanes'.
 template <int BLOCK>
-__device__ __forceinline__ uint32_t quantize_unit(float (&y)[16], uint32_t (&q)[2]) {
-  float top = 0.f;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(y[j]));
+__device__ __forceinline__ uint32_t quantize_unit(const float (&x)[16], float top, float up, float g, uint32_t (&q)[2]) {
   if constexpr (BLOCK == 32) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-  const BlockScale b = block_scale<BLOCK>(top);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float part[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) part[j] = y[8 * h + j];
-    q[h] = round8<BLOCK>(part, b);
-  }
+  const BlockScale b = block_scale<BLOCK>(top * up);
+  q[0] = round8<BLOCK>(x, b, up, g);
+  q[1] = round8<BLOCK>(x + 8, b, up, g);
   return b.code;
 }
 

@@ -154,6 +154,7 @@ __device__ __forceinline__ void stage_tokens(const Fp4Params& p, uint32_t tok, u
   __syncwarp();
   named_bar_sync(2, N);
   rowvec::Unit<X> v[PER];
+  uint32_t tops[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int u = i * N + tid, t = u / width, e = (u - t * width) * 16;
@@ -161,13 +162,7 @@ __device__ __forceinline__ void stage_tokens(const Fp4Params& p, uint32_t tok, u
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < rowvec::Unit<X>::W; ++j) {
-      if constexpr (sizeof(X) == 4) m = max(m, v[i].w[j] & 0x7FFFFFFFu);
-      else m = __vmaxu2(m, v[i].w[j] & 0x7FFF7FFFu);
-    }
-    if constexpr (sizeof(X) == 2) m = abs_bits_to_f32<X>(max(m & 0xFFFFu, m >> 16));
+    uint32_t m = tops[i] = rowvec::magnitude(v[i]);
 #pragma unroll
     for (int o = 1; o < 16; o *= 2) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     const int u = i * N + tid;
@@ -179,12 +174,14 @@ __device__ __forceinline__ void stage_tokens(const Fp4Params& p, uint32_t tok, u
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int u = i * N + tid, t = min(u / width, kFusedTokens - 1), unit = u - u / width * width;
-    const float up = fp4op::row_scale(top[t]).up;
-    float y[16];
+    const fp4op::RowScale s = fp4op::row_scale(top[t]);
+    const bool far = s.far();
+    float y[16], most = __uint_as_float(tops[i]);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) y[j] = up == 0.f ? 0.f : v[i].get(j) * up;
+    for (int j = 0; j < 16; ++j) y[j] = v[i].get(j);
+    if (far) fp4op::bring_near(y, most, s);
     uint32_t q[2];
-    const uint32_t code = fp4op::quantize_unit<BLOCK>(y, q);
+    const uint32_t code = fp4op::quantize_unit<BLOCK>(y, most, far ? 1.f : s.up, far ? 1.f : s.scale, q);
     constexpr int STEP = BLOCK / 16;
     uint32_t w = code << (8 * ((tid / STEP) & 3));
     w |= __shfl_xor_sync(0xFFFFFFFFu, w, STEP);

@@ -8,11 +8,11 @@
 #include "device_guard.cuh"
 #include "fp4_common.cuh"
 #include "gemm_sm100a.h"
-#include "row_vec.cuh"
+#include "row_stream.cuh"
 #include "sm100_ptx.cuh"
 
 using namespace int8op;
-using rowvec::kUnit;
+using namespace rowstream;
 
 namespace {
 
@@ -24,9 +24,11 @@ struct QuantParams {
   uint8_t* scales;
   int64_t tiles;
   float* row_scale;
+  int32_t stages;              // rows ahead, and bytes of a stretch in shared memory (row_stream.cuh)
+  uint32_t place;
 };
 
-// A row belongs to blockDim.x threads (a block holds blockDim.y rows); each keeps NU units in
+// Few or very long rows.  A row belongs to blockDim.x threads (a block holds blockDim.y rows); each keeps NU units in
 // registers between the row's maximum and the rounding, so X is read once.  Longer rows are read
 // again (from L2) chunk by chunk.
 template <typename T, int BLOCK, int NU>
@@ -50,18 +52,12 @@ __global__ void __launch_bounds__(512) quantize_fp4_kernel(const __grid_constant
       v[i] = rowvec::load_unit<T>(x + e, cols - e);
     }
   };
-  uint32_t top = 0;   // largest |x| so far: packed halves (16-bit T) or fp32 bits
+  uint32_t top = 0, tops[NU];   // largest |x| of the row, and of each unit held
   for (int c = 0; c < chunks; ++c) {
     load(c);
 #pragma unroll
-    for (int i = 0; i < NU; ++i)
-#pragma unroll
-      for (int j = 0; j < rowvec::Unit<T>::W; ++j) {
-        if constexpr (sizeof(T) == 4) top = max(top, v[i].w[j] & 0x7FFFFFFFu);
-        else top = __vmaxu2(top, v[i].w[j] & 0x7FFF7FFFu);
-      }
+    for (int i = 0; i < NU; ++i) top = max(top, tops[i] = rowvec::magnitude(v[i]));
   }
-  if constexpr (sizeof(T) == 2) top = abs_bits_to_f32<T>(max(top & 0xFFFFu, top >> 16));
   top = __reduce_max_sync(0xFFFFFFFFu, top);
   if (TX > 32) {
     const int warp = threadIdx.y * (TX >> 5) + (tx >> 5);
@@ -72,20 +68,95 @@ __global__ void __launch_bounds__(512) quantize_fp4_kernel(const __grid_constant
   }
   const fp4op::RowScale s = fp4op::row_scale(top);
   if (live && tx == 0) p.row_scale[row] = s.scale;
+  const bool far = s.far();
+  const float up = far ? 1.f : s.up, g = far ? 1.f : s.scale;
   for (int c = 0; c < chunks; ++c) {
     if (chunks > 1) load(c);
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int unit = c * per_chunk + i * TX + tx;
       if ((unit & ~31) >= units) break;      // whole warps
-      float y[16];
+      if (chunks > 1) tops[i] = rowvec::magnitude(v[i]);
+      float x[16], most = __uint_as_float(tops[i]);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) y[j] = s.up == 0.f ? 0.f : v[i].get(j) * s.up;
+      for (int j = 0; j < 16; ++j) x[j] = v[i].get(j);
+      if (far) fp4op::bring_near(x, most, s);
       uint32_t q[2];
-      const uint32_t code = fp4op::quantize_unit<BLOCK>(y, q);
+      const uint32_t code = fp4op::quantize_unit<BLOCK>(x, most, up, g, q);
       fp4op::store_scale_codes<BLOCK>(p.scales, row, p.tiles, unit, code, live && unit < units);
       const int n = cols - unit * kUnit;
       if (n > 0) fp4op::store_codes(p.values + row * p.ldv + unit * 8, q, n);
+    }
+  }
+}
+
+// Many rows: groups of threads walk down the matrix, NU units to a thread, with the coming rows copied ahead.
+template <typename T, int BLOCK, int NU, bool WIDE>
+__global__ void __launch_bounds__(NU == 2 ? 768 : 512, 1) quantize_fp4_stream_kernel(const __grid_constant__ QuantParams p) {
+  extern __shared__ __align__(16) uint8_t slots[];
+  __shared__ uint32_t warp_max[2][32];
+  constexpr int E = (int)sizeof(T);
+  const int tx = threadIdx.x, TX = blockDim.x, warps = TX >> 5;
+  const int units = (int)(p.tiles * 4 * (BLOCK / 16));
+  const uint32_t per_stage = NU * p.place;
+  const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * warps + (tx >> 5)) * (uint32_t)p.stages * per_stage;
+  const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
+  int n[NU];
+#pragma unroll
+  for (int i = 0; i < NU; ++i) n[i] = (int)p.cols - (i * TX + tx) * kUnit;
+  sm100::grid_dependency_wait();
+  sm100::grid_launch_dependents();
+  auto issue = [&](int64_t row, uint32_t slot) {
+    if (row < p.rows) {
+      const uint8_t* const r = row_of(static_cast<const uint8_t*>(p.x), row, p.ldx * E) + (tx & ~31) * kUnit * E;
+#pragma unroll
+      for (int i = 0; i < NU; ++i) issue_stretch<T, WIDE>(slot + i * p.place, r + i * TX * kUnit * E, n[i] + (tx & 31) * kUnit);
+    }
+    commit_copies();
+  };
+  for (int s = 0; s < p.stages; ++s) issue(first + s * step, mine + (uint32_t)s * per_stage);
+  int stage = 0, flip = 0;
+  for (int64_t row = first; row < p.rows; row += step) {
+    const uint32_t at = mine + (uint32_t)stage * per_stage;
+    wait_copies(p.stages - 1);
+    __syncwarp();
+    const uint32_t off = WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(static_cast<const uint8_t*>(p.x) + row * p.ldx * E) & 15u;
+    Unit<T> v[NU];
+    uint32_t tops[NU], top = 0;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      v[i] = take_unit<T, WIDE>(at + i * p.place, off, n[i]);
+      top = max(top, tops[i] = rowvec::magnitude(v[i]));
+    }
+    __syncwarp();
+    issue(row + p.stages * step, at);
+    if (++stage == p.stages) stage = 0;
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if (warps > 1) {
+      // (A row's maxima are written again by the second row after it, with a barrier between.)
+      uint32_t* const group = warp_max[flip ^= 1] + (int)threadIdx.y * warps;
+      if ((tx & 31) == 0) group[tx >> 5] = top;
+      group_sync();
+      top = __reduce_max_sync(0xFFFFFFFFu, (tx & 31) < warps ? group[tx & 31] : 0u);
+    }
+    const fp4op::RowScale s = fp4op::row_scale(top);
+    if (tx == 0) p.row_scale[row] = s.scale;
+    const bool far = s.far();
+    const float up = far ? 1.f : s.up, g = far ? 1.f : s.scale;
+    uint8_t* const out = row_of(p.values, row, p.ldv);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int unit = i * TX + tx;
+      if ((unit & ~31) >= units) break;      // whole warps
+      forget(v[i]);
+      float x[16], most = __uint_as_float(tops[i]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = v[i].get(j);
+      if (each_row(far)) fp4op::bring_near(x, most, s);
+      uint32_t q[2];
+      const uint32_t code = fp4op::quantize_unit<BLOCK>(x, most, up, g, q);
+      fp4op::store_scale_codes<BLOCK>(p.scales, row, p.tiles, unit, code, unit < units);
+      if (n[i] > 0) fp4op::store_codes(out + unit * 8, q, n[i]);
     }
   }
 }
@@ -99,12 +170,29 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
   const int64_t blocks = (p.rows + ry - 1) / ry;   // at most 2^30
   return launch_overlapped(quantize_fp4_kernel<T, BLOCK, NU>, dim3((unsigned)blocks), dim3((unsigned)tx, (unsigned)ry), 0, 1, st, p);
 }
+template <typename T, int BLOCK, int NU, bool WIDE>
+cudaError_t launch_stream(QuantParams p, cudaStream_t st) {
+  p.place = place_bytes((int)sizeof(T), WIDE);
+  const Shape s = shape_of(p.rows, (int)(p.tiles * 4 * (BLOCK / 16)), NU, NU * (int)p.place, NU == 2 ? 768 : 512);
+  if (s.stages < 1) return cudaErrorInvalidValue;
+  p.stages = s.stages;
+  const auto fn = quantize_fp4_stream_kernel<T, BLOCK, NU, WIDE>;
+  const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+  if (err != cudaSuccess) return err;
+  return launch_overlapped(fn, dim3((unsigned)s.blocks), dim3((unsigned)s.tx, (unsigned)s.ty), s.smem, 1, st, p);
+}
+template <typename T, int BLOCK>
+cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
+  const int64_t units = p.tiles * 4 * (BLOCK / 16);
+  if (p.rows * units <= 148 * 1024) return launch_rows<T, BLOCK, 1>(p, st);
+  if (units > 4 * kMaxThreads) return launch_rows<T, BLOCK, 2>(p, st);
+  const bool wide = all_wide({{p.x, p.ldx * (int64_t)sizeof(T)}});
+  if (units <= 2 * kMaxThreads) return wide ? launch_stream<T, BLOCK, 2, true>(p, st) : launch_stream<T, BLOCK, 2, false>(p, st);
+  return wide ? launch_stream<T, BLOCK, 4, true>(p, st) : launch_stream<T, BLOCK, 4, false>(p, st);
+}
 template <typename T>
 cudaError_t launch_rows(const QuantParams& p, int block, cudaStream_t st) {
-  constexpr int NU = sizeof(T) == 4 ? 2 : 4;
-  const bool small = p.rows * ((p.cols + 15) / 16) <= 148 * 1024;
-  if (block == 16) return small ? launch_rows<T, 16, 1>(p, st) : launch_rows<T, 16, NU>(p, st);
-  return small ? launch_rows<T, 32, 1>(p, st) : launch_rows<T, 32, NU>(p, st);
+  return block == 16 ? launch_rows<T, 16>(p, st) : launch_rows<T, 32>(p, st);
 }
 
 // ----------------------------------------------------------------- back

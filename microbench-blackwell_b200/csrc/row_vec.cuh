@@ -64,6 +64,18 @@ struct Unit {
   }
 };
 
+// Largest |x| of a unit as fp32 bits (integer maximum, so NaN > Inf > finite).
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude(const Unit<T>& u) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < Unit<T>::W; ++j) {
+    if constexpr (sizeof(T) == 4) m = max(m, u.w[j] & 0x7FFFFFFFu);
+    else m = __vmaxu2(m, u.w[j] & 0x7FFF7FFFu);
+  }
+  if constexpr (sizeof(T) == 2) m = abs_bits_to_f32<T>(max(m & 0xFFFFu, m >> 16));
+  return m;
+}
 // Zeros beyond the first `bytes` of a unit.
 template <typename T>
 __device__ __forceinline__ void clip(Unit<T>& u, int bytes) {
