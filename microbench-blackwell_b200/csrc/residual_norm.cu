@@ -71,11 +71,14 @@ __device__ __forceinline__ double squares_wide(const Unit<T>& u) {
 // Where the fp32 part of a sum of squares may have left its range (or come near its end), 64 bits do it again.
 __device__ __forceinline__ bool out_of_range(double s) { return !(s > 1e-30 && s < 1e38); }
 
-// 1 / sqrt(v), rounded to fp32 from an error of 2^-43 or less.
+// 1 / sqrt(v), rounded to fp32 from an error of 2^-43 or so: one Newton step whose 1 - v r^2 has v and r^2 in two fp32
+// words each.
 __device__ __forceinline__ float inverse_root(double v) {
   if (!(v > 1e-30 && v < 1e30)) return (float)(1.0 / sqrt(v));
-  const double r = (double)rsqrtf((float)v);
-  return (float)fma(0.5 * r, fma(-v * r, r, 1.0), r);
+  const float hi = (float)v, lo = (float)(v - (double)hi);
+  const float r = rsqrtf(hi), p = r * r, p_lo = fmaf(r, r, -p);
+  const float t = fmaf(-hi, p, 1.f) - fmaf(hi, p_lo, lo * p);
+  return fmaf(0.5f * r, t, r);
 }
 
 // The sum over the group's warps of a value that the lanes of each warp hold; all threads of the group call, with `part`
@@ -136,7 +139,7 @@ __device__ __forceinline__ void load_params(const void* v, int param32, int e, i
 // Vectors that all groups of a block read, in shared memory: four elements of a unit to a slot, the slots of one kind side by
 // side for all units (no bank conflicts).
 struct SharedVectors {
-  uint32_t base, per_chunk;
+  uint32_t base, per_chunk;      // bytes from a unit's slot to that of its next four elements
   __device__ __forceinline__ uint32_t at(int which, int unit) const { return base + (uint32_t)(which * 4) * per_chunk + (uint32_t)unit * 16u; }
   __device__ __forceinline__ void put(int which, int unit, const F2 (&v)[kUnit / 2]) const {
 #pragma unroll
@@ -620,7 +623,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
       if (lane == 0) {
         // r, q and the coefficients; or -1 for statistics that have to be taken in 64 bits, and what the coefficients need.
         const bool again = out_of_range(t.x) || (POST && out_of_range(t.y));
-        const float r = again ? -1.f : inverse_root(fma((double)t.x, p.inv_n, p.eps)), q = POST && !again ? inverse_root(fma((double)t.y, p.inv_n, p.eps)) : 1.f;
+        const float eps = (float)p.eps, r = again ? -1.f : rsqrtf(fmaf(t.x, inv_n, eps)), q = POST && !again ? rsqrtf(fmaf(t.y, inv_n, eps)) : 1.f;
         const float back = r * r * r * (t.z * inv_n);
         sums.row[threadIdx.y] = again ? make_float4(-1.f, t.z, t.w, 0.f) : make_float4(r, q, back, q * q * q * ((t.w + r * b2 - back * b3) * inv_n));
         if (again) { sums.part[first_warp][0] = b2; sums.part[first_warp][1] = b3; }
@@ -711,7 +714,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
     }
     if (++stage == p.stages) stage = 0;
   }
-  // ---- this block's column sums
+  // ---- this block's column sums (planes of four elements one slot more apart than they have units, for the banks)
+  const SharedVectors columns = {sm100::smem_u32(slots), (uint32_t)(width / kUnit + 1) * 16u};
   wait_copies(0);
   __syncthreads();
   if constexpr (!HELD) {
@@ -719,18 +723,20 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
       if ((int)threadIdx.y == t) {
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-          const int e = unit_at(i);
-          if (e < p.cols) {
+          if (unit_at(i) >= p.cols) continue;
 #pragma unroll
-            for (int j = 0; j < kUnit / 2; ++j) {
-              float a, b;
-              cw[i][j].get(a, b);
-              held[e + 2 * j] = t ? held[e + 2 * j] + a : a;
-              held[e + 2 * j + 1] = t ? held[e + 2 * j + 1] + b : b;
-              cs[i][j].get(a, b);
-              held[width + e + 2 * j] = t ? held[width + e + 2 * j] + a : a;
-              held[width + e + 2 * j + 1] = t ? held[width + e + 2 * j + 1] + b : b;
+          for (int which = 0; which < 2; ++which) {
+            F2* const v = which ? cs[i] : cw[i];
+            if (t > 0) {
+              F2 before[kUnit / 2];
+              columns.get(which, i * TX + tx, before);
+#pragma unroll
+              for (int j = 0; j < kUnit / 2; ++j) v[j] = add2(before[j], v[j]);
             }
+            F2 sum[kUnit / 2];
+#pragma unroll
+            for (int j = 0; j < kUnit / 2; ++j) sum[j] = v[j];
+            columns.put(which, i * TX + tx, sum);
           }
         }
       }
@@ -739,9 +745,23 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
   }
   float* const out = p.parts + (int64_t)blockIdx.x * 2 * p.cols;
   const int all = TX * (int)blockDim.y, me = (int)threadIdx.y * TX + tx;
-  for (int i = me; i < p.cols; i += all) {
-    out[i] = held[i];
-    out[p.cols + i] = held[width + i];
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    for (int q = me; 4 * q < p.cols; q += all) {
+      float f[4];
+      if constexpr (HELD) {
+#pragma unroll
+        for (int l = 0; l < 4; ++l) f[l] = held[which * width + 4 * q + l];
+      } else {
+        F2 a, b;
+        columns.get(which, q >> 2, q & 3, a, b);
+        a.get(f[0], f[1]);
+        b.get(f[2], f[3]);
+      }
+#pragma unroll
+      for (int l = 0; l < 4; ++l)
+        if (4 * q + l < p.cols) out[which * p.cols + 4 * q + l] = f[l];
+    }
   }
 }
 
@@ -822,7 +842,7 @@ cudaError_t launch_backward(BackParams p, const Shape& s, bool wide, cudaStream_
   const int units = (p.cols + kUnit - 1) / kUnit, vectors = nu == 2 && units <= kMaxThreads ? s.tx * 2 * kUnit * 8 : 0;
   p.vectors_at = (int32_t)s.smem;
   size_t smem = s.smem + vectors;
-  const size_t sums = (size_t)units * kUnit * 8;        // the column sums lie over it all in the end
+  const size_t sums = (size_t)(units + 1) * kUnit * 8;  // the column sums lie over it all in the end
   if (smem < sums) smem = sums;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (e != cudaSuccess) return e;
