@@ -69,7 +69,7 @@ __device__ __forceinline__ double squares_wide(const Unit<T>& u) {
   return s;
 }
 // Where the fp32 part of a sum of squares may have left its range (or come near its end), 64 bits do it again.
-__device__ __forceinline__ bool out_of_range(double s) { return !(s > 1e-30 && s < 1e38); }
+__device__ __forceinline__ bool out_of_range(float s) { return !(s > 1e-30f && s < 1e38f); }
 
 // 1 / sqrt(v), rounded to fp32 from an error of 2^-43 or so: one Newton step whose 1 - v r^2 has v and r^2 in two fp32
 // words each.
@@ -81,8 +81,17 @@ __device__ __forceinline__ float inverse_root(double v) {
   return fmaf(0.5f * r, t, r);
 }
 
-// The sum over the group's warps of a value that the lanes of each warp hold; all threads of the group call, with `part`
-// alternating between calls.
+// The sum over the group's threads; all of them call, with `part` alternating between calls.
+__device__ __forceinline__ float group_sum(float v, float* part) {
+  v = warp_sum(v);
+  const int warps = (int)blockDim.x >> 5, lane = (int)(threadIdx.x & 31u);
+  if (warps == 1) return v;
+  float* const mine = part + threadIdx.y * warps;
+  if (lane == 0) mine[threadIdx.x >> 5] = v;
+  group_sync();
+  return warp_sum(lane < warps ? mine[lane] : 0.f);
+}
+// The sum over the group's warps of a value that the lanes of each warp hold, in 64 bits.
 __device__ __forceinline__ double across_warps(double v, double* part) {
   const int warps = (int)blockDim.x >> 5;
   if (warps == 1) return v;
@@ -173,6 +182,7 @@ template <typename T, bool FOUR, int NU, bool WIDE, int KIND>
 __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ double part[2][kManyThreads / 32];
+  __shared__ float part32[2][kManyThreads / 32];
   __shared__ uint32_t warp_max[kManyThreads / 32];
   constexpr int E = (int)sizeof(T);
   constexpr bool KEEP = NU == 1, SHARED = NU == 2 && E == 2, BLOCK = KIND > 0, MATRIX = KIND == 2;
@@ -249,12 +259,16 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
       for (int i = 0; i < NU; ++i) s += squares_wide<T>(v[i]);
       s = across_warps(warp_sum(s), at);
     } else {
-      // Sums of squares of a warp's elements in fp32, beyond in 64 bits.
+      // In fp32, pairwise from a few elements up: 64 bits cost the kernel of 16-bit elements twice its instructions for a last
+      // bit of r that their results do not show.
       float f = 0.f;
 #pragma unroll
       for (int i = 0; i < NU; ++i) f += squares<T>(v[i]);
-      s = across_warps((double)warp_sum(f), at);
-      if (out_of_range(s)) {
+      f = group_sum(f, part32[flip]);
+      if (!out_of_range(f)) {
+        const float m = fmaf(f, (float)p.inv_n, (float)p.eps), r = rsqrtf(m);
+        return fmaf(0.5f * r, fmaf(-m * r, r, 1.f), r);
+      } else {
         group_sync();
         s = 0.0;
 #pragma unroll
