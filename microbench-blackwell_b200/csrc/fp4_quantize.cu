@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(512) quantize_fp4_kernel(const __grid_constant
 }
 
 // Many rows: groups of threads walk down the matrix, NU units to a thread, with the coming rows copied ahead.
-template <typename T, int BLOCK, int NU, bool WIDE>
+template <typename T, int BLOCK, int NU, bool FULL>
 __global__ void __launch_bounds__(NU == 2 ? 768 : 512, 1) quantize_fp4_stream_kernel(const __grid_constant__ QuantParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ uint32_t warp_max[2][32];
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(NU == 2 ? 768 : 512, 1) quantize_fp4_stream_ke
     if (row < p.rows) {
       const uint8_t* const r = row_of(static_cast<const uint8_t*>(p.x), row, p.ldx * E) + (tx & ~31) * kUnit * E;
 #pragma unroll
-      for (int i = 0; i < NU; ++i) issue_stretch<T, WIDE>(slot + i * p.place, r + i * TX * kUnit * E, n[i] + (tx & 31) * kUnit);
+      for (int i = 0; i < NU; ++i) issue_stretch<T, FULL>(slot + i * p.place, r + i * TX * kUnit * E, n[i] + (tx & 31) * kUnit);
     }
     commit_copies();
   };
@@ -120,12 +120,12 @@ __global__ void __launch_bounds__(NU == 2 ? 768 : 512, 1) quantize_fp4_stream_ke
     const uint32_t at = mine + (uint32_t)stage * per_stage;
     wait_copies(p.stages - 1);
     __syncwarp();
-    const uint32_t off = WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(static_cast<const uint8_t*>(p.x) + row * p.ldx * E) & 15u;
+    const uint32_t off = FULL ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(static_cast<const uint8_t*>(p.x) + row * p.ldx * E) & 15u;
     Unit<T> v[NU];
     uint32_t tops[NU], top = 0;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      v[i] = take_unit<T, WIDE>(at + i * p.place, off, n[i]);
+      v[i] = take_unit<T, FULL>(at + i * p.place, off, n[i]);
       top = max(top, tops[i] = rowvec::magnitude(v[i]));
     }
     __syncwarp();
@@ -170,13 +170,13 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
   const int64_t blocks = (p.rows + ry - 1) / ry;   // at most 2^30
   return launch_overlapped(quantize_fp4_kernel<T, BLOCK, NU>, dim3((unsigned)blocks), dim3((unsigned)tx, (unsigned)ry), 0, 1, st, p);
 }
-template <typename T, int BLOCK, int NU, bool WIDE>
+template <typename T, int BLOCK, int NU, bool FULL>
 cudaError_t launch_stream(QuantParams p, cudaStream_t st) {
-  p.place = place_bytes((int)sizeof(T), WIDE);
+  p.place = place_bytes((int)sizeof(T), FULL || all_wide({{p.x, p.ldx * (int64_t)sizeof(T)}}));
   const Shape s = shape_of(p.rows, (int)(p.tiles * 4 * (BLOCK / 16)), NU, NU * (int)p.place, NU == 2 ? 768 : 512);
   if (s.stages < 1) return cudaErrorInvalidValue;
   p.stages = s.stages;
-  const auto fn = quantize_fp4_stream_kernel<T, BLOCK, NU, WIDE>;
+  const auto fn = quantize_fp4_stream_kernel<T, BLOCK, NU, FULL>;
   const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (err != cudaSuccess) return err;
   return launch_overlapped(fn, dim3((unsigned)s.blocks), dim3((unsigned)s.tx, (unsigned)s.ty), s.smem, 1, st, p);
@@ -186,7 +186,8 @@ cudaError_t launch_rows(const QuantParams& p, cudaStream_t st) {
   const int64_t units = p.tiles * 4 * (BLOCK / 16);
   if (p.rows * units <= 148 * 1024) return launch_rows<T, BLOCK, 1>(p, st);
   if (units > 4 * kMaxThreads) return launch_rows<T, BLOCK, 2>(p, st);
-  const bool wide = all_wide({{p.x, p.ldx * (int64_t)sizeof(T)}});
+  const bool wide = all_wide({{p.x, p.ldx * (int64_t)sizeof(T)}}) && p.cols < INT32_MAX / 2 &&
+                    all_full((int)units, (int)p.cols, units <= 2 * kMaxThreads ? 2 : 4);
   if (units <= 2 * kMaxThreads) return wide ? launch_stream<T, BLOCK, 2, true>(p, st) : launch_stream<T, BLOCK, 2, false>(p, st);
   return wide ? launch_stream<T, BLOCK, 4, true>(p, st) : launch_stream<T, BLOCK, 4, false>(p, st);
 }

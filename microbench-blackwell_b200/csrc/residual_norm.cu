@@ -178,7 +178,7 @@ struct SharedVectors {
 //    barriers.  Rows that leave no room for them read them from the caches each time.
 // KIND 0: no y; 1: y; 2: y and a gate matrix.  (What can be absent from call to call is decided here where
 // the compiler would otherwise make a copy of the loop for each case, with the registers of all.)
-template <typename T, bool FOUR, int NU, bool WIDE, int KIND>
+template <typename T, bool FOUR, int NU, bool FULL, int KIND>
 __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ double part[2][kManyThreads / 32];
@@ -206,14 +206,14 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
       const uint8_t* const ry = row_of(p.y, row, p.ldy);
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        issue_stretch<T, WIDE>(slot, rx + (e[i] - lane_e) * E, n[i] + lane_e);
+        issue_stretch<T, FULL>(slot, rx + (e[i] - lane_e) * E, n[i] + lane_e);
         slot += per_unit;
         if (BLOCK) {
-          issue_stretch<T, WIDE>(slot, ry + (e[i] - lane_e) * E, n[i] + lane_e);
+          issue_stretch<T, FULL>(slot, ry + (e[i] - lane_e) * E, n[i] + lane_e);
           slot += per_unit;
         }
         if (MATRIX && p.gate_ahead) {
-          issue_stretch<T, WIDE>(slot, row_of(p.gate, row, p.ldg) + (e[i] - lane_e) * E, n[i] + lane_e);
+          issue_stretch<T, FULL>(slot, row_of(p.gate, row, p.ldg) + (e[i] - lane_e) * E, n[i] + lane_e);
           slot += per_unit;
         }
       }
@@ -293,14 +293,14 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
       uint32_t slot = at;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
-        x[i] = take_unit<T, WIDE>(slot, low(rx), n[i]);
+        x[i] = take_unit<T, FULL>(slot, low(rx), n[i]);
         slot += per_unit;
         if (BLOCK) {
-          y[i] = take_unit<T, WIDE>(slot, low(ry), n[i]);
+          y[i] = take_unit<T, FULL>(slot, low(ry), n[i]);
           slot += per_unit;
         }
         if (MATRIX && p.gate_ahead) {
-          gate[i] = take_unit<T, WIDE>(slot, low(rg), n[i]);
+          gate[i] = take_unit<T, FULL>(slot, low(rg), n[i]);
           slot += per_unit;
         } else if (MATRIX) {
           gate[i] = rowvec::load_unit<T>(reinterpret_cast<const T*>(rg) + e[i], n[i]);
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
             x[i].set2(2 * j, a, b);
           }
         }
-        put_unit<T, WIDE>(out + e[i] * E, x[i], n[i]);
+        put_unit<T, FULL>(out + e[i] * E, x[i], n[i]);
       }
     }
     const F2 r = f2(inverse_rms(x));
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
         Unit<T> o;
 #pragma unroll
         for (int j = 0; j < kUnit; j += 2) o.set2(j, h[j], h[j + 1]);
-        put_unit<T, WIDE>(out + e[i] * E, o, n[i]);
+        put_unit<T, FULL>(out + e[i] * E, o, n[i]);
       }
     } else {
       float h[NU][kUnit], tops[NU];
@@ -409,12 +409,12 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
 
 bool rows_wide(const NormParams& p) { return all_wide({{p.x, p.ldx}, {p.y, p.ldy}, {p.ldg ? p.gate : nullptr, p.ldg}}); }
 
-template <typename T, bool FOUR, int NU, bool WIDE, int KIND>
+template <typename T, bool FOUR, int NU, bool FULL, int KIND>
 cudaError_t launch_forward(const NormParams& p0, cudaStream_t st) {
   NormParams p = p0;
   constexpr bool SHARED = NU == 2 && sizeof(T) == 2;
   const int units = FOUR ? (int)p.tiles * 4 * (p.block / 16) : (p.cols + kUnit - 1) / kUnit;
-  p.place = place_bytes((int)sizeof(T), WIDE || rows_wide(p));
+  p.place = place_bytes((int)sizeof(T), FULL || rows_wide(p));
   const int two = (KIND ? 2 : 1) * NU * (int)p.place, three = two + (KIND == 2 ? NU * (int)p.place : 0);
   const int tx = ((units + NU - 1) / NU + 31) / 32 * 32, vectors = SHARED ? tx * NU * kUnit * 4 * (KIND ? 2 : 1) : 0;
   // A gate matrix is not copied ahead where there is no room for it (rows of more than some 14000 elements).
@@ -423,7 +423,7 @@ cudaError_t launch_forward(const NormParams& p0, cudaStream_t st) {
   if (s.stages < 1) return cudaErrorInvalidValue;
   p.stages = s.stages;
   p.vectors_at = (int32_t)s.smem;
-  const auto fn = residual_norm_kernel<T, FOUR, NU, WIDE, KIND>;
+  const auto fn = residual_norm_kernel<T, FOUR, NU, FULL, KIND>;
   // (Always the same limit: calls of other sizes may be between this line and the launch.)
   const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (err != cudaSuccess) return err;
@@ -432,7 +432,7 @@ cudaError_t launch_forward(const NormParams& p0, cudaStream_t st) {
 template <typename T, bool FOUR, int KIND>
 cudaError_t launch_forward(const NormParams& p, cudaStream_t st) {
   if (p.cols <= kMaxThreads * kUnit && p.rows <= 148) return launch_forward<T, FOUR, 1, false, KIND>(p, st);
-  const bool wide = rows_wide(p) && all_wide({{p.xo, p.ldo}, {p.h, p.ldh}});
+  const bool wide = rows_wide(p) && all_wide({{p.xo, p.ldo}, {p.h, p.ldh}}) && all_full((p.cols + kUnit - 1) / kUnit, p.cols, 2);
   return wide ? launch_forward<T, FOUR, 2, true, KIND>(p, st) : launch_forward<T, FOUR, 2, false, KIND>(p, st);
 }
 template <typename T>
@@ -492,7 +492,7 @@ __device__ __forceinline__ float warp_sums(float (&v)[8]) {
 //  The column sums are two: of dh x r, and of g y q (times a gate matrix' k): dpost and a vector's dgate are the second
 // times what their columns share.
 //  KIND 0: no y; 1: y; 2: y and its norm; 3, 4: 1, 2 with a gate matrix.
-template <typename T, int NU, bool HELD, bool WIDE, int KIND>
+template <typename T, int NU, bool HELD, bool FULL, int KIND>
 __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(const __grid_constant__ BackParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ BackSums sums;
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
           const int e = unit_at(i) - (tx & 31) * kUnit;
-          if (m != DX || each_row(p.in[DX])) issue_stretch<T, WIDE>(slot, r + e * E, p.cols - e);
+          if (m != DX || each_row(p.in[DX])) issue_stretch<T, FULL>(slot, r + e * E, p.cols - e);
           slot += p.place;
         }
       }
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
       Unit<T> u;
       if (m == DX && each_row(!p.in[DX])) u.clear();
       else if constexpr (HELD) u = rowvec::load_unit<T, rowvec::kKeep>(reinterpret_cast<const T*>(row_of(p.in[m], row, p.ld[m])) + e, n);
-      else u = take_unit<T, WIDE>(at + (uint32_t)(m * NU + i) * p.place, WIDE ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(p.in[m] + row * p.ld[m]) & 15u, n);
+      else u = take_unit<T, FULL>(at + (uint32_t)(m * NU + i) * p.place, FULL ? 0u : (uint32_t)reinterpret_cast<uintptr_t>(p.in[m] + row * p.ld[m]) & 15u, n);
       return u;
     };
     // ---- row sums
@@ -689,7 +689,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
           o.set2(2 * j, a, b);
         }
       }
-      put_unit<T, WIDE>(out_x + e * E, o, p.cols - e);
+      put_unit<T, FULL>(out_x + e * E, o, p.cols - e);
       if constexpr (BLOCK) {
         if constexpr (SHARED) vectors.get(1, i * TX + tx, vk);
         const Unit<T> y = get(Y, i);
@@ -717,9 +717,9 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
           t.get(a, b);
           o.set2(2 * j, a, b);
         }
-        put_unit<T, WIDE>(out_y + e * E, o, p.cols - e);
+        put_unit<T, FULL>(out_y + e * E, o, p.cols - e);
         if constexpr (MATRIX)
-          if (each_row(p.dgate)) put_unit<T, WIDE>(row_of(p.dgate, row, p.lddg) + e * E, og, p.cols - e);
+          if (each_row(p.dgate)) put_unit<T, FULL>(row_of(p.dgate, row, p.lddg) + e * E, og, p.cols - e);
       }
     }
     if constexpr (!HELD) {
@@ -843,6 +843,7 @@ template <typename T, int KIND>
 cudaError_t launch_backward(BackParams p, const Shape& s, bool wide, cudaStream_t st) {
   constexpr bool FP32 = sizeof(T) == 4;
   const int nu = back_units(FP32 ? GEMM_TYPE_FP32 : GEMM_TYPE_BF16, p.rows);
+  wide = wide && all_full((p.cols + kUnit - 1) / kUnit, p.cols, nu);
   void (*fn)(BackParams);
   if (p.cols > kMaxThreads * kUnit) {
     fn = residual_norm_backward_kernel<T, 2, true, false, KIND>;

@@ -26,20 +26,21 @@ constexpr int kSmemLimit = 224 * 1024;     // dynamic shared memory of a block, 
 // are what keeps HBM busy while the group goes through a row's sums.  Lanes copy neighbouring 16-byte chunks (whole
 // sectors) and read those of their own unit, so a warp's lanes wait for one another before they read, and before the
 // place is copied to again.  Chunk c lies at c ^ (c / 8 mod E): lanes that read E chunks each then meet all banks.
-// A stretch off 16-byte boundaries (never with WIDE) takes one chunk more, and is shifted when it is read.  Every chunk holds
+// A stretch off 16-byte boundaries takes one chunk more, and is shifted when it is read.  Every chunk holds
 // a byte of the row, so that no copy leaves the 16 bytes around one.
+// FULL: all rows start on 16-byte boundaries and every lane's units lie in the row.
 // n: elements of the row from the stretch's first on.
-template <typename T, bool WIDE>
+template <typename T, bool FULL>
 __device__ __forceinline__ void issue_stretch(uint32_t place, const uint8_t* p, int n) {
   constexpr int E = (int)sizeof(T);
   const int lane = (int)(threadIdx.x & 31u);
-  const int off = WIDE ? 0 : (int)(reinterpret_cast<uintptr_t>(p) & 15u);
+  const int off = FULL ? 0 : (int)(reinterpret_cast<uintptr_t>(p) & 15u);
   const uint32_t dst = place + 16u * (uint32_t)(lane ^ ((lane >> 3) & (E - 1)));
   const uint8_t* const src = p - off + 16 * lane;
-  if (n >= 32 * kUnit) {
+  if (FULL || n >= 32 * kUnit) {
 #pragma unroll
     for (int j = 0; j < E; ++j) sm100::cp_async_16(dst + 512u * j, src + 512 * j, 16u);
-    if (!WIDE && off && lane == 0) sm100::cp_async_16(dst + 512u * E, src + 512 * E, 16u);
+    if (!FULL && off && lane == 0) sm100::cp_async_16(dst + 512u * E, src + 512 * E, 16u);
   } else if (n > 0) {
     const int chunks = (off + n * E + 15) / 16;
 #pragma unroll
@@ -48,11 +49,11 @@ __device__ __forceinline__ void issue_stretch(uint32_t place, const uint8_t* p, 
   }
 }
 // A lane's unit; off: the stretch's offset from a 16-byte boundary, n: elements of the row from the unit's first on.
-template <typename T, bool WIDE>
+template <typename T, bool FULL>
 __device__ __forceinline__ Unit<T> take_unit(uint32_t place, uint32_t off, int n) {
   constexpr int W = Unit<T>::W, E = (int)sizeof(T);
   Unit<T> u;
-  if (n <= 0) {
+  if (!FULL && n <= 0) {
     u.clear();
     return u;
   }
@@ -62,7 +63,7 @@ __device__ __forceinline__ Unit<T> take_unit(uint32_t place, uint32_t off, int n
     const uint4 v = sm100::ld_shared_v4(place + 16u * (uint32_t)(c ^ ((c >> 3) & (E - 1))));
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   };
-  if (WIDE || off == 0) {
+  if (FULL || off == 0) {
 #pragma unroll
     for (int j = 0; j < E; ++j) chunk(j, u.w + 4 * j);
   } else {
@@ -73,12 +74,12 @@ __device__ __forceinline__ Unit<T> take_unit(uint32_t place, uint32_t off, int n
 #pragma unroll
     for (int j = 0; j < W; ++j) u.w[j] = w[j];
   }
-  if (n < kUnit) rowvec::clip(u, n * E);
+  if (!FULL && n < kUnit) rowvec::clip(u, n * E);
   return u;
 }
-template <typename T, bool WIDE>
+template <typename T, bool FULL>
 __device__ __forceinline__ void put_unit(uint8_t* p, const Unit<T>& u, int n) {
-  if constexpr (WIDE) rowvec::store_aligned<T>(p, u, n);
+  if constexpr (FULL) rowvec::store_aligned<T>(p, u, kUnit);
   else rowvec::store_unit<T>(reinterpret_cast<T*>(p), u, n);
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -153,6 +154,8 @@ inline Shape shape_of(int64_t rows, int units, int per_thread, int bytes, int mo
 
 // A stretch in shared memory.
 inline uint32_t place_bytes(int e, bool wide) { return (uint32_t)(32 * e + (wide ? 0 : 1)) * 16u; }
+// `units` of a row among threads of `per_thread` each: every one is there.
+inline bool all_full(int units, int cols, int per_thread) { return units % (32 * per_thread) == 0 && cols == units * kUnit; }
 // Whether the rows of all matrices start on 16-byte boundaries (strides in bytes; an absent one does not count).
 inline bool all_wide(std::initializer_list<std::pair<const void*, int64_t>> matrices) {
   uintptr_t bits = 0;
