@@ -208,51 +208,64 @@ struct DequantParams {
 };
 
 // value * scale has at most seven bits; a row scale that is a power of two keeps it exact within fp32's range.
+// A thread takes a unit of a column of units, two rows at a time.
 template <typename T, int BLOCK>
 __global__ void __launch_bounds__(256) dequantize_fp4_kernel(const __grid_constant__ DequantParams p) {
+  constexpr int UN = 2;
   const int unit = (int)blockIdx.x * (int)blockDim.x + (int)threadIdx.x;
   const int e = unit * kUnit;
   sm100::grid_dependency_wait();
   sm100::grid_launch_dependents();
   const int n = (int)min((int64_t)kUnit, p.cols - e);
-  for (int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row < p.rows; row += (int64_t)gridDim.y * blockDim.y) {
-    uint32_t q[2] = {0u, 0u};
-    float s = 0.f, g = 1.f;
-    if (n > 0) {
-      const uint8_t* const at = p.values + row * p.ldv + unit * 8;
-      if (n == kUnit && (reinterpret_cast<uintptr_t>(at) & 7) == 0) {
-        const uint2 u = *reinterpret_cast<const uint2*>(at);
-        q[0] = u.x;
-        q[1] = u.y;
-      } else {
+  const int64_t step = (int64_t)gridDim.y * blockDim.y;
+  for (int64_t row0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; row0 < p.rows; row0 += UN * step) {
+    uint32_t q[UN][2], code[UN];
+    float g[UN];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (2 * j < n) q[j / 4] |= (uint32_t)at[j] << (8 * (j & 3));
+    for (int u = 0; u < UN; ++u) {
+      const int64_t row = row0 + u * step;
+      q[u][0] = q[u][1] = code[u] = 0u;
+      g[u] = 1.f;
+      if (n > 0 && row < p.rows) {
+        const uint8_t* const at = p.values + row * p.ldv + unit * 8;
+        if (n == kUnit && (reinterpret_cast<uintptr_t>(at) & 7) == 0) {
+          const uint2 w = *reinterpret_cast<const uint2*>(at);
+          q[u][0] = w.x;
+          q[u][1] = w.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (2 * j < n) q[u][j / 4] |= (uint32_t)at[j] << (8 * (j & 3));
+        }
+        code[u] = p.scales[fp4op::scale_at(row, unit / (BLOCK / 16), p.tiles)];
+        if (p.row_scale) g[u] = p.row_scale[row];
       }
-      const uint32_t code = p.scales[fp4op::scale_at(row, unit / (BLOCK / 16), p.tiles)];
-      s = BLOCK == 16 ? fp4op::decode_e4m3(code) : fp4op::decode_e8m0(code);
-      if (p.row_scale) g = p.row_scale[row];
     }
-    rowvec::Unit<T> o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t h;
-      asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
-          : "=r"(h) : "r"(q[j / 4] >> (8 * (j & 3))));
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-      o.set2(2 * j, f.x * s * g, f.y * s * g);
+    for (int u = 0; u < UN; ++u) {
+      const int64_t row = row0 + u * step;
+      if (row >= p.rows) break;          // (whole warps)
+      const float s = BLOCK == 16 ? fp4op::decode_e4m3(code[u]) : fp4op::decode_e8m0(code[u]);
+      rowvec::Unit<T> o;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t h;
+        asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}"
+            : "=r"(h) : "r"(q[u][j / 4] >> (8 * (j & 3))));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        o.set2(2 * j, f.x * s * g[u], f.y * s * g[u]);
+      }
+      rowvec::store_unit<T>(static_cast<T*>(p.y) + row * p.ldy + e, o, n);
     }
-    rowvec::store_unit<T>(static_cast<T*>(p.y) + row * p.ldy + e, o, n);
   }
 }
 
 template <typename T>
 cudaError_t launch_back(const DequantParams& p, int block, cudaStream_t st) {
   const int64_t units = (p.cols + kUnit - 1) / kUnit;
-  int tx = 32;
-  while (tx < 256 && tx < units) tx *= 2;
+  const int64_t gx = (units + 255) / 256;
+  const int tx = (int)(((units + gx - 1) / gx + 31) / 32 * 32);      // even parts of the row
   const int ty = 256 / tx;
-  const int64_t gx = (units + tx - 1) / tx;
   int64_t gy = (p.rows + ty - 1) / ty;
   const int64_t most = (148 * 32 + gx - 1) / gx;
   if (gy > most) gy = most;
