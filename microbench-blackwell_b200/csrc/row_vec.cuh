@@ -180,9 +180,19 @@ __device__ __forceinline__ void store_aligned(uint8_t* p, const Unit<T>& u, int 
   }
 }
 
+// Bytes [from, to) of the 16 at q, from words: at most one 16-bit piece at either end, where a 16-bit element ends there.
+__device__ __forceinline__ void store_part(uint8_t* q, const uint32_t* w, uint32_t from, uint32_t to) {
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    if (from <= 4 * j && 4 * j + 4 <= to) *reinterpret_cast<uint32_t*>(q + 4 * j) = w[j];
+    else if (from <= 4 * j && 4 * j + 2 == to) *reinterpret_cast<uint16_t*>(q + 4 * j) = (uint16_t)w[j];
+    else if (from == 4 * j + 2 && 4 * j + 4 <= to) *reinterpret_cast<uint16_t*>(q + 4 * j + 2) = (uint16_t)(w[j] >> 16);
+  }
+}
+
 // Elements [0, n) of the units of a warp, called by all of its lanes; lane l + 1's unit follows lane l's in the
-// row (in other lanes' rows nothing is assumed).  Off 16-byte boundaries a lane also writes the end of the
-// unit before it, so that whole blocks are written; only at both ends of the warp's stretch elements are.
+// row (of other lanes' rows nothing is assumed).  Off 16-byte boundaries a lane also writes the end of the
+// unit before it, so that whole blocks are written; only at both ends of the warp's stretch, and at the row's end, parts are.
 template <typename T>
 __device__ __forceinline__ void store_unit(T* ptr, const Unit<T>& u, int n) {
   constexpr int W = Unit<T>::W, B = W / 4, E = (int)sizeof(T);
@@ -199,18 +209,26 @@ __device__ __forceinline__ void store_unit(T* ptr, const Unit<T>& u, int n) {
   for (int j = 0; j < W; ++j) w[4 + j] = u.w[j];
   const int head = (16 - (int)off) / E;      // own elements in the block that begins in the unit before
   const int lane = (int)(threadIdx.x & 31u);
-  shift_words<W>(w, 16u - off);              // words of the blocks from p - off
-  const bool first_whole = lane > 0 && n >= head;                 // the unit before a valid one is full
-  if (n > 0 && !first_whole) store_elements<T>(ptr, u, 0, min(n, head));
+  uint8_t* const q = p - off;
+  shift_words<W>(w, 16u - off);              // words of the blocks from q
+  if (n >= kUnit) {
+    if (lane > 0) *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+    else store_part(q, w, off, 16u);
 #pragma unroll
-  for (int j = 0; j < B; ++j) {
-    const bool whole = j == 0 ? first_whole : n >= head + 16 / E * j;
-    if (whole) *reinterpret_cast<uint4*>(p - off + 16 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    for (int j = 1; j < B; ++j) *reinterpret_cast<uint4*>(q + 16 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    if (lane == 31 || n - kUnit < head) {    // the next lane has nothing, or not enough, to fill the block with
+      uint32_t t[8] = {u.w[W - 4], u.w[W - 3], u.w[W - 2], u.w[W - 1], 0u, 0u, 0u, 0u};
+      shift_words<4>(t, 16u - off);
+      store_part(q + 16 * B, t, 0u, off);
+    }
+  } else if (n > 0) {
+    int done = 0;
+    if (lane > 0 && n >= head) {             // the unit before is full
+      *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+      done = head;
+    }
+    store_elements<T>(ptr, u, done, n);
   }
-  // What of this unit lies beyond its last whole block: the next lane writes it, if that has enough to fill the block.
-  const int whole_end = n < head ? n : min(kUnit - (16 / E - head), head + (n - head) / (16 / E) * (16 / E));
-  const bool next_writes = lane < 31 && n >= kUnit && n - kUnit >= head;
-  if (n > whole_end && !next_writes) store_elements<T>(ptr, u, whole_end, min(n, kUnit));
 }
 
 }  // namespace rowvec
