@@ -41,11 +41,13 @@ struct NormParams {
   int32_t param32;             // the vectors are fp32 (else of T)
   int32_t vectors_at;          // many rows: byte of the vectors in shared memory
   int32_t block;               // of the 4-bit form
+  float rest;                  // what is left to multiply with where gate scale is not apart
+  int32_t gate_apart;          // gate scale has a vector of its own; else (no room for three, or no gate) it is part of wp's, and scale 1, or is scale
 };
 
 // NU units to a thread, blockDim.x units apart.
 //  Few rows (NU 1): the vectors stay in registers.
-//  Many rows (NU 2, which halves what the statistics cost per element): the vectors lie in shared memory as w and wp gate scale,
+//  Many rows (NU 2, which halves what the statistics cost per element): the vectors lie in shared memory as w, wp and gate scale,
 //    in fp32, where all groups of the block read them, and up to four groups of 8192-element rows hide one another's
 //    barriers.  Rows that leave no room for them read them from the caches each time.
 // KIND 0: no y; 1: y; 2: y and a gate matrix.  (What can be absent from call to call is decided here where
@@ -54,7 +56,7 @@ template <typename T, bool FOUR, int NU, bool FULL, int KIND>
 __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ double part[2][kManyThreads / 32];
-  __shared__ float part32[2][kManyThreads / 32];
+  __shared__ uint2 part32[2][kManyThreads / 32];
   __shared__ uint32_t warp_max[kManyThreads / 32];
   constexpr int E = (int)sizeof(T);
   constexpr bool KEEP = NU == 1, SHARED = NU == 2 && E == 2, BLOCK = KIND > 0, MATRIX = KIND == 2;
@@ -94,14 +96,18 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
   };
   for (int s = 0; s < p.stages; ++s) issue(first + s * step, mine + (uint32_t)s * per_stage);
 
-  F2 vw[kUnit / 2], vk[kUnit / 2];
+  F2 vw[kUnit / 2], vp[kUnit / 2], vk[kUnit / 2];      // w, wp, gate scale
   auto load_w = [&](int i) { load_params<T>(p.w, p.param32, e[i], n[i], vw); };
   auto load_k = [&](int i) {
-    F2 g[kUnit / 2];
-    load_params<T>(p.wp, p.param32, e[i], n[i], vk);
-    load_params<T>(MATRIX ? nullptr : p.gate, p.param32, e[i], n[i], g);
+    load_params<T>(p.wp, p.param32, e[i], n[i], vp);
+    if constexpr (!MATRIX) {
+      load_params<T>(p.gate, p.param32, e[i], n[i], vk);
 #pragma unroll
-    for (int j = 0; j < kUnit / 2; ++j) vk[j] = mul2(vk[j], mul2(g[j], f2(p.scale)));
+      for (int j = 0; j < kUnit / 2; ++j) {
+        vk[j] = mul2(vk[j], f2(p.scale));
+        if (SHARED && p.gate && !p.gate_apart) vp[j] = mul2(vp[j], vk[j]);
+      }
+    }
   };
   const SharedVectors vectors = {sm100::smem_u32(slots) + (uint32_t)p.vectors_at, (uint32_t)(NU * TX) * 16u};
   if constexpr (KEEP) {
@@ -115,7 +121,8 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
         vectors.put(0, i * TX + tx, vw);
         if (BLOCK) {
           load_k(i);
-          vectors.put(1, i * TX + tx, vk);
+          vectors.put(1, i * TX + tx, vp);
+          if (!MATRIX && p.gate_apart) vectors.put(2, i * TX + tx, vk);
         }
       }
     }
@@ -125,27 +132,23 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
   int flip = 0;       // a call's buffer is written again by the second call after it, with a barrier between
   auto inverse_rms = [&](const Unit<T> (&v)[NU]) {
     double* const at = part[flip ^= 1];
+    // A thread's squares in fp32 (of 16-bit elements), the threads' in 64 bits.
     double s = 0.0;
     if constexpr (E == 4) {
 #pragma unroll
       for (int i = 0; i < NU; ++i) s += squares_wide<T>(v[i]);
-      s = across_warps(warp_sum(s), at);
+      s = group_sum(s, at);
     } else {
-      // In fp32, pairwise from a few elements up: 64 bits cost the kernel of 16-bit elements twice its instructions for a last
-      // bit of r that their results do not show.
       float f = 0.f;
 #pragma unroll
       for (int i = 0; i < NU; ++i) f += squares<T>(v[i]);
-      f = group_sum(f, part32[flip]);
-      if (!out_of_range(f)) {
-        const float m = fmaf(f, (float)p.inv_n, (float)p.eps), r = rsqrtf(m);
-        return fmaf(0.5f * r, fmaf(-m * r, r, 1.f), r);
-      } else {
+      s = group_sum_parts(f, part32[flip]);
+      if (out_of_range((float)s)) {
         group_sync();
         s = 0.0;
 #pragma unroll
         for (int i = 0; i < NU; ++i) s += squares_wide<T>(v[i]);
-        s = across_warps(warp_sum(s), at);
+        s = group_sum(s, at);
       }
     }
     return inverse_root(fma(s, p.inv_n, p.eps));
@@ -190,16 +193,25 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         if (!KEEP && !SHARED) load_k(i);
+        const bool gated = SHARED && !MATRIX && each_row(p.gate_apart);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          F2 k[2] = {vk[2 * c], vk[2 * c + 1]};
-          if (SHARED) vectors.get(1, i * TX + tx, c, k[0], k[1]);
+          F2 w[2] = {vp[2 * c], vp[2 * c + 1]}, k[2] = {vk[2 * c], vk[2 * c + 1]};
+          if (SHARED) {
+            vectors.get(1, i * TX + tx, c, w[0], w[1]);
+            if (!MATRIX) {
+              k[0] = k[1] = f2(p.rest);
+              if (gated) vectors.get(2, i * TX + tx, c, k[0], k[1]);
+            }
+          }
 #pragma unroll
           for (int l = 0; l < 2; ++l) {
             const int j = 2 * c + l;
-            if (MATRIX) k[l] = mul2(k[l], pair(gate[i], j));
+            F2 z = mul2(mul2(pair(y[i], j), q), w[l]);
+            if (MATRIX) k[l] = mul2(pair(gate[i], j), f2(p.scale));
+            z = mul2(z, k[l]);
             float a, b;
-            fma2(mul2(pair(y[i], j), q), k[l], pair(x[i], j)).get(a, b);
+            add2(pair(x[i], j), z).get(a, b);
             x[i].set2(2 * j, a, b);
           }
         }
@@ -288,7 +300,10 @@ cudaError_t launch_forward(const NormParams& p0, cudaStream_t st) {
   const int units = FOUR ? (int)p.tiles * 4 * (p.block / 16) : (p.cols + kUnit - 1) / kUnit;
   p.place = place_bytes((int)sizeof(T), FULL || rows_wide(p));
   const int two = (KIND ? 2 : 1) * NU * (int)p.place, three = two + (KIND == 2 ? NU * (int)p.place : 0);
-  const int tx = ((units + NU - 1) / NU + 31) / 32 * 32, vectors = SHARED ? tx * NU * kUnit * 4 * (KIND ? 2 : 1) : 0;
+  const int tx = ((units + NU - 1) / NU + 31) / 32 * 32, vector = SHARED ? tx * NU * kUnit * 4 : 0;
+  p.rest = p.gate ? 1.f : p.scale;
+  p.gate_apart = SHARED && KIND == 1 && p.gate && 3 * vector + two * (tx / 32) <= kSmemLimit;
+  const int vectors = vector * (KIND == 0 ? 1 : p.gate_apart ? 3 : 2);
   // A gate matrix is not copied ahead where there is no room for it (rows of more than some 14000 elements).
   p.gate_ahead = KIND == 2 && vectors + three * (tx / 32) <= kSmemLimit;
   const Shape s = shape_of(p.rows, units, NU, p.gate_ahead ? three : two, NU == 2 ? many_threads<T>() : kMaxThreads, vectors);

@@ -63,26 +63,41 @@ __device__ __forceinline__ float inverse_root(double v) {
 }
 
 // The sum over the group's threads; all of them call, with `part` alternating between calls.
-__device__ __forceinline__ float group_sum(float v, float* part) {
+__device__ __forceinline__ double group_sum(double v, double* part) {
   v = warp_sum(v);
   const int warps = (int)blockDim.x >> 5, lane = (int)(threadIdx.x & 31u);
   if (warps == 1) return v;
-  float* const mine = part + threadIdx.y * warps;
+  double* const mine = part + threadIdx.y * warps;
   if (lane == 0) mine[threadIdx.x >> 5] = v;
   group_sync();
-  return warp_sum(lane < warps ? mine[lane] : 0.f);
+  v = lane < warps ? mine[lane] : 0.0;
+  // At most 16 warps.
+#pragma unroll
+  for (int o = 8; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return __shfl_sync(0xFFFFFFFFu, v, 0);
 }
-// The sum over the group's warps of a value that the lanes of each warp hold, in 64 bits.
-__device__ __forceinline__ double across_warps(double v, double* part) {
-  const int warps = (int)blockDim.x >> 5;
-  if (warps == 1) return v;
-  double* const mine = part + threadIdx.y * warps;
-  if ((threadIdx.x & 31u) == 0) mine[threadIdx.x >> 5] = v;
-  group_sync();
-  double s[2] = {0.0, 0.0};
-#pragma unroll 4
-  for (int i = 0; i < warps; ++i) s[i & 1] += mine[i];
-  return s[0] + s[1];
+
+// The same for fp32 parts >= 0, in whole numbers of a unit that goes by the largest part: 25 bits of each, so some 2^-28 of the
+// sum are lost, and the hardware's integer reductions take a fraction of the time of a tree of shuffles (of 64 bits
+// above all: 16384 x 8192 bf16 into a 4-bit operand @s1@ us with those, @s2@ with fp32 shuffles, @s3@ with these).
+// A NaN or an infinity gives NaN.
+__device__ __forceinline__ double group_sum_parts(float f, uint2* part) {
+  const int warps = (int)blockDim.x >> 5, lane = (int)(threadIdx.x & 31u);
+  // f = i 2^(e - 151)
+  uint32_t e = max(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f)) >> 23, 24u);
+  uint32_t t = __reduce_add_sync(0xFFFFFFFFu, __float2uint_rn(f * __uint_as_float((278u - e) << 23)));
+  if (warps > 1) {
+    uint2* const mine = part + threadIdx.y * warps;
+    if (lane == 0) mine[threadIdx.x >> 5] = make_uint2(t, e);
+    group_sync();
+    const uint2 w = lane < warps ? mine[lane] : make_uint2(0u, 0u);
+    e = __reduce_max_sync(0xFFFFFFFFu, w.y);
+    const uint32_t down = min(4u + e - w.y, 31u);                             // at most 16 warps of less than 2^30
+    t = __reduce_add_sync(0xFFFFFFFFu, (w.x + (1u << (down - 1u))) >> down);
+    e += 4u;
+  }
+  if (e >= 255u) return __longlong_as_double(0x7FF8000000000000ll);
+  return (double)t * __hiloint2double((int)((e + 1023u - 151u) << 20), 0);
 }
 
 // ----------------------------------------------------------------- vectors

@@ -230,8 +230,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
         if constexpr (POST) sy += squares_wide<T>(get(Y, i));
       }
       group_sync();
-      sx = across_warps(warp_sum(sx), sums.wide[0]);
-      sy = across_warps(warp_sum(sy), sums.wide[1]);
+      sx = group_sum(sx, sums.wide[0]);
+      sy = group_sum(sy, sums.wide[1]);
       const float r = inverse_root(fma(sx, p.inv_n, p.eps)), q = POST ? inverse_root(fma(sy, p.inv_n, p.eps)) : 1.f;
       const float back = r * r * r * (c.y * inv_n);
       c = make_float4(r, q, back, q * q * q * ((c.z + r * b2 - back * b3) * inv_n));
