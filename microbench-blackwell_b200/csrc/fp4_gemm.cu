@@ -170,7 +170,9 @@ __device__ __forceinline__ void stage_tokens(const Fp4Params& p, uint32_t tok, u
   }
   __syncwarp();
   named_bar_sync(2, N);
-  if (tid < p.m) st_shared_u32(sa_s + 4u * tid, __float_as_uint(fp4op::row_scale(top[tid]).scale));
+  // Each of the epilogue's warps writes them for itself (the same values).
+  const int who = tid & 31;
+  if (tid < 128 && who < p.m) st_shared_u32(sa_s + 4u * who, __float_as_uint(fp4op::row_scale(top[who]).scale));
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int u = i * N + tid, t = min(u / width, kFusedTokens - 1), unit = u - u / width * width;
