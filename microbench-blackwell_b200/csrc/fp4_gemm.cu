@@ -20,6 +20,10 @@
 //                  ring fills with weights, 12 warps find the tokens' maxima and
 //                  quantise the CTA's part of them straight into the swizzled
 //                  operand and its scale tiles, which stay in shared memory for all of its tiles.
+//
+// Measured on B200 (from graphs): 8192 x 28672 x 8192 in 773 to 820 us at the clock that the power cap leaves (4.7 to 5.0
+// PFLOP/s), 4096 x 8192 x 8192 in 116 (4.75); 48 x 28672 x 8192 in 26.5, its 132 MB at 5 of the 6.55 TB/s that a copy
+// reaches; one token x 8192 x 8192 in 10.0 in one launch, of which some 4 are launch, first loads and last stores.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -783,7 +787,8 @@ int sm_count() {
   return sms;
 }
 
-// Fused form: CTAs that share a tile of 128 channels.
+// Fused form: CTAs that share a tile of 128 channels.  64 to 128 CTAs stream at HBM's rate, and a part has at least 8 atoms of
+// K (1 x 8192 x 8192: 10.0 us in 2 parts).
 int fused_split(int64_t tiles, int64_t kb) {
   int s = 1;
   while (s < 4 && tiles * s * 2 <= 128 && kb >= 2 * s * 8) s *= 2;
@@ -796,7 +801,9 @@ int fused_split(int64_t tiles, int64_t kb) {
 // from L2 at some 64 a cycle, whichever is more; all of them cannot beat HBM (3400 bytes a cycle); the last
 // tile's epilogue follows, 11 cycles a token.  A split of K over up to 8 CTAs (one wave; the GPU
 // holds few clusters of 8 at a time) adds the exchange of the partial tiles.  Tiles of fewer than 128 tokens
-// take all tokens at once (their scales begin with a tile of 128 rows).
+// take all tokens at once (their scales begin with a tile of 128 rows).  Over 45 problems of 16 to 400 tokens the choice is within 4 %
+// of the best candidate in 37 (48 x 28672 x 8192: 26.4 us with 64 tokens, 27.5 in pairs; 64 x 1000 x 8000: 5.8 in 8 parts, 6.2 in 4,
+// 8.3 in 2).  Farthest off are 192 and 256 x 4096 x 4096: 8.3 us in pairs, 7.5 with single CTAs of 128.
 void choose(const Fp4GemmArgs* a, int num_sms, int& cg, int& bn, int& split) {
   static const int kTiles[6][2] = {{1, 16}, {1, 32}, {1, 64}, {1, 128}, {2, 128}, {2, 256}};
   const int64_t kb = (a->k + kAtomK - 1) / kAtomK, sf = tiles_per_atom(a->block) * 512;
@@ -1009,7 +1016,9 @@ int launch_prepared(const Prepared& q, cudaStream_t st) {
   return GEMM_OK;
 }
 
-// Few tokens, no knob set and X of D's type: one launch.  A D that lies over the tokens (the layer's result
+// Few tokens, no knob set and X of D's type: one launch.  One token x 8192 x 8192 takes 10.6 us a call that way and 13.7 in two
+// launches, 8 tokens x 2048 x 8192 6.5 and 8.3.  (From a graph, where a launch costs less than every CTA's own
+// quantisation, 6.2 and 5.8 for the latter: a knob makes two launches of it.)  A D that lies over the tokens (the layer's result
 // replaces them) needs two launches, the tokens being quantised before the first store.
 bool use_fused(const Fp4GemmArgs& a, const void* x, int32_t x_type, int64_t ldx) {
   if (a.m > kFusedTokens || a.m < 1 || a.n < 1 || a.k < 1 || a.k > kFusedElems) return false;

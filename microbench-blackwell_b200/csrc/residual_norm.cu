@@ -3,6 +3,10 @@
 // the result becomes a 4-bit operand.
 //
 //   z = y r(y) wp,  x' = x + (gate scale) z,  h = x' r(x') w,  r(v) = 1 / sqrt(mean(v^2) + eps)
+//
+// Measured on B200: 16384 x 8192 bf16 with gate and fp32 vectors 174 to 200 us a call (5.4 to 6.2 of the 6.55 TB/s that a copy
+// reaches: the same build gives either, as the memory serves four streams), from fp32 398 us; into a 4-bit operand 206 us, bound by
+// issue slots (62 % busy); one row 3.9 and 4.2 us, launch included.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -48,8 +52,8 @@ struct NormParams {
 // NU units to a thread, blockDim.x units apart.
 //  Few rows (NU 1): the vectors stay in registers.
 //  Many rows (NU 2, which halves what the statistics cost per element): the vectors lie in shared memory as w, wp and gate scale,
-//    in fp32, where all groups of the block read them, and up to four groups of 8192-element rows hide one another's
-//    barriers.  Rows that leave no room for them read them from the caches each time.
+//    in fp32, where all groups of the block read them, and three groups of 8192-element rows hide one another's
+//    barriers (292 us; with the vectors in the registers of one group 353).  Rows that leave no room for them read them from the caches each time.
 // KIND 0: no y; 1: y; 2: y and a gate matrix.  (What can be absent from call to call is decided here where
 // the compiler would otherwise make a copy of the loop for each case, with the registers of all.)
 template <typename T, bool FOUR, int NU, bool FULL, int KIND>

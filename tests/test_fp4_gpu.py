@@ -418,6 +418,36 @@ def test_a_wait_that_runs_out_is_reported(pkg, cuda, knobs):
     assert pkg.read_status(status.data_ptr(), torch.cuda.current_stream().cuda_stream)[0] == pkg.OK
 
 
+def test_offsets_beyond_32_bits(pkg, cuda):
+    """The last rows of matrices of more than 2^31 elements are those of a small call."""
+    x = torch.zeros((140000, 16384), dtype=torch.bfloat16, device="cuda")
+    x[-5:] = normal((5, 16384), 1, torch.bfloat16)
+    f = pkg.quantize_fp4(x)
+    small = pkg.quantize_fp4(x[-5:])
+    assert torch.equal(f.values[-5:], small.values) and torch.equal(f.row_scale[-5:], small.row_scale)
+    del x
+    y = pkg.dequantize_fp4(f)
+    assert torch.equal(y[-5:], pkg.dequantize_fp4(small)) and not y[:100].any()
+    del y, f
+    w = pkg.quantize_fp4(normal((32776, 256), 2), block=32)
+    a = pkg.quantize_fp4(normal((70001, 256), 3), block=32)
+    d = pkg.gemm_fp4(a, w)
+    last = pkg.quantize_fp4(normal((70001, 256), 3)[-6:], block=32)
+    check_sum(d[-6:], stands_for(last, pkg), stands_for(w, pkg))
+
+
+def test_a_graph_captured_before_any_other_call_of_its_size(pkg, cuda):
+    w = pkg.quantize_fp4(normal((333, 1777), 1, scale=0.05), block=32)
+    for m in (3, 77):
+        x = normal((m, 1777), 2, torch.float16)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = pkg.linear_fp4(x, w)
+        graph.replay()
+        check_sum(y, stands_for(pkg.quantize_fp4(x, block=32), pkg), stands_for(w, pkg))
+
+
 def test_refusals_in_python(pkg, cuda):
     w = pkg.quantize_fp4(normal((30, 64), 1))
     x = normal((4, 64), 2, torch.bfloat16)

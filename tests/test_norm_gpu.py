@@ -432,6 +432,42 @@ def test_two_streams(pkg, cuda):
             assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
 
 
+def test_operands_that_are_one_tensor(pkg, cuda):
+    """The same matrix as x, y and gate, and replaced in place; the same vector everywhere."""
+    for cols in (512, 1001):
+        x, w = normal((200, cols), 1, torch.bfloat16), normal((cols,), 2, torch.bfloat16, 0.2) + 1
+        want = pkg.residual_norm(x, x.clone(), weight=w, post_weight=w.clone(), gate=x.clone())
+        got = pkg.residual_norm(x, x, weight=w, post_weight=w, gate=x)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        want = pkg.residual_norm(x, x.clone(), weight=w, post_weight=w)
+        z = x.clone()
+        got = pkg.residual_norm(z, z, weight=w, post_weight=w, out=z)
+        assert got[0] is z and torch.equal(z, want[0]) and torch.equal(got[1], want[1])
+        with pytest.raises(pkg.GemmError):
+            pkg.residual_norm(x, x, weight=w, gate=z, out=z)
+        a = pkg.residual_norm_backward(x, x, x, x, weight=w, post_weight=w, gate=x)
+        b = pkg.residual_norm_backward(x.clone(), x.clone(), x.clone(), x.clone(), weight=w, post_weight=w, gate=x.clone())
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_offsets_beyond_32_bits(pkg, cuda):
+    """The last rows of matrices of more than 2^31 elements are those of a small call."""
+    rows, cols = 131080, 16392 - 8
+    x = torch.zeros((rows, cols), dtype=torch.bfloat16, device="cuda")
+    x[-3:] = normal((3, cols), 1, torch.bfloat16)
+    w = normal((cols,), 2, torch.bfloat16, 0.2) + 1
+    want = pkg.residual_norm(x[-3:], x[-3:].clone(), weight=w, post_weight=w)
+    grads = pkg.residual_norm_backward(x[-3:], x[-3:], x[-3:], x[-3:], weight=w, post_weight=w)
+    got = pkg.residual_norm_backward(x, x, x, x, weight=w, post_weight=w)
+    size = grads.dx.float().abs().max()
+    assert (got.dx[-3:].float() - grads.dx.float()).abs().max() <= 2 ** -7 * size and (got.dy[-3:].float() - grads.dy.float()).abs().max() <= 2 ** -7 * grads.dy.float().abs().max()
+    assert (got.dweight - grads.dweight).abs().max() <= 1e-5 * grads.dweight.abs().max()
+    del got
+    got = pkg.residual_norm(x, x, weight=w, post_weight=w, out=x)
+    assert (x[-3:].float() - want[0].float()).abs().max() <= 2 ** -7 * want[0].float().abs().max()
+    assert (got[1][-3:].float() - want[1].float()).abs().max() <= 2 ** -7 * want[1].float().abs().max() and not got[1][:100].any()
+
+
 def test_refusals_in_python(pkg, cuda):
     s = case(4, 64, torch.bfloat16)
     x, y, w = s["x"], s["y"], s["weight"]
