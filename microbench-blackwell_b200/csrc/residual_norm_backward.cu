@@ -46,7 +46,7 @@ struct BackParams {
 struct BackSums {
   float part[kMaxThreads / 32][8];
   double wide[2][kMaxThreads / 32];
-  float4 row[8];                 // r, q and the two coefficients, one row to a group
+  float4 row[kMaxThreads / 32];  // r, q and the two coefficients, one row to a group
 };
 
 // Sums over the warp of eight values per lane: lane l ends with the one of index l / 4.

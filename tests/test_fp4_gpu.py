@@ -104,6 +104,14 @@ def test_quantize_exact(pkg, cuda, dtype, block, rows, cols):
     check_quantized(pkg.quantize_fp4(x, block=block), x, pkg)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(148 * 40, 600), (20000, 250), (3000, 1024), (400, 8192), (300, 8193), (200, 20000), (160, 32768), (150, 40000)])
+def test_quantize_many_rows(pkg, cuda, dtype, rows, cols):
+    """Rows that groups of threads go down, with as many groups to a block as there can be."""
+    x = normal((rows, cols), rows + cols, dtype, 3.0)
+    check_quantized(pkg.quantize_fp4(x, block=16 if rows % 3 else 32), x, pkg)
+
+
 @pytest.mark.parametrize("block", [16, 32])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_quantize_borders(pkg, cuda, dtype, block):

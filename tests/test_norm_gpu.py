@@ -281,6 +281,21 @@ def test_backward(pkg, cuda, dtype, rows, cols):
     check_backward(pkg, s, dh, dx, x_out)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [1, 16, 100, 512, 513, 1024, 2000])
+def test_many_short_rows(pkg, cuda, dtype, cols):
+    """As many groups to a block as there can be."""
+    rows = 148 * 33 + 5
+    for gate in ("vector", "matrix"):
+        s = case(rows, cols, dtype, True, gate)
+        x_out, dh, dx = (normal((rows, cols), 20 + i, dtype) for i in range(3))
+        check_forward(pkg, s, call(pkg, s))
+        check_backward(pkg, s, dh, dx, x_out)
+    _, f = call(pkg, s, fp4=32)
+    x_out, _ = call(pkg, s)
+    check_four_bits(f, x_out.double() * rms(x_out.double(), 1e-6) * s["weight"].double(), 32)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,cols", [(30, 1001), (170, 8192), (20, 16384)])
 def test_backward_fp32_weights(pkg, cuda, dtype, rows, cols):
