@@ -76,7 +76,6 @@ template <typename T, int NU, bool HELD, bool FULL, int KIND>
 __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(const __grid_constant__ BackParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ BackSums sums;
-  float* const held = reinterpret_cast<float*>(slots);       // [2][cols rounded up to units]
   constexpr int E = (int)sizeof(T);
   constexpr bool BLOCK = KIND > 0, POST = KIND == 2 || KIND == 4, MATRIX = KIND > 2, SHARED = NU == 2 && !HELD;
   enum { X, DH, DX, Y, G };
@@ -85,10 +84,26 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
   const uint32_t per_stage = (uint32_t)((BLOCK ? 4 : 3) + (MATRIX ? 1 : 0)) * NU * p.place;
   const uint32_t mine = sm100::smem_u32(slots) + (uint32_t)((int)threadIdx.y * (TX >> 5) + (tx >> 5)) * (uint32_t)p.stages * per_stage;
   auto unit_at = [&](int i) { return (i * TX + tx) * kUnit; };
+  // Column sums in shared memory (HELD, and in the end): planes of four elements, one slot more apart than there are units, for
+  // the banks.
+  const SharedVectors columns = {sm100::smem_u32(slots), (uint32_t)(width / kUnit + 1) * 16u};
   if constexpr (HELD) {
-    for (int i = tx; i < 2 * width; i += TX) held[i] = 0.f;
-    __syncthreads();
+    const F2 none[kUnit / 2] = {f2(0.f), f2(0.f), f2(0.f), f2(0.f), f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+      if (unit_at(i) < p.cols) {       // a unit's sums are its thread's own
+        columns.put(0, i * TX + tx, none);
+        columns.put(1, i * TX + tx, none);
+      }
   }
+  auto add_held = [&](int which, int i, F2 (&v)[kUnit / 2]) {
+    if (unit_at(i) >= p.cols) return;
+    F2 before[kUnit / 2];
+    columns.get(which, i * TX + tx, before);
+#pragma unroll
+    for (int j = 0; j < kUnit / 2; ++j) v[j] = add2(before[j], v[j]);
+    columns.put(which, i * TX + tx, v);
+  };
   sm100::grid_dependency_wait();
   sm100::grid_launch_dependents();
   const int64_t first = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, step = (int64_t)gridDim.x * blockDim.y;
@@ -257,18 +272,14 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
         for (int j = 0; j < kUnit / 2; ++j) {
           const F2 xv = pair(x, j), dv = pair(dh, j);
           g[j] = fma2(r, mul2(dv, vw[j]), fma2(back, xv, pair(d, j)));
-          if constexpr (HELD) {
-            float a, b;
-            mul2(dv, mul2(xv, r)).get(a, b);
-            if (e + 2 * j < width) { held[e + 2 * j] += a; held[e + 2 * j + 1] += b; }
-          } else {
-            cw[i][j] = fma2(dv, mul2(xv, r), cw[i][j]);
-          }
+          if constexpr (HELD) cw[i][j] = mul2(dv, mul2(xv, r));
+          else cw[i][j] = fma2(dv, mul2(xv, r), cw[i][j]);
           float a, b;
           g[j].get(a, b);
           o.set2(2 * j, a, b);
         }
       }
+      if constexpr (HELD) add_held(0, i, cw[i]);
       put_unit<T, FULL>(out_x + e * E, o, p.cols - e);
       if constexpr (BLOCK) {
         if constexpr (SHARED) vectors.get(1, i * TX + tx, vk);
@@ -287,16 +298,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
             t = mul2(t, k);
             gv = mul2(gv, mul2(k, f2(p.scale)));
           }
-          if constexpr (HELD) {
-            mul2(gv, yn).get(a, b);
-            if (e + 2 * j < width) { held[width + e + 2 * j] += a; held[width + e + 2 * j + 1] += b; }
-          } else {
-            cs[i][j] = fma2(gv, yn, cs[i][j]);
-          }
+          if constexpr (HELD) cs[i][j] = mul2(gv, yn);
+          else cs[i][j] = fma2(gv, yn, cs[i][j]);
           if constexpr (POST) t = fma2(q, t, mul2(back2, yv));
           t.get(a, b);
           o.set2(2 * j, a, b);
         }
+        if constexpr (HELD) add_held(1, i, cs[i]);
         put_unit<T, FULL>(out_y + e * E, o, p.cols - e);
         if constexpr (MATRIX)
           if (each_row(p.dgate)) put_unit<T, FULL>(row_of(p.dgate, row, p.lddg) + e * E, og, p.cols - e);
@@ -308,8 +316,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
     }
     if (++stage == p.stages) stage = 0;
   }
-  // ---- this block's column sums (planes of four elements one slot more apart than they have units, for the banks)
-  const SharedVectors columns = {sm100::smem_u32(slots), (uint32_t)(width / kUnit + 1) * 16u};
+  // ---- this block's column sums
   wait_copies(0);
   __syncthreads();
   if constexpr (!HELD) {
@@ -343,15 +350,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
   for (int which = 0; which < 2; ++which) {
     for (int q = me; 4 * q < p.cols; q += all) {
       float f[4];
-      if constexpr (HELD) {
-#pragma unroll
-        for (int l = 0; l < 4; ++l) f[l] = held[which * width + 4 * q + l];
-      } else {
-        F2 a, b;
-        columns.get(which, q >> 2, q & 3, a, b);
-        a.get(f[0], f[1]);
-        b.get(f[2], f[3]);
-      }
+      F2 a, b;
+      columns.get(which, q >> 2, q & 3, a, b);
+      a.get(f[0], f[1]);
+      b.get(f[2], f[3]);
 #pragma unroll
       for (int l = 0; l < 4; ++l)
         if (4 * q + l < p.cols) out[which * p.cols + 4 * q + l] = f[l];
@@ -405,7 +407,7 @@ Shape back_shape(int type, int64_t rows, int64_t cols, int bytes) {
   const int units = (int)((cols + kUnit - 1) / kUnit);
   if (units > kMaxThreads) {
     Shape s;
-    s.tx = kMaxThreads; s.ty = 1; s.stages = 0;
+    s.tx = ((units + 1) / 2 + 31) / 32 * 32; s.ty = 1; s.stages = 0;
     s.blocks = (int)(rows < 148 ? rows : 148);
     s.smem = (size_t)units * kUnit * 8;
     return s;
