@@ -564,8 +564,7 @@ int gemm_sm100a_fp4_linear_workspace(const Fp4GemmArgs* args, const void* x, int
  *   x_out = x + (gate * scale) * z                          rounded to `type`
  *   h     = x_out * r(x_out) * weight                       of the rounded x_out
  *   r(v)  = 1 / sqrt(mean(v^2) + eps) of a row
- * One fp32 operation after the other, from left to right; the mean to 2^-27 or so (16-bit rows) or in 64 bits
- * (fp32 rows, and wherever squares leave fp32's range).
+ * One fp32 operation after the other, from left to right; the mean in 64 bits (2^-40 or better of its value).
  * x, y, x_out, h and a gate matrix are of `type`, rows x cols with their own strides (elements), any alignment of
  * that type; weight, post_weight and a gate vector (ldg = 0) have cols elements of param_type: `type` or fp32.
  * weight NULL: 1.  gate NULL: 1.  y NULL: x_out is x, which is not written again (x_out NULL too).

@@ -60,7 +60,7 @@ template <typename T, bool FOUR, int NU, bool FULL, int KIND>
 __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ double part[2][kManyThreads / 32];
-  __shared__ uint2 part32[2][kManyThreads / 32];
+  __shared__ WarpSum part32[2][kManyThreads / 32];
   __shared__ uint32_t warp_max[kManyThreads / 32];
   constexpr int E = (int)sizeof(T);
   constexpr bool KEEP = NU == 1, SHARED = NU == 2 && E == 2, BLOCK = KIND > 0, MATRIX = KIND == 2;
@@ -136,17 +136,15 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
   int flip = 0;       // a call's buffer is written again by the second call after it, with a barrier between
   auto inverse_rms = [&](const Unit<T> (&v)[NU]) {
     double* const at = part[flip ^= 1];
-    // A thread's squares in fp32 (of 16-bit elements), the threads' in 64 bits.
     double s = 0.0;
     if constexpr (E == 4) {
 #pragma unroll
       for (int i = 0; i < NU; ++i) s += squares_wide<T>(v[i]);
       s = group_sum(s, at);
     } else {
-      float f = 0.f;
-#pragma unroll
-      for (int i = 0; i < NU; ++i) f += squares<T>(v[i]);
-      s = group_sum_parts(f, part32[flip]);
+      float hi, lo;
+      squares<T, NU>(v, hi, lo);
+      s = group_sum_parts(hi, lo, part32[flip]);
       if (out_of_range((float)s)) {
         group_sync();
         s = 0.0;

@@ -35,12 +35,33 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
 }
-template <typename T>
-__device__ __forceinline__ float squares(const Unit<T>& u) {
-  F2 s = f2(0.f);
+// s + x^2 for the 64-bit number x with these upper 32 bits and zeros below them.
+__device__ __forceinline__ void add_square(double& s, uint32_t upper) {
+  asm volatile("{\n\t.reg .f64 x;\n\tmov.b64 x, {%2, %1};\n\tfma.rn.f64 %0, x, x, %0;\n\t}" : "+d"(s) : "r"(upper), "r"(0));
+}
+// Sum of a thread's squares of 16-bit elements in 64 bits, as hi + lo, |lo| <= 2^-24 hi.  (In fp32 a row whose mean one
+// channel makes up loses 2^-20 of it, and the last bit of r turns elements of x_out and codes of a 4-bit operand.)  The numbers are put
+// together from the elements' bits, exponents moved by 896: conversions would take longer than all the rest
+// (16384 x 8192 bf16: 333 us with them, 170 without; 193 with sums of paired fp32).  A zero or a subnormal bf16 counts as
+// some 2^-127, whose square is nothing beside the least sum that is used (out_of_range).
+template <typename T, int NU>
+__device__ __forceinline__ void squares(const Unit<T> (&u)[NU], float& hi, float& lo) {
+  double s0 = 0.0, s1 = 0.0;
 #pragma unroll
-  for (int j = 0; j < kUnit / 2; ++j) s = fma2(pair(u, j), pair(u, j), s);
-  return both(s);
+  for (int i = 0; i < NU; ++i)
+#pragma unroll
+    for (int j = 0; j < Unit<T>::W; ++j) {
+      if constexpr (std::is_same<T, __half>::value) {
+        add_square(s0, (__float_as_uint(fabsf(u[i].get(2 * j))) >> 3) + 0x38000000u);
+        add_square(s1, (__float_as_uint(fabsf(u[i].get(2 * j + 1))) >> 3) + 0x38000000u);
+      } else {
+        add_square(s0, ((u[i].w[j] & 0x7FFFu) << 13) + 0x38000000u);
+        add_square(s1, ((u[i].w[j] & 0x7FFF0000u) >> 3) + 0x38000000u);
+      }
+    }
+  const double s = s0 + s1;
+  hi = (float)s;
+  lo = (float)(s - (double)hi);
 }
 template <typename T>
 __device__ __forceinline__ double squares_wide(const Unit<T>& u) {
@@ -49,7 +70,7 @@ __device__ __forceinline__ double squares_wide(const Unit<T>& u) {
   for (int j = 0; j < kUnit; ++j) s = fma((double)u.get(j), (double)u.get(j), s);
   return s;
 }
-// Where the fp32 part of a sum of squares may have left its range (or come near its end), 64 bits do it again.
+// Where a sum of squares may have left its parts' range in fp32 (or come near its end), it is taken again, all in 64 bits.
 __device__ __forceinline__ bool out_of_range(float s) { return !(s > 1e-30f && s < 1e38f); }
 
 // 1 / sqrt(v), rounded to fp32 from an error of 2^-43 or so: one Newton step whose 1 - v r^2 has v and r^2 in two fp32
@@ -77,27 +98,35 @@ __device__ __forceinline__ double group_sum(double v, double* part) {
   return __shfl_sync(0xFFFFFFFFu, v, 0);
 }
 
-// The same for fp32 parts >= 0, in whole numbers of a unit that goes by the largest part: 25 bits of each, so some 2^-28 of the
-// sum are lost, and the hardware's integer reductions take a fraction of the time of a tree of shuffles (16384 x 8192 bf16
-// into a 4-bit operand: 235 us with shuffles of 64 bits, 223 with these).
+// The same for parts hi + lo >= 0 as above, in whole numbers of 2^-50 of a unit that goes by the largest part: 25 bits of
+// hi and what is left of it with lo, so that 2^-45 of the sum are lost, and the hardware's integer reductions take a fraction of the
+// time of a tree of 64-bit shuffles.
 // A NaN or an infinity gives NaN.
-__device__ __forceinline__ double group_sum_parts(float f, uint2* part) {
+struct WarpSum {
+  uint64_t sum;      // < 2^55
+  uint32_t e;
+};
+__device__ __forceinline__ double group_sum_parts(float hi, float lo, WarpSum* part) {
   const int warps = (int)blockDim.x >> 5, lane = (int)(threadIdx.x & 31u);
-  // f = i 2^(e - 151)
-  uint32_t e = max(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f)) >> 23, 24u);
-  uint32_t t = __reduce_add_sync(0xFFFFFFFFu, __float2uint_rn(f * __uint_as_float((278u - e) << 23)));
+  // hi + lo = (i + j / 2^25) 2^(e - 151)
+  uint32_t e = max(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(hi)) >> 23, 24u);
+  const float unit = __uint_as_float((278u - e) << 23), f = hi * unit;
+  const uint32_t i = __float2uint_rn(f);
+  const int j = __float2int_rn(fmaf(lo, unit, f - (float)i) * 0x1p25f);
+  uint64_t sum = ((uint64_t)__reduce_add_sync(0xFFFFFFFFu, i) << 25) + (uint64_t)(int64_t)__reduce_add_sync(0xFFFFFFFFu, j);
   if (warps > 1) {
-    uint2* const mine = part + threadIdx.y * warps;
-    if (lane == 0) mine[threadIdx.x >> 5] = make_uint2(t, e);
+    WarpSum* const mine = part + threadIdx.y * warps;
+    if (lane == 0) mine[threadIdx.x >> 5] = {sum, e};
     group_sync();
-    const uint2 w = lane < warps ? mine[lane] : make_uint2(0u, 0u);
-    e = __reduce_max_sync(0xFFFFFFFFu, w.y);
-    const uint32_t down = min(4u + e - w.y, 31u);                             // at most 16 warps of less than 2^30
-    t = __reduce_add_sync(0xFFFFFFFFu, (w.x + (1u << (down - 1u))) >> down);
-    e += 4u;
+    const WarpSum w = lane < warps ? mine[lane] : WarpSum{0ull, 0u};
+    e = __reduce_max_sync(0xFFFFFFFFu, w.e);
+    sum = w.sum >> min(e - w.e, 63u);
+    // At most 16 warps.
+    const uint32_t up = __reduce_add_sync(0xFFFFFFFFu, (uint32_t)(sum >> 28)), low = __reduce_add_sync(0xFFFFFFFFu, (uint32_t)sum & 0xFFFFFFFu);
+    sum = ((uint64_t)up << 28) + low;
   }
   if (e >= 255u) return __longlong_as_double(0x7FF8000000000000ll);
-  return (double)t * __hiloint2double((int)((e + 1023u - 151u) << 20), 0);
+  return (double)sum * __hiloint2double((int)((e + 1023u - 176u) << 20), 0);
 }
 
 // ----------------------------------------------------------------- vectors
