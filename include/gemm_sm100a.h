@@ -601,6 +601,8 @@ int gemm_sm100a_residual_norm(const ResidualNormArgs* args, void* stream);
  * of `type`, and the fp32 sums over rows dweight, dpost_weight and, for a gate vector, dgate; a gate
  * matrix has dgate of `type` (lddg).  y NULL: no dy, dpost_weight, dgate.  dweight, dpost_weight and dgate may be NULL
  * (not wanted).  The same call takes its sums in the same order.  rows = 0 sets the fp32 sums to 0.
+ * Sums over a row or over rows are fp32, of fp32 rows too (a few 2^-24 of what they add up); those of a row far from one, whose
+ * squares sum to 1e20 or more (or, with an eps below 1e-12, to 1e-20 or less) or whose products leave fp32's range, are 64-bit.
  * workspace: gemm_sm100a_residual_norm_workspace(rows, cols) bytes, 16-byte aligned, of this call alone until it has
  * run.  Outputs overlap nothing.
  */

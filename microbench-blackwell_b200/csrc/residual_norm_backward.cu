@@ -1,11 +1,11 @@
 // residual_norm_backward.cu -- gradients of the residual stream around a block (residual_norm.cu).  Bound by the bytes of
 // six matrices.
 //
-// With n columns, dn = dh w, k = gate scale, P = k wp y, r = r(x'), q = r(y):
-//   g  = dx' + r dn - x' r^3 (sum dn x') / n
-//   dy = q (k wp g - y q^2 (sum P g) / n)
-//   sum P g = sum P dx' + r sum P dn - r^3 (sum dn x') / n sum P x'
-// so that all row sums (with those of x'^2 and y^2) come from one pass and one exchange, and no statistics are
+// With c columns, dn = dh w, k = gate scale, P = k wp y, r = r(x'), q = r(y), n = x' r, m = y q:
+//   g  = dx' + r (dn - a n)                a = mean(dn n) = r (sum dn x') / c
+//   dy = q (k wp g - b m)                  b = q mean(P g) = q (sum P g) / c
+//   sum P g = sum P dx' + r (sum P dn - a (r sum P x'))
+// (with n and m, whatever the rows' magnitude; r^3 and q^3 would leave fp32's range long before the gradients do), so that all row sums (with those of x'^2 and y^2) come from one pass and one exchange, and no statistics are
 // kept from the forward call.  The sums over rows (dw, dwp, dgate) stay with the threads of a block, which walks down the
 // matrix; the blocks' parts go through a workspace to a second kernel that adds them in order.
 //
@@ -36,6 +36,7 @@ struct BackParams {
   int32_t cols;
   float scale;
   double eps, inv_n;
+  float low, high;                       // sums of squares that fp32 holds, with what is made of them
   int32_t stages;
   uint32_t place;
   int32_t param32;
@@ -46,7 +47,7 @@ struct BackParams {
 struct BackSums {
   float part[kMaxThreads / 32][8];
   double wide[2][kMaxThreads / 32];
-  float4 row[kMaxThreads / 32];  // r, q and the two coefficients, one row to a group
+  float4 row[kMaxThreads / 32];  // r, q, a and b, one row to a group
 };
 
 // Sums over the warp of eight values per lane: lane l ends with the one of index l / 4.
@@ -228,35 +229,45 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
         t.z += __shfl_xor_sync(0xFFFFFFFFu, t.z, o);
         t.w += __shfl_xor_sync(0xFFFFFFFFu, t.w, o);
       }
-      const float b2 = __shfl_sync(0xFFFFFFFFu, t.x, 1), b3 = __shfl_sync(0xFFFFFFFFu, t.y, 1);
+      const float s4 = __shfl_sync(0xFFFFFFFFu, t.x, 1), s5 = __shfl_sync(0xFFFFFFFFu, t.y, 1);
       if (lane == 0) {
-        // r, q and the coefficients; or -1 for statistics that have to be taken in 64 bits, and what the coefficients need.
-        const bool again = out_of_range(t.x) || (POST && out_of_range(t.y));
-        const float eps = (float)p.eps, r = again ? -1.f : rsqrtf(fmaf(t.x, inv_n, eps)), q = POST && !again ? rsqrtf(fmaf(t.y, inv_n, eps)) : 1.f;
-        const float back = r * r * r * (t.z * inv_n);
-        sums.row[threadIdx.y] = again ? make_float4(-1.f, t.z, t.w, 0.f) : make_float4(r, q, back, q * q * q * ((t.w + r * b2 - back * b3) * inv_n));
-        if (again) { sums.part[first_warp][0] = b2; sums.part[first_warp][1] = b3; }
+        // r, q, a and b; or -1 for sums that have to be taken in 64 bits.
+        const float eps = (float)p.eps, r = rsqrtf(fmaf(t.x, inv_n, eps)), q = POST ? rsqrtf(fmaf(t.y, inv_n, eps)) : 1.f;
+        const float a = r * t.z * inv_n, b = q * ((t.w + r * (s4 - a * (r * s5))) * inv_n);
+        const bool held = t.x > p.low && t.x < p.high && (!POST || (t.y > p.low && t.y < p.high)) && fabsf(a) + fabsf(b) < __int_as_float(0x7F800000);
+        sums.row[threadIdx.y] = make_float4(held ? r : -1.f, q, a, b);
       }
     }
     group_sync();
     float4 c = sums.row[threadIdx.y];
     if (c.x < 0.f) {       // of the whole group
-      const float b2 = sums.part[first_warp][0], b3 = sums.part[first_warp][1];
-      double sx = 0.0, sy = 0.0;
+      double w[6] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+      auto element = [&](int m, int col) { return (double)to_f32(reinterpret_cast<const T*>(p.in[m] + row * p.ld[m])[col]); };
+      auto param = [&](const void* v, int col) {
+        return !v ? 1.f : sizeof(T) == 4 || p.param32 ? static_cast<const float*>(v)[col] : to_f32(static_cast<const T*>(v)[col]);
+      };
 #pragma unroll 1
-      for (int i = 0; i < NU; ++i) {
-        sx += squares_wide<T>(get(X, i));
-        if constexpr (POST) sy += squares_wide<T>(get(Y, i));
+      for (int col = tx; col < p.cols; col += TX) {
+        const double xv = element(X, col), dn = element(DH, col) * param(p.w, col);
+        w[0] = fma(xv, xv, w[0]);
+        w[2] = fma(dn, xv, w[2]);
+        if constexpr (POST) {
+          const double yv = element(Y, col), f = yv * param(p.wp, col) * (MATRIX ? element(G, col) : (double)param(p.gate, col)) * p.scale;
+          w[1] = fma(yv, yv, w[1]);
+          if (p.in[DX]) w[3] = fma(f, element(DX, col), w[3]);
+          w[4] = fma(f, dn, w[4]);
+          w[5] = fma(f, xv, w[5]);
+        }
       }
-      group_sync();
-      sx = group_sum(sx, sums.wide[0]);
-      sy = group_sum(sy, sums.wide[1]);
-      const float r = inverse_root(fma(sx, p.inv_n, p.eps)), q = POST ? inverse_root(fma(sy, p.inv_n, p.eps)) : 1.f;
-      const float back = r * r * r * (c.y * inv_n);
-      c = make_float4(r, q, back, q * q * q * ((c.z + r * b2 - back * b3) * inv_n));
+#pragma unroll
+      for (int k = 0; k < 6; ++k)
+        if (POST || k == 0 || k == 2) w[k] = group_sum(w[k], sums.wide[POST ? k & 1 : k / 2]);
+      const double r = 1.0 / sqrt(fma(w[0], p.inv_n, p.eps)), q = POST ? 1.0 / sqrt(fma(w[1], p.inv_n, p.eps)) : 1.0;
+      const double a = r * w[2] * p.inv_n;
+      c = make_float4((float)r, (float)q, (float)a, (float)(q * ((w[3] + r * (w[4] - a * (r * w[5]))) * p.inv_n)));
     }
     // ---- gradients
-    const F2 r = f2(c.x), q = f2(c.y), back = f2(-c.z), back2 = f2(-c.w);
+    const F2 r = f2(c.x), q = f2(c.y), minus_a = f2(-c.z), minus_b = f2(-c.w);
     uint8_t* const out_x = row_of(p.dx, row, p.lddx);
     uint8_t* const out_y = BLOCK ? row_of(p.dy, row, p.lddy) : nullptr;
 #pragma unroll
@@ -270,10 +281,10 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
         const Unit<T> x = get(X, i), dh = get(DH, i), d = get(DX, i);
 #pragma unroll
         for (int j = 0; j < kUnit / 2; ++j) {
-          const F2 xv = pair(x, j), dv = pair(dh, j);
-          g[j] = fma2(r, mul2(dv, vw[j]), fma2(back, xv, pair(d, j)));
-          if constexpr (HELD) cw[i][j] = mul2(dv, mul2(xv, r));
-          else cw[i][j] = fma2(dv, mul2(xv, r), cw[i][j]);
+          const F2 n = mul2(pair(x, j), r), dv = pair(dh, j);
+          g[j] = fma2(r, fma2(minus_a, n, mul2(dv, vw[j])), pair(d, j));
+          if constexpr (HELD) cw[i][j] = mul2(dv, n);
+          else cw[i][j] = fma2(dv, n, cw[i][j]);
           float a, b;
           g[j].get(a, b);
           o.set2(2 * j, a, b);
@@ -300,7 +311,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) residual_norm_backward_kernel(
           }
           if constexpr (HELD) cs[i][j] = mul2(gv, yn);
           else cs[i][j] = fma2(gv, yn, cs[i][j]);
-          if constexpr (POST) t = fma2(q, t, mul2(back2, yv));
+          if constexpr (POST) t = mul2(q, fma2(minus_b, yn, t));
           t.get(a, b);
           o.set2(2 * j, a, b);
         }
@@ -525,6 +536,9 @@ extern "C" int gemm_sm100a_residual_norm_backward(const ResidualNormBackwardArgs
   p.parts = static_cast<float*>(a->workspace);
   p.rows = a->rows; p.cols = (int32_t)a->cols; p.scale = a->scale; p.eps = a->eps; p.inv_n = 1.0 / (double)a->cols;
   p.param32 = a->param_type == GEMM_TYPE_FP32;
+  // Sums of squares below 1e20 leave room for products with gradients. Small ones lose what eps does not outweigh.
+  p.low = a->eps < 1e-12 ? 1e-20f : -1.f;
+  p.high = a->eps < 1e30 ? 1e20f : 0.f;
   p.place = place;
   PointerDeviceGuard guard(a->dx);
   if (!guard.ok) return GEMM_ERR_LAUNCH;

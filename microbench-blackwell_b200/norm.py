@@ -80,5 +80,6 @@ def residual_norm_backward(dh: torch.Tensor, dx_out: torch.Tensor | None, x_out:
         g = dx_out + (gradient of h towards x_out),  dx = g,  dy = (gradient of (gate * scale) * z towards y for g)
 
     dx, dy and a matrix gate's dgate have x_out's type, dweight, dpost_weight and a vector gate's dgate are fp32 sums
-    over the rows, in the same order for the same call.  No statistics are kept from the forward call."""
+    over the rows, in the same order for the same call.  No statistics are kept from the forward call; its row sums are fp32 here
+    (of fp32 rows too), 64-bit in rows whose squares or products come near the ends of fp32's range."""
     return NormGrads(*_host().residual_norm_backward(dh, dx_out, x_out, y, weight, post_weight, gate, scale, eps))

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from test_fp4_gpu import normal
-from test_norm_gpu import TYPES
+from test_norm_gpu import TYPES, case, check_backward
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,47 @@ def test_statistics_of_uneven_rows(pkg, cuda, dtype, kind, rows, cols):
         ways = [pkg.quantize_fp4(e, block=block) for e in exact]
         assert ((f.values == ways[0].values).all(1) | (f.values == ways[1].values).all(1)).all()
         assert ((f.row_scale == ways[0].row_scale) | (f.row_scale == ways[1].row_scale)).all()
+
+
+# ------------------------------------------------------------------ gradients of rows far from one
+FAR = [1.0, 1e14, 1e16, 1e20, 1e-13, 1e-20]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(72, 1000), (180, 304), (36, 9000), (36, 24)])
+@pytest.mark.parametrize("eps", [1e-6, 0.0, 1e-30, 0.5])
+def test_gradients_of_rows_far_from_one(pkg, cuda, dtype, rows, cols, eps):
+    """Rows of x_out and of y in every pair of magnitudes, within the bounds of ordinary rows: gradients of h about as
+    large as x_out (so that dx is about one where eps does not outweigh the row), and about one; with and without a gradient of x_out."""
+    far = torch.tensor(FAR, device="cuda").repeat((rows + 5) // 6)[:rows, None]
+    other = torch.tensor(FAR, device="cuda").repeat_interleave(6).repeat((rows + 35) // 36)[:rows, None]
+    for gate, post in (("vector", True), ("matrix", True), ("none", False)):
+        s = case(rows, cols, dtype, post, gate, params=torch.float32)
+        s["y"] = (normal((rows, cols), 3) * other).to(dtype)
+        x_out = (normal((rows, cols), 20) * far).to(dtype)
+        dh = normal((rows, cols), 21)
+        check_backward(pkg, s, (dh * far).to(dtype), None, x_out, eps)
+        check_backward(pkg, s, (dh * far).to(dtype), normal((rows, cols), 22, dtype), x_out, eps)
+        # dh about one: r dh y's way leaves the type where both rows are small and eps too.
+        if eps > 1e-9:
+            check_backward(pkg, s, dh.to(dtype), None, x_out, eps)
+            check_backward(pkg, s, dh.to(dtype), (normal((rows, cols), 22) / far.clamp(min=1.0)).to(dtype), x_out, eps)
+
+
+@pytest.mark.parametrize("rows,cols", [(9, 700), (200, 700), (4, 10000)])
+def test_gradients_of_far_fp16_rows(pkg, cuda, rows, cols):
+    """The ends of fp16, with an eps that outweighs none of it."""
+    far = torch.tensor([1.0, 1e4, 2e-6], device="cuda").repeat(rows)[:rows, None]
+    for eps in (0.0, 1e-6):
+        s = case(rows, cols, torch.float16, True, "vector", scale=2.0 ** -10)
+        s["y"] = (normal((rows, cols), 3) * far.flip(0)).clamp(-6e4, 6e4).half()
+        x_out = (normal((rows, cols), 20) * far).clamp(-6e4, 6e4).half()
+        check_backward(pkg, s, (normal((rows, cols), 21) * far * 2.0 ** -6).clamp(-6e4, 6e4).half(), None, x_out, eps)
+
+
+def test_large_gradients_of_ordinary_rows(pkg, cuda):
+    """Row sums that leave fp32 though the rows' squares do not."""
+    s = case(3, 600, torch.float32)
+    x_out, dh = normal((3, 600), 20) * 1e8, normal((3, 600), 21)
+    dh[1] *= 1e32
+    check_backward(pkg, s, dh, None, x_out)
