@@ -20,8 +20,8 @@
 namespace {
 
 constexpr int kManyThreads = 768;          // of a block of many rows
-template <typename T>
-constexpr int many_threads() { return sizeof(T) == 2 ? kManyThreads : kMaxThreads; }
+template <typename T, int KIND>
+constexpr int many_threads() { return sizeof(T) == 2 && KIND != 3 ? kManyThreads : kMaxThreads; }
 
 struct NormParams {
   const uint8_t* x; int64_t ldx;       // strides in bytes
@@ -45,25 +45,27 @@ struct NormParams {
   int32_t param32;             // the vectors are fp32 (else of T)
   int32_t vectors_at;          // many rows: byte of the vectors in shared memory
   int32_t block;               // of the 4-bit form
-  float rest;                  // what is left to multiply with where gate scale is not apart
-  int32_t gate_apart;          // gate scale has a vector of its own; else (no room for three, or no gate) it is part of wp's, and scale 1, or is scale
+  int32_t gate_vector;         // gate scale is a vector in shared memory (KIND 3: its first half is); else it is scale (KIND 3: in the caches)
 };
 
 // NU units to a thread, blockDim.x units apart.
 //  Few rows (NU 1): the vectors stay in registers.
-//  Many rows (NU 2, which halves what the statistics cost per element): the vectors lie in shared memory as w, wp and gate scale,
-//    in fp32, where all groups of the block read them, and three groups of 8192-element rows hide one another's
-//    barriers (292 us; with the vectors in the registers of one group 353).  Rows that leave no room for them read them from the caches each time.
-// KIND 0: no y; 1: y; 2: y and a gate matrix.  (What can be absent from call to call is decided here where
+//  Many rows (NU 2, which halves what the statistics cost per element) of 16-bit elements: the vectors lie in shared memory as w, wp and gate
+//    scale, in fp32, where all groups of the block read them, and three groups of 8192-element rows hide one another's
+//    barriers (292 us; with the vectors in the registers of one group 353).  Rows of fp32 read them from the caches each time.
+// KIND 0: no y; 1: y; 2: y and a gate matrix; 3: y and a gate vector of 16-bit rows that shared memory has no room for (more than
+// 14336 elements, 13312 off 16-byte boundaries): each thread's second unit of it, and where there is no room for half a vector (beyond
+// 15360 off 16-byte boundaries) its first, is read from the caches for each row, before the barriers of the first statistics
+// (4096 x 16384 with an fp32 gate 148 us, 108 without its vector).  (A product of wp and gate made once would round in another order, and may leave fp32's range where z does not.)  (What can be absent from call to call is decided here where
 // the compiler would otherwise make a copy of the loop for each case, with the registers of all.)
 template <typename T, bool FOUR, int NU, bool FULL, int KIND>
-__global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(NU == 2 ? many_threads<T, KIND>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ double part[2][kManyThreads / 32];
   __shared__ WarpSum part32[2][kManyThreads / 32];
   __shared__ uint32_t warp_max[kManyThreads / 32];
   constexpr int E = (int)sizeof(T);
-  constexpr bool KEEP = NU == 1, SHARED = NU == 2 && E == 2, BLOCK = KIND > 0, MATRIX = KIND == 2;
+  constexpr bool KEEP = NU == 1, SHARED = NU == 2 && E == 2, BLOCK = KIND > 0, MATRIX = KIND == 2, CACHED = KIND == 3;
   const int tx = threadIdx.x, TX = blockDim.x;
   // Places of this warp: stage by stage, then unit by unit, then matrix by matrix.
   const uint32_t per_unit = p.place, per_stage = (uint32_t)(((BLOCK ? 2 : 1) + (MATRIX ? p.gate_ahead : 0)) * NU) * per_unit;
@@ -107,13 +109,11 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
     if constexpr (!MATRIX) {
       load_params<T>(p.gate, p.param32, e[i], n[i], vk);
 #pragma unroll
-      for (int j = 0; j < kUnit / 2; ++j) {
-        vk[j] = mul2(vk[j], f2(p.scale));
-        if (SHARED && p.gate && !p.gate_apart) vp[j] = mul2(vp[j], vk[j]);
-      }
+      for (int j = 0; j < kUnit / 2; ++j) vk[j] = mul2(vk[j], f2(p.scale));
     }
   };
   const SharedVectors vectors = {sm100::smem_u32(slots) + (uint32_t)p.vectors_at, (uint32_t)(NU * TX) * 16u};
+  const SharedVectors half_gate = {vectors.base + 8u * vectors.per_chunk, (uint32_t)TX * 16u};
   if constexpr (KEEP) {
     load_w(0);
     if (BLOCK) load_k(0);
@@ -125,8 +125,9 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
         vectors.put(0, i * TX + tx, vw);
         if (BLOCK) {
           load_k(i);
+          if (CACHED && i == 0 && p.gate_vector) half_gate.put(0, tx, vk);
           vectors.put(1, i * TX + tx, vp);
-          if (!MATRIX && p.gate_apart) vectors.put(2, i * TX + tx, vk);
+          if (!MATRIX && !CACHED && p.gate_vector) vectors.put(2, i * TX + tx, vk);
         }
       }
     }
@@ -188,6 +189,12 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
     issue(row + p.stages * step, at);
     if (++stage == p.stages) stage = 0;
     if constexpr (BLOCK) {
+      F2 late[CACHED ? NU : 1][kUnit / 2];
+      if constexpr (CACHED) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+          if (i > 0 || !each_row(p.gate_vector)) load_params<T>(p.gate, p.param32, e[i], n[i], late[i]);
+      }
       const F2 q = f2(p.wp ? inverse_rms(y) : 1.f);
 #pragma unroll
       for (int i = 0; i < NU; ++i) forget(y[i]);
@@ -195,14 +202,21 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T>() : kMaxThreads, 1) 
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         if (!KEEP && !SHARED) load_k(i);
-        const bool gated = SHARED && !MATRIX && each_row(p.gate_apart);
+        const bool gated = SHARED && !MATRIX && !CACHED && each_row(p.gate_vector);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           F2 w[2] = {vp[2 * c], vp[2 * c + 1]}, k[2] = {vk[2 * c], vk[2 * c + 1]};
           if (SHARED) {
             vectors.get(1, i * TX + tx, c, w[0], w[1]);
-            if (!MATRIX) {
-              k[0] = k[1] = f2(p.rest);
+            if constexpr (CACHED) {
+              if (i == 0 && each_row(p.gate_vector)) {
+                half_gate.get(0, tx, c, k[0], k[1]);
+              } else {
+                k[0] = mul2(late[i][2 * c], f2(p.scale));
+                k[1] = mul2(late[i][2 * c + 1], f2(p.scale));
+              }
+            } else if (!MATRIX) {
+              k[0] = k[1] = f2(p.scale);
               if (gated) vectors.get(2, i * TX + tx, c, k[0], k[1]);
             }
           }
@@ -303,12 +317,13 @@ cudaError_t launch_forward(const NormParams& p0, cudaStream_t st) {
   p.place = place_bytes((int)sizeof(T), FULL || rows_wide(p));
   const int two = (KIND ? 2 : 1) * NU * (int)p.place, three = two + (KIND == 2 ? NU * (int)p.place : 0);
   const int tx = ((units + NU - 1) / NU + 31) / 32 * 32, vector = SHARED ? tx * NU * kUnit * 4 : 0;
-  p.rest = p.gate ? 1.f : p.scale;
-  p.gate_apart = SHARED && KIND == 1 && p.gate && 3 * vector + two * (tx / 32) <= kSmemLimit;
-  const int vectors = vector * (KIND == 0 ? 1 : p.gate_apart ? 3 : 2);
-  // A gate matrix is not copied ahead where there is no room for it (rows of more than some 14000 elements).
+  if constexpr (SHARED && KIND == 1)
+    if (p.gate && 3 * vector + two * (tx / 32) > kSmemLimit) return launch_forward<T, FOUR, NU, FULL, 3>(p0, st);
+  p.gate_vector = KIND == 3 ? 2 * vector + vector / 2 + two * (tx / 32) <= kSmemLimit : KIND == 1 && p.gate;
+  const int vectors = KIND == 0 ? vector : 2 * vector + (p.gate_vector ? vector / (KIND == 3 ? 2 : 1) : 0);
+  // A gate matrix is not copied ahead where there is no room for it (16-bit rows of more than 15360 elements off 16-byte boundaries).
   p.gate_ahead = KIND == 2 && vectors + three * (tx / 32) <= kSmemLimit;
-  const Shape s = shape_of(p.rows, units, NU, p.gate_ahead ? three : two, NU == 2 ? many_threads<T>() : kMaxThreads, vectors);
+  const Shape s = shape_of(p.rows, units, NU, p.gate_ahead ? three : two, NU == 2 ? many_threads<T, KIND>() : kMaxThreads, vectors);
   if (s.stages < 1) return cudaErrorInvalidValue;
   p.stages = s.stages;
   p.vectors_at = (int32_t)s.smem;

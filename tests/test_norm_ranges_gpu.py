@@ -55,6 +55,26 @@ def test_statistics_of_uneven_rows(pkg, cuda, dtype, kind, rows, cols):
         assert ((f.row_scale == ways[0].row_scale) | (f.row_scale == ways[1].row_scale)).all()
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("rows,cols", [(300, 16384), (300, 14337), (300, 13313), (170, 12288), (90, 1001), (4, 8192)])
+def test_the_gate_comes_after_the_weight(pkg, cuda, dtype, wide, rows, cols):
+    """z times gate * scale in that order for every number of columns, also where weight times gate leaves fp32's range."""
+    y = normal((rows, cols), 5, dtype)
+    x = torch.zeros_like(y)
+    wp, gate = (normal((cols,), i, torch.float32 if wide else dtype, 0.3) + 1 for i in (3, 4))
+    if wide:
+        y[:, 7] *= 2.0 ** -13
+        wp[7], gate[7] = 1e20, 1e20 if dtype == torch.bfloat16 else 1e-16
+        gate[8], wp[9] = 1e-30, 1e-20
+    for shift in (0, 1):      # vectors off 16-byte boundaries
+        v = [torch.nn.functional.pad(t, (shift, 0))[shift:] for t in (wp, gate)]
+        x_out, _ = pkg.residual_norm(x, y, post_weight=v[0], gate=v[1], scale=0.3)
+        k = gate.float() * torch.tensor(0.3, device="cuda")
+        ways = [(((y.float() * q) * wp.float()) * k).to(dtype) for q in inverse_roots(y, 1e-6)]
+        assert ((x_out == ways[0]) | (x_out == ways[1])).all(), (x_out != ways[0]).sum().item()
+
+
 # ------------------------------------------------------------------ gradients of rows far from one
 FAR = [1.0, 1e14, 1e16, 1e20, 1e-13, 1e-20]
 
