@@ -11,7 +11,7 @@
 // each; in a pair warps 6..9 take every other chunk).
 //   whole-K form   persistent CTAs (CTA pairs for large problems), two
 //                  accumulators, so a tile's epilogue overlaps the next mainloop.  Two of 256
-//                  tokens and the scales do not fit in tensor memory: their positions overlap by 64 columns, which
+//                  tokens and two atoms' scales do not fit in tensor memory: their positions overlap by 96 columns, which
 //                  the epilogue reads first.
 //   split-K form   for few tiles: the CTAs of a cluster share one tile's K and
 //                  add their fp32 partial tiles in the order of their ranks through distributed shared
@@ -52,7 +52,7 @@ constexpr int kFusedBN = 16;            // its MMA N, the smallest there is for 
 constexpr int kStageWarps = 12;         // warps of the fused form that quantise tokens (the epilogue's four among them)
 constexpr int kFusedElems = 16384;      // most tokens x K (in whole atoms) of the fused form: at most 96 KB of shared memory
 constexpr int kMaxGroups = 2;           // epilogue groups of a CTA pair's kernel (four warps each)
-constexpr int kOverlap = 64;            // columns that the two positions of a 256-token accumulator share
+constexpr int kOverlap = 96;            // columns that the two positions of a 256-token accumulator share: three chunks of the epilogue
 constexpr int kTmemCols = 512;          // all of it: one CTA per SM
 // Most threads of a CTA.
 __host__ __device__ constexpr int threads_for(int cg, bool fuse) {
@@ -66,6 +66,7 @@ constexpr int kMinSmemPerCta = 120 * 1024;
 constexpr int kBarrierBytes = 1024;
 constexpr int kStaticSmem = 512;        // bound of the static shared memory of the fused form
 constexpr int kMaxStages = 32;
+constexpr int kScaleBars = 4;
 constexpr int kCBufs = 4;               // most staging buffers of an epilogue group that reads C by TMA:
                                         // all but two hold chunks of C on their way
 constexpr int kAtom = 128;              // bytes of one swizzled K atom
@@ -74,6 +75,17 @@ constexpr uint32_t kTokAtom = 8 * kAtom;  // fused form: bytes of one K atom of 
 constexpr uint32_t kTokTile = 128;      // fused form: bytes of one scale tile of 8 tokens x 4 scales (rows 16 bytes apart)
 __host__ __device__ constexpr int tiles_per_atom(int block) { return kAtomK / 4 / block; }
 constexpr int kChannels = 128;          // channels per CTA
+constexpr int kMaxStages4 = 12;         // most stages of a ring (the barriers have room for kMaxStages)
+// A copy of scales to tensor memory is ordered behind the MMAs that read what it overwrites by nothing but their commit.  They have as
+// many slots as there are stages, whose loads have waited for that commit: then nothing more has to be waited for.  The 256-token
+// tile has room for two slots (blocks of 16) or four (blocks of 32), each with a barrier that its issuer waits for (4096 x 8192 x 8192,
+// blocks of 16: 105.8 us; 103.3 with one slot that nothing guarded, 117 with four slots of half an atom).
+__host__ __device__ constexpr int slot_columns(int bn, int block) { return tiles_per_atom(block) * 4 * (1 + (bn + 127) / 128); }
+__host__ __device__ constexpr int first_slot(int bn) { return bn == 256 ? 2 * bn - kOverlap : 2 * bn; }           // behind the accumulators
+__host__ __device__ constexpr int scale_slots(int bn, int block) {
+  const int n = (kTmemCols - first_slot(bn)) / slot_columns(bn, block);
+  return n < kMaxStages4 ? n : kMaxStages4;
+}
 constexpr int kMaxSplit = 8;            // CTAs that may share a tile's K (portable cluster size)
 
 template <int V>
@@ -248,10 +260,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channe
   constexpr int NSF = tiles_per_atom(BLOCK);        // scale tiles of a K atom
   constexpr int TB = (BN + 127) / 128;              // row blocks of 128 tokens
   constexpr int OV = BN == 256 ? kOverlap : 0;      // columns that the accumulator's two positions share
-  constexpr uint32_t SF0 = BN == 256 ? 2 * BN - OV : 2 * BN;      // first scale column
-  constexpr uint32_t SF_COLS = NSF * 4 * (1 + TB);  // scale columns of a K atom
-  constexpr uint32_t SF_SLOTS = (kTmemCols - SF0) / SF_COLS < 8 ? (kTmemCols - SF0) / SF_COLS : 8;
-  static_assert(SF_SLOTS >= 1, "scales fit behind the accumulators");
+  constexpr uint32_t SF0 = first_slot(BN), SF_COLS = slot_columns(BN, BLOCK), SF_SLOTS = scale_slots(BN, BLOCK);
+  constexpr bool SF_WAIT = BN == 256;
+  static_assert(!SF_WAIT || (CG == 2 && SF_SLOTS >= 2 && SF_SLOTS <= kScaleBars), "scales of two atoms fit behind the accumulators");
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_base = smem_u32(smem_raw);
@@ -269,6 +280,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channe
   const uint32_t tok_bar = abort_flag + 4u;              // fused form: the tokens are in place
   const uint32_t c_bar = tok_bar + 8u;                   // [groups][kCBufs]: a chunk of C is in its buffer
   const uint32_t lost_flag0 = c_bar + 8u * kCBufs * kMaxGroups;   // [groups]: a warp of the group has given up a wait
+  const uint32_t scale_bar = lost_flag0 + 4u * kMaxGroups;        // [kScaleBars]: the MMAs have read a slot's scales
   __shared__ uint32_t tok_top[FUSE ? kFusedTokens : 1];
 
   const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -300,6 +312,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channe
     mbar_init(drain_bar, 1);
     mbar_init(tok_bar, kStageWarps);
     for (int b = 0; b < kCBufs * kMaxGroups; ++b) mbar_init(c_bar + 8u * b, 1);
+    for (int b = 0; b < kScaleBars; ++b) mbar_init(scale_bar + 8u * b, 1);
     st_shared_u32(abort_flag, 0u);
     for (int g = 0; g < kMaxGroups; ++g) st_shared_u32(lost_flag0 + 4u * g, 0u);
     fence_mbar_init();
@@ -405,7 +418,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channe
     if (leader) {
       const uint32_t issue = elect_one() ? 1u : 0u;
       int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0, pos = 0, slot = 0;
+      uint32_t phase = 0, acc_phase = 0, pos = 0, slot = 0, slot_phase = 0;
       bool ok = true, issued = false;
       if constexpr (FUSE) {
         const bool wt = wait_bar<false>(tok_bar, 0, ctl, ROLE_MMA, 0x90u);
@@ -423,24 +436,25 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channe
           if (!w) { ok = false; break; }
           tc_fence_after();
           const uint32_t w_src = base + (uint32_t)stage * p.stage_bytes;
+          const uint32_t t_src = w_src + p.a_bytes;
+          const uint32_t ws_src = FUSE ? t_src : t_src + (uint32_t)(TROWS * kAtom);
+          const uint32_t ts_src = FUSE ? base + p.tok_tiles + (uint32_t)((kb - kb_begin) * NSF) * kTokTile : ws_src + NSF * 512u;
+          const uint64_t wd = sw128_kmajor_desc(w_src);
+          const uint64_t td = sw128_kmajor_desc(FUSE ? base + p.tok_offset + (uint32_t)(kb - kb_begin) * kTokAtom : t_src);
+          if constexpr (SF_WAIT) {
+            if (!wait_bar<false>(scale_bar + 8u * slot, slot_phase ^ 1u, ctl, ROLE_MMA, 0xA0u | slot)) { ok = false; break; }
+            tc_fence_after();
+          }
           if (CG == 1 || issue) {
-            // This atom's scales go to the next of the slots, so that their copy never overwrites scales
-            // that the MMAs of the atom before still read.
-            const uint32_t t_src = w_src + p.a_bytes;
-            const uint32_t ws_src = FUSE ? t_src : t_src + (uint32_t)(TROWS * kAtom);
-            const uint32_t ts_src = FUSE ? base + p.tok_tiles + (uint32_t)((kb - kb_begin) * NSF) * kTokTile : ws_src + NSF * 512u;
             const uint32_t ws_t = tmem_base + SF0 + slot * SF_COLS, ts_t = ws_t + NSF * 4u;
-            if (++slot == SF_SLOTS) slot = 0;
+            const uint64_t ws_desc = plain_desc(ws_src), ts_desc = plain_desc(ts_src);      // (in units of 16 bytes)
 #pragma unroll
             for (int q = 0; q < NSF; ++q) {
-              tmem_cp_32x128b_warpx4<CG>(ws_t + 4u * q, plain_desc(ws_src + 512u * q), issue);
+              tmem_cp_32x128b_warpx4<CG>(ws_t + 4u * q, ws_desc + 32u * q, issue);
 #pragma unroll
               for (int b = 0; b < TB; ++b)
-                tmem_cp_32x128b_warpx4<CG>(ts_t + (uint32_t)(q * TB + b) * 4u,
-                                           plain_desc(FUSE ? ts_src + kTokTile * q : ts_src + (uint32_t)(b * NSF + q) * 512u), issue);
+                tmem_cp_32x128b_warpx4<CG>(ts_t + (uint32_t)(q * TB + b) * 4u, ts_desc + (FUSE ? kTokTile / 16u * q : (uint32_t)(b * NSF + q) * 32u), issue);
             }
-            const uint64_t wd = sw128_kmajor_desc(w_src);
-            const uint64_t td = sw128_kmajor_desc(FUSE ? base + p.tok_offset + (uint32_t)(kb - kb_begin) * kTokAtom : t_src);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
               const uint32_t acc_on = (kb != kb_begin || kk) ? 1u : 0u;
@@ -450,10 +464,12 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channe
                 mma_mxf4<CG>(d_tmem, wd + 2u * kk, td + 2u * kk, p.idesc | (kk & 1 ? kUpperScales : 0u), ws_t + 4u * (kk / 2),
                              ts_t + 4u * TB * (kk / 2), acc_on, issue);
             }
+            if constexpr (SF_WAIT) mma_commit_pair(scale_bar + 8u * slot, 0x1, issue);
             if constexpr (CG == 2) mma_commit_pair(empty_bar + 8u * stage, 0x3, issue);
             else mma_commit(empty_bar + 8u * stage, issue);
           }
           issued = true;
+          if (++slot == SF_SLOTS) { slot = 0; slot_phase ^= 1u; }
           if (++stage == p.stages) { stage = 0; phase ^= 1u; }
           ready = CG == 2 ? mbar_test_wait_cluster(full_bar + 8u * stage, phase)
                           : mbar_test_wait(full_bar + 8u * stage, phase);
@@ -881,7 +897,9 @@ int resolve(const Fp4GemmArgs* a, bool fused, Resolved& r) {
   const int64_t tok_tiles = fused ? ((int64_t)kb_cta * sf * kTokTile + 384 + 511) / 512 * 512 : 0;
   const int64_t fixed = 1024 + kBarrierBytes + (int64_t)p.groups * p.stg_bufs * p.stg_bytes + p.groups * 4 * r.bn * 4 + tok_bytes + tok_tiles + kStaticSmem;
   r.max_stages = (int)((kSmemLimit - fixed) / p.stage_bytes);
-  if (r.max_stages > 12) r.max_stages = 12;
+  if (r.max_stages > kMaxStages4) r.max_stages = kMaxStages4;
+  // (No tile but that of 256 tokens has more stages than slots as it is.)
+  if (r.bn != 256 && r.max_stages > scale_slots(r.bn, a->block)) r.max_stages = scale_slots(r.bn, a->block);
   r.stages = r.max_stages;
   if (r.split > 1) {
     if (r.stages > kb_cta) r.stages = kb_cta;
