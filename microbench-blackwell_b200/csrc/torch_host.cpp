@@ -213,11 +213,20 @@ void* stream_of(int index) { return c10::cuda::getCurrentCUDAStream((c10::Device
 // The output of a product or of dropout: `o`, or a new packed one.
 struct Output {
   at::Tensor fresh;
-  PyObject* given;
+  PyObject* given = nullptr;
+  bool written = false;      // `given` is (or is about to be) overwritten
   void* ptr;
   int64_t ld;
+  // After the launch.  Autograd then sees that a tensor which it has saved is no longer what it was.
   PyObject* wrap() {
-    if (given) { Py_INCREF(given); return given; }
+    if (given) {
+      if (written) {
+        const at::Tensor& t = THPVariable_Unpack(given);
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+      }
+      Py_INCREF(given);
+      return given;
+    }
     return THPVariable_Wrap(std::move(fresh));
   }
 };
@@ -229,10 +238,10 @@ Output output(PyObject* o, int64_t rows, int64_t cols, at::ScalarType t, int ind
     same_type(m, "out", t);
     shape(m, "out", rows, cols);
     out.given = o;
+    out.written = true;
     out.ptr = m.ptr;
     out.ld = m.ld;
   } else {
-    out.given = nullptr;
     out.fresh = empty({rows, cols}, t, index);
     out.ptr = out.fresh.data_ptr();
     out.ld = cols > 0 ? cols : 1;
