@@ -117,3 +117,29 @@ def test_large_gradients_of_ordinary_rows(pkg, cuda):
     x_out, dh = normal((3, 600), 20) * 1e8, normal((3, 600), 21)
     dh[1] *= 1e32
     check_backward(pkg, s, dh, None, x_out)
+
+
+# ------------------------------------------------------------------ many rows in place
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(5000, 512), (4001, 1001), (3000, 4096), (1200, 8192), (700, 16384), (20000, 24)])
+def test_many_rows_in_place(pkg, cuda, dtype, rows, cols):
+    """Groups that walk down many rows with the coming ones copied ahead: x_out over x or y, aligned and off 16-byte
+    boundaries, is that of a call apart."""
+    s = case(rows, cols, dtype, True, "vector")
+    for shift in (0, 3):
+        for name in ("x", "y"):
+            store = torch.full((rows + 1, cols + 8 + shift), 7.0, dtype=dtype, device="cuda")
+            t = dict(x=s["x"], y=s["y"])
+            t[name] = store[:rows, shift:shift + cols]
+            t[name].copy_(s[name])
+            around = dict(weight=s["weight"], post_weight=s["post"], gate=s["gate"], scale=0.5)
+            want = pkg.residual_norm(t["x"], t["y"], **around)
+            want4 = pkg.residual_norm(t["x"], t["y"], fp4=16, **around)[1]
+            got = pkg.residual_norm(t["x"], t["y"], out=t[name], **around)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            t[name].copy_(s[name])
+            _, four = pkg.residual_norm(t["x"], t["y"], fp4=16, out=t[name], **around)
+            assert torch.equal(t[name], want[0])
+            assert torch.equal(four.values, want4.values) and torch.equal(four.row_scale, want4.row_scale)
+            store[:rows, shift:shift + cols] = 7.0
+            assert (store == 7.0).all()
