@@ -214,33 +214,23 @@ __device__ __forceinline__ void stage_tokens(const Fp4Params& p, uint32_t tok, u
 // One element of a staged chunk.
 template <typename T>
 __device__ __forceinline__ float staged(uint32_t addr) {
-  if constexpr (sizeof(T) == 4) {
-    return __uint_as_float(ld_shared_u32(addr));
-  } else {
-    const uint16_t h = ld_shared_u16(addr);
-    T v;
-    __builtin_memcpy(&v, &h, 2);
-    return to_f32(v);
-  }
+  const uint16_t h = ld_shared_u16(addr);
+  T v;
+  __builtin_memcpy(&v, &h, 2);
+  return to_f32(v);
 }
 
 // A thread's column of a chunk, `tokens` rows of D from `d`, `step` bytes apart: for
 // a D that TMA cannot store.  With one warp per scheduler every instruction counts, hence the running
-// pointer and the paired conversions (777 x 5001 x 2048: 18.1 us through shared memory in
-// aligned 16-byte stores).
+// pointer and the paired conversions.
 template <typename T, int CW>
 __device__ __forceinline__ void store_column(uint8_t* d, int64_t step, const float (&v)[CW], int tokens) {
 #pragma unroll
   for (int j = 0; j < CW; j += 2) {
     uint8_t* const d1 = d + step;
-    if constexpr (sizeof(T) == 4) {
-      if (j < tokens) *reinterpret_cast<float*>(d) = v[j];
-      if (j + 1 < tokens) *reinterpret_cast<float*>(d1) = v[j + 1];
-    } else {
-      const uint32_t h = pack2<T>(v[j], v[j + 1]);
-      if (j < tokens) *reinterpret_cast<uint16_t*>(d) = (uint16_t)h;
-      if (j + 1 < tokens) *reinterpret_cast<uint16_t*>(d1) = (uint16_t)(h >> 16);
-    }
+    const uint32_t h = pack2<T>(v[j], v[j + 1]);
+    if (j < tokens) *reinterpret_cast<uint16_t*>(d) = (uint16_t)h;
+    if (j + 1 < tokens) *reinterpret_cast<uint16_t*>(d1) = (uint16_t)(h >> 16);
     d = d1 + step;
   }
 }
@@ -552,9 +542,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channe
           if (t < BN) st_shared_u32(sa_s + 4u * t, __float_as_uint(sa));
         }
         __syncwarp();
-      } else {
-        // The staging warps' scales: in place before any sum is.
       }
+      // (Fused form: the staging warps' scales are in place before any sum is.)
       const bool ok = __all_sync(0xffffffffu, wait_bar<false>(tfull_bar + 8u * acc, acc_phase, ctl, ROLE_EPILOGUE, acc));
       if (!p.tma_store) {
         if (!ok) break;
@@ -646,14 +635,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w,   // weights: channe
           }
 #pragma unroll
           for (int j = 0; j < CW; j += 2) {
-            if constexpr (sizeof(T) == 4) {
-              st_shared_u32(at + (uint32_t)(j * kChannels * 4), __float_as_uint(v[j]));
-              st_shared_u32(at + (uint32_t)((j + 1) * kChannels * 4), __float_as_uint(v[j + 1]));
-            } else {
-              const uint32_t h = pack2<T>(v[j], v[j + 1]);
-              st_shared_u16(at + (uint32_t)(j * kChannels * 2), (uint16_t)h);
-              st_shared_u16(at + (uint32_t)((j + 1) * kChannels * 2), (uint16_t)(h >> 16));
-            }
+            const uint32_t h = pack2<T>(v[j], v[j + 1]);
+            st_shared_u16(at + (uint32_t)(j * kChannels * 2), (uint16_t)h);
+            st_shared_u16(at + (uint32_t)((j + 1) * kChannels * 2), (uint16_t)(h >> 16));
           }
           fence_proxy_async_shared();
           named_bar_sync(bar_id, 128);
