@@ -56,7 +56,7 @@ struct NormParams {
 // KIND 0: no y; 1: y; 2: y and a gate matrix; 3: y and a gate vector of 16-bit rows that shared memory has no room for (more than
 // 14336 elements, 13312 off 16-byte boundaries): each thread's second unit of it, and where there is no room for half a vector (beyond
 // 15360 off 16-byte boundaries) its first, is read from the caches for each row, before the barriers of the first statistics
-// (4096 x 16384 with an fp32 gate 148 us, 108 without its vector).  (A product of wp and gate made once would round in another order, and may leave fp32's range where z does not.)  (What can be absent from call to call is decided here where
+// (4096 x 16384 with an fp32 gate 159 us, 108 with one product of wp and gate).  (A product of wp and gate made once would round in another order, and may leave fp32's range where z does not.)  (What can be absent from call to call is decided here where
 // the compiler would otherwise make a copy of the loop for each case, with the registers of all.)
 template <typename T, bool FOUR, int NU, bool FULL, int KIND>
 __global__ void __launch_bounds__(NU == 2 ? many_threads<T, KIND>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
@@ -225,10 +225,10 @@ __global__ void __launch_bounds__(NU == 2 ? many_threads<T, KIND>() : kMaxThread
             const int j = 2 * c + l;
             F2 z = mul2(mul2(pair(y[i], j), q), w[l]);
             if (MATRIX) k[l] = mul2(pair(gate[i], j), f2(p.scale));
-            z = mul2(z, k[l]);
+            // (A product and a sum of pairs become one multiply-add, whatever their rounding modes say; two sums do not.)
             float a, b;
-            add2(pair(x[i], j), z).get(a, b);
-            x[i].set2(2 * j, a, b);
+            mul2(z, k[l]).get(a, b);
+            x[i].set2(2 * j, __fadd_rn(x[i].get(2 * j), a), __fadd_rn(x[i].get(2 * j + 1), b));
           }
         }
         put_unit<T, FULL>(out + e[i] * E, x[i], n[i]);

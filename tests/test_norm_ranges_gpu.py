@@ -75,6 +75,16 @@ def test_the_gate_comes_after_the_weight(pkg, cuda, dtype, wide, rows, cols):
         assert ((x_out == ways[0]) | (x_out == ways[1])).all(), (x_out != ways[0]).sum().item()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gate", ["vector", "matrix", "none"])
+@pytest.mark.parametrize("rows,cols", [(900, 4096), (700, 1001), (5, 8192), (200, 16384)])
+def test_the_product_is_rounded_before_the_sum(pkg, cuda, dtype, gate, rows, cols):
+    s = case(rows, cols, dtype, False, gate)
+    k = torch.tensor(0.3, device="cuda") * (1.0 if s["gate"] is None else s["gate"].float())
+    x_out, _ = pkg.residual_norm(s["x"], s["y"], gate=s["gate"], scale=0.3)
+    assert torch.equal(x_out, (s["x"].float() + s["y"].float() * k).to(dtype))
+
+
 # ------------------------------------------------------------------ gradients of rows far from one
 FAR = [1.0, 1e14, 1e16, 1e20, 1e-13, 1e-20]
 
