@@ -464,7 +464,8 @@ int64_t gemm_sm100a_fp4_scale_bytes(int64_t rows, int64_t cols, int32_t block);
  * Quantise the rows of X:
  *   row_scale g = 2^(floor(log2 max|x|) - 10), at least 2^-126;  y = x / g in fp32 (exact from 2^-126 on)
  *   scale     s = the least e4m3 number (block 16) or power of two from 2^-126 on (block 32) with
- *                 6 s >= max|y| over the block
+ *                 6 s >= max|y| over the block (so nothing is clipped; the OCP conversion to blocks of 32 takes
+ *                 2^(floor(log2 max) - 2) and saturates)
  *   value     q = y / s rounded to e2m1, ties to the even code, decided exactly
  * A row with a NaN or an infinity gets that as its row scale and zeros as values: what is computed from
  * it is NaN, and no other row is touched.  The three outputs overlap neither X nor one another.

@@ -21,8 +21,8 @@
 //                  quantise the CTA's part of them straight into the swizzled
 //                  operand and its scale tiles, which stay in shared memory for all of its tiles.
 //
-// Measured on B200 (from graphs): 8192 x 28672 x 8192 in 773 to 820 us at the clock that the power cap leaves (4.7 to 5.0
-// PFLOP/s), 4096 x 8192 x 8192 in 116 (4.75); 48 x 28672 x 8192 in 26.5, its 132 MB at 5 of the 6.55 TB/s that a copy
+// Measured on B200: 8192 x 28672 x 8192 in 748 to 790 us at the clock that the power cap leaves (4.9 to 5.1
+// PFLOP/s), 4096 x 8192 x 8192 in 106 (5.2); 48 x 28672 x 8192 in 26.5, its 132 MB at 5 of the 6.55 TB/s that a copy
 // reaches; one token x 8192 x 8192 in 10.0 in one launch, of which some 4 are launch, first loads and last stores.
 #include <cuda.h>
 #include <cudaTypedefs.h>

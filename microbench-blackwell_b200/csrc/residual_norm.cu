@@ -4,9 +4,9 @@
 //
 //   z = y r(y) wp,  x' = x + (gate scale) z,  h = x' r(x') w,  r(v) = 1 / sqrt(mean(v^2) + eps)
 //
-// Measured on B200: 16384 x 8192 bf16 with gate and fp32 vectors 174 to 200 us a call (5.4 to 6.2 of the 6.55 TB/s that a copy
-// reaches: the same build gives either, as the memory serves four streams), from fp32 398 us; into a 4-bit operand 206 us, bound by
-// issue slots (62 % busy); one row 3.9 and 4.2 us, launch included.
+// Measured on B200: 16384 x 8192 bf16 with gate and fp32 vectors 172 to 200 us a call (5.4 to 6.2 of the 6.55 TB/s that a copy
+// reaches: the same build gives either, as the memory serves four streams), with a gate matrix 236, from fp32 398 us; into a 4-bit
+// operand 223 us, bound by issue slots (67 % busy); one row 4.8 and 6.9 us a call.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -56,8 +56,10 @@ struct NormParams {
 // KIND 0: no y; 1: y; 2: y and a gate matrix; 3: y and a gate vector of 16-bit rows that shared memory has no room for (more than
 // 14336 elements, 13312 off 16-byte boundaries): each thread's second unit of it, and where there is no room for half a vector (beyond
 // 15360 off 16-byte boundaries) its first, is read from the caches for each row, before the barriers of the first statistics
-// (4096 x 16384 with an fp32 gate 159 us, 108 with one product of wp and gate).  (A product of wp and gate made once would round in another order, and may leave fp32's range where z does not.)  (What can be absent from call to call is decided here where
-// the compiler would otherwise make a copy of the loop for each case, with the registers of all.)
+// (4096 x 16384 with an fp32 gate 159 us, 108 with one product of wp and gate made before, which rounds in another order
+// and may leave fp32's range where z does not).
+// (What can be absent from call to call is decided here where the compiler would otherwise make a copy of the loop for each
+// case, with the registers of all.)
 template <typename T, bool FOUR, int NU, bool FULL, int KIND>
 __global__ void __launch_bounds__(NU == 2 ? many_threads<T, KIND>() : kMaxThreads, 1) residual_norm_kernel(const __grid_constant__ NormParams p) {
   extern __shared__ __align__(16) uint8_t slots[];

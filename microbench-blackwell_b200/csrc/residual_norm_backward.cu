@@ -9,9 +9,11 @@
 // kept from the forward call.  The sums over rows (dw, dwp, dgate) stay with the threads of a block, which walks down the
 // matrix; the blocks' parts go through a workspace to a second kernel that adds them in order.
 //
-// Measured on B200: 16384 x 8192 bf16 with gate and fp32 vectors 341 us a call (306 from a graph with bf16 vectors, 5.3 of the
-// 6.55 TB/s that a copy reaches), fp32 578; bound by issue slots, 48 % busy with the 16 warps that the column sums' registers
-// leave room for.  333 x 1001 fp32 with a gate matrix 13 us, of which the host's call is 9.
+// Measured on B200: 16384 x 8192 bf16 with gate and fp32 vectors 327 to 347 us a call (4.6 to 4.9 of the 6.55 TB/s that a copy
+// reaches); bound by latency: the column sums' registers and the vectors leave room for two groups of 8 warps and one row
+// each, the next row is asked for after the second pass of the one before, and between its two barriers a group's first warp
+// works alone (issue slots 48 % busy).  With a gate matrix 412, fp32 694; 4096 x 8192 rows of zeros 99.
+// 333 x 1001 fp32 with a gate matrix 13 us, of which the host's call is 9.
 #include <cuda_runtime.h>
 
 #include <cstdint>

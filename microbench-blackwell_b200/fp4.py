@@ -82,7 +82,11 @@ def quantize_fp4(x: torch.Tensor, *, block: int = 16) -> Fp4:
 
     row scale g = 2^(floor(log2 max|x|) - 10), at least 2^-126; block scale s = the least e4m3 number
     (``block`` 16) or power of two from 2^-126 on (32) with 6 s >= max|x / g| over the block; values x / (g s) rounded to
-    e2m1, ties to the even code, decided exactly.  A row with NaN or Inf gets that as its row scale."""
+    e2m1, ties to the even code, decided exactly.  A row with NaN or Inf gets that as its row scale.
+
+    No element is clipped.  The conversion of the OCP microscaling formats takes 2^(floor(log2 max|x|) - 2) for blocks of 32
+    instead and saturates what lies above 6 of it, so codes of its quantisers differ from these in blocks whose largest
+    element is more than 1.5 times a power of two."""
     return Fp4(*_host().quantize_fp4(x, block), x.shape[1], block)
 
 

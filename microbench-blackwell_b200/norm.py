@@ -67,7 +67,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor | None = None, *, weight: tor
     x_out is x.  ``fp4`` = 16 or 32: h is an ``Fp4`` with blocks of that size, from its fp32 values.  ``out`` takes
     x_out; it may be x or y.
 
-    One fp32 operation follows the other from left to right, means of squares are taken in 64 bits; x_out is rounded to x's type, and h is that of the rounded x_out."""
+    One fp32 operation follows the other from left to right, means of squares are taken in 64 bits; x_out is rounded to x's
+    type, and h is that of the rounded x_out."""
     got = _host().residual_norm(x, y, weight, post_weight, gate, scale, eps, fp4, out)
     return (got[0], Fp4(got[1], got[2], got[3], x.shape[1], fp4)) if fp4 else got
 
